@@ -189,7 +189,7 @@ def prepare(case: dict, seed: int) -> dict:
         if own:  # the program's weights: laid out once
             import trntensor_amd as tt
 
-            state["w"] = tt.Q4Matrix(codes, scales, k, zeros=zeros)
+            state["w"] = tt.Q4Matrix(codes, scales, k, case["group"], zeros=zeros)
         else:
             state["codes"], state["scales"], state["zeros"] = codes, scales, zeros
         return state
