@@ -41,7 +41,7 @@
 extern "C" {
 #endif
 
-#define TT_ABI_VERSION 4
+#define TT_ABI_VERSION 5
 #define TT_MAX_DIMS 8
 
 enum { TT_OK = 0, TT_INVALID = 1, TT_UNSUPPORTED = 2, TT_HIP_ERROR = 3 };
@@ -252,6 +252,110 @@ int tt_strided_contract(int dtype, int n_out, const int64_t* out_shape,
                         const void* A, const void* B, double alpha, double beta,
                         const void* C, void* D, void* workspace, size_t workspace_bytes,
                         void* stream);
+
+/* ------------------------------------------------------------------------
+ * Serving operators of language models (no counterpart in the reference).
+ *
+ * Their arguments travel in structs whose fields are all 8 bytes wide, in the
+ * order given. Element strides count elements, pitches count bytes. dtype is
+ * TT_F32, TT_BF16 or TT_F16; sums, softmax statistics and rotations are held
+ * in 32 bits and rounded once at the store.
+ * --------------------------------------------------------------------- */
+
+/*
+ * y[m][n] = sum_k x[m][k] * scale[k / group][n] * (code[n][k] - zero[k / group][n])
+ * with 4-bit codes: row n of `codes` starts at n * code_pitch and byte j of it
+ * holds code 2j in its low and code 2j + 1 in its high half. code_pitch is a
+ * multiple of 64 and at least K / 2 rounded up to one (what the bytes past K
+ * hold does not matter); `codes` is 16-byte aligned. `scales` and `zeros`
+ * (NULL: every zero is 8) are [ceil(K / group)][N] in scale_dtype (TT_F32,
+ * TT_BF16, TT_F16). group is 32, 64 or a multiple of 128. x and y are rows of
+ * unit stride at ldx and ldy elements.
+ */
+typedef struct {
+    int64_t dtype, scale_dtype, M, N, K, group, ldx, code_pitch, ldy;
+    const void *x, *codes, *scales, *zeros;
+    void *y, *workspace;
+    int64_t workspace_bytes;
+} tt_q4_args;
+
+/* Device bytes of workspace that tt_q4_matmul needs (may be 0). */
+size_t tt_q4_matmul_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
+
+int tt_q4_matmul(const tt_q4_args* args, void* stream);
+
+/*
+ * A paged cache of keys and values in 8-bit floats (OCP e4m3, no infinities)
+ * with one power-of-two scale for each page and head: value = scale * code.
+ *   k       [pages][heads][page][width]   k_scale [pages][heads] (float)
+ *   v       [pages][heads][width][page]   v_scale [pages][heads]
+ * width is dim rounded up to a multiple of 64; a key's codes past dim are
+ * zeros. page (tokens a page) is a multiple of 16, dim at most 256. Token p of
+ * sequence b lies in page table[b * table_stride + p / page], slot p % page.
+ * A page number outside [0, pages) stands for no page: nothing is written
+ * there, and its tokens are not seen.
+ */
+typedef struct {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int64_t pages, heads, page, dim;
+} tt_kv_cache;
+
+/*
+ * Appends `tokens` keys and values of each sequence (counts[b] of them where
+ * counts is given) behind the lengths[b] tokens it holds. Where cos is given,
+ * the first rot elements of each key and query are rotated in pairs
+ * (a, b) -> (a cos - b sin, b cos + a sin), products and sums each rounded to
+ * 32 bits; pair i is (i, i + rot / 2), or (2i, 2i + 1) if interleaved; cos and
+ * sin are [positions][rot / 2] with positions >= table_width * page, and a
+ * token's position is its place in its sequence. q_out (contiguous) gets the
+ * rotated queries, zeros in rows past counts[b]. q may be NULL.
+ *
+ * A block's scale is the smallest power of two, at least 2^-64, that brings
+ * its new tokens' largest finite magnitude to 448 or below, or the one it has
+ * where that is larger and the block holds earlier tokens; if it grows, the
+ * earlier tokens' codes are rounded to it. Codes are rounded to nearest even
+ * and saturate at 448; NaN stays NaN. Tokens past table_width * page are
+ * dropped. Pages written to belong to one sequence each.
+ */
+typedef struct {
+    int64_t dtype, batch, tokens, q_heads, rot, interleaved, table_width, table_stride;
+    int64_t k_stride[3], v_stride[3], q_stride[3]; /* batch, token, head */
+    const void *k, *v, *q;
+    void* q_out;
+    const float *cos, *sin;
+    const int32_t *table, *lengths, *counts;
+    tt_kv_cache cache;
+} tt_kv_append_args;
+
+int tt_kv_append(const tt_kv_append_args* args, void* stream);
+
+/*
+ * Attention of `tokens` queries a sequence (counts[b] of them where counts is
+ * given) over its lengths[b] cached tokens, the queries being the last ones of
+ * them: query i is at position lengths[b] - counts[b] + i and sees token j if
+ * j <= position and, where window > 0, j > position - window or j < sinks.
+ * q is [batch][tokens][q_heads][dim] with strides, out the same, contiguous;
+ * q_heads is a multiple of the cache's heads and query head h reads cache head
+ * h / (q_heads / heads). Queries that see nothing, and rows past counts[b],
+ * give zeros. What masked slots of a page hold has no influence, NaN included.
+ */
+typedef struct {
+    int64_t dtype, batch, tokens, q_heads, window, sinks, table_width, table_stride;
+    int64_t q_stride[3]; /* batch, token, head */
+    double scale;
+    const void* q;
+    void* out;
+    const int32_t *table, *lengths, *counts;
+    tt_kv_cache cache;
+    void* workspace;
+    int64_t workspace_bytes;
+} tt_kv_attention_args;
+
+/* Device bytes of workspace that tt_kv_attention needs for these sizes (may be 0). */
+size_t tt_kv_attention_workspace_bytes(const tt_kv_attention_args* args);
+
+int tt_kv_attention(const tt_kv_attention_args* args, void* stream);
 
 /*
  * Measurement aid with no counterpart in the reference: `workgroups`

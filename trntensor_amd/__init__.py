@@ -23,6 +23,7 @@ from .plan import (
     plan_contraction,
 )
 from .quantum import ao_to_mo_transform, mp2_energy, mp2_energy_shard
+from .serving import KVCache, Q4Matrix, kv_append, kv_attention, q4_matmul
 
 __all__ = [
     "einsum",
@@ -43,4 +44,9 @@ __all__ = [
     "mp2_energy",
     "mp2_energy_shard",
     "ao_to_mo_transform",
+    "Q4Matrix",
+    "q4_matmul",
+    "KVCache",
+    "kv_append",
+    "kv_attention",
 ]

@@ -31,8 +31,11 @@ SOURCES = [
     "tt_gemm_big.hip",
     "tt_gemm_mid.hip",
     "tt_gemm_small.hip",
+    "tt_kv_append.hip",
+    "tt_kv_attention.hip",
     "tt_mp2.hip",
     "tt_probe.hip",
+    "tt_q4.hip",
     "tt_strided.hip",
 ]
 # Sources whose MFMA accumulators belong in AGPRs (256 fp32 per lane): built
