@@ -1,4 +1,11 @@
-// Attention over a paged cache of 8-bit floats.
+// Attention over a paged cache of 8-bit floats (tt_kv_attention).
+//
+//   o_r = sum_j softmax_j(scale * q_r . k_j) v_j over the keys j that row r sees
+//
+// in one pass over the keys with the running maximum and sum of a softmax;
+// neither scores nor widened keys and values ever leave registers.
+#include <type_traits>
+
 #include "tt_serving.hpp"
 
 namespace tt {
@@ -6,85 +13,849 @@ namespace tt {
 namespace {
 
 struct AttnParams {
-    int64_t tokens, q_heads, window, sinks, table_width, table_stride, q_stride[3];
-    float scale;
     const void* q;
     void* out;
     const int32_t *table, *lengths, *counts;
-    tt_kv_cache c;
-    int64_t width;
+    const uint8_t *k, *v;
+    const float *k_scale, *v_scale;
+    float* part;  // partial results: slots of rows * (width + 2) floats
+    int64_t q_stride[3], table_stride, pages;
+    int batch, tokens, q_heads, heads, share, page, dim, window, sinks;
+    int capacity;    // tokens that the table covers
+    int row_blocks;  // blocks of query rows of one cache head
+    int groups;      // workgroups that share the key tiles
+    int direct;      // each workgroup takes one pair, whole
+    FastDiv by_page, by_share;
+    float scale;  // times log2(e)
 };
 
-// One workgroup per query row: chunks of 256 keys, running maximum and sum.
+constexpr int kTile = 64;     // keys a wavefront takes at a time
+constexpr int kMinTiles = 4;  // fewest tiles worth a workgroup: one per wavefront
+
+// Which keys the query rows of one block see: those of [0, end) that are in a
+// row's window or among the sinks lie in tiles [0, sink_tiles) and [start, ..).
+struct Span {
+    int first_pos, last_pos;   // positions of the block's live rows
+    int held;                  // tokens that exist
+    int sink_tiles, start, tiles;
+    int live;                  // live rows of the block
+};
+
+__device__ __forceinline__ Span span_of(const AttnParams& p, int b, int row0, int rows) {
+    Span s = {0, -1, 0, 0, 0, 0, 0};
+    const int len = p.lengths[b];
+    const int n = p.counts ? p.counts[b] : p.tokens;
+    const int live_tokens = n < p.tokens ? n : p.tokens;
+    if (live_tokens <= 0 || len <= 0) return s;
+    const int64_t all = (int64_t)live_tokens * p.share;
+    s.live = all > row0 ? (int)(all - row0 < rows ? all - row0 : rows) : 0;
+    if (s.live <= 0) return s;
+    s.held = len < p.capacity ? len : p.capacity;
+    const int64_t base = (int64_t)len - n;
+    const int64_t first = base + (int)fdiv(row0, p.by_share), last = base + (int)fdiv(row0 + s.live - 1, p.by_share);
+    if (last < 0) return s;
+    s.first_pos = first < -1 ? -1 : (int)first;
+    s.last_pos = (int)last;
+    const int end = s.last_pos + 1 < s.held ? s.last_pos + 1 : s.held;
+    const int64_t low = p.window > 0 ? (int64_t)s.first_pos - p.window + 1 : 0;
+    s.start = low > 0 ? (int)(low / kTile) : 0;
+    if (s.start > 0) {
+        const int st = p.sinks / kTile + (p.sinks % kTile ? 1 : 0);
+        s.sink_tiles = st < s.start ? st : s.start;
+    }
+    const int last_tile = (end + kTile - 1) / kTile;
+    if (last_tile < s.start) s.start = last_tile;
+    if (s.sink_tiles > last_tile) s.sink_tiles = last_tile;
+    s.tiles = s.sink_tiles + last_tile - s.start;
+    return s;
+}
+
+// How a dtype's queries and probabilities enter the 16-bit matrix units. Codes
+// are exact in either 16-bit type. float32 splits into three bfloat16 parts
+// (24 bits); float16 queries are taken as they are, and their probabilities as
+// two bfloat16 parts (16 bits), since scaled values may pass float16's range.
 template <typename T>
-__global__ __launch_bounds__(256) void kv_attention_simple_kernel(AttnParams p) {
-    __shared__ float q[256], prob[256], part[4];
-    const int tid = threadIdx.x;
-    const int64_t H = p.c.heads, P = p.c.page, W = p.width, D = p.c.dim;
-    const int64_t h = blockIdx.x % p.q_heads, t = blockIdx.x / p.q_heads % p.tokens, b = blockIdx.x / p.q_heads / p.tokens;
-    const int64_t kh = h / (p.q_heads / H);
-    T* out = static_cast<T*>(p.out) + blockIdx.x * D;
-    int64_t len = p.lengths[b], n = p.counts ? p.counts[b] : p.tokens;
-    const int64_t pos = len - n + t;
-    if (len > p.table_width * P) len = p.table_width * P;
-    const bool live = t < n && pos >= 0;
-    const int64_t end = live ? (pos + 1 < len ? pos + 1 : len) : 0;  // keys [0, end)
-    const int64_t low = p.window > 0 ? pos - p.window + 1 : 0;        // and of them [low, ..) or [0, sinks)
-    const T* qrow = static_cast<const T*>(p.q) + b * p.q_stride[0] + t * p.q_stride[1] + h * p.q_stride[2];
-    if (tid < D) q[tid] = to_f32(qrow[tid]);
-    float top = -INFINITY, sum = 0.f, acc = 0.f;
-    bool any = false;
-    for (int64_t base = 0; base < end; base += 256) {
-        if (base + 256 <= low && base >= p.sinks) continue;
-        __syncthreads();
-        const int64_t j = base + tid;
-        float s = -INFINITY;
-        bool seen = j < end && (j >= low || j < p.sinks);
-        if (seen) {
-            const int64_t page = p.table[b * p.table_stride + j / P];
-            seen = page >= 0 && page < p.c.pages;
-            if (seen) {
-                const uint8_t* k = static_cast<const uint8_t*>(p.c.k) + ((page * H + kh) * P + j % P) * W;
-                s = 0.f;
-                for (int64_t d = 0; d < D; ++d) s += q[d] * fp8_value(k[d]);
-                s *= p.c.k_scale[page * H + kh] * p.scale;
+struct Parts {
+    static constexpr int q = 1, p = 1;
+    typedef bf16x8 qv;
+};
+template <>
+struct Parts<_Float16> {
+    static constexpr int q = 1, p = 2;
+    typedef f16x8 qv;
+};
+template <>
+struct Parts<float> {
+    static constexpr int q = 3, p = 3;
+    typedef bf16x8 qv;
+};
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    bf16x2 v = {(__bf16)a, (__bf16)b};
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+__device__ __forceinline__ float bf16_of(uint32_t pair, int i) {
+    return __uint_as_float(i ? pair & 0xffff0000u : pair << 16);
+}
+
+// Eight floats as N bfloat16 parts whose sum is the float to 8 N bits.
+template <int N>
+__device__ __forceinline__ void split8(const float* x, u32x4* out) {
+    float rest[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rest[i] = x[i];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            out[n][i] = pack_bf16(rest[2 * i], rest[2 * i + 1]);
+            if (n + 1 < N) {
+                rest[2 * i] -= bf16_of(out[n][i], 0);
+                rest[2 * i + 1] -= bf16_of(out[n][i], 1);
             }
         }
-        float m = s;
-        for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-        if ((tid & 63) == 0) part[tid / 64] = m;
-        any = __syncthreads_or(seen) || any;
-        m = fmaxf(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])), top);
-        const float shift = m == -INFINITY ? 0.f : m;
-        const float keep = expf(top - shift);
-        const float e = seen ? expf(s - shift) : 0.f;
-        prob[tid] = seen ? e : -1.f;
-        sum = sum * keep + e;  // this thread's keys
-        acc *= keep;
-        top = m;
+    }
+}
+
+template <bool Half>
+__device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi) {
+    u32x4 r;
+    if constexpr (Half) {
+        r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false));
+        r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true));
+        r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false));
+        r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true));
+    } else {
+        r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false));
+        r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true));
+        r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false));
+        r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true));
+    }
+    return r;
+}
+
+__device__ __forceinline__ f32x4 mma_bf16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma_f16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Maximum and sum over the four lanes that share a query column (l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float column_max(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float column_sum(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// One wavefront's running state for MT blocks of 16 query rows. With lane l,
+// column c = l % 16 is a query row and g = l / 16 a group of four lanes' rows:
+//   scores  s[mt][t][r]  key 16 g + 4 t + r of the tile, query row c
+//   output  o[mt][d][r]  element 16 d + 4 g + r of query row c
+// A tile's keys are dealt to the MFMA rows so that lane group g holds the
+// scores of the run of keys 16 g .. 16 g + 15: these are the keys whose values
+// the same lane reads as 16 contiguous bytes for the second product, so that
+// probabilities pass from one product to the next in their registers, and a
+// run lies in one page (pages are multiples of 16), so that a lane needs one
+// scale. Keys are read as 16 bytes along d, two products' worth.
+template <typename T, int W, int MT>
+struct Wave {
+    static constexpr int QP = Parts<T>::q, PP = Parts<T>::p;
+    static constexpr bool kHalf = std::is_same<T, _Float16>::value;
+    u32x4 q[MT][QP][W / 32];
+    f32x4 o[MT][W / 16];
+    float m[MT], l[MT];
+    bool any[MT];
+    int end[MT], low[MT];  // this lane's query row sees keys of [0, end) that are >= low or < sinks
+
+    __device__ __forceinline__ void load_q(const AttnParams& p, int b, int kh, int row0, const Span& sp, int base) {
+        const int c = threadIdx.x & 15, h = (threadIdx.x & 63) >> 4;
+        const int len = p.lengths[b], n = p.counts ? p.counts[b] : p.tokens;
+        const int limit = (n < p.tokens ? n : p.tokens);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const int row = row0 + mt * 16 + c;
+            const int t = (int)fdiv(row, p.by_share), g = row - t * p.share;
+            const bool live = t < limit && row - base < sp.live;
+            const int64_t pos = (int64_t)len - n + t;
+            end[mt] = live && pos >= 0 ? (pos + 1 < sp.held ? (int)pos + 1 : sp.held) : 0;
+            const int64_t lo = p.window > 0 ? pos - p.window + 1 : 0;
+            low[mt] = lo > 0 ? (int)lo : 0;
+            m[mt] = -INFINITY;
+            l[mt] = 0.f;
+            any[mt] = false;
+#pragma unroll
+            for (int d = 0; d < W / 16; ++d) o[mt][d] = f32x4{0, 0, 0, 0};
+            const T* src = static_cast<const T*>(p.q) + b * p.q_stride[0] + (int64_t)(live ? t : 0) * p.q_stride[1] +
+                           (int64_t)(kh * p.share + (live ? g : 0)) * p.q_stride[2];
+#pragma unroll
+            for (int s = 0; s < W / 32; ++s) {
+                const int d0 = s / 2 * 64 + h * 16 + (s & 1) * 8;
+                T x[8];
+                if (live && d0 + 8 <= p.dim) {
+                    __builtin_memcpy(x, src + d0, sizeof x);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = live && d0 + i < p.dim ? src[d0 + i] : (T)0.f;
+                }
+                if constexpr (QP == 1) {
+                    q[mt][0][s] = __builtin_bit_cast(u32x4, x);
+                } else {
+                    u32x4 parts[QP];
+                    split8<QP>(x, parts);
+#pragma unroll
+                    for (int n2 = 0; n2 < QP; ++n2) q[mt][n2][s] = parts[n2];
+                }
+            }
+        }
+    }
+};
+
+// A tile's place in the cache for one lane: the run whose keys it reads as
+// rows, and the run whose values (and whose keys' scores) it holds.
+struct Runs {
+    int64_t k_page, v_page;
+    int k_slot, v_slot;
+    bool v_ok;
+};
+
+template <typename T, int W, int MT>
+__device__ __forceinline__ Runs find_runs(const AttnParams& p, const int32_t* table, int tile, int held) {
+    const int lane = threadIdx.x & 63;
+    Runs r;
+    const int k_at = tile * kTile + ((lane & 15) >> 2) * 16, v_at = tile * kTile + (lane >> 4) * 16;
+    const int kp = (int)fdiv(k_at, p.by_page), vp = (int)fdiv(v_at, p.by_page);
+    r.k_slot = k_at - kp * p.page;
+    r.v_slot = v_at - vp * p.page;
+    r.k_page = k_at < held ? table[kp] : -1;
+    r.v_page = v_at < held ? table[vp] : -1;
+    r.v_ok = r.v_page >= 0 && r.v_page < p.pages;
+    // What lies in no page is read from page 0 and masked.
+    if (r.k_page < 0 || r.k_page >= p.pages) r.k_page = 0;
+    if (!r.v_ok) r.v_page = 0;
+    return r;
+}
+
+template <typename T, int W, int MT>
+struct Tile {
+    u32x4 k[4][W / 64], v[W / 16];
+    float k_scale, v_scale;
+    bool ok;
+
+    __device__ __forceinline__ void load_k(const AttnParams& p, const Runs& r, int kh) {
+        const int lane = threadIdx.x & 63;
+        const uint8_t* src =
+            p.k + ((r.k_page * p.heads + kh) * p.page + r.k_slot + (lane & 3)) * W + (lane >> 4) * 16;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int c = 0; c < W / 64; ++c) k[t][c] = *reinterpret_cast<const u32x4*>(src + t * 4 * W + c * 64);
+        ok = r.v_ok;
+        const int64_t at = r.v_page * p.heads + kh;
+        k_scale = ok ? p.k_scale[at] : 0.f;
+        v_scale = ok ? p.v_scale[at] : 0.f;
+    }
+    __device__ __forceinline__ void load_v(const AttnParams& p, const Runs& r, int kh) {
+        const int lane = threadIdx.x & 63;
+        const uint8_t* src = p.v + ((r.v_page * p.heads + kh) * W + (lane & 15)) * p.page + r.v_slot;
+#pragma unroll
+        for (int d = 0; d < W / 16; ++d) v[d] = *reinterpret_cast<const u32x4*>(src + (int64_t)d * 16 * p.page);
+    }
+};
+
+// Scores of one tile, and its keys' weights folded into the running state.
+// `full`: every live row sees every key.
+template <typename T, int W, int MT>
+__device__ __forceinline__ void tile_scores(Wave<T, W, MT>& w, const Tile<T, W, MT>& x, f32x4 (&s)[MT][4]) {
+    typedef Wave<T, W, MT> WV;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) s[mt][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < W / 64; ++c)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const u32x4 a = widen8<WV::kHalf>(x.k[t][c][2 * u], x.k[t][c][2 * u + 1]);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int n = 0; n < WV::QP; ++n) {
+                        if constexpr (WV::kHalf)
+                            s[mt][t] = mma_f16(a, w.q[mt][n][2 * c + u], s[mt][t]);
+                        else
+                            s[mt][t] = mma_bf16(a, w.q[mt][n][2 * c + u], s[mt][t]);
+                    }
+            }
+}
+
+template <typename T, int W, int MT>
+__device__ __forceinline__ void tile_fold(const AttnParams& p, Wave<T, W, MT>& w, Tile<T, W, MT>& x, f32x4 (&s)[MT][4],
+                                          int tile, bool full) {
+    typedef Wave<T, W, MT> WV;
+    const int lane = threadIdx.x & 63;
+    const int key0 = tile * kTile + (lane >> 4) * 16;
+    const float c = x.k_scale * p.scale;
+    u32x4 prob[MT][WV::PP][2];
+    bool bad_values = false;
+    u32x4 seen[MT][2];  // 1.0 where a row sees a key, for values that are NaN
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float v = s[mt][t][r] * c;
+                if (!full) {
+                    const int j = key0 + 4 * t + r;
+                    const bool see = x.ok && j < w.end[mt] && (j >= w.low[mt] || j < p.sinks);
+                    v = see ? v : -INFINITY;
+                    w.any[mt] |= see;
+                    seen[mt][t >> 1][(t & 1) * 2 + (r >> 1)] =
+                        (r & 1 ? seen[mt][t >> 1][(t & 1) * 2 + (r >> 1)] : 0u) | (see ? 0x3f80u << (r & 1) * 16 : 0u);
+                }
+                s[mt][t][r] = v;
+                top = fmaxf(top, v);
+            }
+        if (full) w.any[mt] = true;
+        // The maximum is moved only where some score passes it by over 8 (its
+        // weight would be over 256): until then weights and sums keep it.
+        const float m_old = w.m[mt];
+        if (__any(top > m_old + 8.f)) {
+            const float m_new = fmaxf(m_old, column_max(top));
+            const float keep = m_new == -INFINITY ? 1.f : exp2f(m_old - m_new);
+            w.m[mt] = m_new;
+            w.l[mt] *= keep;
+#pragma unroll
+            for (int d = 0; d < W / 16; ++d) w.o[mt][d] *= keep;
+        }
+        const float shift = w.m[mt] == -INFINITY ? 0.f : w.m[mt];
+        float sum = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                e[i] = __builtin_amdgcn_exp2f(s[mt][2 * h + i / 4][i & 3] - shift);
+                sum += e[i];
+                e[i] *= x.v_scale;
+            }
+            u32x4 parts[WV::PP];
+            split8<WV::PP>(e, parts);
+#pragma unroll
+            for (int n = 0; n < WV::PP; ++n) prob[mt][n][h] = parts[n];
+        }
+        w.l[mt] += sum;
+    }
+    if (!full) {
+        // Values of keys that no row sees may be anything: zeros in their
+        // place. NaN among the others belongs only to the rows that see it.
+        u32x4 dead;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t some = 0;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const uint32_t a = seen[mt][i >> 1][(i & 1) * 2], b = seen[mt][i >> 1][(i & 1) * 2 + 1];
+                some |= (a & 0x80u) | (a >> 16 & 0x80u) << 8 | (b & 0x80u) << 16 | (b >> 16 & 0x80u) << 24;
+            }
+            // over the 16 columns
+#pragma unroll
+            for (int off = 1; off < 16; off <<= 1) some |= __shfl_xor(some, off, 64);
+            dead[i] = ~((some >> 7) * 0xffu);
+        }
+        bool nan_here = false;
+#pragma unroll
+        for (int d = 0; d < W / 16; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x.v[d][i] &= ~dead[i];
+                nan_here |= (((x.v[d][i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+            }
+        bad_values = __any(nan_here);
+        if (bad_values) {
+#pragma unroll
+            for (int d = 0; d < W / 16; ++d) {
+                u32x4 flag;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t nan = ((((x.v[d][i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
+                    flag[i] = nan & 0x38383838u;  // 1.0
+                    x.v[d][i] &= ~nan;
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    f32x4 hit = {0, 0, 0, 0};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        hit = mma_bf16(widen8<false>(flag[2 * h], flag[2 * h + 1]), seen[mt][h], hit);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (hit[r] > 0.f) w.o[mt][d][r] = NAN;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < W / 16; ++d)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const u32x4 a = widen8<false>(x.v[d][2 * h], x.v[d][2 * h + 1]);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int n = 0; n < WV::PP; ++n) w.o[mt][d] = mma_bf16(a, prob[mt][n][h], w.o[mt][d]);
+        }
+}
+
+// Folds tiles first, first + step, ... below last of the span into the wave's state.
+template <typename T, int W, int MT>
+__device__ __forceinline__ void walk(const AttnParams& p, Wave<T, W, MT>& w, const Span& sp, int b, int kh, int first,
+                                     int last, int step) {
+    if (first >= last) return;
+    const int32_t* table = p.table + b * p.table_stride;
+    auto tile_at = [&](int i) { return i < sp.sink_tiles ? i : sp.start + i - sp.sink_tiles; };
+    // Keys [sure_low, sure_end) are seen by every live row, as are those below sure_sinks.
+    const int sure_end = sp.first_pos + 1 < sp.held ? sp.first_pos + 1 : sp.held;
+    const int64_t lo = p.window > 0 ? (int64_t)sp.last_pos - p.window + 1 : 0;
+    const int sure_low = lo > 0 ? (int)lo : 0;
+    Tile<T, W, MT> x;
+    Runs r = find_runs<T, W, MT>(p, table, tile_at(first), sp.held);
+    x.load_k(p, r, kh);
+    for (int i = first; i < last; i += step) {
+        const int tile = tile_at(i);
+        x.load_v(p, r, kh);
+        const int next = i + step < last ? i + step : i;
+        const Runs rn = find_runs<T, W, MT>(p, table, tile_at(next), sp.held);
+        f32x4 s[MT][4];
+        tile_scores<T, W, MT>(w, x, s);
+        Tile<T, W, MT> y;
+        if (i + step < last) y.load_k(p, rn, kh);
+        const int key = tile * kTile;
+        const bool full = key + kTile <= sure_end && (key >= sure_low || key + kTile <= p.sinks) && __all(x.ok);
+        tile_fold<T, W, MT>(p, w, x, s, tile, full);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int c = 0; c < W / 64; ++c) x.k[t][c] = y.k[t][c];
+        x.k_scale = y.k_scale;
+        x.v_scale = y.v_scale;
+        x.ok = y.ok;
+        r = rn;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* dst, const float* v, int count) {
+    if (count >= 4) {
+        T x[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+        __builtin_memcpy(dst, x, sizeof x);
+    } else {
+        for (int i = 0; i < count; ++i) dst[i] = (T)v[i];
+    }
+}
+
+// Address of query row `row` of (b, kh) in the contiguous output.
+template <typename T>
+__device__ __forceinline__ T* out_row(const AttnParams& p, int b, int kh, int row) {
+    const int t = (int)fdiv(row, p.by_share), g = row - t * p.share;
+    return static_cast<T*>(p.out) + (((int64_t)b * p.tokens + t) * p.q_heads + kh * p.share + g) * p.dim;
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void zero_rows(const AttnParams& p, int b, int kh, int row0, int row1) {
+    const int rows = p.tokens * p.share;
+    if (row1 > rows) row1 = rows;
+    for (int i = threadIdx.x; i < (row1 - row0) * W; i += 256) {
+        const int d = i % W;
+        if (d < p.dim) out_row<T>(p, b, kh, row0 + i / W)[d] = (T)0.f;
+    }
+}
+
+// The four wavefronts' states of the same 16 query rows, joined; to the output
+// or to a slot of partial results.
+template <typename T, int W>
+__device__ __forceinline__ void join_waves(const AttnParams& p, Wave<T, W, 1>& w, const Span& sp, int b, int kh, int row0,
+                                           float* slot) {
+    __shared__ float sm[4][16], sl[4][16];
+    __shared__ float so[4][16][68];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const float l = column_sum(w.l[0]);
+    const bool any = column_sum(w.any[0] ? 1.f : 0.f) > 0.f;
+    if (g == 0) {
+        sm[wave][c] = w.m[0];
+        sl[wave][c] = any ? l : -1.f;
+    }
+    __syncthreads();
+    float m = -INFINITY, sum = 0.f;
+    bool some = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, sm[i][c]);
+    const float shift = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool has = sl[i][c] != -1.f;
+        if (has) sum += sl[i][c] * exp2f(sm[i][c] - shift);
+        some |= has;
+    }
+    const float mine = any ? exp2f(w.m[0] - shift) * (slot ? 1.f : 1.f / sum) : 0.f;
+    if (slot && threadIdx.x < 16 && c < sp.live) {
+        slot[16 * W + c] = m;
+        slot[16 * W + 16 + c] = some ? sum : -1.f;
+    }
+    const int oc = threadIdx.x >> 4, od = (threadIdx.x & 15) * 4;
+#pragma unroll
+    for (int d0 = 0; d0 < W / 64; ++d0) {
+        if (d0) __syncthreads();
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            f32x4 v = any ? w.o[0][d0 * 4 + d] * mine : f32x4{0, 0, 0, 0};
+            *reinterpret_cast<f32x4*>(&so[wave][c][d * 16 + g * 4]) = v;
+        }
         __syncthreads();
-        if (tid < D) {
-            for (int i = 0; i < 256 && base + i < end; ++i) {
-                if (prob[i] == -1.f) continue;
-                const int64_t jj = base + i, page = p.table[b * p.table_stride + jj / P];
-                const uint8_t* v = static_cast<const uint8_t*>(p.c.v) + ((page * H + kh) * W + tid) * P;
-                acc += prob[i] * (fp8_value(v[jj % P]) * p.c.v_scale[page * H + kh]);
+        f32x4 v = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v += *reinterpret_cast<const f32x4*>(&so[i][oc][od]);
+        if (oc < sp.live) {
+            if (slot) {
+                *reinterpret_cast<f32x4*>(slot + oc * W + d0 * 64 + od) = v;
+            } else {
+                float x[4] = {v[0], v[1], v[2], v[3]};
+                const int d = d0 * 64 + od;
+                if (d < p.dim) store4<T>(out_row<T>(p, b, kh, row0 + oc) + d, x, p.dim - d);
             }
         }
     }
     __syncthreads();
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-    if ((tid & 63) == 0) part[tid / 64] = sum;
+}
+
+// Few query rows (at most 16 a cache head): the four wavefronts of a workgroup
+// take every fourth tile of the same keys. The key tiles of all (sequence,
+// head) pairs form one list, which the workgroups share evenly whatever the
+// sequences' lengths; a pair cut by a workgroup's end leaves partial results.
+// Wavefronts a SIMD is to hold: two where the state of one fits half its registers.
+template <typename T, int W, int MT>
+constexpr int kWavesPerSimd = Parts<T>::q * MT * W > 256 || W > 128 ? 1 : 2;
+
+template <typename T, int W>
+__global__ __launch_bounds__(256, (kWavesPerSimd<T, W, 1>)) void kv_attention_few_kernel(AttnParams p) {
+    __shared__ int64_t scan[256];
+    const int wave = threadIdx.x >> 6;
+    Wave<T, W, 1> w;
+    if (p.direct) {
+        const int b = blockIdx.x / p.heads, kh = blockIdx.x - b * p.heads;
+        const Span sp = span_of(p, b, 0, 16);
+        if (sp.tiles > 0) {
+            w.load_q(p, b, kh, 0, sp, 0);
+            walk<T, W, 1>(p, w, sp, b, kh, wave, sp.tiles, 4);
+            join_waves<T, W>(p, w, sp, b, kh, 0, nullptr);
+            zero_rows<T, W>(p, b, kh, sp.live, 16);
+        } else {
+            zero_rows<T, W>(p, b, kh, 0, 16);
+        }
+        return;
+    }
+    // All tiles, and where this workgroup's share of them begins.
+    int64_t total = 0;
+    for (int b = threadIdx.x; b < p.batch; b += 256) total += (int64_t)span_of(p, b, 0, 16).tiles * p.heads;
+    scan[threadIdx.x] = total;
     __syncthreads();
-    sum = (part[0] + part[1]) + (part[2] + part[3]);
-    if (tid < D) out[tid] = (T)(any ? acc / sum : 0.f);
+    for (int off = 128; off > 0; off >>= 1) {
+        if ((int)threadIdx.x < off) scan[threadIdx.x] += scan[threadIdx.x + off];
+        __syncthreads();
+    }
+    total = scan[0];
+    __syncthreads();
+    int64_t per = (total + p.groups - 1) / p.groups;
+    if (per < kMinTiles) per = kMinTiles;
+    const int64_t begin = blockIdx.x * per, stop = begin + per < total ? begin + per : total;
+    // Sequences that see nothing: their zeros, dealt out over the workgroups.
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+        const Span sp = span_of(p, b, 0, 16);
+        if (sp.tiles == 0 || sp.live < 16)
+            for (int kh = 0; kh < p.heads; ++kh) zero_rows<T, W>(p, b, kh, sp.tiles == 0 ? 0 : sp.live, 16);
+    }
+    if (begin >= stop) return;
+    int64_t at = 0;
+    int b = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 256) {
+        const int mine = b0 + (int)threadIdx.x;
+        __syncthreads();
+        scan[threadIdx.x] = mine < p.batch ? (int64_t)span_of(p, mine, 0, 16).tiles * p.heads : 0;
+        __syncthreads();
+        for (int off = 1; off < 256; off <<= 1) {
+            const int64_t v = (int)threadIdx.x >= off ? scan[threadIdx.x - off] : 0;
+            __syncthreads();
+            scan[threadIdx.x] += v;
+            __syncthreads();
+        }
+        if (at + scan[255] > begin) {
+            // the first sequence of these whose tiles reach past `begin`
+            int lo = 0, hi = 255;
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (at + scan[mid] > begin)
+                    hi = mid;
+                else
+                    lo = mid + 1;
+            }
+            b = b0 + lo;
+            at += lo ? scan[lo - 1] : 0;
+            break;
+        }
+        at += scan[255];
+    }
+    // `at` is the place of sequence b's first tile.
+    int64_t pos = begin;
+    while (pos < stop) {
+        const Span sp = span_of(p, b, 0, 16);
+        const int64_t size = (int64_t)sp.tiles * p.heads;
+        if (pos >= at + size) {
+            at += size;
+            ++b;
+            continue;
+        }
+        const int kh = (int)((pos - at) / sp.tiles);
+        const int64_t pair = at + (int64_t)kh * sp.tiles;
+        const int first = (int)(pos - pair), last = (int)(stop - pair < sp.tiles ? stop - pair : sp.tiles);
+        w.load_q(p, b, kh, 0, sp, 0);
+        walk<T, W, 1>(p, w, sp, b, kh, first + wave, last, 4);
+        const bool whole = first == 0 && last == sp.tiles;
+        float* slot = whole ? nullptr : p.part + ((int64_t)blockIdx.x * 2 + (first == 0 ? 1 : 0)) * (16 * (W + 2));
+        join_waves<T, W>(p, w, sp, b, kh, 0, slot);
+        pos = pair + last;
+    }
+}
+
+// Joins the partial results of the pairs that were cut: one wavefront a query row.
+template <typename T, int W>
+__global__ __launch_bounds__(256) void kv_attention_few_join_kernel(AttnParams p) {
+    __shared__ int64_t scan[2][256];
+    const int b = blockIdx.x / p.heads, kh = blockIdx.x - b * p.heads;
+    int64_t total = 0, before = 0;
+    for (int i = threadIdx.x; i < p.batch; i += 256) {
+        const int64_t n = (int64_t)span_of(p, i, 0, 16).tiles * p.heads;
+        total += n;
+        if (i < b) before += n;
+    }
+    scan[0][threadIdx.x] = total;
+    scan[1][threadIdx.x] = before;
+    __syncthreads();
+    for (int off = 128; off > 0; off >>= 1) {
+        if ((int)threadIdx.x < off) {
+            scan[0][threadIdx.x] += scan[0][threadIdx.x + off];
+            scan[1][threadIdx.x] += scan[1][threadIdx.x + off];
+        }
+        __syncthreads();
+    }
+    total = scan[0][0];
+    int64_t per = (total + p.groups - 1) / p.groups;
+    if (per < kMinTiles) per = kMinTiles;
+    const Span sp = span_of(p, b, 0, 16);
+    if (sp.tiles == 0) return;
+    const int64_t at = scan[1][0] + (int64_t)kh * sp.tiles;
+    const int64_t g0 = at / per, g1 = (at + sp.tiles - 1) / per;
+    if (g0 == g1) return;
+    const int lane = threadIdx.x & 63;
+    for (int row = threadIdx.x >> 6; row < sp.live; row += 4) {
+        float m = -INFINITY;
+        for (int64_t g = g0; g <= g1; ++g) m = fmaxf(m, p.part[(g * 2 + (g == g0)) * (16 * (W + 2)) + 16 * W + row]);
+        const float shift = m == -INFINITY ? 0.f : m;
+        float sum = 0.f, o[W / 64] = {};
+        bool some = false;
+        for (int64_t g = g0; g <= g1; ++g) {
+            const float* slot = p.part + (g * 2 + (g == g0)) * (16 * (W + 2));
+            const float l = slot[16 * W + 16 + row];
+            if (l == -1.f) continue;
+            some = true;
+            const float f = exp2f(slot[16 * W + row] - shift);
+            sum += l * f;
+#pragma unroll
+            for (int d = 0; d < W / 64; ++d) o[d] += f * slot[row * W + d * 64 + lane];
+        }
+        T* out = out_row<T>(p, b, kh, row);
+#pragma unroll
+        for (int d = 0; d < W / 64; ++d)
+            if (d * 64 + lane < p.dim) out[d * 64 + lane] = (T)(some ? o[d] / sum : 0.f);
+    }
+}
+
+// Many query rows: each wavefront takes MT blocks of 16 rows of its own, and
+// the four of a workgroup walk the same keys. With `groups` > 1 the keys of a
+// row block are cut into that many ranges, joined afterwards.
+template <typename T, int W, int MT>
+__global__ __launch_bounds__(256, (kWavesPerSimd<T, W, MT>)) void kv_attention_many_kernel(AttnParams p) {
+    constexpr int kRows = 64 * MT;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    int id = blockIdx.x;
+    const int part = id % p.groups;
+    id /= p.groups;
+    const int kh = id % p.heads;
+    id /= p.heads;
+    // The last row blocks of a sequence see the most keys: they go first.
+    const int b = id % p.batch, rb = p.row_blocks - 1 - id / p.batch;
+    const int row0 = rb * kRows, mine = row0 + wave * 16 * MT;
+    const Span all = span_of(p, b, row0, kRows);
+    const int per = all.tiles > 0 ? (all.tiles + p.groups - 1) / p.groups : 1;
+    const int first = part * per, last = first + per < all.tiles ? first + per : all.tiles;
+    if (part > 0 && first >= last) return;
+    Wave<T, W, MT> w;
+    const Span sp = span_of(p, b, mine, 16 * MT);
+    w.load_q(p, b, kh, mine, sp, mine);
+    walk<T, W, MT>(p, w, all, b, kh, first, last, 1);
+    float* slot = p.groups > 1 && per < all.tiles
+                      ? p.part + ((((int64_t)b * p.row_blocks + rb) * p.heads + kh) * p.groups + part) * (kRows * (W + 2))
+                      : nullptr;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int r = wave * 16 * MT + mt * 16 + c;
+        const float l = column_sum(w.l[mt]);
+        const bool any = column_sum(w.any[mt] ? 1.f : 0.f) > 0.f;
+        if (row0 + r >= p.tokens * p.share) continue;
+        const bool dead = r >= all.live || !any;
+        if (slot) {
+            if (g == 0) {
+                slot[kRows * W + r] = w.m[mt];
+                slot[kRows * W + kRows + r] = dead ? -1.f : l;
+            }
+#pragma unroll
+            for (int d = 0; d < W / 16; ++d) *reinterpret_cast<f32x4*>(slot + r * W + d * 16 + g * 4) = w.o[mt][d];
+        } else {
+            T* out = out_row<T>(p, b, kh, row0 + r);
+            const float f = 1.f / l;
+#pragma unroll
+            for (int d = 0; d < W / 16; ++d) {
+                const int d0 = d * 16 + g * 4;
+                float x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = dead ? 0.f : w.o[mt][d][i] * f;
+                if (d0 < p.dim) store4<T>(out + d0, x, p.dim - d0);
+            }
+        }
+    }
+}
+
+template <typename T, int W, int MT>
+__global__ __launch_bounds__(256) void kv_attention_many_join_kernel(AttnParams p) {
+    constexpr int kRows = 64 * MT;
+    int id = blockIdx.x;
+    const int chunk = id % (kRows / 4);
+    id /= kRows / 4;
+    const int kh = id % p.heads;
+    id /= p.heads;
+    const int rb = id % p.row_blocks, b = id / p.row_blocks;
+    const int row0 = rb * kRows, r = chunk * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const Span all = span_of(p, b, row0, kRows);
+    if (row0 + r >= p.tokens * p.share || all.tiles <= 0) return;
+    const int per = (all.tiles + p.groups - 1) / p.groups;
+    if (per >= all.tiles) return;
+    const int parts = (all.tiles + per - 1) / per;
+    const float* base = p.part + (((int64_t)b * p.row_blocks + rb) * p.heads + kh) * p.groups * (int64_t)(kRows * (W + 2));
+    float m = -INFINITY;
+    for (int i = 0; i < parts; ++i) m = fmaxf(m, base[(int64_t)i * (kRows * (W + 2)) + kRows * W + r]);
+    const float shift = m == -INFINITY ? 0.f : m;
+    float sum = 0.f, o[W / 64] = {};
+    bool some = false;
+    for (int i = 0; i < parts; ++i) {
+        const float* slot = base + (int64_t)i * (kRows * (W + 2));
+        const float l = slot[kRows * W + kRows + r];
+        if (l == -1.f) continue;
+        some = true;
+        const float f = exp2f(slot[kRows * W + r] - shift);
+        sum += l * f;
+#pragma unroll
+        for (int d = 0; d < W / 64; ++d) o[d] += f * slot[r * W + d * 64 + lane];
+    }
+    T* out = out_row<T>(p, b, kh, row0 + r);
+#pragma unroll
+    for (int d = 0; d < W / 64; ++d)
+        if (d * 64 + lane < p.dim) out[d * 64 + lane] = (T)(some ? o[d] / sum : 0.f);
+}
+
+// How a call is cut, from what the host knows of it.
+struct Cut {
+    bool few, direct;
+    int mt, row_blocks, groups;
+    int64_t grid, slots, slot_floats;
+};
+
+Cut cut_of(const tt_kv_attention_args* a) {
+    Cut c = {};
+    const int64_t share = a->q_heads / a->cache.heads, rows = a->tokens * share, W = kv_width(a->cache.dim);
+    const int64_t cap = a->table_width * a->cache.page;
+    int64_t keys = cap;  // the most a row block may have to walk
+    if (a->window > 0 && a->window < cap && a->sinks < cap) {
+        const int64_t w = a->window + a->sinks + a->tokens + 2 * kTile;
+        keys = w < cap ? w : cap;
+    }
+    const int64_t tiles = (keys + kTile - 1) / kTile;
+    const int64_t pairs = a->batch * a->cache.heads;
+    c.few = rows <= 16;
+    if (c.few) {
+        c.mt = 1;
+        c.row_blocks = 1;
+        c.direct = tiles <= 16;
+        c.groups = 512;
+        c.grid = c.direct ? pairs : c.groups;
+        c.slots = c.direct ? 0 : 2 * c.groups;
+        c.slot_floats = 16 * (W + 2);
+    } else {
+        c.mt = rows > 64 && W <= 128 ? 2 : 1;
+        c.row_blocks = (int)((rows + 64 * c.mt - 1) / (64 * c.mt));
+        const int64_t blocks = pairs * c.row_blocks;
+        int64_t g = blocks >= 512 ? 1 : (512 + blocks - 1) / blocks;
+        if (g > tiles / 4) g = tiles / 4 > 0 ? tiles / 4 : 1;
+        c.groups = (int)g;
+        c.grid = blocks * g;
+        c.slots = g > 1 ? blocks * g : 0;
+        c.slot_floats = 64 * c.mt * (W + 2);
+    }
+    return c;
+}
+
+template <typename T, int W>
+int attn_launch(AttnParams& p, const Cut& c, hipStream_t st) {
+    if (c.few) {
+        kv_attention_few_kernel<T, W><<<(uint32_t)c.grid, 256, 0, st>>>(p);
+        if (!c.direct) kv_attention_few_join_kernel<T, W><<<(uint32_t)(p.batch * p.heads), 256, 0, st>>>(p);
+        return check_launch("tt_kv_attention");
+    }
+    const uint32_t join = (uint32_t)((int64_t)p.batch * p.heads * p.row_blocks * 16 * c.mt);
+    if constexpr (W <= 128) {
+        if (c.mt == 2) {
+            kv_attention_many_kernel<T, W, 2><<<(uint32_t)c.grid, 256, 0, st>>>(p);
+            if (c.groups > 1) kv_attention_many_join_kernel<T, W, 2><<<join, 256, 0, st>>>(p);
+            return check_launch("tt_kv_attention");
+        }
+    }
+    kv_attention_many_kernel<T, W, 1><<<(uint32_t)c.grid, 256, 0, st>>>(p);
+    if (c.groups > 1) kv_attention_many_join_kernel<T, W, 1><<<join, 256, 0, st>>>(p);
+    return check_launch("tt_kv_attention");
 }
 
 template <typename T>
-int attn_launch(const AttnParams& p, int64_t rows, hipStream_t st) {
-    if (rows > kMaxGrid) return set_error(TT_UNSUPPORTED, "tt_kv_attention: %lld query rows", (long long)rows);
-    kv_attention_simple_kernel<T><<<(uint32_t)rows, 256, 0, st>>>(p);
-    return check_launch("tt_kv_attention");
+int attn_typed(AttnParams& p, const Cut& c, hipStream_t st) {
+    switch (kv_width(p.dim)) {
+        case 64:
+            return attn_launch<T, 64>(p, c, st);
+        case 128:
+            return attn_launch<T, 128>(p, c, st);
+        case 192:
+            return attn_launch<T, 192>(p, c, st);
+        default:
+            return attn_launch<T, 256>(p, c, st);
+    }
 }
 
 int check_attention(const tt_kv_attention_args* a) {
@@ -100,37 +871,68 @@ int check_attention(const tt_kv_attention_args* a) {
     if (a->batch == 0 || a->tokens == 0) return TT_OK;
     if (!a->q || !a->out || !a->lengths || (a->table_width > 0 && !a->table))
         return set_error(TT_INVALID, "tt_kv_attention: NULL pointer");
+    constexpr int64_t kMost = int64_t(1) << 30;
+    if (a->batch >= kMost || a->tokens >= kMost || a->q_heads >= kMost || a->batch * a->cache.heads >= kMost ||
+        a->tokens * a->q_heads >= kMost || a->cache.pages >= kMost || a->table_width > kMost / a->cache.page)
+        return set_error(TT_UNSUPPORTED, "tt_kv_attention: extents of 2^30 or more");
     return TT_OK;
 }
 
 }  // namespace
 }  // namespace tt
 
-extern "C" size_t tt_kv_attention_workspace_bytes(const tt_kv_attention_args*) { return 0; }
+extern "C" size_t tt_kv_attention_workspace_bytes(const tt_kv_attention_args* a) {
+    using namespace tt;
+    if (check_attention(a) != TT_OK || a->batch == 0 || a->tokens == 0) return 0;
+    const Cut c = cut_of(a);
+    return (size_t)(c.slots * c.slot_floats * 4);
+}
 
 extern "C" int tt_kv_attention(const tt_kv_attention_args* a, void* stream) {
     using namespace tt;
     if (int rc = check_attention(a)) return rc;
     if (a->batch == 0 || a->tokens == 0) return TT_OK;
+    const Cut c = cut_of(a);
+    const int64_t join = a->batch * a->cache.heads * c.row_blocks * 16 * c.mt;
+    if (c.grid > kMaxGrid || join > kMaxGrid)
+        return set_error(TT_UNSUPPORTED, "tt_kv_attention: %lld workgroups", (long long)c.grid);
+    const int64_t need = c.slots * c.slot_floats * 4;
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need || (uintptr_t)a->workspace % 16))
+        return set_error(TT_INVALID, "tt_kv_attention: workspace of %lld bytes, need %lld", (long long)a->workspace_bytes,
+                         (long long)need);
     AttnParams p;
-    p.tokens = a->tokens;
-    p.q_heads = a->q_heads;
-    p.window = a->window;
-    p.sinks = a->sinks;
-    p.table_width = a->table_width;
-    p.table_stride = a->table_stride;
-    for (int i = 0; i < 3; ++i) p.q_stride[i] = a->q_stride[i];
-    p.scale = (float)a->scale;
     p.q = a->q;
     p.out = a->out;
     p.table = a->table;
     p.lengths = a->lengths;
     p.counts = a->counts;
-    p.c = a->cache;
-    p.width = kv_width(a->cache.dim);
-    const int64_t rows = a->batch * a->tokens * a->q_heads;
+    p.k = static_cast<const uint8_t*>(a->cache.k);
+    p.v = static_cast<const uint8_t*>(a->cache.v);
+    p.k_scale = a->cache.k_scale;
+    p.v_scale = a->cache.v_scale;
+    p.part = static_cast<float*>(a->workspace);
+    for (int i = 0; i < 3; ++i) p.q_stride[i] = a->q_stride[i];
+    p.table_stride = a->table_stride;
+    p.pages = a->cache.pages;
+    p.batch = (int)a->batch;
+    p.tokens = (int)a->tokens;
+    p.q_heads = (int)a->q_heads;
+    p.heads = (int)a->cache.heads;
+    p.share = p.q_heads / p.heads;
+    p.page = (int)a->cache.page;
+    p.dim = (int)a->cache.dim;
+    constexpr int64_t kInt = 0x7fffffff;
+    p.window = (int)(a->window < kInt ? a->window : kInt);
+    p.sinks = (int)(a->sinks < kInt ? a->sinks : kInt);
+    p.capacity = a->cache.pages > 0 ? (int)(a->table_width * a->cache.page) : 0;
+    p.row_blocks = c.row_blocks;
+    p.groups = c.groups;
+    p.direct = c.direct;
+    p.by_page = make_fastdiv((uint32_t)p.page);
+    p.by_share = make_fastdiv((uint32_t)p.share);
+    p.scale = (float)(a->scale * 1.4426950408889634074);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (a->dtype == TT_F32) return attn_launch<float>(p, rows, st);
-    if (a->dtype == TT_BF16) return attn_launch<__bf16>(p, rows, st);
-    return attn_launch<_Float16>(p, rows, st);
+    if (a->dtype == TT_F32) return attn_typed<float>(p, c, st);
+    if (a->dtype == TT_BF16) return attn_typed<__bf16>(p, c, st);
+    return attn_typed<_Float16>(p, c, st);
 }
