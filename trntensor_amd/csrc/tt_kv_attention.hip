@@ -90,34 +90,6 @@ struct Parts<float> {
     typedef bf16x8 qv;
 };
 
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-    bf16x2 v = {(__bf16)a, (__bf16)b};
-    return __builtin_bit_cast(uint32_t, v);
-}
-
-__device__ __forceinline__ float bf16_of(uint32_t pair, int i) {
-    return __uint_as_float(i ? pair & 0xffff0000u : pair << 16);
-}
-
-// Eight floats as N bfloat16 parts whose sum is the float to 8 N bits.
-template <int N>
-__device__ __forceinline__ void split8(const float* x, u32x4* out) {
-    float rest[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) rest[i] = x[i];
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            out[n][i] = pack_bf16(rest[2 * i], rest[2 * i + 1]);
-            if (n + 1 < N) {
-                rest[2 * i] -= bf16_of(out[n][i], 0);
-                rest[2 * i + 1] -= bf16_of(out[n][i], 1);
-            }
-        }
-    }
-}
-
 template <bool Half>
 __device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi) {
     u32x4 r;

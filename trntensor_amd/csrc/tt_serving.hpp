@@ -30,6 +30,34 @@ __device__ __forceinline__ uint32_t fp8_pair(float a, float b) {
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu;
 }
 
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    bf16x2 v = {(__bf16)a, (__bf16)b};
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+__device__ __forceinline__ float bf16_of(uint32_t pair, int i) {
+    return __uint_as_float(i ? pair & 0xffff0000u : pair << 16);
+}
+
+// Eight floats as N bfloat16 parts whose sum is the float to 8 N bits.
+template <int N>
+__device__ __forceinline__ void split8(const float* x, u32x4* out) {
+    float rest[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rest[i] = x[i];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            out[n][i] = pack_bf16(rest[2 * i], rest[2 * i + 1]);
+            if (n + 1 < N) {
+                rest[2 * i] -= bf16_of(out[n][i], 0);
+                rest[2 * i + 1] -= bf16_of(out[n][i], 1);
+            }
+        }
+    }
+}
+
 // Codes of one cache row: dim rounded up to a multiple of 64.
 inline int64_t kv_width(int64_t dim) { return (dim + 63) / 64 * 64; }
 
