@@ -7,7 +7,7 @@ namespace tt {
 namespace {
 
 struct AppendParams {
-    int64_t tokens, q_heads, rot, interleaved, table_width, table_stride;
+    int64_t batch, tokens, q_heads, rot, interleaved, table_width, table_stride;
     int64_t k_stride[3], v_stride[3], q_stride[3];
     const void *k, *v, *q;
     void* q_out;
@@ -44,15 +44,75 @@ __device__ __forceinline__ int scale_exponent(float amax) {
 
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
+// What one workgroup of the cache part appends to: the new tokens [lo, hi) of
+// one block (page and head), keys or values.
+struct Block {
+    bool is_v;
+    int lo, hi;         // slots of the page
+    int64_t first;      // position of the page's first slot
+    const void* x;      // row of slot 0 (its head), which need not exist
+    int64_t row_stride;
+    uint8_t* codes;
+    float* scale;
+};
+
 template <typename T>
-__global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p) {
+__device__ __forceinline__ bool find_block(const AppendParams& p, int64_t w, Block& k) {
+    const int64_t H = p.c.heads, P = p.c.page;
+    k.is_v = w & 1;
+    w >>= 1;
+    const int64_t h = w % H, j = w / H % p.blocks, b = w / H / p.blocks;
+    const int64_t len = p.lengths[b];
+    int64_t n = p.counts ? p.counts[b] : p.tokens;
+    n = n > p.tokens ? p.tokens : n;
+    if (len < 0) return false;
+    const int64_t end = len + n < p.table_width * P ? len + n : p.table_width * P;
+    k.first = (len / P + j) * P;
+    k.lo = (int)((len > k.first ? len : k.first) - k.first);
+    const int64_t hi = (end < k.first + P ? end : k.first + P) - k.first;
+    if (k.lo >= hi) return false;
+    k.hi = (int)hi;
+    const int64_t page = p.table[b * p.table_stride + k.first / P];
+    if (page < 0 || page >= p.c.pages) return false;
+    const int64_t* stride = k.is_v ? p.v_stride : p.k_stride;
+    k.x = static_cast<const T*>(k.is_v ? p.v : p.k) + b * stride[0] + h * stride[2] + (k.first - len) * stride[1];
+    k.row_stride = stride[1];
+    k.codes = static_cast<uint8_t*>(k.is_v ? p.c.v : p.c.k) + (page * H + h) * p.width * P;
+    k.scale = (k.is_v ? p.c.v_scale : p.c.k_scale) + page * H + h;
+    return true;
+}
+
+// The block's new scale, from the largest finite magnitude among the new
+// values (each thread's in `amax`) and, if it holds earlier tokens, its old one.
+__device__ __forceinline__ float settle_scale(const Block& k, float amax, float& old) {
     __shared__ float part[4];
-    int64_t w = blockIdx.x;
-    const int64_t H = p.c.heads, P = p.c.page, W = p.width;
-    if (w >= p.kv_groups) {
-        // queries: one workgroup per token
-        w -= p.kv_groups;
-        const int64_t b = w / p.tokens, t = w % p.tokens;
+    for (int off = 32; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off, 64));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x / 64] = amax;
+    old = k.lo > 0 ? *k.scale : 0.f;
+    __syncthreads();
+    amax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    return fmaxf(power_of_two(scale_exponent(amax)), old);
+}
+
+__device__ __forceinline__ void take_max(float& amax, float x) {
+    const float a = fabsf(x);
+    if (a < INFINITY) amax = fmaxf(amax, a);
+}
+
+// Four codes at another scale.
+__device__ __forceinline__ uint32_t rescaled(uint32_t c, float f) {
+    const uint32_t lo = fp8_pair(__builtin_amdgcn_cvt_f32_fp8(c, 0) * f, __builtin_amdgcn_cvt_f32_fp8(c, 1) * f);
+    const uint32_t hi = fp8_pair(__builtin_amdgcn_cvt_f32_fp8(c, 2) * f, __builtin_amdgcn_cvt_f32_fp8(c, 3) * f);
+    return lo | hi << 16;
+}
+
+// Element by element, for head sizes and rotations that are no multiples of
+// the pieces below.
+template <typename T>
+__global__ __launch_bounds__(256) void kv_append_any_kernel(AppendParams p) {
+    const int64_t P = p.c.page, W = p.width;
+    if (blockIdx.x >= p.kv_groups) {
+        const int64_t w = blockIdx.x - p.kv_groups, b = w / p.tokens, t = w % p.tokens;
         const int64_t n = p.counts ? p.counts[b] : p.tokens, pos = (int64_t)p.lengths[b] + t;
         const bool live = t < n && pos >= 0 && pos < p.table_width * P;
         const T* q = static_cast<const T*>(p.q) + b * p.q_stride[0] + t * p.q_stride[1];
@@ -63,57 +123,296 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p) {
         }
         return;
     }
-    const bool is_v = w & 1;
-    w >>= 1;
-    const int64_t j = w % p.blocks, h = w / p.blocks % H, b = w / p.blocks / H;
-    const int64_t len = p.lengths[b];
-    int64_t n = p.counts ? p.counts[b] : p.tokens;
-    n = n > p.tokens ? p.tokens : n;
-    if (len < 0) return;
-    const int64_t end = len + n < p.table_width * P ? len + n : p.table_width * P;
-    const int64_t first = (len / P + j) * P;
-    const int64_t lo = (len > first ? len : first) - first, hi = (end < first + P ? end : first + P) - first;
-    if (lo >= hi) return;
-    const int64_t page = p.table[b * p.table_stride + first / P];
-    if (page < 0 || page >= p.c.pages) return;
-    const int64_t* stride = is_v ? p.v_stride : p.k_stride;
-    const T* x = static_cast<const T*>(is_v ? p.v : p.k) + b * stride[0] + h * stride[2] + (first - len) * stride[1];
-    uint8_t* codes = static_cast<uint8_t*>(is_v ? p.c.v : p.c.k) + (page * H + h) * W * P;
-    float* scales = (is_v ? p.c.v_scale : p.c.k_scale) + page * H + h;
+    Block k;
+    if (!find_block<T>(p, blockIdx.x, k)) return;
+    const T* x = static_cast<const T*>(k.x);
     auto value = [&](int64_t t, int d) -> float {
         if (d >= p.c.dim) return 0.f;
-        return is_v ? to_f32(x[t * stride[1] + d]) : rotated<T>(p, x + t * stride[1], first + t, d);
+        return k.is_v ? to_f32(x[t * k.row_stride + d]) : rotated<T>(p, x + t * k.row_stride, k.first + t, d);
     };
-    auto place = [&](int64_t t, int64_t d) { return is_v ? d * P + t : t * W + d; };
-
-    float amax = 0.f;
-    for (int64_t i = lo * W + threadIdx.x; i < hi * W; i += 256) {
-        const float a = fabsf(value(i / W, (int)(i % W)));
-        if (a < INFINITY) amax = fmaxf(amax, a);
-    }
-    for (int off = 32; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off, 64));
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x / 64] = amax;
-    const float old = lo > 0 ? *scales : 0.f;
-    __syncthreads();
-    amax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-    const float scale = fmaxf(power_of_two(scale_exponent(amax)), old);
-    const float inv = 1.f / scale;
-    if (lo > 0 && scale > old) {
-        for (int64_t i = threadIdx.x; i < lo * W; i += 256) {
-            uint8_t* c = codes + place(i / W, i % W);
+    auto place = [&](int64_t t, int64_t d) { return k.is_v ? d * P + t : t * W + d; };
+    float amax = 0.f, old;
+    for (int64_t i = k.lo * W + threadIdx.x; i < k.hi * W; i += 256) take_max(amax, value(i / W, (int)(i % W)));
+    const float scale = settle_scale(k, amax, old), inv = 1.f / scale;
+    if (k.lo > 0 && scale > old) {
+        for (int64_t i = threadIdx.x; i < k.lo * W; i += 256) {
+            uint8_t* c = k.codes + place(i / W, i % W);
             *c = (uint8_t)fp8_pair(fp8_value(*c) * (old * inv), 0.f);
         }
     }
-    for (int64_t i = lo * W + threadIdx.x; i < hi * W; i += 256) {
+    for (int64_t i = k.lo * W + threadIdx.x; i < k.hi * W; i += 256) {
         const int64_t t = i / W, d = i % W;
-        codes[place(t, d)] = (uint8_t)fp8_pair(value(t, (int)d) * inv, 0.f);
+        k.codes[place(t, d)] = (uint8_t)fp8_pair(value(t, (int)d) * inv, 0.f);
     }
-    if (threadIdx.x == 0) *scales = scale;
+    if (threadIdx.x == 0) *k.scale = scale;
 }
 
 template <typename T>
-int append_launch(const AppendParams& p, int64_t grid, hipStream_t st) {
-    kv_append_kernel<T><<<(uint32_t)grid, 256, 0, st>>>(p);
+__device__ __forceinline__ void load8(const T* src, float* x) {
+    T v[8];
+    __builtin_memcpy(v, src, sizeof v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32(v[i]);
+}
+
+// The two pieces of eight elements that one thread takes of a row: for the
+// rotated part a piece and the one it is paired with (the same distance into
+// the other half, or its neighbour), after that neighbours.
+struct Pieces {
+    int a, b;   // first elements
+    int turn;   // first of their cos and sin, or -1
+};
+
+__device__ __forceinline__ Pieces pieces_of(const AppendParams& p, int i, bool rotate) {
+    const int rot = rotate ? (int)p.rot : 0;
+    if (16 * i >= rot) return {16 * i, 16 * i + 8, -1};
+    if (p.interleaved) return {16 * i, 16 * i + 8, 8 * i};
+    return {8 * i, 8 * i + rot / 2, 8 * i};
+}
+
+// Rotates the pieces a and b by eight angles; each product and sum is rounded.
+__device__ __forceinline__ void turn_pieces(const float* c, const float* s, bool interleaved, float* a, float* b) {
+#pragma clang fp contract(off)
+    if (interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float a0 = a[2 * i], a1 = a[2 * i + 1], b0 = b[2 * i], b1 = b[2 * i + 1];
+            const float p0 = a0 * c[i], p1 = a1 * s[i], p2 = a1 * c[i], p3 = a0 * s[i];
+            const float r0 = b0 * c[4 + i], r1 = b1 * s[4 + i], r2 = b1 * c[4 + i], r3 = b0 * s[4 + i];
+            a[2 * i] = p0 - p1;
+            a[2 * i + 1] = p2 + p3;
+            b[2 * i] = r0 - r1;
+            b[2 * i + 1] = r2 + r3;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float p0 = a[i] * c[i], p1 = b[i] * s[i], p2 = b[i] * c[i], p3 = a[i] * s[i];
+            a[i] = p0 - p1;
+            b[i] = p2 + p3;
+        }
+    }
+}
+
+// Bytes-bound: keys, values and queries are read once, codes and rotated
+// queries written once.
+//   keys     a thread takes 16 elements of a token at a time and keeps them in
+//            registers between the block's maximum and its codes
+//   values   a thread takes two neighbouring elements of the 16 tokens of a
+//            run, whose codes lie together in the cache
+//   queries  a wavefront takes a token; a lane's elements are in the same
+//            place of every head, so that it reads its angles once
+// Head sizes are multiples of 8 here and rotated parts of 16.
+template <typename T, int W>
+__global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p) {
+    constexpr int kRow = W / 16;  // threads a row
+    const int tid = threadIdx.x, D = (int)p.c.dim;
+    if (blockIdx.x >= p.kv_groups) {
+        const int64_t row = (int64_t)(blockIdx.x - p.kv_groups) * 4 + (tid >> 6);
+        const int64_t b = row / p.tokens, t = row - b * p.tokens;
+        if (b >= p.batch) return;
+        const int64_t n = p.counts ? p.counts[b] : p.tokens, pos = (int64_t)p.lengths[b] + t;
+        const bool live = t < n && pos >= 0 && pos < p.table_width * p.c.page;
+        const T* q = static_cast<const T*>(p.q) + b * p.q_stride[0] + t * p.q_stride[1];
+        T* out = static_cast<T*>(p.q_out) + row * p.q_heads * D;
+        constexpr int kLanes = 64 / kRow * kRow;  // lanes at work: whole rows
+        const int lane = tid & 63;
+        if (lane >= kLanes) return;
+        const Pieces at = pieces_of(p, lane % kRow, true);
+        float c[8], s[8];
+        if (live && at.turn >= 0) {
+            __builtin_memcpy(c, p.cos + pos * (p.rot / 2) + at.turn, sizeof c);
+            __builtin_memcpy(s, p.sin + pos * (p.rot / 2) + at.turn, sizeof s);
+        }
+        constexpr int kHeads = 64 / kRow;
+        for (int h0 = lane / kRow; h0 < p.q_heads; h0 += 4 * kHeads) {
+            float x[4][2][8];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int h = h0 + u * kHeads;
+                const T* src = q + h * p.q_stride[2];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[u][0][i] = x[u][1][i] = 0.f;
+                if (live && h < p.q_heads) {
+                    if (at.a < D) load8(src + at.a, x[u][0]);
+                    if (at.b < D) load8(src + at.b, x[u][1]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int h = h0 + u * kHeads;
+                if (h >= p.q_heads) break;
+                if (live && at.turn >= 0) turn_pieces(c, s, p.interleaved, x[u][0], x[u][1]);
+                T y[2][8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    y[0][i] = (T)x[u][0][i];
+                    y[1][i] = (T)x[u][1][i];
+                }
+                if (at.a < D) __builtin_memcpy(out + (int64_t)h * D + at.a, y[0], sizeof y[0]);
+                if (at.b < D) __builtin_memcpy(out + (int64_t)h * D + at.b, y[1], sizeof y[1]);
+            }
+        }
+        return;
+    }
+    Block k;
+    if (!find_block<T>(p, blockIdx.x, k)) return;
+    const T* x = static_cast<const T*>(k.x);
+    float amax = 0.f, old;
+    if (!k.is_v) {
+        // keys
+        constexpr int kHold = 2;  // rows of threads held in registers
+        const Pieces at = pieces_of(p, tid % kRow, p.cos != nullptr);
+        auto load = [&](int t, float* a, float* b) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+            const T* src = x + t * k.row_stride;
+            if (at.a < D) load8(src + at.a, a);
+            if (at.b < D) load8(src + at.b, b);
+            if (at.turn >= 0) {
+                float c[8], s[8];
+                __builtin_memcpy(c, p.cos + (k.first + t) * (p.rot / 2) + at.turn, sizeof c);
+                __builtin_memcpy(s, p.sin + (k.first + t) * (p.rot / 2) + at.turn, sizeof s);
+                turn_pieces(c, s, p.interleaved, a, b);
+            }
+        };
+        constexpr int kStep = 256 / kRow;  // rows a pass
+        const bool works = tid < kStep * kRow;
+        const int t0 = works ? k.lo + tid / kRow : k.hi;
+        float held[kHold][2][8];
+#pragma unroll
+        for (int u = 0; u < kHold; ++u)
+            if (t0 + u * kStep < k.hi) load(t0 + u * kStep, held[u][0], held[u][1]);
+#pragma unroll
+        for (int u = 0; u < kHold; ++u)
+            if (t0 + u * kStep < k.hi)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) take_max(amax, held[u][i / 8][i % 8]);
+        for (int t = t0 + kHold * kStep; t < k.hi; t += kStep) {
+            float a[8], b[8];
+            load(t, a, b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                take_max(amax, a[i]);
+                take_max(amax, b[i]);
+            }
+        }
+        const float scale = settle_scale(k, amax, old), inv = 1.f / scale;
+        auto store = [&](int t, const float* a, const float* b) {
+            u32x2 u, v;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                u[i] = fp8_pair(a[4 * i] * inv, a[4 * i + 1] * inv) | fp8_pair(a[4 * i + 2] * inv, a[4 * i + 3] * inv) << 16;
+                v[i] = fp8_pair(b[4 * i] * inv, b[4 * i + 1] * inv) | fp8_pair(b[4 * i + 2] * inv, b[4 * i + 3] * inv) << 16;
+            }
+            *reinterpret_cast<u32x2*>(k.codes + (int64_t)t * W + at.a) = u;
+            *reinterpret_cast<u32x2*>(k.codes + (int64_t)t * W + at.b) = v;
+        };
+#pragma unroll
+        for (int u = 0; u < kHold; ++u)
+            if (t0 + u * kStep < k.hi) store(t0 + u * kStep, held[u][0], held[u][1]);
+        for (int t = t0 + kHold * kStep; t < k.hi; t += kStep) {
+            float a[8], b[8];
+            load(t, a, b);
+            store(t, a, b);
+        }
+        if (k.lo > 0 && scale > old) {
+            for (int64_t i = tid; i < (int64_t)k.lo * W / 4; i += 256) {
+                uint32_t* c = reinterpret_cast<uint32_t*>(k.codes) + i;
+                *c = rescaled(*c, old * inv);
+            }
+        }
+        if (tid == 0) *k.scale = scale;
+        return;
+    }
+    // values
+    const int run0 = k.lo / 16, runs = (k.hi + 15) / 16 - run0, P = (int)p.c.page;
+    auto load = [&](int unit, float* v) {
+        const int t = (run0 + unit / (W / 2)) * 16, d = unit % (W / 2) * 2;
+        const T* src = x + t * k.row_stride + d;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const bool in = t + i >= k.lo && t + i < k.hi && d < D;
+            T two[2] = {(T)0.f, (T)0.f};
+            if (in) __builtin_memcpy(two, src + i * k.row_stride, sizeof two);
+            v[i] = to_f32(two[0]);
+            v[16 + i] = to_f32(two[1]);
+        }
+    };
+    const int units = runs * (W / 2);
+    float held[32];
+    if (tid < units) {
+        load(tid, held);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) take_max(amax, held[i]);
+    }
+    for (int u = tid + 256; u < units; u += 256) {
+        float v[32];
+        load(u, v);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) take_max(amax, v[i]);
+    }
+    const float scale = settle_scale(k, amax, old), inv = 1.f / scale;
+    const bool grown = k.lo > 0 && scale > old;
+    for (int u = tid; u < units; u += 256) {
+        if (u != tid) load(u, held);
+        const int t = (run0 + u / (W / 2)) * 16, d = u % (W / 2) * 2;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            u32x4* dst = reinterpret_cast<u32x4*>(k.codes + (int64_t)(d + e) * P + t);
+            u32x4 c;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float* v = held + e * 16 + i * 4;
+                c[i] = fp8_pair(v[0] * inv, v[1] * inv) | fp8_pair(v[2] * inv, v[3] * inv) << 16;
+            }
+            if (t < k.lo || t + 16 > k.hi) {
+                // a run that holds other tokens: earlier ones, or slots not yet taken
+                const u32x4 was = *dst;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t again = grown ? rescaled(was[i], old * inv) : was[i];
+                    uint32_t r = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int slot = t + 4 * i + j;
+                        r |= (slot < k.lo ? again : slot < k.hi ? c[i] : was[i]) & (0xffu << 8 * j);
+                    }
+                    c[i] = r;
+                }
+            }
+            *dst = c;
+        }
+    }
+    if (grown) {
+        // runs of earlier tokens only
+        for (int64_t u = tid; u < (int64_t)run0 * W; u += 256) {
+            u32x4* dst = reinterpret_cast<u32x4*>(k.codes + u / run0 * P + u % run0 * 16);
+            u32x4 c = *dst;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[i] = rescaled(c[i], old * inv);
+            *dst = c;
+        }
+    }
+    if (tid == 0) *k.scale = scale;
+}
+
+template <typename T>
+int append_launch(AppendParams& p, bool queries, hipStream_t st) {
+    const bool pieces = p.c.dim % 8 == 0 && p.rot % 16 == 0;
+    const int64_t rows = queries ? p.batch * p.tokens : 0, grid = p.kv_groups + (pieces ? (rows + 3) / 4 : rows);
+    if (grid > kMaxGrid) return set_error(TT_UNSUPPORTED, "tt_kv_append: %lld workgroups", (long long)grid);
+    const uint32_t g = (uint32_t)grid;
+    if (!pieces)
+        kv_append_any_kernel<T><<<g, 256, 0, st>>>(p);
+    else if (p.width == 64)
+        kv_append_kernel<T, 64><<<g, 256, 0, st>>>(p);
+    else if (p.width == 128)
+        kv_append_kernel<T, 128><<<g, 256, 0, st>>>(p);
+    else if (p.width == 192)
+        kv_append_kernel<T, 192><<<g, 256, 0, st>>>(p);
+    else
+        kv_append_kernel<T, 256><<<g, 256, 0, st>>>(p);
     return check_launch("tt_kv_append");
 }
 
@@ -137,9 +436,10 @@ extern "C" int tt_kv_append(const tt_kv_append_args* a, void* stream) {
     if (!a->k || !a->v || !a->lengths || (a->table_width > 0 && !a->table))
         return set_error(TT_INVALID, "tt_kv_append: NULL pointer");
     AppendParams p;
+    p.batch = a->batch;
     p.tokens = a->tokens;
     p.q_heads = a->q_heads;
-    p.rot = a->rot;
+    p.rot = a->cos ? a->rot : 0;
     p.interleaved = a->interleaved;
     p.table_width = a->table_width;
     p.table_stride = a->table_stride;
@@ -160,11 +460,13 @@ extern "C" int tt_kv_append(const tt_kv_append_args* a, void* stream) {
     p.c = a->cache;
     p.width = kv_width(a->cache.dim);
     p.blocks = (a->tokens + a->cache.page - 2) / a->cache.page + 1;
+    if (a->batch > kMaxGrid || a->tokens > kMaxGrid || a->cache.heads > kMaxGrid / a->batch ||
+        p.blocks > kMaxGrid / 2 / (a->batch * a->cache.heads))
+        return set_error(TT_UNSUPPORTED, "tt_kv_append: %lld sequences of %lld tokens", (long long)a->batch,
+                         (long long)a->tokens);
     p.kv_groups = 2 * a->batch * a->cache.heads * p.blocks;
-    const int64_t grid = p.kv_groups + (a->q ? a->batch * a->tokens : 0);
-    if (grid > kMaxGrid) return set_error(TT_UNSUPPORTED, "tt_kv_append: %lld workgroups", (long long)grid);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (a->dtype == TT_F32) return append_launch<float>(p, grid, st);
-    if (a->dtype == TT_BF16) return append_launch<__bf16>(p, grid, st);
-    return append_launch<_Float16>(p, grid, st);
+    if (a->dtype == TT_F32) return append_launch<float>(p, a->q != nullptr, st);
+    if (a->dtype == TT_BF16) return append_launch<__bf16>(p, a->q != nullptr, st);
+    return append_launch<_Float16>(p, a->q != nullptr, st);
 }
