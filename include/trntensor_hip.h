@@ -268,8 +268,8 @@ int tt_strided_contract(int dtype, int n_out, const int64_t* out_shape,
  * holds code 2j in its low and code 2j + 1 in its high half. code_pitch is a
  * multiple of 64 and at least K / 2 rounded up to one (what the bytes past K
  * hold does not matter); `codes` is 16-byte aligned. `scales` and `zeros`
- * (NULL: every zero is 8) are [ceil(K / group)][N] in scale_dtype (TT_F32,
- * TT_BF16, TT_F16). group is 32, 64 or a multiple of 128. x and y are rows of
+ * (NULL: every zero is 8) are [ceil(K / group)][N rounded up to a multiple of
+ * 16] in scale_dtype (TT_F32, TT_BF16, TT_F16), 16-byte aligned. group is 32, 64 or a multiple of 128. x and y are rows of
  * unit stride at ldx and ldy elements.
  */
 typedef struct {

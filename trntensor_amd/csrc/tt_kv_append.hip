@@ -82,21 +82,47 @@ __device__ __forceinline__ bool find_block(const AppendParams& p, int64_t w, Blo
     return true;
 }
 
-// The block's new scale, from the largest finite magnitude among the new
-// values (each thread's in `amax`) and, if it holds earlier tokens, its old one.
-__device__ __forceinline__ float settle_scale(const Block& k, float amax, float& old) {
-    __shared__ float part[4];
-    for (int off = 32; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off, 64));
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x / 64] = amax;
-    old = k.lo > 0 ? *k.scale : 0.f;
-    __syncthreads();
-    amax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-    return fmaxf(power_of_two(scale_exponent(amax)), old);
+// The largest magnitude as bits, which order as magnitudes do; anything from
+// 0x7f800000 on says that an infinity or NaN is among them.
+constexpr uint32_t kNotFinite = 0x7f800000u;
+
+__device__ __forceinline__ void take_max(uint32_t& top, float x) {
+    const uint32_t a = __float_as_uint(x) & 0x7fffffffu;
+    top = a > top ? a : top;
 }
 
-__device__ __forceinline__ void take_max(float& amax, float x) {
-    const float a = fabsf(x);
-    if (a < INFINITY) amax = fmaxf(amax, a);
+__device__ __forceinline__ void take_finite_max(uint32_t& top, float x) {
+    const uint32_t a = __float_as_uint(x) & 0x7fffffffu;
+    if (a < kNotFinite) top = a > top ? a : top;
+}
+
+// Over the workgroup.
+__device__ __forceinline__ uint32_t top_of_all(uint32_t top) {
+    __shared__ uint32_t part[4];
+    for (int off = 32; off > 0; off >>= 1) {
+        const uint32_t o = __shfl_xor(top, off, 64);
+        top = o > top ? o : top;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x / 64] = top;
+    __syncthreads();
+    const uint32_t a = part[0] > part[1] ? part[0] : part[1], b = part[2] > part[3] ? part[2] : part[3];
+    return a > b ? a : b;
+}
+
+// The block's new scale: its new values' (the largest finite magnitude's), or
+// its old one if that is larger and the block holds earlier tokens.
+__device__ __forceinline__ float new_scale(uint32_t top, float old) {
+    return fmaxf(power_of_two(scale_exponent(__uint_as_float(top))), old);
+}
+
+// Four values as codes. Finite ones are within the format's range at their
+// block's scale; with others about (`wild`) each is saturated.
+__device__ __forceinline__ uint32_t codes_of(const float* x, float inv, bool wild) {
+    const float a = x[0] * inv, b = x[1] * inv, c = x[2] * inv, d = x[3] * inv;
+    if (wild) return fp8_pair(a, b) | fp8_pair(c, d) << 16;
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
 }
 
 // Four codes at another scale.
@@ -131,9 +157,10 @@ __global__ __launch_bounds__(256) void kv_append_any_kernel(AppendParams p) {
         return k.is_v ? to_f32(x[t * k.row_stride + d]) : rotated<T>(p, x + t * k.row_stride, k.first + t, d);
     };
     auto place = [&](int64_t t, int64_t d) { return k.is_v ? d * P + t : t * W + d; };
-    float amax = 0.f, old;
-    for (int64_t i = k.lo * W + threadIdx.x; i < k.hi * W; i += 256) take_max(amax, value(i / W, (int)(i % W)));
-    const float scale = settle_scale(k, amax, old), inv = 1.f / scale;
+    const float old = k.lo > 0 ? *k.scale : 0.f;
+    uint32_t top = 0;
+    for (int64_t i = k.lo * W + threadIdx.x; i < k.hi * W; i += 256) take_finite_max(top, value(i / W, (int)(i % W)));
+    const float scale = new_scale(top_of_all(top), old), inv = 1.f / scale;
     if (k.lo > 0 && scale > old) {
         for (int64_t i = threadIdx.x; i < k.lo * W; i += 256) {
             uint8_t* c = k.codes + place(i / W, i % W);
@@ -258,63 +285,68 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p) {
     Block k;
     if (!find_block<T>(p, blockIdx.x, k)) return;
     const T* x = static_cast<const T*>(k.x);
-    float amax = 0.f, old;
+    const float old = k.lo > 0 ? *k.scale : 0.f;
+    uint32_t top = 0;
     if (!k.is_v) {
         // keys
         constexpr int kHold = 2;  // rows of threads held in registers
         const Pieces at = pieces_of(p, tid % kRow, p.cos != nullptr);
-        auto load = [&](int t, float* a, float* b) {
+        auto load = [&](int t, float* v) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+            for (int i = 0; i < 16; ++i) v[i] = 0.f;
             const T* src = x + t * k.row_stride;
-            if (at.a < D) load8(src + at.a, a);
-            if (at.b < D) load8(src + at.b, b);
+            if (at.a < D) load8(src + at.a, v);
+            if (at.b < D) load8(src + at.b, v + 8);
             if (at.turn >= 0) {
                 float c[8], s[8];
                 __builtin_memcpy(c, p.cos + (k.first + t) * (p.rot / 2) + at.turn, sizeof c);
                 __builtin_memcpy(s, p.sin + (k.first + t) * (p.rot / 2) + at.turn, sizeof s);
-                turn_pieces(c, s, p.interleaved, a, b);
+                turn_pieces(c, s, p.interleaved, v, v + 8);
             }
         };
         constexpr int kStep = 256 / kRow;  // rows a pass
-        const bool works = tid < kStep * kRow;
-        const int t0 = works ? k.lo + tid / kRow : k.hi;
-        float held[kHold][2][8];
+        const int t0 = tid < kStep * kRow ? k.lo + tid / kRow : k.hi;
+        float held[kHold][16];
 #pragma unroll
         for (int u = 0; u < kHold; ++u)
-            if (t0 + u * kStep < k.hi) load(t0 + u * kStep, held[u][0], held[u][1]);
+            if (t0 + u * kStep < k.hi) load(t0 + u * kStep, held[u]);
 #pragma unroll
         for (int u = 0; u < kHold; ++u)
             if (t0 + u * kStep < k.hi)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) take_max(amax, held[u][i / 8][i % 8]);
+                for (int i = 0; i < 16; ++i) take_max(top, held[u][i]);
         for (int t = t0 + kHold * kStep; t < k.hi; t += kStep) {
-            float a[8], b[8];
-            load(t, a, b);
+            float v[16];
+            load(t, v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                take_max(amax, a[i]);
-                take_max(amax, b[i]);
-            }
+            for (int i = 0; i < 16; ++i) take_max(top, v[i]);
         }
-        const float scale = settle_scale(k, amax, old), inv = 1.f / scale;
-        auto store = [&](int t, const float* a, const float* b) {
-            u32x2 u, v;
+        top = top_of_all(top);
+        const bool wild = top >= kNotFinite;
+        if (wild) {
+            uint32_t finite = 0;
+            for (int t = t0; t < k.hi; t += kStep) {
+                float v[16];
+                load(t, v);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                u[i] = fp8_pair(a[4 * i] * inv, a[4 * i + 1] * inv) | fp8_pair(a[4 * i + 2] * inv, a[4 * i + 3] * inv) << 16;
-                v[i] = fp8_pair(b[4 * i] * inv, b[4 * i + 1] * inv) | fp8_pair(b[4 * i + 2] * inv, b[4 * i + 3] * inv) << 16;
+                for (int i = 0; i < 16; ++i) take_finite_max(finite, v[i]);
             }
-            *reinterpret_cast<u32x2*>(k.codes + (int64_t)t * W + at.a) = u;
-            *reinterpret_cast<u32x2*>(k.codes + (int64_t)t * W + at.b) = v;
+            top = top_of_all(finite);
+        }
+        const float scale = new_scale(top, old), inv = 1.f / scale;
+        auto store = [&](int t, const float* v) {
+            u32x2 a = {codes_of(v, inv, wild), codes_of(v + 4, inv, wild)};
+            u32x2 b = {codes_of(v + 8, inv, wild), codes_of(v + 12, inv, wild)};
+            *reinterpret_cast<u32x2*>(k.codes + (int64_t)t * W + at.a) = a;
+            *reinterpret_cast<u32x2*>(k.codes + (int64_t)t * W + at.b) = b;
         };
 #pragma unroll
         for (int u = 0; u < kHold; ++u)
-            if (t0 + u * kStep < k.hi) store(t0 + u * kStep, held[u][0], held[u][1]);
+            if (t0 + u * kStep < k.hi) store(t0 + u * kStep, held[u]);
         for (int t = t0 + kHold * kStep; t < k.hi; t += kStep) {
-            float a[8], b[8];
-            load(t, a, b);
-            store(t, a, b);
+            float v[16];
+            load(t, v);
+            store(t, v);
         }
         if (k.lo > 0 && scale > old) {
             for (int64_t i = tid; i < (int64_t)k.lo * W / 4; i += 256) {
@@ -329,30 +361,55 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p) {
     const int run0 = k.lo / 16, runs = (k.hi + 15) / 16 - run0, P = (int)p.c.page;
     auto load = [&](int unit, float* v) {
         const int t = (run0 + unit / (W / 2)) * 16, d = unit % (W / 2) * 2;
-        const T* src = x + t * k.row_stride + d;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const bool in = t + i >= k.lo && t + i < k.hi && d < D;
-            T two[2] = {(T)0.f, (T)0.f};
-            if (in) __builtin_memcpy(two, src + i * k.row_stride, sizeof two);
-            v[i] = to_f32(two[0]);
-            v[16 + i] = to_f32(two[1]);
+        for (int i = 0; i < 32; ++i) v[i] = 0.f;
+        if (d >= D) return;
+        const T* src = x + t * k.row_stride + d;
+        T two[16][2];
+        if (t >= k.lo && t + 16 <= k.hi) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) __builtin_memcpy(two[i], src + i * k.row_stride, sizeof two[i]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                v[i] = to_f32(two[i][0]);
+                v[16 + i] = to_f32(two[i][1]);
+            }
+            return;
         }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (t + i >= k.lo && t + i < k.hi) {
+                __builtin_memcpy(two[i], src + i * k.row_stride, sizeof two[i]);
+                v[i] = to_f32(two[i][0]);
+                v[16 + i] = to_f32(two[i][1]);
+            }
     };
     const int units = runs * (W / 2);
     float held[32];
     if (tid < units) {
         load(tid, held);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) take_max(amax, held[i]);
+        for (int i = 0; i < 32; ++i) take_max(top, held[i]);
     }
     for (int u = tid + 256; u < units; u += 256) {
         float v[32];
         load(u, v);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) take_max(amax, v[i]);
+        for (int i = 0; i < 32; ++i) take_max(top, v[i]);
     }
-    const float scale = settle_scale(k, amax, old), inv = 1.f / scale;
+    top = top_of_all(top);
+    const bool wild = top >= kNotFinite;
+    if (wild) {
+        uint32_t finite = 0;
+        for (int u = tid; u < units; u += 256) {
+            float v[32];
+            load(u, v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) take_finite_max(finite, v[i]);
+        }
+        top = top_of_all(finite);
+    }
+    const float scale = new_scale(top, old), inv = 1.f / scale;
     const bool grown = k.lo > 0 && scale > old;
     for (int u = tid; u < units; u += 256) {
         if (u != tid) load(u, held);
@@ -362,23 +419,17 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p) {
             u32x4* dst = reinterpret_cast<u32x4*>(k.codes + (int64_t)(d + e) * P + t);
             u32x4 c;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float* v = held + e * 16 + i * 4;
-                c[i] = fp8_pair(v[0] * inv, v[1] * inv) | fp8_pair(v[2] * inv, v[3] * inv) << 16;
-            }
+            for (int i = 0; i < 4; ++i) c[i] = codes_of(held + e * 16 + i * 4, inv, wild);
             if (t < k.lo || t + 16 > k.hi) {
                 // a run that holds other tokens: earlier ones, or slots not yet taken
                 const u32x4 was = *dst;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
+                    const int slot = t + 4 * i;
+                    auto below = [&](int n) { return n <= slot ? 0u : n >= slot + 4 ? ~0u : (1u << 8 * (n - slot)) - 1; };
+                    const uint32_t earlier = below(k.lo), taken = below(k.hi);
                     const uint32_t again = grown ? rescaled(was[i], old * inv) : was[i];
-                    uint32_t r = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int slot = t + 4 * i + j;
-                        r |= (slot < k.lo ? again : slot < k.hi ? c[i] : was[i]) & (0xffu << 8 * j);
-                    }
-                    c[i] = r;
+                    c[i] = (again & earlier) | (c[i] & taken & ~earlier) | (was[i] & ~taken);
                 }
             }
             *dst = c;

@@ -31,6 +31,7 @@ struct AttnParams {
 
 constexpr int kTile = 64;     // keys a wavefront takes at a time
 constexpr int kMinTiles = 4;  // fewest tiles worth a workgroup: one per wavefront
+constexpr int kPairCost = 4;  // what starting and joining a pair costs, in tiles
 
 // Which keys the query rows of one block see: those of [0, end) that are in a
 // row's window or among the sinks lie in tiles [0, sink_tiles) and [start, ..).
@@ -512,18 +513,48 @@ __device__ __forceinline__ void join_waves(const AttnParams& p, Wave<T, W, 1>& w
     __syncthreads();
 }
 
+// The work of a sequence's pairs, in tiles, and of all sequences.
+__device__ __forceinline__ int64_t weight_of(const AttnParams& p, int b) {
+    const int tiles = span_of(p, b, 0, 16).tiles;
+    return tiles > 0 ? (int64_t)(tiles + kPairCost) * p.heads : 0;
+}
+
+struct Weights {
+    int64_t total, before;  // of all sequences, and of those before a given one
+};
+
+// By one wavefront.
+__device__ __forceinline__ Weights all_weights(const AttnParams& p, int limit) {
+    Weights w = {0, 0};
+    for (int b = threadIdx.x & 63; b < p.batch; b += 64) {
+        const int64_t v = weight_of(p, b);
+        w.total += v;
+        if (b < limit) w.before += v;
+    }
+    for (int off = 32; off > 0; off >>= 1) {
+        w.total += __shfl_xor(w.total, off, 64);
+        w.before += __shfl_xor(w.before, off, 64);
+    }
+    return w;
+}
+
+__device__ __forceinline__ int64_t share_of(const AttnParams& p, int64_t total) {
+    const int64_t per = (total + p.groups - 1) / p.groups;
+    return per < kMinTiles + kPairCost ? kMinTiles + kPairCost : per;
+}
+
 // Few query rows (at most 16 a cache head): the four wavefronts of a workgroup
 // take every fourth tile of the same keys. The key tiles of all (sequence,
-// head) pairs form one list, which the workgroups share evenly whatever the
-// sequences' lengths; a pair cut by a workgroup's end leaves partial results.
+// head) pairs form one list, in which each pair also takes the room of what
+// starting it costs; the workgroups share it evenly whatever the sequences'
+// lengths, and a pair cut by a workgroup's end leaves partial results.
 // Wavefronts a SIMD is to hold: two where the state of one fits half its registers.
 template <typename T, int W, int MT>
 constexpr int kWavesPerSimd = Parts<T>::q * MT * W > 256 || W > 128 ? 1 : 2;
 
 template <typename T, int W>
 __global__ __launch_bounds__(256, (kWavesPerSimd<T, W, 1>)) void kv_attention_few_kernel(AttnParams p) {
-    __shared__ int64_t scan[256];
-    const int wave = threadIdx.x >> 6;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     Wave<T, W, 1> w;
     if (p.direct) {
         const int b = blockIdx.x / p.heads, kh = blockIdx.x - b * p.heads;
@@ -538,19 +569,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, W, 1>)) void kv_attention_fe
         }
         return;
     }
-    // All tiles, and where this workgroup's share of them begins.
-    int64_t total = 0;
-    for (int b = threadIdx.x; b < p.batch; b += 256) total += (int64_t)span_of(p, b, 0, 16).tiles * p.heads;
-    scan[threadIdx.x] = total;
-    __syncthreads();
-    for (int off = 128; off > 0; off >>= 1) {
-        if ((int)threadIdx.x < off) scan[threadIdx.x] += scan[threadIdx.x + off];
-        __syncthreads();
-    }
-    total = scan[0];
-    __syncthreads();
-    int64_t per = (total + p.groups - 1) / p.groups;
-    if (per < kMinTiles) per = kMinTiles;
+    const int64_t total = all_weights(p, p.batch).total, per = share_of(p, total);
     const int64_t begin = blockIdx.x * per, stop = begin + per < total ? begin + per : total;
     // Sequences that see nothing: their zeros, dealt out over the workgroups.
     for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
@@ -559,108 +578,115 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, W, 1>)) void kv_attention_fe
             for (int kh = 0; kh < p.heads; ++kh) zero_rows<T, W>(p, b, kh, sp.tiles == 0 ? 0 : sp.live, 16);
     }
     if (begin >= stop) return;
+    // The sequence that `begin` lies in, and the place `at` of its first pair.
     int64_t at = 0;
     int b = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += 256) {
-        const int mine = b0 + (int)threadIdx.x;
-        __syncthreads();
-        scan[threadIdx.x] = mine < p.batch ? (int64_t)span_of(p, mine, 0, 16).tiles * p.heads : 0;
-        __syncthreads();
-        for (int off = 1; off < 256; off <<= 1) {
-            const int64_t v = (int)threadIdx.x >= off ? scan[threadIdx.x - off] : 0;
-            __syncthreads();
-            scan[threadIdx.x] += v;
-            __syncthreads();
+    for (int b0 = 0;; b0 += 64) {
+        const int64_t mine = b0 + lane < p.batch ? weight_of(p, b0 + lane) : 0;
+        int64_t upto = mine;
+        for (int off = 1; off < 64; off <<= 1) {
+            const int64_t v = __shfl_up(upto, off, 64);
+            upto += lane >= off ? v : 0;
         }
-        if (at + scan[255] > begin) {
-            // the first sequence of these whose tiles reach past `begin`
-            int lo = 0, hi = 255;
-            while (lo < hi) {
-                const int mid = (lo + hi) / 2;
-                if (at + scan[mid] > begin)
-                    hi = mid;
-                else
-                    lo = mid + 1;
-            }
-            b = b0 + lo;
-            at += lo ? scan[lo - 1] : 0;
+        const uint64_t past = __ballot(at + upto > begin);
+        if (past) {
+            const int f = __builtin_ctzll(past);
+            b = b0 + f;
+            at += __shfl(upto - mine, f, 64);
             break;
         }
-        at += scan[255];
+        at += __shfl(upto, 63, 64);
     }
-    // `at` is the place of sequence b's first tile.
     int64_t pos = begin;
     while (pos < stop) {
         const Span sp = span_of(p, b, 0, 16);
-        const int64_t size = (int64_t)sp.tiles * p.heads;
+        const int64_t pair_weight = sp.tiles + kPairCost, size = sp.tiles > 0 ? pair_weight * p.heads : 0;
         if (pos >= at + size) {
             at += size;
             ++b;
             continue;
         }
-        const int kh = (int)((pos - at) / sp.tiles);
-        const int64_t pair = at + (int64_t)kh * sp.tiles;
-        const int first = (int)(pos - pair), last = (int)(stop - pair < sp.tiles ? stop - pair : sp.tiles);
+        const int kh = (int)((pos - at) / pair_weight);
+        const int64_t pair = at + kh * pair_weight + kPairCost, end = stop < pair + sp.tiles ? stop : pair + sp.tiles;
+        const int first = pos > pair ? (int)(pos - pair) : 0, last = end > pair ? (int)(end - pair) : 0;
+        pos = end > pos ? end : stop;
+        if (first >= last) continue;
         w.load_q(p, b, kh, 0, sp, 0);
         walk<T, W, 1>(p, w, sp, b, kh, first + wave, last, 4);
+        // A pair is cut at most at this workgroup's ends: in its first or its last tiles.
         const bool whole = first == 0 && last == sp.tiles;
         float* slot = whole ? nullptr : p.part + ((int64_t)blockIdx.x * 2 + (first == 0 ? 1 : 0)) * (16 * (W + 2));
         join_waves<T, W>(p, w, sp, b, kh, 0, slot);
-        pos = pair + last;
     }
+}
+
+// One query row of `parts` partial results by one wavefront: slot 0 is `first`
+// and slot i > 0 `rest` + i * stride; a slot holds its rows' sums of W elements,
+// and the row's maximum and weight at m_at and l_at (weight -1: no key seen).
+template <typename T, int W>
+__device__ __forceinline__ void join_row(const float* first, const float* rest, int64_t stride, int parts, int row, int m_at,
+                                         int l_at, int dim, T* out) {
+    const int lane = threadIdx.x & 63;
+    auto slot = [&](int i) { return i ? rest + i * stride : first; };
+    float m = -INFINITY;
+    for (int i = lane; i < parts; i += 64) m = fmaxf(m, slot(i)[m_at]);
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    const float shift = m == -INFINITY ? 0.f : m;
+    float sum = 0.f, o[W / 64] = {};
+    bool some = false;
+    for (int i0 = 0; i0 < parts; i0 += 64) {
+        float f = 0.f;
+        if (i0 + lane < parts) {
+            const float* s = slot(i0 + lane);
+            const float l = s[l_at];
+            if (l != -1.f) {
+                f = exp2f(s[m_at] - shift);
+                sum += l * f;
+                some = true;
+            }
+        }
+        const int n = parts - i0 < 64 ? parts - i0 : 64;
+        constexpr int kDeep = 8;
+        for (int i = 0; i < n; i += kDeep) {
+            float x[kDeep][W / 64];
+#pragma unroll
+            for (int u = 0; u < kDeep; ++u) {
+                const float* s = slot(i0 + (i + u < n ? i + u : n - 1)) + row * W + lane;
+#pragma unroll
+                for (int d = 0; d < W / 64; ++d) x[u][d] = s[d * 64];
+            }
+#pragma unroll
+            for (int u = 0; u < kDeep; ++u) {
+                if (i + u >= n) break;
+                const float g = __shfl(f, i + u, 64);
+#pragma unroll
+                for (int d = 0; d < W / 64; ++d) o[d] += g * x[u][d];
+            }
+        }
+    }
+    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+    some = __any(some);
+#pragma unroll
+    for (int d = 0; d < W / 64; ++d)
+        if (d * 64 + lane < dim) out[d * 64 + lane] = (T)(some ? o[d] / sum : 0.f);
 }
 
 // Joins the partial results of the pairs that were cut: one wavefront a query row.
 template <typename T, int W>
 __global__ __launch_bounds__(256) void kv_attention_few_join_kernel(AttnParams p) {
-    __shared__ int64_t scan[2][256];
+    constexpr int64_t kSlot = 16 * (W + 2);
     const int b = blockIdx.x / p.heads, kh = blockIdx.x - b * p.heads;
-    int64_t total = 0, before = 0;
-    for (int i = threadIdx.x; i < p.batch; i += 256) {
-        const int64_t n = (int64_t)span_of(p, i, 0, 16).tiles * p.heads;
-        total += n;
-        if (i < b) before += n;
-    }
-    scan[0][threadIdx.x] = total;
-    scan[1][threadIdx.x] = before;
-    __syncthreads();
-    for (int off = 128; off > 0; off >>= 1) {
-        if ((int)threadIdx.x < off) {
-            scan[0][threadIdx.x] += scan[0][threadIdx.x + off];
-            scan[1][threadIdx.x] += scan[1][threadIdx.x + off];
-        }
-        __syncthreads();
-    }
-    total = scan[0][0];
-    int64_t per = (total + p.groups - 1) / p.groups;
-    if (per < kMinTiles) per = kMinTiles;
     const Span sp = span_of(p, b, 0, 16);
+    const Weights w = all_weights(p, b);
     if (sp.tiles == 0) return;
-    const int64_t at = scan[1][0] + (int64_t)kh * sp.tiles;
-    const int64_t g0 = at / per, g1 = (at + sp.tiles - 1) / per;
+    const int64_t per = share_of(p, w.total);
+    const int64_t pair = w.before + kh * (int64_t)(sp.tiles + kPairCost) + kPairCost;
+    const int64_t g0 = pair / per, g1 = (pair + sp.tiles - 1) / per;
     if (g0 == g1) return;
-    const int lane = threadIdx.x & 63;
-    for (int row = threadIdx.x >> 6; row < sp.live; row += 4) {
-        float m = -INFINITY;
-        for (int64_t g = g0; g <= g1; ++g) m = fmaxf(m, p.part[(g * 2 + (g == g0)) * (16 * (W + 2)) + 16 * W + row]);
-        const float shift = m == -INFINITY ? 0.f : m;
-        float sum = 0.f, o[W / 64] = {};
-        bool some = false;
-        for (int64_t g = g0; g <= g1; ++g) {
-            const float* slot = p.part + (g * 2 + (g == g0)) * (16 * (W + 2));
-            const float l = slot[16 * W + 16 + row];
-            if (l == -1.f) continue;
-            some = true;
-            const float f = exp2f(slot[16 * W + row] - shift);
-            sum += l * f;
-#pragma unroll
-            for (int d = 0; d < W / 64; ++d) o[d] += f * slot[row * W + d * 64 + lane];
-        }
-        T* out = out_row<T>(p, b, kh, row);
-#pragma unroll
-        for (int d = 0; d < W / 64; ++d)
-            if (d * 64 + lane < p.dim) out[d * 64 + lane] = (T)(some ? o[d] / sum : 0.f);
-    }
+    const float* base = p.part + g0 * 2 * kSlot;
+    for (int row = threadIdx.x >> 6; row < sp.live; row += 4)
+        join_row<T, W>(base + kSlot, base, 2 * kSlot, (int)(g1 - g0 + 1), row, 16 * W + row, 16 * W + 16 + row, p.dim,
+                       out_row<T>(p, b, kh, row));
 }
 
 // Many query rows: each wavefront takes MT blocks of 16 rows of its own, and
@@ -727,32 +753,15 @@ __global__ __launch_bounds__(256) void kv_attention_many_join_kernel(AttnParams 
     const int kh = id % p.heads;
     id /= p.heads;
     const int rb = id % p.row_blocks, b = id / p.row_blocks;
-    const int row0 = rb * kRows, r = chunk * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int row0 = rb * kRows, r = chunk * 4 + (threadIdx.x >> 6);
     const Span all = span_of(p, b, row0, kRows);
     if (row0 + r >= p.tokens * p.share || all.tiles <= 0) return;
     const int per = (all.tiles + p.groups - 1) / p.groups;
     if (per >= all.tiles) return;
-    const int parts = (all.tiles + per - 1) / per;
-    const float* base = p.part + (((int64_t)b * p.row_blocks + rb) * p.heads + kh) * p.groups * (int64_t)(kRows * (W + 2));
-    float m = -INFINITY;
-    for (int i = 0; i < parts; ++i) m = fmaxf(m, base[(int64_t)i * (kRows * (W + 2)) + kRows * W + r]);
-    const float shift = m == -INFINITY ? 0.f : m;
-    float sum = 0.f, o[W / 64] = {};
-    bool some = false;
-    for (int i = 0; i < parts; ++i) {
-        const float* slot = base + (int64_t)i * (kRows * (W + 2));
-        const float l = slot[kRows * W + kRows + r];
-        if (l == -1.f) continue;
-        some = true;
-        const float f = exp2f(slot[kRows * W + r] - shift);
-        sum += l * f;
-#pragma unroll
-        for (int d = 0; d < W / 64; ++d) o[d] += f * slot[r * W + d * 64 + lane];
-    }
-    T* out = out_row<T>(p, b, kh, row0 + r);
-#pragma unroll
-    for (int d = 0; d < W / 64; ++d)
-        if (d * 64 + lane < p.dim) out[d * 64 + lane] = (T)(some ? o[d] / sum : 0.f);
+    constexpr int64_t kSlot = kRows * (W + 2);
+    const float* base = p.part + (((int64_t)b * p.row_blocks + rb) * p.heads + kh) * p.groups * kSlot;
+    join_row<T, W>(base, base, kSlot, (all.tiles + per - 1) / per, r, kRows * W + r, kRows * W + kRows + r, p.dim,
+                   out_row<T>(p, b, kh, row0 + r));
 }
 
 // How a call is cut, from what the host knows of it.

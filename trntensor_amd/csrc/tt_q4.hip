@@ -138,6 +138,7 @@ __global__ __launch_bounds__(64 * KW, 2) void q4_matmul_kernel(Q4Params p) {
     const int per = (p.chunks + KW - 1) / KW;
     const int first = wave * per, last = first + per < p.chunks ? first + per : p.chunks;
 
+    // Rows past the end repeat the last one: what they give is not stored.
     const uint8_t* code_row[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -145,26 +146,31 @@ __global__ __launch_bounds__(64 * KW, 2) void q4_matmul_kernel(Q4Params p) {
         code_row[r] = p.codes + (int64_t)(n < p.N ? n : p.N - 1) * p.code_pitch + g * 16;
     }
     const T* x_row[MT];
-    bool x_live[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const int m = m0 + mt * 16 + c;
-        x_live[mt] = m < p.M;
-        x_row[mt] = static_cast<const T*>(p.x) + (int64_t)(x_live[mt] ? m : 0) * p.ldx;
+        x_row[mt] = static_cast<const T*>(p.x) + (int64_t)(m < p.M ? m : p.M - 1) * p.ldx + g * 8;
+    }
+    // A last chunk that the columns do not fill, with zeros behind them.
+    __shared__ __attribute__((aligned(16))) T filled[MT * 16][128 + 16 / sizeof(T)];
+    const bool ragged = last == p.chunks && p.K % 128 != 0 && first < last;
+    if (ragged) {
+        const int k0 = (p.chunks - 1) * 128;
+        for (int i = lane; i < MT * 16 * 128; i += 64) {
+            const int m = m0 + i / 128, k = k0 + i % 128;
+            filled[i / 128][i % 128] = k < p.K ? static_cast<const T*>(p.x)[(int64_t)(m < p.M ? m : p.M - 1) * p.ldx + k] : (T)0.f;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
     const bool bf16 = p.scale_bf16;
-    auto load_four = [&](const void* base, int group, int n) {
+    const int scale_pitch = (p.N + 15) / 16 * 16;
+    auto load_four = [&](const void* base, int group, int r) {
         Four<SW> f;
-        const uint8_t* src = static_cast<const uint8_t*>(base) + (int64_t)(group < p.groups ? group : p.groups - 1) * p.N * SW;
-        if (n + 4 <= p.N) {
-            __builtin_memcpy(f.raw, src + (int64_t)n * SW, sizeof f.raw);
-        } else {
-            uint8_t edge[4 * SW];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                __builtin_memcpy(edge + i * SW, src + (int64_t)(n + i < p.N ? n + i : p.N - 1) * SW, SW);
-            __builtin_memcpy(f.raw, edge, sizeof f.raw);
-        }
+        group = group < p.groups ? group : p.groups - 1;
+        const int n = n0 + r * 16 < scale_pitch ? n0 + r * 16 + g * 4 : 0;
+        __builtin_memcpy(f.raw, static_cast<const uint8_t*>(base) + ((int64_t)group * scale_pitch + n) * SW, sizeof f.raw);
         return f;
     };
     typedef Stage<T, SW, U, R, MT, GPC> St;
@@ -174,26 +180,27 @@ __global__ __launch_bounds__(64 * KW, 2) void q4_matmul_kernel(Q4Params p) {
             const int k = chunk + u < last ? chunk + u : last - 1;
 #pragma unroll
             for (int r = 0; r < R; ++r) st.codes[u][r] = *reinterpret_cast<const u32x4*>(code_row[r] + (int64_t)k * 64);
+            const bool edge = ragged && k == p.chunks - 1;
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int mt = 0; mt < MT; ++mt) {
+                if (edge) {
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const int k0 = k * 128 + s * 32 + g * 8;
-                    if (x_live[mt] && k0 + 8 <= p.K) {
-                        __builtin_memcpy(st.x[u][mt][s], x_row[mt] + k0, sizeof st.x[u][mt][s]);
-                    } else {
+                    for (int s = 0; s < 4; ++s)
+                        __builtin_memcpy(st.x[u][mt][s], __builtin_assume_aligned(&filled[mt * 16 + c][s * 32 + g * 8], 16),
+                                         sizeof st.x[u][mt][s]);
+                } else {
+                    const T* src = x_row[mt] + k * 128;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            st.x[u][mt][s][i] = x_live[mt] && k0 + i < p.K ? x_row[mt][k0 + i] : (T)0.f;
-                    }
+                    for (int s = 0; s < 4; ++s) __builtin_memcpy(st.x[u][mt][s], src + s * 32, sizeof st.x[u][mt][s]);
                 }
+            }
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
                 for (int q = 0; q < GPC; ++q) {
                     const int group = GPC > 1 ? (k * GPC + q) >> p.group_shift : k / p.chunks_per_group;
-                    st.scales[u][r][q] = load_four(p.scales, group, n0 + r * 16 + g * 4);
-                    if (p.zeros) st.zeros[u][r][q] = load_four(p.zeros, group, n0 + r * 16 + g * 4);
+                    st.scales[u][r][q] = load_four(p.scales, group, r);
+                    if (p.zeros) st.zeros[u][r][q] = load_four(p.zeros, group, r);
                 }
         }
     };

@@ -111,11 +111,17 @@ class Q4Matrix:
             laid[:, : codes.shape[1]] = codes
             codes = laid
         self.codes = codes
-        self.scales = scales.detach().to(device).t().contiguous()
-        self.zeros = None if zeros is None else zeros.detach().to(device).t().contiguous()
+        self.scales, self.zeros = (None if t is None else self._by_group(t.detach().to(device)) for t in (scales, zeros))
         self.shape = (n, k)
         self.group_size = int(group_size)
         self.device = device
+
+    @staticmethod
+    def _by_group(t: torch.Tensor) -> torch.Tensor:
+        """(out_features, groups) as (groups, out_features rounded up to a multiple of 16)."""
+        out = torch.zeros((t.shape[1], -(-t.shape[0] // 16) * 16), dtype=t.dtype, device=t.device)
+        out[:, : t.shape[0]] = t.t()
+        return out
 
     def __repr__(self) -> str:
         return f"Q4Matrix({self.shape[0]}, {self.shape[1]}, group_size={self.group_size}, device={self.device})"
