@@ -263,17 +263,28 @@ int tt_strided_contract(int dtype, int n_out, const int64_t* out_shape,
  * --------------------------------------------------------------------- */
 
 /*
+ * Lays out 4-bit codes for tt_q4_matmul. Row n of `codes` starts at n * pitch
+ * bytes, and byte j of it holds code 2j in its low and code 2j + 1 in its high
+ * half. `packed` (16-byte aligned) takes tt_q4_packed_bytes(N, K) bytes: tiles
+ * of 16 rows and 128 columns, 1024 bytes each, those of the same rows
+ * together; codes past N and K become zeros. In a tile, byte 16 l + 4 s + j
+ * holds columns 32 s + 8 (l / 16) + 4 (j % 2) + .. of row l % 16: in its low
+ * half column 0 and in its high half column 2 of those four for j < 2, column
+ * 1 and 3 for j >= 2.
+ */
+size_t tt_q4_packed_bytes(int64_t N, int64_t K);
+
+int tt_q4_pack(int64_t N, int64_t K, const void* codes, int64_t pitch, void* packed, void* stream);
+
+/*
  * y[m][n] = sum_k x[m][k] * scale[k / group][n] * (code[n][k] - zero[k / group][n])
- * with 4-bit codes: row n of `codes` starts at n * code_pitch and byte j of it
- * holds code 2j in its low and code 2j + 1 in its high half. code_pitch is a
- * multiple of 64 and at least K / 2 rounded up to one (what the bytes past K
- * hold does not matter); `codes` is 16-byte aligned. `scales` and `zeros`
- * (NULL: every zero is 8) are [ceil(K / group)][N rounded up to a multiple of
- * 16] in scale_dtype (TT_F32, TT_BF16, TT_F16), 16-byte aligned. group is 32, 64 or a multiple of 128. x and y are rows of
- * unit stride at ldx and ldy elements.
+ * with codes laid out by tt_q4_pack. `scales` and `zeros` (NULL: every zero is
+ * 8) are [ceil(K / group)][N rounded up to a multiple of 16] in scale_dtype
+ * (TT_F32, TT_BF16, TT_F16), 16-byte aligned. group is 32, 64 or a multiple of
+ * 128. x and y are rows of unit stride at ldx and ldy elements.
  */
 typedef struct {
-    int64_t dtype, scale_dtype, M, N, K, group, ldx, code_pitch, ldy;
+    int64_t dtype, scale_dtype, M, N, K, group, ldx, ldy;
     const void *x, *codes, *scales, *zeros;
     void *y, *workspace;
     int64_t workspace_bytes;

@@ -26,6 +26,7 @@ class _Cache:
 
     head_dim, num_heads, page_size = 64, 2, 16
     device = torch.device("cpu")
+    _host = None
 
 
 def _args(tokens=3, table=4):
@@ -153,20 +154,30 @@ def _cache_fields(**kw):
 
 
 def _q4(lib, **kw):
-    f = dict(dtype=0, scale_dtype=0, M=2, N=8, K=128, group=32, ldx=128, pitch=64, ldy=8, x=256, codes=256, scales=256,
-             zeros=0, y=256, ws=0, ws_bytes=0) | kw
-    return lib.tt_q4_matmul(struct.pack("=16q", *f.values()), None)
+    f = dict(dtype=0, scale_dtype=0, M=2, N=8, K=128, group=32, ldx=128, ldy=8, x=256, codes=256, scales=256, zeros=0, y=256,
+             ws=0, ws_bytes=0) | kw
+    return lib.tt_q4_matmul(struct.pack("=15q", *f.values()), None)
 
 
 def test_c_q4_refusals(lib):
     assert lib.tt_q4_matmul(None, None) == _lib.TT_INVALID
-    for kw in (dict(M=-1), dict(K=-1), dict(group=33), dict(group=16), dict(group=192), dict(ldx=127), dict(ldy=7), dict(pitch=63),
-               dict(pitch=0), dict(codes=257), dict(x=0), dict(codes=0), dict(scales=0), dict(y=0)):
+    for kw in (dict(M=-1), dict(K=-1), dict(group=33), dict(group=16), dict(group=192), dict(ldx=127), dict(ldy=7), dict(codes=257),
+               dict(scales=264), dict(zeros=8), dict(N=-1), dict(K=0), dict(x=0), dict(codes=0), dict(scales=0), dict(y=0)):
         assert _q4(lib, **kw) == _lib.TT_INVALID, kw
         assert lib.tt_last_error().startswith(b"tt_q4_matmul")
     for kw in (dict(dtype=1), dict(scale_dtype=1), dict(dtype=9)):
         assert _q4(lib, **kw) == _lib.TT_UNSUPPORTED, kw
     assert _q4(lib, M=0) == _lib.TT_OK and _q4(lib, N=0) == _lib.TT_OK
+
+
+def test_c_q4_pack_refusals(lib):
+    assert lib.tt_q4_packed_bytes(17, 129) == 2 * 2 * 1024 and lib.tt_q4_packed_bytes(0, 5) == 0
+    for args in ((-1, 8, 256, 4, 256), (4, 0, 256, 4, 256), (4, 8, 0, 4, 256), (4, 8, 256, 4, 0), (4, 9, 256, 4, 256),
+                 (4, 8, 256, 4, 264)):
+        assert lib.tt_q4_pack(*args, None) == _lib.TT_INVALID, args
+        assert lib.tt_last_error().startswith(b"tt_q4_pack")
+    assert lib.tt_q4_pack(1 << 31, 8, 256, 4, 256, None) == _lib.TT_UNSUPPORTED
+    assert lib.tt_q4_pack(0, 8, 0, 4, 0, None) == _lib.TT_OK
 
 
 def _append(lib, cache=None, **kw):

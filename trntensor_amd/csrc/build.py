@@ -5,8 +5,9 @@ Usage: python trntensor_amd/csrc/build.py [--jobs N] [--no-fastpath]
 Each source is compiled to an object with hipcc in parallel, then linked
 into ``trntensor_amd/_lib/libtrntensor_hip.so`` (in-tree, so it travels
 with the source tree). Packed-FP32 instruction selection is disabled for all
-device code. Then the host launch table (tt_fastpath.cpp, a torch C++
-extension) is built into ``trntensor_amd/_lib/fastpath/``.
+device code. Then the host launch table and the serving operators' host path
+(FASTPATH_SOURCES, a torch C++ extension) are built into
+``trntensor_amd/_lib/fastpath/``.
 """
 
 from __future__ import annotations
@@ -104,10 +105,11 @@ def build(jobs: int = 4, verbose: bool = False, extra: list[str] | None = None) 
 
 FASTPATH_DIR = os.path.join(OUT_DIR, "fastpath")
 FASTPATH = os.path.join(FASTPATH_DIR, "tt_fastpath.so")
+FASTPATH_SOURCES = ["tt_fastpath.cpp", "tt_serving_host.cpp"]
 
 
 def build_fastpath(verbose: bool = False) -> str:
-    """Compile tt_fastpath.cpp (host C++ against torch's headers, no device
+    """Compile FASTPATH_SOURCES (host C++ against torch's headers, no device
     code) into ``_lib/fastpath/tt_fastpath.so``, from scratch each time."""
     import torch.utils.cpp_extension as ce
 
@@ -118,7 +120,7 @@ def build_fastpath(verbose: bool = False) -> str:
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
     ce.load(
         "tt_fastpath",
-        [os.path.join(HERE, "tt_fastpath.cpp")],
+        [os.path.join(HERE, src) for src in FASTPATH_SOURCES],
         build_directory=FASTPATH_DIR,
         extra_cflags=["-O2", "-D__HIP_PLATFORM_AMD__", f"-I{rocm}/include", f"-I{os.path.join(os.path.dirname(PKG), 'include')}"],
         extra_ldflags=["-lc10_hip", f"-L{rocm}/lib", "-lamdhip64"],

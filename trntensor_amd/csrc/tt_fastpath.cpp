@@ -233,8 +233,11 @@ class LaunchTable {
 
 }  // namespace
 
+void bind_serving(py::module_& m);  // tt_serving_host.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-    m.doc() = "Launch table for repeated two-operand contractions (one GEMM launch each)";
+    m.doc() = "Launch table for repeated two-operand contractions (one GEMM launch each); the serving operators' host path";
+    bind_serving(m);
     py::class_<LaunchTable>(m, "LaunchTable")
         .def(py::init<int64_t, int64_t, int64_t, int64_t>(), py::arg("packed"), py::arg("last_error"),
              py::arg("status_string"), py::arg("max_entries"))

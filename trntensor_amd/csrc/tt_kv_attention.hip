@@ -556,48 +556,44 @@ template <typename T, int W>
 __global__ __launch_bounds__(256, (kWavesPerSimd<T, W, 1>)) void kv_attention_few_kernel(AttnParams p) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     Wave<T, W, 1> w;
-    if (p.direct) {
-        const int b = blockIdx.x / p.heads, kh = blockIdx.x - b * p.heads;
-        const Span sp = span_of(p, b, 0, 16);
-        if (sp.tiles > 0) {
-            w.load_q(p, b, kh, 0, sp, 0);
-            walk<T, W, 1>(p, w, sp, b, kh, wave, sp.tiles, 4);
-            join_waves<T, W>(p, w, sp, b, kh, 0, nullptr);
-            zero_rows<T, W>(p, b, kh, sp.live, 16);
-        } else {
-            zero_rows<T, W>(p, b, kh, 0, 16);
-        }
-        return;
-    }
-    const int64_t total = all_weights(p, p.batch).total, per = share_of(p, total);
-    const int64_t begin = blockIdx.x * per, stop = begin + per < total ? begin + per : total;
-    // Sequences that see nothing: their zeros, dealt out over the workgroups.
-    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-        const Span sp = span_of(p, b, 0, 16);
-        if (sp.tiles == 0 || sp.live < 16)
-            for (int kh = 0; kh < p.heads; ++kh) zero_rows<T, W>(p, b, kh, sp.tiles == 0 ? 0 : sp.live, 16);
-    }
-    if (begin >= stop) return;
-    // The sequence that `begin` lies in, and the place `at` of its first pair.
-    int64_t at = 0;
+    // This workgroup's places [pos, stop) of the list, and sequence b, whose first pair is at `at`.
+    int64_t pos, stop, at = 0;
     int b = 0;
-    for (int b0 = 0;; b0 += 64) {
-        const int64_t mine = b0 + lane < p.batch ? weight_of(p, b0 + lane) : 0;
-        int64_t upto = mine;
-        for (int off = 1; off < 64; off <<= 1) {
-            const int64_t v = __shfl_up(upto, off, 64);
-            upto += lane >= off ? v : 0;
+    if (p.direct) {
+        b = blockIdx.x / p.heads;
+        const Span sp = span_of(p, b, 0, 16);
+        const int kh = blockIdx.x - b * p.heads;
+        zero_rows<T, W>(p, b, kh, sp.tiles > 0 ? sp.live : 0, 16);
+        pos = (int64_t)kh * (sp.tiles + kPairCost);
+        stop = sp.tiles > 0 ? pos + sp.tiles + kPairCost : pos;
+    } else {
+        const int64_t total = all_weights(p, p.batch).total, per = share_of(p, total);
+        pos = blockIdx.x * per;
+        stop = pos + per < total ? pos + per : total;
+        // Rows that see nothing: their zeros, dealt out over the workgroups.
+        for (int i = blockIdx.x; i < p.batch; i += gridDim.x) {
+            const Span sp = span_of(p, i, 0, 16);
+            if (sp.tiles == 0 || sp.live < 16)
+                for (int kh = 0; kh < p.heads; ++kh) zero_rows<T, W>(p, i, kh, sp.tiles == 0 ? 0 : sp.live, 16);
         }
-        const uint64_t past = __ballot(at + upto > begin);
-        if (past) {
-            const int f = __builtin_ctzll(past);
-            b = b0 + f;
-            at += __shfl(upto - mine, f, 64);
-            break;
+        if (pos >= stop) return;
+        for (int b0 = 0;; b0 += 64) {
+            const int64_t mine = b0 + lane < p.batch ? weight_of(p, b0 + lane) : 0;
+            int64_t upto = mine;
+            for (int off = 1; off < 64; off <<= 1) {
+                const int64_t v = __shfl_up(upto, off, 64);
+                upto += lane >= off ? v : 0;
+            }
+            const uint64_t past = __ballot(at + upto > pos);
+            if (past) {
+                const int f = __builtin_ctzll(past);
+                b = b0 + f;
+                at += __shfl(upto - mine, f, 64);
+                break;
+            }
+            at += __shfl(upto, 63, 64);
         }
-        at += __shfl(upto, 63, 64);
     }
-    int64_t pos = begin;
     while (pos < stop) {
         const Span sp = span_of(p, b, 0, 16);
         const int64_t pair_weight = sp.tiles + kPairCost, size = sp.tiles > 0 ? pair_weight * p.heads : 0;

@@ -16,10 +16,8 @@ namespace tt {
 
 namespace {
 
-constexpr int KW = 8;  // wavefronts a workgroup
-
 struct Q4Params {
-    int64_t ldx, code_pitch, ldy;
+    int64_t ldx, ldy;
     const void *x, *scales, *zeros;
     const uint8_t* codes;
     void* y;
@@ -48,8 +46,7 @@ struct Act<float> {
     static constexpr int parts = 3;
 };
 
-// Eight codes of one word (code i in bits 4 i ..) as v = 1 + c / 16, in the
-// order 0 4 1 5 2 6 3 7.
+// The eight codes of a packed word as v = 1 + c / 16, in their columns' order.
 __device__ __forceinline__ u32x4 widen_codes(uint32_t w, __bf16) {
     u32x4 r;
     r[0] = ((w << 3) & 0x00780078u) | 0x3f803f80u;
@@ -69,35 +66,18 @@ __device__ __forceinline__ u32x4 widen_codes(uint32_t w, _Float16) {
 __device__ __forceinline__ uint32_t one_pair(__bf16) { return 0x3f803f80u; }
 __device__ __forceinline__ uint32_t one_pair(_Float16) { return 0x3c003c00u; }
 
-// Eight 16-bit values in the codes' order.
-__device__ __forceinline__ u32x4 code_order(u32x4 x) {
-    u32x4 r;
-    r[0] = __builtin_amdgcn_perm(x[2], x[0], 0x05040100u);
-    r[1] = __builtin_amdgcn_perm(x[2], x[0], 0x07060302u);
-    r[2] = __builtin_amdgcn_perm(x[3], x[1], 0x05040100u);
-    r[3] = __builtin_amdgcn_perm(x[3], x[1], 0x07060302u);
-    return r;
-}
-
-// Exchanges word i of lane group j with word j of lane group i (groups of 16
-// lanes): a lane that read 16 bytes of a row then holds, word by word, its part
-// of four runs of 32 columns instead of one run of its own.
-__device__ __forceinline__ u32x4 swap_words(u32x4 x) {
-    auto a = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
-    auto b = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
-    auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
-    auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
-    return u32x4{c[0], c[1], d[0], d[1]};
-}
-
 // Scales or zero points of four neighbouring rows, as stored (SW bytes each).
 template <int SW>
 struct Four {
     uint32_t raw[SW];
-    __device__ __forceinline__ float get(int i, bool bf16) const {
-        if constexpr (SW == 4) return __uint_as_float(raw[i]);
-        const uint32_t h = i & 1 ? raw[i / 2] >> 16 : raw[i / 2] & 0xffffu;
-        return bf16 ? __uint_as_float(h << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+    __device__ __forceinline__ f32x4 get(bool bf16) const {
+        if constexpr (SW == 4)
+            return f32x4{__uint_as_float(raw[0]), __uint_as_float(raw[1]), __uint_as_float(raw[2]), __uint_as_float(raw[3])};
+        if (bf16)
+            return f32x4{__uint_as_float(raw[0] << 16), __uint_as_float(raw[0] & 0xffff0000u), __uint_as_float(raw[1] << 16),
+                         __uint_as_float(raw[1] & 0xffff0000u)};
+        const f16x2 a = __builtin_bit_cast(f16x2, raw[0]), b = __builtin_bit_cast(f16x2, raw[1]);
+        return f32x4{(float)a[0], (float)a[1], (float)b[0], (float)b[1]};
     }
 };
 
@@ -114,8 +94,8 @@ struct Stage {
 // wavefronts of a workgroup take contiguous shares of the columns, which are
 // summed at the end in their order. GPC: the pieces of a chunk of 128 columns
 // that are scaled one by one, 1 for groups of at least a chunk, else 4.
-template <typename T, int SW, int U, int R, int MT, int GPC>
-__global__ __launch_bounds__(64 * KW, 2) void q4_matmul_kernel(Q4Params p) {
+template <typename T, int SW, int U, int R, int MT, int GPC, int KW>
+__global__ __launch_bounds__(64 * KW, KW / 4 < 2 ? 2 : KW / 4) void q4_matmul_kernel(Q4Params p) {
     typedef typename Act<T>::half H;
     constexpr int NP = Act<T>::parts;
     constexpr int kSteps = 4 / GPC;  // MFMA steps of 32 columns a piece
@@ -138,12 +118,13 @@ __global__ __launch_bounds__(64 * KW, 2) void q4_matmul_kernel(Q4Params p) {
     const int per = (p.chunks + KW - 1) / KW;
     const int first = wave * per, last = first + per < p.chunks ? first + per : p.chunks;
 
-    // Rows past the end repeat the last one: what they give is not stored.
+    // Rows past the end repeat the last ones: what they give is not stored.
+    const int tiles = (p.N + 15) / 16;
     const uint8_t* code_row[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int n = n0 + r * 16 + c;
-        code_row[r] = p.codes + (int64_t)(n < p.N ? n : p.N - 1) * p.code_pitch + g * 16;
+        const int t = rb * R + r;
+        code_row[r] = p.codes + (int64_t)(t < tiles ? t : tiles - 1) * p.chunks * 1024 + lane * 16;
     }
     const T* x_row[MT];
 #pragma unroll
@@ -179,7 +160,7 @@ __global__ __launch_bounds__(64 * KW, 2) void q4_matmul_kernel(Q4Params p) {
         for (int u = 0; u < U; ++u) {
             const int k = chunk + u < last ? chunk + u : last - 1;
 #pragma unroll
-            for (int r = 0; r < R; ++r) st.codes[u][r] = *reinterpret_cast<const u32x4*>(code_row[r] + (int64_t)k * 64);
+            for (int r = 0; r < R; ++r) st.codes[u][r] = *reinterpret_cast<const u32x4*>(code_row[r] + (int64_t)k * 1024);
             const bool edge = ragged && k == p.chunks - 1;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
@@ -215,9 +196,6 @@ __global__ __launch_bounds__(64 * KW, 2) void q4_matmul_kernel(Q4Params p) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (chunk + u >= last) break;
-            u32x4 w[R];
-#pragma unroll
-            for (int r = 0; r < R; ++r) w[r] = swap_words(st.codes[u][r]);
 #pragma unroll
             for (int q = 0; q < GPC; ++q) {
                 f32x4 sum[R][MT], total[MT];
@@ -234,19 +212,16 @@ __global__ __launch_bounds__(64 * KW, 2) void q4_matmul_kernel(Q4Params p) {
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) {
                         if constexpr (NP == 1) {
-                            b[mt][0] = code_order(__builtin_bit_cast(u32x4, st.x[u][mt][s]));
+                            b[mt][0] = __builtin_bit_cast(u32x4, st.x[u][mt][s]);
                         } else {
-                            u32x4 part[NP];
-                            split8<NP>(st.x[u][mt][s], part);
-#pragma unroll
-                            for (int i = 0; i < NP; ++i) b[mt][i] = code_order(part[i]);
+                            split8<NP>(st.x[u][mt][s], b[mt]);
                         }
 #pragma unroll
                         for (int i = 0; i < NP; ++i) total[mt] = q4_mma(one, b[mt][i], total[mt], H());
                     }
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
-                        const u32x4 a = widen_codes(w[r][s], H());
+                        const u32x4 a = widen_codes(st.codes[u][r][s], H());
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -254,14 +229,13 @@ __global__ __launch_bounds__(64 * KW, 2) void q4_matmul_kernel(Q4Params p) {
                     }
                 }
 #pragma unroll
-                for (int r = 0; r < R; ++r)
+                for (int r = 0; r < R; ++r) {
+                    const f32x4 scale = st.scales[u][r][q].get(bf16) * 16.f;
+                    f32x4 off = {1.5f, 1.5f, 1.5f, 1.5f};
+                    if (p.zeros) off = st.zeros[u][r][q].get(bf16) * 0.0625f + 1.f;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float sc = 16.f * st.scales[u][r][q].get(i, bf16);
-                        const float off = p.zeros ? 1.f + 0.0625f * st.zeros[u][r][q].get(i, bf16) : 1.5f;
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) out[r][mt][i] += sc * (sum[r][mt][i] - off * total[mt][i]);
-                    }
+                    for (int mt = 0; mt < MT; ++mt) out[r][mt] += scale * (sum[r][mt] - off * total[mt]);
+                }
             }
         }
     };
@@ -297,20 +271,33 @@ __global__ __launch_bounds__(64 * KW, 2) void q4_matmul_kernel(Q4Params p) {
     }
 }
 
-template <typename T, int SW, int U, int R, int MT, int GPC>
+template <typename T, int SW, int U, int R, int MT, int GPC, int KW>
 int q4_run(const Q4Params& p, hipStream_t st) {
     const int64_t grid = (int64_t)((p.N + 16 * R - 1) / (16 * R)) * ((p.M + 16 * MT - 1) / (16 * MT));
-    if (grid > kMaxGrid / 2) return set_error(TT_UNSUPPORTED, "tt_q4_matmul: %lld workgroups", (long long)grid);
-    q4_matmul_kernel<T, SW, U, R, MT, GPC><<<(uint32_t)grid, 64 * KW, 0, st>>>(p);
+    if (grid > kMaxGrid / 4) return set_error(TT_UNSUPPORTED, "tt_q4_matmul: %lld workgroups", (long long)grid);
+    q4_matmul_kernel<T, SW, U, R, MT, GPC, KW><<<(uint32_t)grid, 64 * KW, 0, st>>>(p);
     return check_launch("tt_q4_matmul");
 }
 
 template <typename T, int SW, int GPC>
 int q4_shape(const Q4Params& p, hipStream_t st) {
+    // R weight tiles a wavefront read the same activations: fewer of their bytes
+    // a byte of codes, but fewer wavefronts. us for R = 1 / 2 / 4 (bfloat16,
+    // groups of 128): one row, 4096 x 4096 4.9 / 6.6 / 9.8, 8192 x 4096 7.4 /
+    // 8.5 / 11.2, 16384 x 8192 20.4 / 18.1 / 20.1; 16 rows, 16384 x 8192 36.9 /
+    // 24.5 / 22.7; 32 rows, 4096 x 4096 11.2 / 12.5 / 15.9, 16384 x 8192 69.9 /
+    // 41.9 / 31.2. Four or sixteen wavefronts a workgroup, or two chunks a
+    // stage, were slower at all of these or level.
     constexpr bool kWide = sizeof(T) == 4;  // three parts an activation: no room for two blocks of rows
-    if (p.N <= 8192 && (p.M <= 16 || kWide)) return q4_run<T, SW, kWide ? 1 : 2, 1, 1, GPC>(p, st);
-    if (p.M <= 16 || kWide) return q4_run<T, SW, 1, 2, 1, GPC>(p, st);
-    if constexpr (!kWide) return q4_run<T, SW, 1, 2, 2, GPC>(p, st);
+    const int tiles = (p.N + 15) / 16;
+    if (p.M <= 16 || kWide) {
+        if (tiles <= 512) return q4_run<T, SW, 1, 1, 1, GPC, 8>(p, st);
+        return q4_run<T, SW, 1, 2, 1, GPC, 8>(p, st);
+    }
+    if constexpr (!kWide) {
+        if (tiles <= 256) return q4_run<T, SW, 1, 1, 2, GPC, 8>(p, st);
+        return q4_run<T, SW, 1, GPC == 1 ? 4 : 2, 2, GPC, 8>(p, st);
+    }
     return TT_OK;
 }
 
@@ -320,8 +307,62 @@ int q4_typed(int64_t scale_dtype, const Q4Params& p, bool small_groups, hipStrea
     return small_groups ? q4_shape<T, 2, 4>(p, st) : q4_shape<T, 2, 1>(p, st);
 }
 
+// One thread a lane's 16 bytes of a tile.
+__global__ __launch_bounds__(256) void q4_pack_kernel(int N, int K, int chunks, const uint8_t* codes, int64_t pitch,
+                                                      u32x4* out, int64_t count) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= count) return;
+    const int lane = i & 63;
+    const int64_t tile = i >> 6;
+    const int chunk = (int)(tile % chunks);
+    const int64_t n = tile / chunks * 16 + (lane & 15);
+    const int bytes = (K + 1) / 2;
+    u32x4 w;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        const int at = chunk * 64 + s * 16 + (lane >> 4) * 4;
+        uint32_t x = 0;
+        if (n < N) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (at + j < bytes) x |= (uint32_t)codes[n * pitch + at + j] << 8 * j;
+        }
+        uint32_t even = x & 0x0f0f0f0fu, odd = x >> 4 & 0x0f0f0f0fu;
+        even = (even | even >> 4) & 0x00ff00ffu;
+        odd = (odd | odd >> 4) & 0x00ff00ffu;
+        w[s] = ((even | even >> 8) & 0xffffu) | (odd | odd >> 8) << 16;
+    }
+    out[i] = w;
+}
+
+int check_q4_size(const char* who, int64_t N, int64_t K) {
+    constexpr int64_t kMost = int64_t(1) << 30;
+    if (N < 0 || K < 1) return set_error(TT_INVALID, "%s: %lld rows of %lld columns", who, (long long)N, (long long)K);
+    if (N > kMost || K > kMost) return set_error(TT_UNSUPPORTED, "%s: extents beyond 2^30", who);
+    return TT_OK;
+}
+
 }  // namespace
 }  // namespace tt
+
+extern "C" size_t tt_q4_packed_bytes(int64_t N, int64_t K) {
+    if (N < 1 || K < 1) return 0;
+    return (size_t)((N + 15) / 16) * (size_t)((K + 127) / 128) * 1024;
+}
+
+extern "C" int tt_q4_pack(int64_t N, int64_t K, const void* codes, int64_t pitch, void* packed, void* stream) {
+    using namespace tt;
+    if (int rc = check_q4_size("tt_q4_pack", N, K)) return rc;
+    if (N == 0) return TT_OK;
+    if (!codes || !packed) return set_error(TT_INVALID, "tt_q4_pack: NULL pointer");
+    if (pitch < (K + 1) / 2 || (uintptr_t)packed % 16)
+        return set_error(TT_INVALID, "tt_q4_pack: pitch %lld, or alignment", (long long)pitch);
+    const int64_t count = (int64_t)(tt_q4_packed_bytes(N, K) / 16), blocks = (count + 255) / 256;
+    if (blocks > kMaxGrid) return set_error(TT_UNSUPPORTED, "tt_q4_pack: %lld by %lld codes", (long long)N, (long long)K);
+    q4_pack_kernel<<<(uint32_t)blocks, 256, 0, static_cast<hipStream_t>(stream)>>>(
+        (int)N, (int)K, (int)((K + 127) / 128), static_cast<const uint8_t*>(codes), pitch, static_cast<u32x4*>(packed), count);
+    return check_launch("tt_q4_pack");
+}
 
 extern "C" size_t tt_q4_matmul_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
     (void)dtype, (void)M, (void)N, (void)K;
@@ -334,22 +375,18 @@ extern "C" int tt_q4_matmul(const tt_q4_args* a, void* stream) {
     if (!serving_dtype(a->dtype) || !serving_dtype(a->scale_dtype))
         return set_error(TT_UNSUPPORTED, "tt_q4_matmul: dtypes %lld, %lld (TT_F32, TT_BF16, TT_F16)",
                          (long long)a->dtype, (long long)a->scale_dtype);
-    if (a->M < 0 || a->N < 0 || a->K < 1)
-        return set_error(TT_INVALID, "tt_q4_matmul: extents %lld, %lld, %lld", (long long)a->M, (long long)a->N,
-                         (long long)a->K);
+    if (int rc = check_q4_size("tt_q4_matmul", a->N, a->K)) return rc;
+    if (a->M < 0) return set_error(TT_INVALID, "tt_q4_matmul: %lld rows", (long long)a->M);
+    if (a->M > int64_t(1) << 30) return set_error(TT_UNSUPPORTED, "tt_q4_matmul: extents beyond 2^30");
     if (a->group != 32 && a->group != 64 && (a->group < 128 || a->group % 128))
         return set_error(TT_INVALID, "tt_q4_matmul: group of %lld (32, 64 or a multiple of 128)", (long long)a->group);
     if (a->M == 0 || a->N == 0) return TT_OK;
     if (!a->y || !a->x || !a->codes || !a->scales) return set_error(TT_INVALID, "tt_q4_matmul: NULL pointer");
     if (a->ldx < a->K || a->ldy < a->N) return set_error(TT_INVALID, "tt_q4_matmul: leading dimension below the width");
-    if (a->code_pitch % 64 || a->code_pitch < (a->K + 1) / 2 || (uintptr_t)a->codes % 16)
-        return set_error(TT_INVALID, "tt_q4_matmul: code pitch %lld or alignment", (long long)a->code_pitch);
-    constexpr int64_t kMost = int64_t(1) << 30;
-    if (a->M > kMost || a->N > kMost || a->K > kMost)
-        return set_error(TT_UNSUPPORTED, "tt_q4_matmul: extents beyond 2^30");
+    if (((uintptr_t)a->codes | (uintptr_t)a->scales | (uintptr_t)a->zeros) % 16)
+        return set_error(TT_INVALID, "tt_q4_matmul: weights are not 16-byte aligned");
     Q4Params p;
     p.ldx = a->ldx;
-    p.code_pitch = a->code_pitch;
     p.ldy = a->ldy;
     p.x = a->x;
     p.scales = a->scales;

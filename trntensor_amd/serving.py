@@ -28,13 +28,13 @@ import struct
 
 import torch
 
-from .hip import _lib, dispatch, engine
+from .hip import _fastpath, _lib, dispatch, engine
 
 _CODES = {torch.float32: _lib.TT_F32, torch.bfloat16: _lib.TT_BF16, torch.float16: _lib.TT_F16}
 FP8 = torch.float8_e4m3fn
 
 # The argument structs of include/trntensor_hip.h, eight bytes a field.
-_Q4_ARGS = struct.Struct("=16q")
+_Q4_ARGS = struct.Struct("=15q")
 _CACHE = struct.Struct("=8q")
 _APPEND_ARGS = struct.Struct("=26q")
 _ATTENTION_ARGS = struct.Struct("=11qd5q")
@@ -55,14 +55,14 @@ def _check_grad(what: str, *tensors) -> None:
                 raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or detach its operands")
 
 
-def _launch(name: str, device: torch.device, packed: bytes) -> None:
+def _launch(name: str, device: torch.device, *args) -> None:
     """One library call on torch's current stream of `device`."""
     fn = getattr(_lib.load(), name)
     if device.index == torch.cuda.current_device():
-        st = fn(packed, engine._stream_ptr(device))
+        st = fn(*args, engine._stream_ptr(device))
     else:
         with torch.cuda.device(device):
-            st = fn(packed, engine._stream_ptr(device))
+            st = fn(*args, engine._stream_ptr(device))
     if st:
         _lib.check(st, name)
 
@@ -80,13 +80,12 @@ class Q4Matrix:
     group_size)) in one of float32, bfloat16, float16; without ``zeros`` every
     zero point is 8. ``group_size`` is 32, 64 or a multiple of 128.
 
-    The weights are laid out once, here: scales with the output features
-    contiguous, and rows of codes padded to 64 bytes where they are no such
-    multiple (otherwise ``codes`` is kept as it is, not copied). They live on
-    ``codes``' device if that is a GPU, else on the current one.
+    The weights are laid out once, here, in copies on ``codes``' device (the
+    current GPU if that is the host): codes in the tiles that the matrix units
+    take, scales with the output features contiguous.
     """
 
-    __slots__ = ("codes", "scales", "zeros", "shape", "group_size", "device", "_code")
+    __slots__ = ("packed", "scales", "zeros", "shape", "group_size", "device", "_code", "_host")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, in_features: int, group_size: int,
                  zeros: torch.Tensor | None = None):
@@ -104,17 +103,17 @@ class Q4Matrix:
                 raise ValueError(f"{name} must be {scales.dtype} ({n}, {groups}); got {t.dtype} {tuple(t.shape)}")
         dispatch.require_hip()
         device = codes.device if codes.device.type == "cuda" else dispatch._device()
-        codes = codes.to(device)
-        pitch = -(-k // 128) * 64
-        if pitch != codes.shape[1] or not codes.is_contiguous() or codes.data_ptr() % 16:
-            laid = torch.zeros((n, pitch), dtype=torch.uint8, device=device)
-            laid[:, : codes.shape[1]] = codes
-            codes = laid
-        self.codes = codes
+        codes = codes.to(device).contiguous()
+        lib = _lib.load()
+        self.packed = torch.empty(lib.tt_q4_packed_bytes(n, k), dtype=torch.uint8, device=device)
+        _launch("tt_q4_pack", device, n, k, codes.data_ptr(), codes.shape[1], self.packed.data_ptr())
         self.scales, self.zeros = (None if t is None else self._by_group(t.detach().to(device)) for t in (scales, zeros))
         self.shape = (n, k)
         self.group_size = int(group_size)
         self.device = device
+        host = _fastpath.module()
+        self._host = None if host is None else host.Q4Host(_fastpath.serving_entries(), self.packed, self.scales, self.zeros,
+                                                           n, k, self.group_size, self._code)
 
     @staticmethod
     def _by_group(t: torch.Tensor) -> torch.Tensor:
@@ -135,6 +134,10 @@ def q4_matmul(x: torch.Tensor, w: Q4Matrix) -> torch.Tensor:
     and the result is rounded once to x's dtype. Rows of x need a unit stride
     and one row pitch, else they are copied.
     """
+    if w._host is not None and dispatch._use_hip() and isinstance(x, torch.Tensor):
+        y = w._host.run(x)
+        if y is not None:
+            return y
     n, k = w.shape
     if x.dim() < 1 or x.shape[-1] != k:
         raise ValueError(f"x must be (..., {k}); got {tuple(x.shape)}")
@@ -155,8 +158,8 @@ def q4_matmul(x: torch.Tensor, w: Q4Matrix) -> torch.Tensor:
     need = _lib.load().tt_q4_matmul_workspace_bytes(code, m, n, k)
     ws = torch.empty(need, dtype=torch.uint8, device=w.device) if need else None
     _launch("tt_q4_matmul", w.device, _Q4_ARGS.pack(
-        code, w._code, m, n, k, w.group_size, max(x2.stride(0), k), w.codes.shape[1], n, x2.data_ptr(),
-        w.codes.data_ptr(), w.scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(), y.data_ptr(),
+        code, w._code, m, n, k, w.group_size, max(x2.stride(0), k), n, x2.data_ptr(), w.packed.data_ptr(),
+        w.scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(), y.data_ptr(),
         0 if ws is None else ws.data_ptr(), need))
     return y if home == w.device else y.to(home)
 
@@ -177,7 +180,8 @@ class KVCache:
     business: calls take a page table.
     """
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "head_dim", "page_size", "num_pages", "num_heads", "device", "_packed")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "head_dim", "page_size", "num_pages", "num_heads", "device", "_packed",
+                 "_scale", "_host")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, head_dim: int):
         if k.dim() != 4:
@@ -203,8 +207,12 @@ class KVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.head_dim, self.page_size, self.num_pages, self.num_heads = int(head_dim), page, pages, heads
         self.device = k.device
+        self._scale = 1.0 / math.sqrt(self.head_dim)
         self._packed = _CACHE.pack(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, heads, page,
                                    self.head_dim)
+        host = _fastpath.module()
+        self._host = None if host is None else host.CacheHost(_fastpath.serving_entries(), k, v, k_scale, v_scale,
+                                                              self.head_dim)
 
     @classmethod
     def empty(cls, num_pages: int, num_heads: int, head_dim: int, page_size: int = 64,
@@ -300,6 +308,10 @@ def kv_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table: torc
     table's end, or whose page number is none of the cache's, are dropped. A
     page that is written to must belong to one sequence.
     """
+    if cache._host is not None and dispatch._use_hip():
+        done, out = cache._host.append(k, v, page_table, lengths, counts, q, cos, sin, interleaved)
+        if done:
+            return out
     if k.dim() != 4:
         raise ValueError(f"k must be 4D (batch, tokens, heads, head_dim); got shape {tuple(k.shape)}")
     batch, tokens = k.shape[0], k.shape[1]
@@ -360,6 +372,11 @@ def kv_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, leng
     rows past their count) give zeros. No masked slot has any influence,
     whatever its page holds.
     """
+    if cache._host is not None and dispatch._use_hip():
+        out = cache._host.attention(q, page_table, lengths, counts, cache._scale if scale is None else scale,
+                                    0 if window is None else window or -1, sinks)
+        if out is not None:
+            return out
     if q.dim() != 4:
         raise ValueError(f"q must be 4D (batch, tokens, heads, head_dim); got shape {tuple(q.shape)}")
     batch, tokens, heads, dim = q.shape
@@ -379,7 +396,7 @@ def kv_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, leng
     if batch and tokens:
         sq = q.stride()
         head = (code, batch, tokens, heads, window or 0, sinks, table.shape[1], table.stride(0), sq[0], sq[1], sq[2],
-                1.0 / math.sqrt(dim) if scale is None else float(scale), q.data_ptr(), out.data_ptr(), table.data_ptr(),
+                cache._scale if scale is None else float(scale), q.data_ptr(), out.data_ptr(), table.data_ptr(),
                 lengths.data_ptr(), 0 if counts is None else counts.data_ptr())
         packed = _ATTENTION_ARGS.pack(*head) + cache._packed
         need = _lib.load().tt_kv_attention_workspace_bytes(packed + _WORKSPACE.pack(0, 0))
