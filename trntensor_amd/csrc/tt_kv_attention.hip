@@ -20,7 +20,7 @@ struct AttnParams {
     const float *k_scale, *v_scale;
     float* part;  // partial results: slots of rows * (width + 2) floats
     int64_t q_stride[3], table_stride, pages;
-    int batch, tokens, q_heads, heads, share, page, dim, window, sinks;
+    int batch, tokens, q_heads, heads, share, page, dim, window, sinks, table_width;
     int capacity;    // tokens that the table covers
     int row_blocks;  // blocks of query rows of one cache head
     int groups;      // workgroups that share the key tiles
@@ -36,6 +36,8 @@ constexpr int kPairCost = 4;  // what starting and joining a pair costs, in tile
 // Which keys the query rows of one block see: those of [0, end) that are in a
 // row's window or among the sinks lie in tiles [0, sink_tiles) and [start, ..).
 struct Span {
+    int64_t base;              // position of the sequence's first query
+    int tokens;                // its queries
     int first_pos, last_pos;   // positions of the block's live rows
     int held;                  // tokens that exist
     int sink_tiles, start, tiles;
@@ -43,17 +45,17 @@ struct Span {
 };
 
 __device__ __forceinline__ Span span_of(const AttnParams& p, int b, int row0, int rows) {
-    Span s = {0, -1, 0, 0, 0, 0, 0};
+    Span s = {0, 0, 0, -1, 0, 0, 0, 0, 0};
     const int len = p.lengths[b];
     const int n = p.counts ? p.counts[b] : p.tokens;
-    const int live_tokens = n < p.tokens ? n : p.tokens;
-    if (live_tokens <= 0 || len <= 0) return s;
-    const int64_t all = (int64_t)live_tokens * p.share;
+    s.tokens = n < p.tokens ? n : p.tokens;
+    if (s.tokens <= 0 || len <= 0) return s;
+    const int64_t all = (int64_t)s.tokens * p.share;
     s.live = all > row0 ? (int)(all - row0 < rows ? all - row0 : rows) : 0;
     if (s.live <= 0) return s;
     s.held = len < p.capacity ? len : p.capacity;
-    const int64_t base = (int64_t)len - n;
-    const int64_t first = base + (int)fdiv(row0, p.by_share), last = base + (int)fdiv(row0 + s.live - 1, p.by_share);
+    s.base = (int64_t)len - n;
+    const int64_t first = s.base + (int)fdiv(row0, p.by_share), last = s.base + (int)fdiv(row0 + s.live - 1, p.by_share);
     if (last < 0) return s;
     s.first_pos = first < -1 ? -1 : (int)first;
     s.last_pos = (int)last;
@@ -139,6 +141,19 @@ __device__ __forceinline__ float column_sum(float x) {
 // probabilities pass from one product to the next in their registers, and a
 // run lies in one page (pages are multiples of 16), so that a lane needs one
 // scale. Keys are read as 16 bytes along d, two products' worth.
+//
+// What starting and joining a pair compute from the lane and the head size is
+// hidden from the compiler (fresh): it would keep the addresses and masks that
+// follow, hundreds of registers of them, across the tiles' loop.
+__device__ __forceinline__ int fresh(int uniform) {
+    asm volatile("" : "+s"(uniform));
+    return uniform;
+}
+__device__ __forceinline__ int fresh_lane(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 template <typename T, int W, int MT>
 struct Wave {
     static constexpr int QP = Parts<T>::q, PP = Parts<T>::p;
@@ -146,46 +161,59 @@ struct Wave {
     u32x4 q[MT][QP][W / 32];
     f32x4 o[MT][W / 16];
     float m[MT], l[MT];
-    bool any[MT];
+    uint32_t any[MT];      // not 0 once the row has seen a key
     int end[MT], low[MT];  // this lane's query row sees keys of [0, end) that are >= low or < sinks
 
-    __device__ __forceinline__ void load_q(const AttnParams& p, int b, int kh, int row0, const Span& sp, int base) {
-        const int c = threadIdx.x & 15, h = (threadIdx.x & 63) >> 4;
-        const int len = p.lengths[b], n = p.counts ? p.counts[b] : p.tokens;
-        const int limit = (n < p.tokens ? n : p.tokens);
+    // Rows from row0 on, of which `sp` (the span of them) has the live ones.
+    __device__ __forceinline__ void load_q(const AttnParams& p, int b, int kh, int row0, const Span& sp) {
+        const int lane = fresh_lane(threadIdx.x & 63), c = lane & 15, h = lane >> 4;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            const int row = row0 + mt * 16 + c;
+            const bool live = mt * 16 + c < sp.live;
+            // Rows past the end repeat the first: what they give is not stored.
+            const int row = live ? row0 + mt * 16 + c : 0;
             const int t = (int)fdiv(row, p.by_share), g = row - t * p.share;
-            const bool live = t < limit && row - base < sp.live;
-            const int64_t pos = (int64_t)len - n + t;
+            const int64_t pos = sp.base + t;
             end[mt] = live && pos >= 0 ? (pos + 1 < sp.held ? (int)pos + 1 : sp.held) : 0;
             const int64_t lo = p.window > 0 ? pos - p.window + 1 : 0;
             low[mt] = lo > 0 ? (int)lo : 0;
             m[mt] = -INFINITY;
             l[mt] = 0.f;
-            any[mt] = false;
+            any[mt] = 0;
 #pragma unroll
             for (int d = 0; d < W / 16; ++d) o[mt][d] = f32x4{0, 0, 0, 0};
-            const T* src = static_cast<const T*>(p.q) + b * p.q_stride[0] + (int64_t)(live ? t : 0) * p.q_stride[1] +
-                           (int64_t)(kh * p.share + (live ? g : 0)) * p.q_stride[2];
+            const T* src = static_cast<const T*>(p.q) + b * p.q_stride[0] + (int64_t)t * p.q_stride[1] +
+                           (int64_t)(kh * p.share + g) * p.q_stride[2];
+            T x[W / 32][8];
+            const int dim = fresh(p.dim);
+            if (dim % 8 == 0) {
+#pragma unroll
+                for (int s = 0; s < W / 32; ++s) {
+                    const int d0 = s / 2 * 64 + h * 16 + (s & 1) * 8;
+                    __builtin_memcpy(x[s], src + (d0 < dim ? d0 : 0), sizeof x[s]);
+                    if (d0 >= dim)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x[s][i] = (T)0.f;
+                }
+            } else {
+#pragma unroll
+                for (int s = 0; s < W / 32; ++s)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int d = s / 2 * 64 + h * 16 + (s & 1) * 8 + i;
+                        const T v = src[d < dim ? d : 0];
+                        x[s][i] = d < dim ? v : (T)0.f;
+                    }
+            }
 #pragma unroll
             for (int s = 0; s < W / 32; ++s) {
-                const int d0 = s / 2 * 64 + h * 16 + (s & 1) * 8;
-                T x[8];
-                if (live && d0 + 8 <= p.dim) {
-                    __builtin_memcpy(x, src + d0, sizeof x);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = live && d0 + i < p.dim ? src[d0 + i] : (T)0.f;
-                }
                 if constexpr (QP == 1) {
-                    q[mt][0][s] = __builtin_bit_cast(u32x4, x);
+                    q[mt][0][s] = __builtin_bit_cast(u32x4, x[s]);
                 } else {
                     u32x4 parts[QP];
-                    split8<QP>(x, parts);
+                    split8<QP>(x[s], parts);
 #pragma unroll
-                    for (int n2 = 0; n2 < QP; ++n2) q[mt][n2][s] = parts[n2];
+                    for (int n = 0; n < QP; ++n) q[mt][n][s] = parts[n];
                 }
             }
         }
@@ -200,30 +228,36 @@ struct Runs {
     bool v_ok;
 };
 
-template <typename T, int W, int MT>
-__device__ __forceinline__ Runs find_runs(const AttnParams& p, const int32_t* table, int tile, int held) {
+__device__ __forceinline__ Runs find_runs(const AttnParams& p, const int32_t* table, int tile) {
     const int lane = threadIdx.x & 63;
     Runs r;
     const int k_at = tile * kTile + ((lane & 15) >> 2) * 16, v_at = tile * kTile + (lane >> 4) * 16;
     const int kp = (int)fdiv(k_at, p.by_page), vp = (int)fdiv(v_at, p.by_page);
     r.k_slot = k_at - kp * p.page;
     r.v_slot = v_at - vp * p.page;
-    r.k_page = k_at < held ? table[kp] : -1;
-    r.v_page = v_at < held ? table[vp] : -1;
-    r.v_ok = r.v_page >= 0 && r.v_page < p.pages;
-    // What lies in no page is read from page 0 and masked.
-    if (r.k_page < 0 || r.k_page >= p.pages) r.k_page = 0;
-    if (!r.v_ok) r.v_page = 0;
+    r.k_page = table[kp < p.table_width ? kp : p.table_width - 1];
+    r.v_page = table[vp < p.table_width ? vp : p.table_width - 1];
     return r;
 }
 
-template <typename T, int W, int MT>
+// What lies past the sequence's end or in no page is read from page 0 and masked.
+__device__ __forceinline__ void settle_runs(const AttnParams& p, Runs& r, int tile, int held) {
+    const int lane = threadIdx.x & 63;
+    r.v_ok = r.v_page >= 0 && r.v_page < p.pages && tile * kTile + (lane >> 4) * 16 < held;
+    if (r.k_page < 0 || r.k_page >= p.pages) r.k_page = 0;
+    if (!r.v_ok) r.v_page = 0;
+}
+
+struct Scales {
+    float k, v;
+    bool ok;
+};
+
+template <int W>
 struct Tile {
     u32x4 k[4][W / 64], v[W / 16];
-    float k_scale, v_scale;
-    bool ok;
 
-    __device__ __forceinline__ void load_k(const AttnParams& p, const Runs& r, int kh) {
+    __device__ __forceinline__ Scales load_k(const AttnParams& p, const Runs& r, int kh) {
         const int lane = threadIdx.x & 63;
         const uint8_t* src =
             p.k + ((r.k_page * p.heads + kh) * p.page + r.k_slot + (lane & 3)) * W + (lane >> 4) * 16;
@@ -231,23 +265,23 @@ struct Tile {
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int c = 0; c < W / 64; ++c) k[t][c] = *reinterpret_cast<const u32x4*>(src + t * 4 * W + c * 64);
-        ok = r.v_ok;
         const int64_t at = r.v_page * p.heads + kh;
-        k_scale = ok ? p.k_scale[at] : 0.f;
-        v_scale = ok ? p.v_scale[at] : 0.f;
+        return {r.v_ok ? p.k_scale[at] : 0.f, r.v_ok ? p.v_scale[at] : 0.f, r.v_ok};
     }
     __device__ __forceinline__ void load_v(const AttnParams& p, const Runs& r, int kh) {
         const int lane = threadIdx.x & 63;
         const uint8_t* src = p.v + ((r.v_page * p.heads + kh) * W + (lane & 15)) * p.page + r.v_slot;
 #pragma unroll
-        for (int d = 0; d < W / 16; ++d) v[d] = *reinterpret_cast<const u32x4*>(src + (int64_t)d * 16 * p.page);
+        for (int d = 0; d < W / 16; ++d) {
+            v[d] = *reinterpret_cast<const u32x4*>(src);
+            src += 16 * p.page;
+        }
     }
 };
 
-// Scores of one tile, and its keys' weights folded into the running state.
-// `full`: every live row sees every key.
+// Products of one tile's keys with the queries.
 template <typename T, int W, int MT>
-__device__ __forceinline__ void tile_scores(Wave<T, W, MT>& w, const Tile<T, W, MT>& x, f32x4 (&s)[MT][4]) {
+__device__ __forceinline__ void tile_scores(Wave<T, W, MT>& w, const Tile<W>& x, f32x4 (&s)[MT][4]) {
     typedef Wave<T, W, MT> WV;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -272,36 +306,102 @@ __device__ __forceinline__ void tile_scores(Wave<T, W, MT>& w, const Tile<T, W, 
             }
 }
 
+// Bit i: i < n.
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 16 ? 0xffffu : (1u << n) - 1; }
+
+// Four bits as the low bits of four bytes.
+__device__ __forceinline__ uint32_t bits_to_bytes(uint32_t m) { return (m & 15u) * 0x00204081u & 0x01010101u; }
+
+// Bytes that are NaN codes, as 1.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t v) { return ((v & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u; }
+
+// A tile that some row does not see whole: bit i of mask[mt] says whether this
+// lane's row sees key i of its run. Values of keys that no row of the wavefront
+// sees may be anything, so zeros are put in their place. NaN among the others
+// belongs only to the rows that see it: its elements are found, zeroed, and
+// their rows' output set to NaN through a product of their places with `mask`.
 template <typename T, int W, int MT>
-__device__ __forceinline__ void tile_fold(const AttnParams& p, Wave<T, W, MT>& w, Tile<T, W, MT>& x, f32x4 (&s)[MT][4],
-                                          int tile, bool full) {
+__device__ __forceinline__ void clear_values(Wave<T, W, MT>& w, Tile<W>& x, const uint32_t (&mask)[MT]) {
+    uint32_t some = mask[0];
+#pragma unroll
+    for (int mt = 1; mt < MT; ++mt) some |= mask[mt];
+    some |= __builtin_amdgcn_mov_dpp(some, 0x128, 0xf, 0xf, true);  // row_ror: over the 16 columns
+    some |= __builtin_amdgcn_mov_dpp(some, 0x124, 0xf, 0xf, true);
+    some |= __builtin_amdgcn_mov_dpp(some, 0x122, 0xf, 0xf, true);
+    some |= __builtin_amdgcn_mov_dpp(some, 0x121, 0xf, 0xf, true);
+    uint32_t keep[4], nan = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) keep[i] = bits_to_bytes(some >> 4 * i) * 0xffu;
+#pragma unroll
+    for (int d = 0; d < W / 16; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x.v[d][i] &= keep[i];
+            nan |= nan_bytes(x.v[d][i]);
+        }
+    if (!__any(nan != 0)) return;
+    u32x4 seen[MT][2];  // 1.0 where the row sees the key
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            seen[mt][i / 4][i % 4] = (mask[mt] >> 2 * i & 1 ? 0x3f80u : 0u) | (mask[mt] >> 2 * i & 2 ? 0x3f800000u : 0u);
+#pragma unroll
+    for (int d = 0; d < W / 16; ++d) {
+        u32x4 flag;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t at = nan_bytes(x.v[d][i]);
+            flag[i] = at * 0x38u;  // the code of 1.0
+            x.v[d][i] &= ~(at * 0xffu);
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            f32x4 hit = {0, 0, 0, 0};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) hit = mma_bf16(widen8<false>(flag[2 * h], flag[2 * h + 1]), seen[mt][h], hit);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (hit[r] > 0.f) w.o[mt][d][r] = NAN;
+        }
+    }
+}
+
+// Folds one tile's keys, of products s, into the running state. `full`: every
+// live row sees every key of the tile.
+template <typename T, int W, int MT>
+__device__ __forceinline__ void tile_fold(const AttnParams& p, Wave<T, W, MT>& w, Tile<W>& x, const Scales& sc,
+                                          f32x4 (&s)[MT][4], int tile, bool full) {
     typedef Wave<T, W, MT> WV;
-    const int lane = threadIdx.x & 63;
-    const int key0 = tile * kTile + (lane >> 4) * 16;
-    const float c = x.k_scale * p.scale;
+    const float c = sc.k * p.scale;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) s[mt][t] *= c;
+    if (full) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) w.any[mt] = 1;
+    } else {
+        const int key0 = tile * kTile + (threadIdx.x >> 4 & 3) * 16;
+        uint32_t mask[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            mask[mt] = sc.ok ? bits_below(w.end[mt] - key0) & (~bits_below(w.low[mt] - key0) | bits_below(p.sinks - key0)) : 0u;
+            w.any[mt] |= mask[mt];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const uint32_t on = (uint32_t)((int)(mask[mt] << (31 - i)) >> 31);
+                s[mt][i / 4][i % 4] = __uint_as_float((__float_as_uint(s[mt][i / 4][i % 4]) & on) | (0xff800000u & ~on));
+            }
+        }
+        clear_values<T, W, MT>(w, x, mask);
+    }
     u32x4 prob[MT][WV::PP][2];
-    bool bad_values = false;
-    u32x4 seen[MT][2];  // 1.0 where a row sees a key, for values that are NaN
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         float top = -INFINITY;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float v = s[mt][t][r] * c;
-                if (!full) {
-                    const int j = key0 + 4 * t + r;
-                    const bool see = x.ok && j < w.end[mt] && (j >= w.low[mt] || j < p.sinks);
-                    v = see ? v : -INFINITY;
-                    w.any[mt] |= see;
-                    seen[mt][t >> 1][(t & 1) * 2 + (r >> 1)] =
-                        (r & 1 ? seen[mt][t >> 1][(t & 1) * 2 + (r >> 1)] : 0u) | (see ? 0x3f80u << (r & 1) * 16 : 0u);
-                }
-                s[mt][t][r] = v;
-                top = fmaxf(top, v);
-            }
-        if (full) w.any[mt] = true;
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[mt][i / 4][i % 4]);
         // The maximum is moved only where some score passes it by over 8 (its
         // weight would be over 256): until then weights and sums keep it.
         const float m_old = w.m[mt];
@@ -322,7 +422,7 @@ __device__ __forceinline__ void tile_fold(const AttnParams& p, Wave<T, W, MT>& w
             for (int i = 0; i < 8; ++i) {
                 e[i] = __builtin_amdgcn_exp2f(s[mt][2 * h + i / 4][i & 3] - shift);
                 sum += e[i];
-                e[i] *= x.v_scale;
+                e[i] *= sc.v;
             }
             u32x4 parts[WV::PP];
             split8<WV::PP>(e, parts);
@@ -330,55 +430,6 @@ __device__ __forceinline__ void tile_fold(const AttnParams& p, Wave<T, W, MT>& w
             for (int n = 0; n < WV::PP; ++n) prob[mt][n][h] = parts[n];
         }
         w.l[mt] += sum;
-    }
-    if (!full) {
-        // Values of keys that no row sees may be anything: zeros in their
-        // place. NaN among the others belongs only to the rows that see it.
-        u32x4 dead;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t some = 0;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const uint32_t a = seen[mt][i >> 1][(i & 1) * 2], b = seen[mt][i >> 1][(i & 1) * 2 + 1];
-                some |= (a & 0x80u) | (a >> 16 & 0x80u) << 8 | (b & 0x80u) << 16 | (b >> 16 & 0x80u) << 24;
-            }
-            // over the 16 columns
-#pragma unroll
-            for (int off = 1; off < 16; off <<= 1) some |= __shfl_xor(some, off, 64);
-            dead[i] = ~((some >> 7) * 0xffu);
-        }
-        bool nan_here = false;
-#pragma unroll
-        for (int d = 0; d < W / 16; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x.v[d][i] &= ~dead[i];
-                nan_here |= (((x.v[d][i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
-            }
-        bad_values = __any(nan_here);
-        if (bad_values) {
-#pragma unroll
-            for (int d = 0; d < W / 16; ++d) {
-                u32x4 flag;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t nan = ((((x.v[d][i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
-                    flag[i] = nan & 0x38383838u;  // 1.0
-                    x.v[d][i] &= ~nan;
-                }
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    f32x4 hit = {0, 0, 0, 0};
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        hit = mma_bf16(widen8<false>(flag[2 * h], flag[2 * h + 1]), seen[mt][h], hit);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (hit[r] > 0.f) w.o[mt][d][r] = NAN;
-                }
-            }
-        }
     }
 #pragma unroll
     for (int d = 0; d < W / 16; ++d)
@@ -392,40 +443,40 @@ __device__ __forceinline__ void tile_fold(const AttnParams& p, Wave<T, W, MT>& w
         }
 }
 
-// Folds tiles first, first + step, ... below last of the span into the wave's state.
+__device__ __forceinline__ int tile_at(const Span& sp, int i) { return i < sp.sink_tiles ? i : sp.start + i - sp.sink_tiles; }
+
+// Folds tiles first, first + step, ... below last of the span into the wave's
+// state; `r` is where the first of them lies.
 template <typename T, int W, int MT>
-__device__ __forceinline__ void walk(const AttnParams& p, Wave<T, W, MT>& w, const Span& sp, int b, int kh, int first,
-                                     int last, int step) {
+__device__ __forceinline__ void walk(const AttnParams& p, Wave<T, W, MT>& w, const Span& sp, int b, int kh, Runs r,
+                                     int first, int last, int step) {
     if (first >= last) return;
     const int32_t* table = p.table + b * p.table_stride;
-    auto tile_at = [&](int i) { return i < sp.sink_tiles ? i : sp.start + i - sp.sink_tiles; };
-    // Keys [sure_low, sure_end) are seen by every live row, as are those below sure_sinks.
+    // Keys [sure_low, sure_end) are seen by every live row, as are those below the sinks' end.
     const int sure_end = sp.first_pos + 1 < sp.held ? sp.first_pos + 1 : sp.held;
     const int64_t lo = p.window > 0 ? (int64_t)sp.last_pos - p.window + 1 : 0;
     const int sure_low = lo > 0 ? (int)lo : 0;
-    Tile<T, W, MT> x;
-    Runs r = find_runs<T, W, MT>(p, table, tile_at(first), sp.held);
-    x.load_k(p, r, kh);
+    Tile<W> x;
+    int tile = tile_at(sp, first);
+    settle_runs(p, r, tile, sp.held);
+    Scales sc = x.load_k(p, r, kh);
     for (int i = first; i < last; i += step) {
-        const int tile = tile_at(i);
         x.load_v(p, r, kh);
-        const int next = i + step < last ? i + step : i;
-        const Runs rn = find_runs<T, W, MT>(p, table, tile_at(next), sp.held);
+        __builtin_amdgcn_sched_barrier(0);  // in flight while the scores are formed
+        const int next = tile_at(sp, i + step < last ? i + step : i);
+        r = find_runs(p, table, next);
         f32x4 s[MT][4];
         tile_scores<T, W, MT>(w, x, s);
-        Tile<T, W, MT> y;
-        if (i + step < last) y.load_k(p, rn, kh);
+        const Scales now = sc;
+        if (i + step < last) {
+            settle_runs(p, r, next, sp.held);
+            sc = x.load_k(p, r, kh);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // in flight while the tile is folded
         const int key = tile * kTile;
-        const bool full = key + kTile <= sure_end && (key >= sure_low || key + kTile <= p.sinks) && __all(x.ok);
-        tile_fold<T, W, MT>(p, w, x, s, tile, full);
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int c = 0; c < W / 64; ++c) x.k[t][c] = y.k[t][c];
-        x.k_scale = y.k_scale;
-        x.v_scale = y.v_scale;
-        x.ok = y.ok;
-        r = rn;
+        const bool full = key + kTile <= sure_end && (key >= sure_low || key + kTile <= p.sinks) && __all(now.ok);
+        tile_fold<T, W, MT>(p, w, x, now, s, tile, full);
+        tile = next;
     }
 }
 
@@ -450,7 +501,7 @@ template <typename T, int W>
 __device__ __forceinline__ void zero_rows(const AttnParams& p, int b, int kh, int row0, int row1) {
     const int rows = p.tokens * p.share;
     if (row1 > rows) row1 = rows;
-    for (int i = threadIdx.x; i < (row1 - row0) * W; i += 256) {
+    for (int i = fresh_lane(threadIdx.x); i < (row1 - row0) * W; i += 256) {
         const int d = i % W;
         if (d < p.dim) out_row<T>(p, b, kh, row0 + i / W)[d] = (T)0.f;
     }
@@ -463,7 +514,8 @@ __device__ __forceinline__ void join_waves(const AttnParams& p, Wave<T, W, 1>& w
                                            float* slot) {
     __shared__ float sm[4][16], sl[4][16];
     __shared__ float so[4][16][68];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const int tid = fresh_lane(threadIdx.x), dim = fresh(p.dim);
+    const int lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
     const float l = column_sum(w.l[0]);
     const bool any = column_sum(w.any[0] ? 1.f : 0.f) > 0.f;
     if (g == 0) {
@@ -483,11 +535,11 @@ __device__ __forceinline__ void join_waves(const AttnParams& p, Wave<T, W, 1>& w
         some |= has;
     }
     const float mine = any ? exp2f(w.m[0] - shift) * (slot ? 1.f : 1.f / sum) : 0.f;
-    if (slot && threadIdx.x < 16 && c < sp.live) {
+    if (slot && tid < 16 && c < sp.live) {
         slot[16 * W + c] = m;
         slot[16 * W + 16 + c] = some ? sum : -1.f;
     }
-    const int oc = threadIdx.x >> 4, od = (threadIdx.x & 15) * 4;
+    const int oc = tid >> 4, od = (tid & 15) * 4;
 #pragma unroll
     for (int d0 = 0; d0 < W / 64; ++d0) {
         if (d0) __syncthreads();
@@ -506,7 +558,7 @@ __device__ __forceinline__ void join_waves(const AttnParams& p, Wave<T, W, 1>& w
             } else {
                 float x[4] = {v[0], v[1], v[2], v[3]};
                 const int d = d0 * 64 + od;
-                if (d < p.dim) store4<T>(out_row<T>(p, b, kh, row0 + oc) + d, x, p.dim - d);
+                if (d < dim) store4<T>(out_row<T>(p, b, kh, row0 + oc) + d, x, dim - d);
             }
         }
     }
@@ -559,9 +611,14 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, W, 1>)) void kv_attention_fe
     // This workgroup's places [pos, stop) of the list, and sequence b, whose first pair is at `at`.
     int64_t pos, stop, at = 0;
     int b = 0;
+    Span sp;
+    Runs r;
     if (p.direct) {
         b = blockIdx.x / p.heads;
-        const Span sp = span_of(p, b, 0, 16);
+        // Where a wavefront's first tile lies is looked up beside the lengths
+        // (without a window: which tile it is follows from nothing else).
+        if (p.capacity > 0) r = find_runs(p, p.table + b * p.table_stride, wave);
+        sp = span_of(p, b, 0, 16);
         const int kh = blockIdx.x - b * p.heads;
         zero_rows<T, W>(p, b, kh, sp.tiles > 0 ? sp.live : 0, 16);
         pos = (int64_t)kh * (sp.tiles + kPairCost);
@@ -572,9 +629,9 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, W, 1>)) void kv_attention_fe
         stop = pos + per < total ? pos + per : total;
         // Rows that see nothing: their zeros, dealt out over the workgroups.
         for (int i = blockIdx.x; i < p.batch; i += gridDim.x) {
-            const Span sp = span_of(p, i, 0, 16);
-            if (sp.tiles == 0 || sp.live < 16)
-                for (int kh = 0; kh < p.heads; ++kh) zero_rows<T, W>(p, i, kh, sp.tiles == 0 ? 0 : sp.live, 16);
+            const Span z = span_of(p, i, 0, 16);
+            if (z.tiles == 0 || z.live < 16)
+                for (int kh = 0; kh < p.heads; ++kh) zero_rows<T, W>(p, i, kh, z.tiles == 0 ? 0 : z.live, 16);
         }
         if (pos >= stop) return;
         for (int b0 = 0;; b0 += 64) {
@@ -595,7 +652,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, W, 1>)) void kv_attention_fe
         }
     }
     while (pos < stop) {
-        const Span sp = span_of(p, b, 0, 16);
+        if (!p.direct) sp = span_of(p, b, 0, 16);
         const int64_t pair_weight = sp.tiles + kPairCost, size = sp.tiles > 0 ? pair_weight * p.heads : 0;
         if (pos >= at + size) {
             at += size;
@@ -607,8 +664,9 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, W, 1>)) void kv_attention_fe
         const int first = pos > pair ? (int)(pos - pair) : 0, last = end > pair ? (int)(end - pair) : 0;
         pos = end > pos ? end : stop;
         if (first >= last) continue;
-        w.load_q(p, b, kh, 0, sp, 0);
-        walk<T, W, 1>(p, w, sp, b, kh, first + wave, last, 4);
+        if (!p.direct || p.window > 0) r = find_runs(p, p.table + b * p.table_stride, tile_at(sp, first + wave));
+        w.load_q(p, b, kh, 0, sp);
+        walk<T, W, 1>(p, w, sp, b, kh, r, first + wave, last, 4);
         // A pair is cut at most at this workgroup's ends: in its first or its last tiles.
         const bool whole = first == 0 && last == sp.tiles;
         float* slot = whole ? nullptr : p.part + ((int64_t)blockIdx.x * 2 + (first == 0 ? 1 : 0)) * (16 * (W + 2));
@@ -706,27 +764,29 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, W, MT>)) void kv_attention_m
     if (part > 0 && first >= last) return;
     Wave<T, W, MT> w;
     const Span sp = span_of(p, b, mine, 16 * MT);
-    w.load_q(p, b, kh, mine, sp, mine);
-    walk<T, W, MT>(p, w, all, b, kh, first, last, 1);
+    Runs r;
+    if (first < last) r = find_runs(p, p.table + b * p.table_stride, tile_at(all, first));
+    w.load_q(p, b, kh, mine, sp);
+    walk<T, W, MT>(p, w, all, b, kh, r, first, last, 1);
     float* slot = p.groups > 1 && per < all.tiles
                       ? p.part + ((((int64_t)b * p.row_blocks + rb) * p.heads + kh) * p.groups + part) * (kRows * (W + 2))
                       : nullptr;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        const int r = wave * 16 * MT + mt * 16 + c;
+        const int row = wave * 16 * MT + mt * 16 + c;
         const float l = column_sum(w.l[mt]);
         const bool any = column_sum(w.any[mt] ? 1.f : 0.f) > 0.f;
-        if (row0 + r >= p.tokens * p.share) continue;
-        const bool dead = r >= all.live || !any;
+        if (row0 + row >= p.tokens * p.share) continue;
+        const bool dead = row >= all.live || !any;
         if (slot) {
             if (g == 0) {
-                slot[kRows * W + r] = w.m[mt];
-                slot[kRows * W + kRows + r] = dead ? -1.f : l;
+                slot[kRows * W + row] = w.m[mt];
+                slot[kRows * W + kRows + row] = dead ? -1.f : l;
             }
 #pragma unroll
-            for (int d = 0; d < W / 16; ++d) *reinterpret_cast<f32x4*>(slot + r * W + d * 16 + g * 4) = w.o[mt][d];
+            for (int d = 0; d < W / 16; ++d) *reinterpret_cast<f32x4*>(slot + row * W + d * 16 + g * 4) = w.o[mt][d];
         } else {
-            T* out = out_row<T>(p, b, kh, row0 + r);
+            T* out = out_row<T>(p, b, kh, row0 + row);
             const float f = 1.f / l;
 #pragma unroll
             for (int d = 0; d < W / 16; ++d) {
@@ -902,6 +962,7 @@ extern "C" int tt_kv_attention(const tt_kv_attention_args* a, void* stream) {
     p.window = (int)(a->window < kInt ? a->window : kInt);
     p.sinks = (int)(a->sinks < kInt ? a->sinks : kInt);
     p.capacity = a->cache.pages > 0 ? (int)(a->table_width * a->cache.page) : 0;
+    p.table_width = (int)a->table_width;
     p.row_blocks = c.row_blocks;
     p.groups = c.groups;
     p.direct = c.direct;
