@@ -26,7 +26,8 @@ struct AttnParams {
     int groups;      // workgroups that share the key tiles
     int direct;      // each workgroup takes one pair, whole
     FastDiv by_page, by_share;
-    float scale;  // times log2(e)
+    float scale;    // magnitude, times log2(e)
+    uint32_t flip;  // the sign bits of two 16-bit values where the scale is negative
 };
 
 constexpr int kTile = 64;     // keys a wavefront takes at a time
@@ -160,7 +161,8 @@ struct Wave {
     static constexpr bool kHalf = std::is_same<T, _Float16>::value;
     u32x4 q[MT][QP][W / 32];
     f32x4 o[MT][W / 16];
-    float m[MT], l[MT];
+    f32x4 l[MT];           // the weights' sum, in every element and lane of a column
+    float m[MT];
     uint32_t any[MT];      // not 0 once the row has seen a key
     int end[MT], low[MT];  // this lane's query row sees keys of [0, end) that are >= low or < sinks
 
@@ -178,7 +180,7 @@ struct Wave {
             const int64_t lo = p.window > 0 ? pos - p.window + 1 : 0;
             low[mt] = lo > 0 ? (int)lo : 0;
             m[mt] = -INFINITY;
-            l[mt] = 0.f;
+            l[mt] = f32x4{0, 0, 0, 0};
             any[mt] = 0;
 #pragma unroll
             for (int d = 0; d < W / 16; ++d) o[mt][d] = f32x4{0, 0, 0, 0};
@@ -207,14 +209,13 @@ struct Wave {
             }
 #pragma unroll
             for (int s = 0; s < W / 32; ++s) {
-                if constexpr (QP == 1) {
-                    q[mt][0][s] = __builtin_bit_cast(u32x4, x[s]);
-                } else {
-                    u32x4 parts[QP];
+                u32x4 parts[QP];
+                if constexpr (QP == 1)
+                    parts[0] = __builtin_bit_cast(u32x4, x[s]);
+                else
                     split8<QP>(x[s], parts);
 #pragma unroll
-                    for (int n = 0; n < QP; ++n) q[mt][n][s] = parts[n];
-                }
+                for (int n = 0; n < QP; ++n) q[mt][n][s] = parts[n] ^ p.flip;
             }
         }
     }
@@ -248,10 +249,21 @@ __device__ __forceinline__ void settle_runs(const AttnParams& p, Runs& r, int ti
     if (!r.v_ok) r.v_page = 0;
 }
 
+// The scales of the run whose keys' scores a lane holds. A value's scale is
+// 2^v_exp: probabilities are formed times it, as exp2 of one sum, and sums of
+// probabilities are taken with 2^-v_exp (two bfloat16 values of it in v_inv).
 struct Scales {
-    float k, v;
+    float k, v_exp;
+    uint32_t v_inv;
     bool ok;
 };
+
+__device__ __forceinline__ Scales load_scales(const AttnParams& p, const Runs& r, int kh) {
+    const int64_t at = r.v_page * p.heads + kh;
+    const int e = r.v_ok ? (int)(__float_as_uint(p.v_scale[at]) >> 23 & 255) - 127 : 0;
+    const uint32_t inv = (uint32_t)(127 - e) << 7;
+    return {r.v_ok ? p.k_scale[at] : 0.f, (float)e, inv | inv << 16, r.v_ok};
+}
 
 template <int W>
 struct Tile {
@@ -265,8 +277,7 @@ struct Tile {
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int c = 0; c < W / 64; ++c) k[t][c] = *reinterpret_cast<const u32x4*>(src + t * 4 * W + c * 64);
-        const int64_t at = r.v_page * p.heads + kh;
-        return {r.v_ok ? p.k_scale[at] : 0.f, r.v_ok ? p.v_scale[at] : 0.f, r.v_ok};
+        return load_scales(p, r, kh);
     }
     __device__ __forceinline__ void load_v(const AttnParams& p, const Runs& r, int kh) {
         const int lane = threadIdx.x & 63;
@@ -317,91 +328,90 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t v) { return ((v & 0x7f7f7
 
 // A tile that some row does not see whole: bit i of mask[mt] says whether this
 // lane's row sees key i of its run. Values of keys that no row of the wavefront
-// sees may be anything, so zeros are put in their place. NaN among the others
-// belongs only to the rows that see it: its elements are found, zeroed, and
-// their rows' output set to NaN through a product of their places with `mask`.
-template <typename T, int W, int MT>
-__device__ __forceinline__ void clear_values(Wave<T, W, MT>& w, Tile<W>& x, const uint32_t (&mask)[MT]) {
-    uint32_t some = mask[0];
+// sees may be anything, so zeros are put in their place (`keep`: the bytes that
+// stay). NaN among the others belongs only to the rows that see it: it is
+// zeroed as well, and those rows' output set to NaN through a product of its
+// places with `seen` (1.0 where the row sees the key).
+template <int MT>
+struct Edge {
+    uint32_t keep[4];
+    u32x4 seen[MT][2];
+
+    __device__ __forceinline__ explicit Edge(const uint32_t (&mask)[MT]) {
+        uint32_t some = mask[0];
 #pragma unroll
-    for (int mt = 1; mt < MT; ++mt) some |= mask[mt];
-    some |= __builtin_amdgcn_mov_dpp(some, 0x128, 0xf, 0xf, true);  // row_ror: over the 16 columns
-    some |= __builtin_amdgcn_mov_dpp(some, 0x124, 0xf, 0xf, true);
-    some |= __builtin_amdgcn_mov_dpp(some, 0x122, 0xf, 0xf, true);
-    some |= __builtin_amdgcn_mov_dpp(some, 0x121, 0xf, 0xf, true);
-    uint32_t keep[4], nan = 0;
+        for (int mt = 1; mt < MT; ++mt) some |= mask[mt];
+        some |= __builtin_amdgcn_mov_dpp(some, 0x128, 0xf, 0xf, true);  // row_ror: over the 16 columns
+        some |= __builtin_amdgcn_mov_dpp(some, 0x124, 0xf, 0xf, true);
+        some |= __builtin_amdgcn_mov_dpp(some, 0x122, 0xf, 0xf, true);
+        some |= __builtin_amdgcn_mov_dpp(some, 0x121, 0xf, 0xf, true);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) keep[i] = bits_to_bytes(some >> 4 * i) * 0xffu;
+        for (int i = 0; i < 4; ++i) keep[i] = bits_to_bytes(some >> 4 * i) * 0xffu;
 #pragma unroll
-    for (int d = 0; d < W / 16; ++d)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x.v[d][i] &= keep[i];
-            nan |= nan_bytes(x.v[d][i]);
-        }
-    if (!__any(nan != 0)) return;
-    u32x4 seen[MT][2];  // 1.0 where the row sees the key
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            seen[mt][i / 4][i % 4] = (mask[mt] >> 2 * i & 1 ? 0x3f80u : 0u) | (mask[mt] >> 2 * i & 2 ? 0x3f800000u : 0u);
-#pragma unroll
-    for (int d = 0; d < W / 16; ++d) {
+            for (int i = 0; i < 8; ++i)
+                seen[mt][i / 4][i % 4] = (mask[mt] >> 2 * i & 1 ? 0x3f80u : 0u) | (mask[mt] >> 2 * i & 2 ? 0x3f800000u : 0u);
+    }
+    // Clears the codes v of one block of 16 elements, o[mt] its output.
+    __device__ __forceinline__ u32x4 clear(u32x4 v, f32x4 (&o)[MT]) const {
         u32x4 flag;
+        uint32_t nan = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t at = nan_bytes(x.v[d][i]);
+            v[i] &= keep[i];
+            const uint32_t at = nan_bytes(v[i]);
             flag[i] = at * 0x38u;  // the code of 1.0
-            x.v[d][i] &= ~(at * 0xffu);
+            v[i] &= ~(at * 0xffu);
+            nan |= at;
         }
+        if (__any(nan != 0)) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            f32x4 hit = {0, 0, 0, 0};
+            for (int mt = 0; mt < MT; ++mt) {
+                f32x4 hit = {0, 0, 0, 0};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) hit = mma_bf16(widen8<false>(flag[2 * h], flag[2 * h + 1]), seen[mt][h], hit);
+                for (int h = 0; h < 2; ++h) hit = mma_bf16(widen8<false>(flag[2 * h], flag[2 * h + 1]), seen[mt][h], hit);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (hit[r] > 0.f) w.o[mt][d][r] = NAN;
+                for (int r = 0; r < 4; ++r)
+                    if (hit[r] > 0.f) o[mt][r] = NAN;
+            }
+        }
+        return v;
+    }
+};
+
+// Which keys of its run a lane's rows see of a tile, and scores of the others set to -inf.
+template <typename T, int W, int MT>
+__device__ __forceinline__ void mask_scores(const AttnParams& p, Wave<T, W, MT>& w, bool ok, f32x4 (&s)[MT][4], int tile,
+                                            uint32_t (&mask)[MT]) {
+    const int key0 = tile * kTile + (threadIdx.x >> 4 & 3) * 16;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        mask[mt] = ok ? bits_below(w.end[mt] - key0) & (~bits_below(w.low[mt] - key0) | bits_below(p.sinks - key0)) : 0u;
+        w.any[mt] |= mask[mt];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t on = (uint32_t)((int)(mask[mt] << (31 - i)) >> 31);
+            s[mt][i / 4][i % 4] = __uint_as_float((__float_as_uint(s[mt][i / 4][i % 4]) & on) | (0xff800000u & ~on));
         }
     }
 }
 
-// Folds one tile's keys, of products s, into the running state. `full`: every
-// live row sees every key of the tile.
+// The weights of one tile's keys, of products s (-inf where masked), as the
+// operands of the second product, and their sum and maximum in the running state.
 template <typename T, int W, int MT>
-__device__ __forceinline__ void tile_fold(const AttnParams& p, Wave<T, W, MT>& w, Tile<W>& x, const Scales& sc,
-                                          f32x4 (&s)[MT][4], int tile, bool full) {
+__device__ __forceinline__ void tile_weights(const AttnParams& p, Wave<T, W, MT>& w, const Scales& sc, f32x4 (&s)[MT][4],
+                                             u32x4 (&prob)[MT][Wave<T, W, MT>::PP][2]) {
     typedef Wave<T, W, MT> WV;
-    const float c = sc.k * p.scale;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) s[mt][t] *= c;
-    if (full) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) w.any[mt] = 1;
-    } else {
-        const int key0 = tile * kTile + (threadIdx.x >> 4 & 3) * 16;
-        uint32_t mask[MT];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            mask[mt] = sc.ok ? bits_below(w.end[mt] - key0) & (~bits_below(w.low[mt] - key0) | bits_below(p.sinks - key0)) : 0u;
-            w.any[mt] |= mask[mt];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const uint32_t on = (uint32_t)((int)(mask[mt] << (31 - i)) >> 31);
-                s[mt][i / 4][i % 4] = __uint_as_float((__float_as_uint(s[mt][i / 4][i % 4]) & on) | (0xff800000u & ~on));
-            }
-        }
-        clear_values<T, W, MT>(w, x, mask);
-    }
-    u32x4 prob[MT][WV::PP][2];
+    // Not zero, so that a masked score stays -inf whatever the scale.
+    const float c = fmaxf(sc.k * p.scale, 1e-30f);
+    const u32x4 one = {sc.v_inv, sc.v_inv, sc.v_inv, sc.v_inv};
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        float top = -INFINITY;
+        float top = s[mt][0][0];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[mt][i / 4][i % 4]);
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[mt][i / 4][i % 4]);
+        top *= c;
         // The maximum is moved only where some score passes it by over 8 (its
         // weight would be over 256): until then weights and sums keep it.
         const float m_old = w.m[mt];
@@ -413,49 +423,50 @@ __device__ __forceinline__ void tile_fold(const AttnParams& p, Wave<T, W, MT>& w
 #pragma unroll
             for (int d = 0; d < W / 16; ++d) w.o[mt][d] *= keep;
         }
-        const float shift = w.m[mt] == -INFINITY ? 0.f : w.m[mt];
-        float sum = 0.f;
+        const float shift = sc.v_exp - (w.m[mt] == -INFINITY ? 0.f : w.m[mt]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             float e[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                e[i] = __builtin_amdgcn_exp2f(s[mt][2 * h + i / 4][i & 3] - shift);
-                sum += e[i];
-                e[i] *= sc.v;
-            }
+            for (int i = 0; i < 8; ++i)
+                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][2 * h + i / 4][i & 3], c, shift));
             u32x4 parts[WV::PP];
             split8<WV::PP>(e, parts);
 #pragma unroll
-            for (int n = 0; n < WV::PP; ++n) prob[mt][n][h] = parts[n];
+            for (int n = 0; n < WV::PP; ++n) {
+                prob[mt][n][h] = parts[n];
+                w.l[mt] = mma_bf16(one, parts[n], w.l[mt]);
+            }
         }
-        w.l[mt] += sum;
     }
-#pragma unroll
-    for (int d = 0; d < W / 16; ++d)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const u32x4 a = widen8<false>(x.v[d][2 * h], x.v[d][2 * h + 1]);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int n = 0; n < WV::PP; ++n) w.o[mt][d] = mma_bf16(a, prob[mt][n][h], w.o[mt][d]);
-        }
 }
 
 __device__ __forceinline__ int tile_at(const Span& sp, int i) { return i < sp.sink_tiles ? i : sp.start + i - sp.sink_tiles; }
+
+// Keys [low, end) are seen by every live row of a span, as are those below the sinks' end.
+struct Sure {
+    int low, end;
+
+    __device__ __forceinline__ Sure(const AttnParams& p, const Span& sp) {
+        end = sp.first_pos + 1 < sp.held ? sp.first_pos + 1 : sp.held;
+        const int64_t lo = p.window > 0 ? (int64_t)sp.last_pos - p.window + 1 : 0;
+        low = lo > 0 ? (int)lo : 0;
+    }
+    __device__ __forceinline__ bool sees(const AttnParams& p, int tile) const {
+        const int key = tile * kTile;
+        return key + kTile <= end && (key >= low || key + kTile <= p.sinks);
+    }
+};
 
 // Folds tiles first, first + step, ... below last of the span into the wave's
 // state; `r` is where the first of them lies.
 template <typename T, int W, int MT>
 __device__ __forceinline__ void walk(const AttnParams& p, Wave<T, W, MT>& w, const Span& sp, int b, int kh, Runs r,
                                      int first, int last, int step) {
+    typedef Wave<T, W, MT> WV;
     if (first >= last) return;
     const int32_t* table = p.table + b * p.table_stride;
-    // Keys [sure_low, sure_end) are seen by every live row, as are those below the sinks' end.
-    const int sure_end = sp.first_pos + 1 < sp.held ? sp.first_pos + 1 : sp.held;
-    const int64_t lo = p.window > 0 ? (int64_t)sp.last_pos - p.window + 1 : 0;
-    const int sure_low = lo > 0 ? (int)lo : 0;
+    const Sure sure(p, sp);
     Tile<W> x;
     int tile = tile_at(sp, first);
     settle_runs(p, r, tile, sp.held);
@@ -473,9 +484,36 @@ __device__ __forceinline__ void walk(const AttnParams& p, Wave<T, W, MT>& w, con
             sc = x.load_k(p, r, kh);
         }
         __builtin_amdgcn_sched_barrier(0);  // in flight while the tile is folded
-        const int key = tile * kTile;
-        const bool full = key + kTile <= sure_end && (key >= sure_low || key + kTile <= p.sinks) && __all(now.ok);
-        tile_fold<T, W, MT>(p, w, x, now, s, tile, full);
+        const bool full = sure.sees(p, tile) && __all(now.ok);
+        if (full) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) w.any[mt] = 1;
+        } else {
+            uint32_t mask[MT];
+            mask_scores<T, W, MT>(p, w, now.ok, s, tile, mask);
+            const Edge<MT> edge(mask);
+#pragma unroll
+            for (int d = 0; d < W / 16; ++d) {
+                f32x4 o[MT];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) o[mt] = w.o[mt][d];
+                x.v[d] = edge.clear(x.v[d], o);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) w.o[mt][d] = o[mt];
+            }
+        }
+        u32x4 prob[MT][WV::PP][2];
+        tile_weights<T, W, MT>(p, w, now, s, prob);
+#pragma unroll
+        for (int d = 0; d < W / 16; ++d)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const u32x4 a = widen8<false>(x.v[d][2 * h], x.v[d][2 * h + 1]);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int n = 0; n < WV::PP; ++n) w.o[mt][d] = mma_bf16(a, prob[mt][n][h], w.o[mt][d]);
+            }
         tile = next;
     }
 }
@@ -516,7 +554,7 @@ __device__ __forceinline__ void join_waves(const AttnParams& p, Wave<T, W, 1>& w
     __shared__ float so[4][16][68];
     const int tid = fresh_lane(threadIdx.x), dim = fresh(p.dim);
     const int lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
-    const float l = column_sum(w.l[0]);
+    const float l = w.l[0][0];
     const bool any = column_sum(w.any[0] ? 1.f : 0.f) > 0.f;
     if (g == 0) {
         sm[wave][c] = w.m[0];
@@ -743,12 +781,19 @@ __global__ __launch_bounds__(256) void kv_attention_few_join_kernel(AttnParams p
                        out_row<T>(p, b, kh, row));
 }
 
-// Many query rows: each wavefront takes MT blocks of 16 rows of its own, and
-// the four of a workgroup walk the same keys. With `groups` > 1 the keys of a
-// row block are cut into that many ranges, joined afterwards.
-template <typename T, int W, int MT>
-__global__ __launch_bounds__(256, (kWavesPerSimd<T, W, MT>)) void kv_attention_many_kernel(AttnParams p) {
-    constexpr int kRows = 64 * MT;
+// Many query rows: each of NW wavefronts takes MT blocks of 16 rows, and all of
+// them walk the same keys, whose codes the workgroup widens once and puts into
+// LDS as the operands of the products, tile by tile in two buffers: what widens
+// a tile, loads it and reads it is shared by 16 MT NW rows. With `groups` > 1
+// the keys of a row block are cut into that many ranges, joined afterwards.
+template <typename T, int W, int MT, int NW>
+__global__ __launch_bounds__(64 * NW, (NW == 8 ? 2 : 1)) void kv_attention_many_kernel(AttnParams p) {
+    typedef Wave<T, W, MT> WV;
+    constexpr int kRows = 16 * MT * NW;
+    constexpr int kKeys = W / 16, kLoads = 2 * kKeys, kMine = kLoads / NW;  // 16-byte pieces a lane: of keys, of a tile, a wavefront's
+    static_assert(kLoads % NW == 0, "pieces divide evenly");
+    __shared__ u32x4 lds[2][2 * kLoads][64];
+    __shared__ int nan_values[3];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     int id = blockIdx.x;
     const int part = id % p.groups;
@@ -762,19 +807,159 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, W, MT>)) void kv_attention_m
     const int per = all.tiles > 0 ? (all.tiles + p.groups - 1) / p.groups : 1;
     const int first = part * per, last = first + per < all.tiles ? first + per : all.tiles;
     if (part > 0 && first >= last) return;
-    Wave<T, W, MT> w;
+    WV w;
     const Span sp = span_of(p, b, mine, 16 * MT);
-    Runs r;
-    if (first < last) r = find_runs(p, p.table + b * p.table_stride, tile_at(all, first));
     w.load_q(p, b, kh, mine, sp);
-    walk<T, W, MT>(p, w, all, b, kh, r, first, last, 1);
+    if (first < last) {
+        const int32_t* table = p.table + b * p.table_stride;
+        const Sure sure(p, all);
+        const int end = all.last_pos + 1 < all.held ? all.last_pos + 1 : all.held;  // no row sees further
+        u32x4 raw[kMine];
+        Scales sc;
+        // Piece n of a tile: of its keys (row block n % 4, elements 64 (n / 4) ..) or, from kKeys on, of its values.
+        auto load = [&](const Runs& r) {
+            const uint8_t* k = p.k + ((r.k_page * p.heads + kh) * p.page + r.k_slot + (lane & 3)) * W + (lane >> 4) * 16;
+            const uint8_t* v = p.v + ((r.v_page * p.heads + kh) * W + c) * p.page + r.v_slot;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                const int n = wave + i * NW;
+                const uint8_t* src = n < kKeys ? k + n % 4 * 4 * W + n / 4 * 64 : v + (int64_t)(n - kKeys) * 16 * p.page;
+                raw[i] = *reinterpret_cast<const u32x4*>(src);
+            }
+            sc = load_scales(p, r, kh);
+        };
+        auto stage = [&](int buffer, int flag, int tile, bool ok) {
+            uint32_t nan = 0;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                const int n = wave + i * NW;
+                u32x4 x = raw[i];
+                if (n < kKeys) {
+                    const int at = n % 4 * (W / 32) + n / 4 * 2;
+                    lds[buffer][at][lane] = widen8<WV::kHalf>(x[0], x[1]);
+                    lds[buffer][at + 1][lane] = widen8<WV::kHalf>(x[2], x[3]);
+                } else {
+                    if (!sure.sees(p, tile) || !ok) {
+                        const uint32_t live = ok ? bits_below(end - tile * kTile - g * 16) : 0u;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            x[j] &= bits_to_bytes(live >> 4 * j) * 0xffu;
+                            nan |= nan_bytes(x[j]);
+                        }
+                    }
+                    const int at = kLoads + (n - kKeys) * 2;
+                    lds[buffer][at][lane] = widen8<false>(x[0], x[1]);
+                    lds[buffer][at + 1][lane] = widen8<false>(x[2], x[3]);
+                }
+            }
+            if (nan) nan_values[flag] = 1;
+        };
+        if (threadIdx.x < 3) nan_values[threadIdx.x] = 0;
+        __syncthreads();
+        int tile = tile_at(all, first), turn = 0;
+        Runs r = find_runs(p, table, tile);
+        settle_runs(p, r, tile, all.held);
+        load(r);
+        stage(0, 0, tile, sc.ok);
+        Scales now = sc;
+        Runs at = r;
+        int next = first + 1 < last ? tile_at(all, first + 1) : tile;
+        r = find_runs(p, table, next);
+        __syncthreads();
+        for (int i = first; i < last; ++i) {
+            const bool more = i + 1 < last;
+            if (more) {
+                settle_runs(p, r, next, all.held);
+                load(r);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // in flight while this tile is worked on
+            const Runs after = r;
+            const int tile2 = i + 2 < last ? tile_at(all, i + 2) : next;
+            r = find_runs(p, table, tile2);
+            const u32x4(*keys)[64] = lds[(i - first) & 1];
+            const u32x4(*values)[64] = keys + kLoads;
+            f32x4 s[MT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) s[mt][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < W / 32; ++e)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const u32x4 a = keys[t * (W / 32) + e][lane];
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int n = 0; n < WV::QP; ++n) {
+                            if constexpr (WV::kHalf)
+                                s[mt][t] = mma_f16(a, w.q[mt][n][e], s[mt][t]);
+                            else
+                                s[mt][t] = mma_bf16(a, w.q[mt][n][e], s[mt][t]);
+                        }
+                }
+            const bool full = sure.sees(p, tile) && __all(now.ok);
+            uint32_t mask[MT];
+            if (full) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) w.any[mt] = 1;
+            } else {
+                mask_scores<T, W, MT>(p, w, now.ok, s, tile, mask);
+            }
+            u32x4 prob[MT][WV::PP][2];
+            tile_weights<T, W, MT>(p, w, now, s, prob);
+            if (!full && nan_values[turn]) {
+                // NaN among values that not every row sees: from the codes, as
+                // rarely as that happens.
+                const Edge<MT> edge(mask);
+                const uint8_t* v = p.v + ((at.v_page * p.heads + kh) * W + c) * p.page + at.v_slot;
+#pragma unroll
+                for (int d = 0; d < W / 16; ++d) {
+                    f32x4 o[MT];
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) o[mt] = w.o[mt][d];
+                    const u32x4 x = edge.clear(*reinterpret_cast<const u32x4*>(v + (int64_t)d * 16 * p.page), o);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const u32x4 a = widen8<false>(x[2 * h], x[2 * h + 1]);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                            for (int n = 0; n < WV::PP; ++n) o[mt] = mma_bf16(a, prob[mt][n][h], o[mt]);
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) w.o[mt][d] = o[mt];
+                }
+            } else {
+#pragma unroll
+                for (int d = 0; d < W / 16; ++d)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const u32x4 a = values[d * 2 + h][lane];
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                            for (int n = 0; n < WV::PP; ++n) w.o[mt][d] = mma_bf16(a, prob[mt][n][h], w.o[mt][d]);
+                    }
+            }
+            const int turn1 = turn == 2 ? 0 : turn + 1, turn2 = turn1 == 2 ? 0 : turn1 + 1;
+            if (threadIdx.x == 0) nan_values[turn2] = 0;
+            if (more) stage((i + 1 - first) & 1, turn1, next, sc.ok);
+            now = sc;
+            at = after;
+            tile = next;
+            next = tile2;
+            turn = turn1;
+            __syncthreads();
+        }
+    }
     float* slot = p.groups > 1 && per < all.tiles
                       ? p.part + ((((int64_t)b * p.row_blocks + rb) * p.heads + kh) * p.groups + part) * (kRows * (W + 2))
                       : nullptr;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const int row = wave * 16 * MT + mt * 16 + c;
-        const float l = column_sum(w.l[mt]);
+        const float l = w.l[mt][0];
         const bool any = column_sum(w.any[mt] ? 1.f : 0.f) > 0.f;
         if (row0 + row >= p.tokens * p.share) continue;
         const bool dead = row >= all.live || !any;
@@ -786,6 +971,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, W, MT>)) void kv_attention_m
 #pragma unroll
             for (int d = 0; d < W / 16; ++d) *reinterpret_cast<f32x4*>(slot + row * W + d * 16 + g * 4) = w.o[mt][d];
         } else {
+            const int dim = fresh(p.dim);
             T* out = out_row<T>(p, b, kh, row0 + row);
             const float f = 1.f / l;
 #pragma unroll
@@ -794,15 +980,14 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, W, MT>)) void kv_attention_m
                 float x[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[i] = dead ? 0.f : w.o[mt][d][i] * f;
-                if (d0 < p.dim) store4<T>(out + d0, x, p.dim - d0);
+                if (d0 < dim) store4<T>(out + d0, x, dim - d0);
             }
         }
     }
 }
 
-template <typename T, int W, int MT>
+template <typename T, int W, int kRows>
 __global__ __launch_bounds__(256) void kv_attention_many_join_kernel(AttnParams p) {
-    constexpr int kRows = 64 * MT;
     int id = blockIdx.x;
     const int chunk = id % (kRows / 4);
     id /= kRows / 4;
@@ -823,7 +1008,7 @@ __global__ __launch_bounds__(256) void kv_attention_many_join_kernel(AttnParams 
 // How a call is cut, from what the host knows of it.
 struct Cut {
     bool few, direct;
-    int mt, row_blocks, groups;
+    int mt, waves, row_blocks, groups;
     int64_t grid, slots, slot_floats;
 };
 
@@ -848,37 +1033,44 @@ Cut cut_of(const tt_kv_attention_args* a) {
         c.slots = c.direct ? 0 : 2 * c.groups;
         c.slot_floats = 16 * (W + 2);
     } else {
-        c.mt = rows > 64 && W <= 128 ? 2 : 1;
-        c.row_blocks = (int)((rows + 64 * c.mt - 1) / (64 * c.mt));
-        const int64_t blocks = pairs * c.row_blocks;
-        int64_t g = blocks >= 512 ? 1 : (512 + blocks - 1) / blocks;
+        const bool wide = W > 128;
+        c.mt = rows > 128 && !wide && a->dtype != TT_F32 ? 2 : 1;
+        c.waves = rows <= 64 || (wide && a->dtype == TT_F32) ? 4 : 8;
+        const int64_t block = 16 * c.mt * c.waves;
+        c.row_blocks = (int)((rows + block - 1) / block);
+        const int64_t blocks = pairs * c.row_blocks, want = c.waves == 4 ? 512 : 256;
+        int64_t g = blocks >= want ? 1 : (want + blocks - 1) / blocks;
         if (g > tiles / 4) g = tiles / 4 > 0 ? tiles / 4 : 1;
         c.groups = (int)g;
         c.grid = blocks * g;
         c.slots = g > 1 ? blocks * g : 0;
-        c.slot_floats = 64 * c.mt * (W + 2);
+        c.slot_floats = block * (W + 2);
     }
     return c;
 }
 
+template <typename T, int W, int MT, int NW>
+int attn_many(const AttnParams& p, const Cut& c, hipStream_t st) {
+    kv_attention_many_kernel<T, W, MT, NW><<<(uint32_t)c.grid, 64 * NW, 0, st>>>(p);
+    if (c.groups > 1) {
+        const uint32_t join = (uint32_t)((int64_t)p.batch * p.heads * p.row_blocks * 4 * MT * NW);
+        kv_attention_many_join_kernel<T, W, 16 * MT * NW><<<join, 256, 0, st>>>(p);
+    }
+    return check_launch("tt_kv_attention");
+}
+
 template <typename T, int W>
-int attn_launch(AttnParams& p, const Cut& c, hipStream_t st) {
+int attn_launch(const AttnParams& p, const Cut& c, hipStream_t st) {
     if (c.few) {
         kv_attention_few_kernel<T, W><<<(uint32_t)c.grid, 256, 0, st>>>(p);
         if (!c.direct) kv_attention_few_join_kernel<T, W><<<(uint32_t)(p.batch * p.heads), 256, 0, st>>>(p);
         return check_launch("tt_kv_attention");
     }
-    const uint32_t join = (uint32_t)((int64_t)p.batch * p.heads * p.row_blocks * 16 * c.mt);
-    if constexpr (W <= 128) {
-        if (c.mt == 2) {
-            kv_attention_many_kernel<T, W, 2><<<(uint32_t)c.grid, 256, 0, st>>>(p);
-            if (c.groups > 1) kv_attention_many_join_kernel<T, W, 2><<<join, 256, 0, st>>>(p);
-            return check_launch("tt_kv_attention");
-        }
-    }
-    kv_attention_many_kernel<T, W, 1><<<(uint32_t)c.grid, 256, 0, st>>>(p);
-    if (c.groups > 1) kv_attention_many_join_kernel<T, W, 1><<<join, 256, 0, st>>>(p);
-    return check_launch("tt_kv_attention");
+    if (c.waves == 4) return attn_many<T, W, 1, 4>(p, c, st);
+    if constexpr (sizeof(T) == 2 && W <= 128)
+        if (c.mt == 2) return attn_many<T, W, 2, 8>(p, c, st);
+    if constexpr (sizeof(T) == 2 || W <= 128) return attn_many<T, W, 1, 8>(p, c, st);
+    return set_error(TT_HIP_ERROR, "tt_kv_attention: no kernel");
 }
 
 template <typename T>
@@ -930,7 +1122,7 @@ extern "C" int tt_kv_attention(const tt_kv_attention_args* a, void* stream) {
     if (int rc = check_attention(a)) return rc;
     if (a->batch == 0 || a->tokens == 0) return TT_OK;
     const Cut c = cut_of(a);
-    const int64_t join = a->batch * a->cache.heads * c.row_blocks * 16 * c.mt;
+    const int64_t join = a->batch * a->cache.heads * c.row_blocks * 4 * c.mt * c.waves;
     if (c.grid > kMaxGrid || join > kMaxGrid)
         return set_error(TT_UNSUPPORTED, "tt_kv_attention: %lld workgroups", (long long)c.grid);
     const int64_t need = c.slots * c.slot_floats * 4;
@@ -968,7 +1160,8 @@ extern "C" int tt_kv_attention(const tt_kv_attention_args* a, void* stream) {
     p.direct = c.direct;
     p.by_page = make_fastdiv((uint32_t)p.page);
     p.by_share = make_fastdiv((uint32_t)p.share);
-    p.scale = (float)(a->scale * 1.4426950408889634074);
+    p.scale = (float)((a->scale < 0 ? -a->scale : a->scale) * 1.4426950408889634074);
+    p.flip = a->scale < 0 ? 0x80008000u : 0u;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (a->dtype == TT_F32) return attn_typed<float>(p, c, st);
     if (a->dtype == TT_BF16) return attn_typed<__bf16>(p, c, st);

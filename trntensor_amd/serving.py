@@ -204,6 +204,9 @@ class KVCache:
                 raise RuntimeError(f"a cache's tensors are on one HIP device; {name} is on {t.device}")
             if not t.is_contiguous() or t.data_ptr() % 16:
                 raise ValueError(f"{name} must be contiguous and 16-byte aligned")
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if not (torch.frexp(t)[0] == 0.5).all():
+                raise ValueError(f"{name} must be positive powers of two")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.head_dim, self.page_size, self.num_pages, self.num_heads = int(head_dim), page, pages, heads
         self.device = k.device
