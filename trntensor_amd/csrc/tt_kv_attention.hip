@@ -34,6 +34,12 @@ constexpr int kTile = 64;     // keys a wavefront takes at a time
 constexpr int kMinTiles = 4;  // fewest tiles worth a workgroup: one per wavefront
 constexpr int kPairCost = 4;  // what starting and joining a pair costs, in tiles
 
+// A value that all lanes of a wavefront share, for scalar registers.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    return (int64_t)((uint64_t)(uint32_t)uniform((int)x) | (uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32);
+}
+
 // Which keys the query rows of one block see: those of [0, end) that are in a
 // row's window or among the sinks lie in tiles [0, sink_tiles) and [start, ..).
 struct Span {
@@ -224,68 +230,74 @@ struct Wave {
 // A tile's place in the cache for one lane: the run whose keys it reads as
 // rows, and the run whose values (and whose keys' scores) it holds.
 struct Runs {
-    int64_t k_page, v_page;
-    int k_slot, v_slot;
-    bool v_ok;
+    int k_page, v_page;
 };
+
+// First keys of a tile's runs that this lane reads as rows, and whose values it reads.
+__device__ __forceinline__ int k_first(int tile) { return tile * kTile + (threadIdx.x >> 2 & 3) * 16; }
+__device__ __forceinline__ int v_first(int tile) { return tile * kTile + (threadIdx.x >> 4 & 3) * 16; }
 
 __device__ __forceinline__ Runs find_runs(const AttnParams& p, const int32_t* table, int tile) {
-    const int lane = threadIdx.x & 63;
-    Runs r;
-    const int k_at = tile * kTile + ((lane & 15) >> 2) * 16, v_at = tile * kTile + (lane >> 4) * 16;
-    const int kp = (int)fdiv(k_at, p.by_page), vp = (int)fdiv(v_at, p.by_page);
-    r.k_slot = k_at - kp * p.page;
-    r.v_slot = v_at - vp * p.page;
-    r.k_page = table[kp < p.table_width ? kp : p.table_width - 1];
-    r.v_page = table[vp < p.table_width ? vp : p.table_width - 1];
-    return r;
+    const int kp = (int)fdiv(k_first(tile), p.by_page), vp = (int)fdiv(v_first(tile), p.by_page);
+    return {table[kp < p.table_width ? kp : p.table_width - 1], table[vp < p.table_width ? vp : p.table_width - 1]};
 }
 
-// What lies past the sequence's end or in no page is read from page 0 and masked.
-__device__ __forceinline__ void settle_runs(const AttnParams& p, Runs& r, int tile, int held) {
-    const int lane = threadIdx.x & 63;
-    r.v_ok = r.v_page >= 0 && r.v_page < p.pages && tile * kTile + (lane >> 4) * 16 < held;
+// What lies past the sequence's end or in no page is read from page 0 and
+// masked; whether the values' run does not.
+__device__ __forceinline__ bool settle_runs(const AttnParams& p, Runs& r, int tile, int held) {
+    const bool ok = r.v_page >= 0 && r.v_page < p.pages && v_first(tile) < held;
     if (r.k_page < 0 || r.k_page >= p.pages) r.k_page = 0;
-    if (!r.v_ok) r.v_page = 0;
+    if (!ok) r.v_page = 0;
+    return ok;
 }
 
-// The scales of the run whose keys' scores a lane holds. A value's scale is
-// 2^v_exp: probabilities are formed times it, as exp2 of one sum, and sums of
-// probabilities are taken with 2^-v_exp (two bfloat16 values of it in v_inv).
+__device__ __forceinline__ const uint8_t* k_run(const AttnParams& p, const Runs& r, int tile, int kh, int W) {
+    const int at = k_first(tile), slot = at - (int)fdiv(at, p.by_page) * p.page;
+    return p.k + (((int64_t)r.k_page * p.heads + kh) * p.page + slot + (threadIdx.x & 3)) * W + (threadIdx.x >> 4 & 3) * 16;
+}
+
+__device__ __forceinline__ const uint8_t* v_run(const AttnParams& p, const Runs& r, int tile, int kh, int W) {
+    const int at = v_first(tile), slot = at - (int)fdiv(at, p.by_page) * p.page;
+    return p.v + (((int64_t)r.v_page * p.heads + kh) * W + (threadIdx.x & 15)) * p.page + slot;
+}
+
+// The scales of the run whose keys' scores a lane holds, as loaded: what is
+// made of them is made where they are used, not where that would be a wait for
+// them. A value's scale is 2^v_exp(): probabilities are formed times it, as
+// exp2 of one sum, and sums of probabilities are taken with 2^-v_exp().
 struct Scales {
-    float k, v_exp;
-    uint32_t v_inv;
+    float k, v;
     bool ok;
+
+    __device__ __forceinline__ float key() const { return ok ? k : 0.f; }
+    __device__ __forceinline__ float v_exp() const { return ok ? (float)((int)(__float_as_uint(v) >> 23 & 255) - 127) : 0.f; }
+    // 2^-v_exp() as two bfloat16 values; the low one is that of a float in its upper half.
+    __device__ __forceinline__ uint32_t v_inv() const {
+        const uint32_t inv = (ok ? 254 - (__float_as_uint(v) >> 23 & 255) : 127u) << 7;
+        return inv | inv << 16;
+    }
 };
 
-__device__ __forceinline__ Scales load_scales(const AttnParams& p, const Runs& r, int kh) {
-    const int64_t at = r.v_page * p.heads + kh;
-    const int e = r.v_ok ? (int)(__float_as_uint(p.v_scale[at]) >> 23 & 255) - 127 : 0;
-    const uint32_t inv = (uint32_t)(127 - e) << 7;
-    return {r.v_ok ? p.k_scale[at] : 0.f, (float)e, inv | inv << 16, r.v_ok};
+__device__ __forceinline__ Scales load_scales(const AttnParams& p, const Runs& r, int kh, bool ok) {
+    const int64_t at = (int64_t)r.v_page * p.heads + kh;
+    return {p.k_scale[at], p.v_scale[at], ok};
 }
 
 template <int W>
 struct Tile {
     u32x4 k[4][W / 64], v[W / 16];
 
-    __device__ __forceinline__ Scales load_k(const AttnParams& p, const Runs& r, int kh) {
-        const int lane = threadIdx.x & 63;
-        const uint8_t* src =
-            p.k + ((r.k_page * p.heads + kh) * p.page + r.k_slot + (lane & 3)) * W + (lane >> 4) * 16;
+    __device__ __forceinline__ void load_k(const uint8_t* src) {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int c = 0; c < W / 64; ++c) k[t][c] = *reinterpret_cast<const u32x4*>(src + t * 4 * W + c * 64);
-        return load_scales(p, r, kh);
     }
-    __device__ __forceinline__ void load_v(const AttnParams& p, const Runs& r, int kh) {
-        const int lane = threadIdx.x & 63;
-        const uint8_t* src = p.v + ((r.v_page * p.heads + kh) * W + (lane & 15)) * p.page + r.v_slot;
+    __device__ __forceinline__ void load_v(const uint8_t* src, int page) {
 #pragma unroll
         for (int d = 0; d < W / 16; ++d) {
             v[d] = *reinterpret_cast<const u32x4*>(src);
-            src += 16 * p.page;
+            src += 16 * page;
         }
     }
 };
@@ -399,13 +411,15 @@ __device__ __forceinline__ void mask_scores(const AttnParams& p, Wave<T, W, MT>&
 
 // The weights of one tile's keys, of products s (-inf where masked), as the
 // operands of the second product, and their sum and maximum in the running state.
-template <typename T, int W, int MT>
+template <typename T, int W, int MT, bool SumOnMfma>
 __device__ __forceinline__ void tile_weights(const AttnParams& p, Wave<T, W, MT>& w, const Scales& sc, f32x4 (&s)[MT][4],
                                              u32x4 (&prob)[MT][Wave<T, W, MT>::PP][2]) {
     typedef Wave<T, W, MT> WV;
     // Not zero, so that a masked score stays -inf whatever the scale.
-    const float c = fmaxf(sc.k * p.scale, 1e-30f);
-    const u32x4 one = {sc.v_inv, sc.v_inv, sc.v_inv, sc.v_inv};
+    const float c = fmaxf(sc.key() * p.scale, 1e-30f);
+    const uint32_t inv = sc.v_inv();
+    const u32x4 one = {inv, inv, inv, inv};
+    const float v_exp = sc.v_exp();
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         float top = s[mt][0][0];
@@ -423,7 +437,7 @@ __device__ __forceinline__ void tile_weights(const AttnParams& p, Wave<T, W, MT>
 #pragma unroll
             for (int d = 0; d < W / 16; ++d) w.o[mt][d] *= keep;
         }
-        const float shift = sc.v_exp - (w.m[mt] == -INFINITY ? 0.f : w.m[mt]);
+        const float shift = v_exp - (w.m[mt] == -INFINITY ? 0.f : w.m[mt]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             float e[8];
@@ -432,10 +446,14 @@ __device__ __forceinline__ void tile_weights(const AttnParams& p, Wave<T, W, MT>
                 e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][2 * h + i / 4][i & 3], c, shift));
             u32x4 parts[WV::PP];
             split8<WV::PP>(e, parts);
+            if constexpr (!SumOnMfma) {
+                const float sum = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+                w.l[mt][0] += sum * __uint_as_float(inv << 16);
+            }
 #pragma unroll
             for (int n = 0; n < WV::PP; ++n) {
                 prob[mt][n][h] = parts[n];
-                w.l[mt] = mma_bf16(one, parts[n], w.l[mt]);
+                if constexpr (SumOnMfma) w.l[mt] = mma_bf16(one, parts[n], w.l[mt]);
             }
         }
     }
@@ -468,21 +486,27 @@ __device__ __forceinline__ void walk(const AttnParams& p, Wave<T, W, MT>& w, con
     const int32_t* table = p.table + b * p.table_stride;
     const Sure sure(p, sp);
     Tile<W> x;
-    int tile = tile_at(sp, first);
-    settle_runs(p, r, tile, sp.held);
-    Scales sc = x.load_k(p, r, kh);
+    // Loads return in order, so what is needed first is asked for first: the
+    // pages of the tile after next, this tile's values, the next one's keys.
+    int tile = tile_at(sp, first), next = tile_at(sp, first + step < last ? first + step : first);
+    Scales sc = load_scales(p, r, kh, settle_runs(p, r, tile, sp.held));
+    x.load_k(k_run(p, r, tile, kh, W));
+    Runs rn = find_runs(p, table, next);
     for (int i = first; i < last; i += step) {
-        x.load_v(p, r, kh);
+        const int after = i + 2 * step < last ? tile_at(sp, i + 2 * step) : next;
+        const Runs ra = find_runs(p, table, after);
+        x.load_v(v_run(p, r, tile, kh, W), p.page);
         __builtin_amdgcn_sched_barrier(0);  // in flight while the scores are formed
-        const int next = tile_at(sp, i + step < last ? i + step : i);
-        r = find_runs(p, table, next);
         f32x4 s[MT][4];
         tile_scores<T, W, MT>(w, x, s);
         const Scales now = sc;
         if (i + step < last) {
-            settle_runs(p, r, next, sp.held);
-            sc = x.load_k(p, r, kh);
+            r = rn;
+            const bool ok = settle_runs(p, r, next, sp.held);
+            sc = load_scales(p, r, kh, ok);
+            x.load_k(k_run(p, r, next, kh, W));
         }
+        rn = ra;
         __builtin_amdgcn_sched_barrier(0);  // in flight while the tile is folded
         const bool full = sure.sees(p, tile) && __all(now.ok);
         if (full) {
@@ -503,7 +527,7 @@ __device__ __forceinline__ void walk(const AttnParams& p, Wave<T, W, MT>& w, con
             }
         }
         u32x4 prob[MT][WV::PP][2];
-        tile_weights<T, W, MT>(p, w, now, s, prob);
+        tile_weights<T, W, MT, false>(p, w, now, s, prob);
 #pragma unroll
         for (int d = 0; d < W / 16; ++d)
 #pragma unroll
@@ -515,6 +539,7 @@ __device__ __forceinline__ void walk(const AttnParams& p, Wave<T, W, MT>& w, con
                     for (int n = 0; n < WV::PP; ++n) w.o[mt][d] = mma_bf16(a, prob[mt][n][h], w.o[mt][d]);
             }
         tile = next;
+        next = after;
     }
 }
 
@@ -553,8 +578,8 @@ __device__ __forceinline__ void join_waves(const AttnParams& p, Wave<T, W, 1>& w
     __shared__ float sm[4][16], sl[4][16];
     __shared__ float so[4][16][68];
     const int tid = fresh_lane(threadIdx.x), dim = fresh(p.dim);
-    const int lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
-    const float l = w.l[0][0];
+    const int lane = tid & 63, wave = uniform(tid >> 6), c = lane & 15, g = lane >> 4;
+    const float l = column_sum(w.l[0][0]);
     const bool any = column_sum(w.any[0] ? 1.f : 0.f) > 0.f;
     if (g == 0) {
         sm[wave][c] = w.m[0];
@@ -625,7 +650,7 @@ __device__ __forceinline__ Weights all_weights(const AttnParams& p, int limit) {
         w.total += __shfl_xor(w.total, off, 64);
         w.before += __shfl_xor(w.before, off, 64);
     }
-    return w;
+    return {uniform(w.total), uniform(w.before)};
 }
 
 __device__ __forceinline__ int64_t share_of(const AttnParams& p, int64_t total) {
@@ -644,7 +669,7 @@ constexpr int kWavesPerSimd = Parts<T>::q * MT * W > 256 || W > 128 ? 1 : 2;
 
 template <typename T, int W>
 __global__ __launch_bounds__(256, (kWavesPerSimd<T, W, 1>)) void kv_attention_few_kernel(AttnParams p) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
     Wave<T, W, 1> w;
     // This workgroup's places [pos, stop) of the list, and sequence b, whose first pair is at `at`.
     int64_t pos, stop, at = 0;
@@ -683,10 +708,10 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, W, 1>)) void kv_attention_fe
             if (past) {
                 const int f = __builtin_ctzll(past);
                 b = b0 + f;
-                at += __shfl(upto - mine, f, 64);
+                at += uniform((int64_t)__shfl(upto - mine, f, 64));
                 break;
             }
-            at += __shfl(upto, 63, 64);
+            at += uniform((int64_t)__shfl(upto, 63, 64));
         }
     }
     while (pos < stop) {
@@ -776,7 +801,7 @@ __global__ __launch_bounds__(256) void kv_attention_few_join_kernel(AttnParams p
     const int64_t g0 = pair / per, g1 = (pair + sp.tiles - 1) / per;
     if (g0 == g1) return;
     const float* base = p.part + g0 * 2 * kSlot;
-    for (int row = threadIdx.x >> 6; row < sp.live; row += 4)
+    for (int row = uniform((int)threadIdx.x >> 6); row < sp.live; row += 4)
         join_row<T, W>(base + kSlot, base, 2 * kSlot, (int)(g1 - g0 + 1), row, 16 * W + row, 16 * W + 16 + row, p.dim,
                        out_row<T>(p, b, kh, row));
 }
@@ -794,7 +819,7 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 ? 2 : 1)) void kv_attention_many_
     static_assert(kLoads % NW == 0, "pieces divide evenly");
     __shared__ u32x4 lds[2][2 * kLoads][64];
     __shared__ int nan_values[3];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     int id = blockIdx.x;
     const int part = id % p.groups;
     id /= p.groups;
@@ -817,16 +842,15 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 ? 2 : 1)) void kv_attention_many_
         u32x4 raw[kMine];
         Scales sc;
         // Piece n of a tile: of its keys (row block n % 4, elements 64 (n / 4) ..) or, from kKeys on, of its values.
-        auto load = [&](const Runs& r) {
-            const uint8_t* k = p.k + ((r.k_page * p.heads + kh) * p.page + r.k_slot + (lane & 3)) * W + (lane >> 4) * 16;
-            const uint8_t* v = p.v + ((r.v_page * p.heads + kh) * W + c) * p.page + r.v_slot;
+        auto load = [&](const Runs& r, int tile, bool ok) {
+            sc = load_scales(p, r, kh, ok);
+            const uint8_t *k = k_run(p, r, tile, kh, W), *v = v_run(p, r, tile, kh, W);
 #pragma unroll
             for (int i = 0; i < kMine; ++i) {
                 const int n = wave + i * NW;
                 const uint8_t* src = n < kKeys ? k + n % 4 * 4 * W + n / 4 * 64 : v + (int64_t)(n - kKeys) * 16 * p.page;
                 raw[i] = *reinterpret_cast<const u32x4*>(src);
             }
-            sc = load_scales(p, r, kh);
         };
         auto stage = [&](int buffer, int flag, int tile, bool ok) {
             uint32_t nan = 0;
@@ -858,9 +882,9 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 ? 2 : 1)) void kv_attention_many_
         __syncthreads();
         int tile = tile_at(all, first), turn = 0;
         Runs r = find_runs(p, table, tile);
-        settle_runs(p, r, tile, all.held);
-        load(r);
-        stage(0, 0, tile, sc.ok);
+        const bool ok = settle_runs(p, r, tile, all.held);
+        load(r, tile, ok);
+        stage(0, 0, tile, ok);
         Scales now = sc;
         Runs at = r;
         int next = first + 1 < last ? tile_at(all, first + 1) : tile;
@@ -868,14 +892,12 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 ? 2 : 1)) void kv_attention_many_
         __syncthreads();
         for (int i = first; i < last; ++i) {
             const bool more = i + 1 < last;
-            if (more) {
-                settle_runs(p, r, next, all.held);
-                load(r);
-            }
-            __builtin_amdgcn_sched_barrier(0);  // in flight while this tile is worked on
-            const Runs after = r;
             const int tile2 = i + 2 < last ? tile_at(all, i + 2) : next;
+            const bool fits = more && settle_runs(p, r, next, all.held);
+            const Runs after = r;
             r = find_runs(p, table, tile2);
+            if (more) load(after, next, fits);
+            __builtin_amdgcn_sched_barrier(0);  // in flight while this tile is worked on
             const u32x4(*keys)[64] = lds[(i - first) & 1];
             const u32x4(*values)[64] = keys + kLoads;
             f32x4 s[MT][4];
@@ -907,12 +929,12 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 ? 2 : 1)) void kv_attention_many_
                 mask_scores<T, W, MT>(p, w, now.ok, s, tile, mask);
             }
             u32x4 prob[MT][WV::PP][2];
-            tile_weights<T, W, MT>(p, w, now, s, prob);
+            tile_weights<T, W, MT, true>(p, w, now, s, prob);
             if (!full && nan_values[turn]) {
                 // NaN among values that not every row sees: from the codes, as
                 // rarely as that happens.
                 const Edge<MT> edge(mask);
-                const uint8_t* v = p.v + ((at.v_page * p.heads + kh) * W + c) * p.page + at.v_slot;
+                const uint8_t* v = v_run(p, at, tile, kh, W);
 #pragma unroll
                 for (int d = 0; d < W / 16; ++d) {
                     f32x4 o[MT];
@@ -994,7 +1016,7 @@ __global__ __launch_bounds__(256) void kv_attention_many_join_kernel(AttnParams 
     const int kh = id % p.heads;
     id /= p.heads;
     const int rb = id % p.row_blocks, b = id / p.row_blocks;
-    const int row0 = rb * kRows, r = chunk * 4 + (threadIdx.x >> 6);
+    const int row0 = rb * kRows, r = chunk * 4 + uniform((int)threadIdx.x >> 6);
     const Span all = span_of(p, b, row0, kRows);
     if (row0 + r >= p.tokens * p.share || all.tiles <= 0) return;
     const int per = (all.tiles + p.groups - 1) / p.groups;
