@@ -365,13 +365,22 @@ struct Edge {
             for (int i = 0; i < 8; ++i)
                 seen[mt][i / 4][i % 4] = (mask[mt] >> 2 * i & 1 ? 0x3f80u : 0u) | (mask[mt] >> 2 * i & 2 ? 0x3f800000u : 0u);
     }
-    // Clears the codes v of one block of 16 elements, o[mt] its output.
-    __device__ __forceinline__ u32x4 clear(u32x4 v, f32x4 (&o)[MT]) const {
-        u32x4 flag;
+    // Clears the codes v of one block of 16 elements and tells of NaN among the rest.
+    __device__ __forceinline__ uint32_t clear(u32x4& v) const {
         uint32_t nan = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             v[i] &= keep[i];
+            nan |= nan_bytes(v[i]);
+        }
+        return nan;
+    }
+    // Takes NaN out of cleared codes, o[mt] being the block's output.
+    __device__ __forceinline__ u32x4 settle_nan(u32x4 v, f32x4 (&o)[MT]) const {
+        u32x4 flag;
+        uint32_t nan = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
             const uint32_t at = nan_bytes(v[i]);
             flag[i] = at * 0x38u;  // the code of 1.0
             v[i] &= ~(at * 0xffu);
@@ -516,14 +525,19 @@ __device__ __forceinline__ void walk(const AttnParams& p, Wave<T, W, MT>& w, con
             uint32_t mask[MT];
             mask_scores<T, W, MT>(p, w, now.ok, s, tile, mask);
             const Edge<MT> edge(mask);
+            uint32_t nan = 0;
 #pragma unroll
-            for (int d = 0; d < W / 16; ++d) {
-                f32x4 o[MT];
+            for (int d = 0; d < W / 16; ++d) nan |= edge.clear(x.v[d]);
+            if (__any(nan != 0)) {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) o[mt] = w.o[mt][d];
-                x.v[d] = edge.clear(x.v[d], o);
+                for (int d = 0; d < W / 16; ++d) {
+                    f32x4 o[MT];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) w.o[mt][d] = o[mt];
+                    for (int mt = 0; mt < MT; ++mt) o[mt] = w.o[mt][d];
+                    x.v[d] = edge.settle_nan(x.v[d], o);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) w.o[mt][d] = o[mt];
+                }
             }
         }
         u32x4 prob[MT][WV::PP][2];
@@ -940,7 +954,9 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 ? 2 : 1)) void kv_attention_many_
                     f32x4 o[MT];
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) o[mt] = w.o[mt][d];
-                    const u32x4 x = edge.clear(*reinterpret_cast<const u32x4*>(v + (int64_t)d * 16 * p.page), o);
+                    u32x4 x = *reinterpret_cast<const u32x4*>(v + (int64_t)d * 16 * p.page);
+                    edge.clear(x);
+                    x = edge.settle_nan(x, o);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const u32x4 a = widen8<false>(x[2 * h], x[2 * h + 1]);
