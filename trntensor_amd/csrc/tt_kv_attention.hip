@@ -832,7 +832,7 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 ? 2 : 1)) void kv_attention_many_
     constexpr int kKeys = W / 16, kLoads = 2 * kKeys, kMine = kLoads / NW;  // 16-byte pieces a lane: of keys, of a tile, a wavefront's
     static_assert(kLoads % NW == 0, "pieces divide evenly");
     __shared__ u32x4 lds[2][2 * kLoads][64];
-    __shared__ int nan_values[3];
+    __shared__ int nan_values[3];  // whether tile n's values, if some row does not see them all, hold NaN: at n % 3
     const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     int id = blockIdx.x;
     const int part = id % p.groups;
@@ -866,14 +866,15 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 ? 2 : 1)) void kv_attention_many_
                 raw[i] = *reinterpret_cast<const u32x4*>(src);
             }
         };
-        auto stage = [&](int buffer, int flag, int tile, bool ok) {
+        auto stage = [&](int n, int tile, bool ok) {
+            const int buffer = n & 1;
             uint32_t nan = 0;
 #pragma unroll
             for (int i = 0; i < kMine; ++i) {
-                const int n = wave + i * NW;
+                const int piece = wave + i * NW;
                 u32x4 x = raw[i];
-                if (n < kKeys) {
-                    const int at = n % 4 * (W / 32) + n / 4 * 2;
+                if (piece < kKeys) {
+                    const int at = piece % 4 * (W / 32) + piece / 4 * 2;
                     lds[buffer][at][lane] = widen8<WV::kHalf>(x[0], x[1]);
                     lds[buffer][at + 1][lane] = widen8<WV::kHalf>(x[2], x[3]);
                 } else {
@@ -882,58 +883,71 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 ? 2 : 1)) void kv_attention_many_
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             x[j] &= bits_to_bytes(live >> 4 * j) * 0xffu;
-                            nan |= nan_bytes(x[j]);
+                            const uint32_t at = nan_bytes(x[j]);
+                            nan |= at;
+                            x[j] &= ~(at * 0xffu);
                         }
                     }
-                    const int at = kLoads + (n - kKeys) * 2;
+                    const int at = kLoads + (piece - kKeys) * 2;
                     lds[buffer][at][lane] = widen8<false>(x[0], x[1]);
                     lds[buffer][at + 1][lane] = widen8<false>(x[2], x[3]);
                 }
             }
-            if (nan) nan_values[flag] = 1;
+            if (nan) nan_values[n % 3] = 1;
         };
         if (threadIdx.x < 3) nan_values[threadIdx.x] = 0;
         __syncthreads();
-        int tile = tile_at(all, first), turn = 0;
+        const int tiles = last - first;
+        auto tile_of = [&](int n) { return tile_at(all, first + (n < tiles ? n : tiles - 1)); };
+        int tile = tile_of(0);
         Runs r = find_runs(p, table, tile);
         const bool ok = settle_runs(p, r, tile, all.held);
         load(r, tile, ok);
-        stage(0, 0, tile, ok);
+        stage(0, tile, ok);
         Scales now = sc;
         Runs at = r;
-        int next = first + 1 < last ? tile_at(all, first + 1) : tile;
-        r = find_runs(p, table, next);
+        r = find_runs(p, table, tile_of(1));
+        f32x4 s[MT][4];
         __syncthreads();
-        for (int i = first; i < last; ++i) {
-            const bool more = i + 1 < last;
-            const int tile2 = i + 2 < last ? tile_at(all, i + 2) : next;
-            const bool fits = more && settle_runs(p, r, next, all.held);
-            const Runs after = r;
-            r = find_runs(p, table, tile2);
-            if (more) load(after, next, fits);
-            __builtin_amdgcn_sched_barrier(0);  // in flight while this tile is worked on
-            const u32x4(*keys)[64] = lds[(i - first) & 1];
-            const u32x4(*values)[64] = keys + kLoads;
-            f32x4 s[MT][4];
+        auto scores = [&](const u32x4(*keys)[64]) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int t = 0; t < 4; ++t) s[mt][t] = f32x4{0, 0, 0, 0};
+            u32x4 a[2][4];
 #pragma unroll
-            for (int e = 0; e < W / 32; ++e)
+            for (int t = 0; t < 4; ++t) a[0][t] = keys[t * (W / 32)][lane];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const u32x4 a = keys[t * (W / 32) + e][lane];
+            for (int e = 0; e < W / 32; ++e) {
+                if (e + 1 < W / 32) {
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int n = 0; n < WV::QP; ++n) {
-                            if constexpr (WV::kHalf)
-                                s[mt][t] = mma_f16(a, w.q[mt][n][e], s[mt][t]);
-                            else
-                                s[mt][t] = mma_bf16(a, w.q[mt][n][e], s[mt][t]);
-                        }
+                    for (int t = 0; t < 4; ++t) a[(e + 1) & 1][t] = keys[t * (W / 32) + e + 1][lane];
                 }
+                __builtin_amdgcn_sched_barrier(0);  // read a step ahead
+#pragma unroll
+                for (int n = 0; n < WV::QP; ++n)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            if constexpr (WV::kHalf)
+                                s[mt][t] = mma_f16(a[e & 1][t], w.q[mt][n][e], s[mt][t]);
+                            else
+                                s[mt][t] = mma_bf16(a[e & 1][t], w.q[mt][n][e], s[mt][t]);
+                        }
+            }
+        };
+        // Between two barriers, tile n of the walk is worked on in buffer n % 2 and
+        // tile n + 1 loaded, then staged in the other.
+        for (int n = 0; n < tiles; ++n) {
+            const bool more = n + 1 < tiles;
+            const int next = tile_of(n + 1);
+            const bool fits = more && settle_runs(p, r, next, all.held);
+            const Runs after = r;
+            r = find_runs(p, table, tile_of(n + 2));
+            if (more) load(after, next, fits);
+            __builtin_amdgcn_sched_barrier(0);  // in flight while this tile is worked on
+            scores(lds[n & 1]);
             const bool full = sure.sees(p, tile) && __all(now.ok);
             uint32_t mask[MT];
             if (full) {
@@ -944,9 +958,9 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 ? 2 : 1)) void kv_attention_many_
             }
             u32x4 prob[MT][WV::PP][2];
             tile_weights<T, W, MT, true>(p, w, now, s, prob);
-            if (!full && nan_values[turn]) {
-                // NaN among values that not every row sees: from the codes, as
-                // rarely as that happens.
+            if (!full && nan_values[n % 3]) {
+                // Values staged without their NaN, which not every row
+                // sees: it is given to those that do.
                 const Edge<MT> edge(mask);
                 const uint8_t* v = v_run(p, at, tile, kh, W);
 #pragma unroll
@@ -956,38 +970,34 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 ? 2 : 1)) void kv_attention_many_
                     for (int mt = 0; mt < MT; ++mt) o[mt] = w.o[mt][d];
                     u32x4 x = *reinterpret_cast<const u32x4*>(v + (int64_t)d * 16 * p.page);
                     edge.clear(x);
-                    x = edge.settle_nan(x, o);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const u32x4 a = widen8<false>(x[2 * h], x[2 * h + 1]);
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                            for (int n = 0; n < WV::PP; ++n) o[mt] = mma_bf16(a, prob[mt][n][h], o[mt]);
-                    }
+                    edge.settle_nan(x, o);
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) w.o[mt][d] = o[mt];
+                    __builtin_amdgcn_sched_barrier(0);  // one at a time: registers matter more
                 }
-            } else {
-#pragma unroll
-                for (int d = 0; d < W / 16; ++d)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const u32x4 a = values[d * 2 + h][lane];
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                            for (int n = 0; n < WV::PP; ++n) w.o[mt][d] = mma_bf16(a, prob[mt][n][h], w.o[mt][d]);
-                    }
             }
-            const int turn1 = turn == 2 ? 0 : turn + 1, turn2 = turn1 == 2 ? 0 : turn1 + 1;
-            if (threadIdx.x == 0) nan_values[turn2] = 0;
-            if (more) stage((i + 1 - first) & 1, turn1, next, sc.ok);
+            const u32x4(*values)[64] = lds[n & 1] + kLoads;
+            u32x4 a[2][2] = {{values[0][lane], values[1][lane]}};
+#pragma unroll
+            for (int d = 0; d < W / 16; ++d) {
+                if (d + 1 < W / 16) {
+                    a[(d + 1) & 1][0] = values[d * 2 + 2][lane];
+                    a[(d + 1) & 1][1] = values[d * 2 + 3][lane];
+                }
+                __builtin_amdgcn_sched_barrier(0);  // read a block ahead
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < WV::PP; ++i) w.o[mt][d] = mma_bf16(a[d & 1][h], prob[mt][i][h], w.o[mt][d]);
+            }
+            // Marks of NaN: tile n's is read here, n + 1's set, n + 2's cleared.
+            if (threadIdx.x == 0) nan_values[(n + 2) % 3] = 0;
+            if (more) stage(n + 1, next, fits);
             now = sc;
             at = after;
             tile = next;
-            next = tile2;
-            turn = turn1;
             __syncthreads();
         }
     }
