@@ -231,55 +231,64 @@ __device__ __forceinline__ void turn_pieces(const float* c, const float* s, bool
 //            place of every head, so that it reads its angles once
 // Head sizes are multiples of 8 here and rotated parts of 16.
 template <typename T, int W>
-__global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p) {
+__device__ __forceinline__ void rotate_token(const AppendParams& p, int64_t row) {
+    constexpr int kRow = W / 16;  // lanes a head
+    const int tid = threadIdx.x, D = (int)p.c.dim;
+    const int64_t b = row / p.tokens, t = row - b * p.tokens;
+    if (b >= p.batch) return;
+    const int64_t n = p.counts ? p.counts[b] : p.tokens, pos = (int64_t)p.lengths[b] + t;
+    const bool live = t < n && pos >= 0 && pos < p.table_width * p.c.page;
+    const T* q = static_cast<const T*>(p.q) + b * p.q_stride[0] + t * p.q_stride[1];
+    T* out = static_cast<T*>(p.q_out) + row * p.q_heads * D;
+    constexpr int kLanes = 64 / kRow * kRow;  // lanes at work: whole rows
+    const int lane = tid & 63;
+    if (lane >= kLanes) return;
+    const Pieces at = pieces_of(p, lane % kRow, true);
+    float c[8], s[8];
+    if (live && at.turn >= 0) {
+        __builtin_memcpy(c, p.cos + pos * (p.rot / 2) + at.turn, sizeof c);
+        __builtin_memcpy(s, p.sin + pos * (p.rot / 2) + at.turn, sizeof s);
+    }
+    constexpr int kHeads = 64 / kRow;
+    for (int h0 = lane / kRow; h0 < p.q_heads; h0 += 4 * kHeads) {
+        T x[4][2][8];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int h = h0 + u * kHeads;
+            const T* src = q + h * p.q_stride[2];
+            if (live && h < p.q_heads) {
+                if (at.a < D) __builtin_memcpy(x[u][0], src + at.a, sizeof x[u][0]);
+                if (at.b < D) __builtin_memcpy(x[u][1], src + at.b, sizeof x[u][1]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int h = h0 + u * kHeads;
+            if (h >= p.q_heads) break;
+            float v[2][8];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i / 8][i % 8] = live ? to_f32(x[u][i / 8][i % 8]) : 0.f;
+            if (live && at.turn >= 0) turn_pieces(c, s, p.interleaved, v[0], v[1]);
+            T y[2][8];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i / 8][i % 8] = (T)v[i / 8][i % 8];
+            if (at.a < D) __builtin_memcpy(out + (int64_t)h * D + at.a, y[0], sizeof y[0]);
+            if (at.b < D) __builtin_memcpy(out + (int64_t)h * D + at.b, y[1], sizeof y[1]);
+        }
+    }
+}
+
+template <typename T, int W>
+__global__ __launch_bounds__(256) void rotate_queries_kernel(AppendParams p) {
+    rotate_token<T, W>(p, (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6));
+}
+
+template <typename T, int W, bool Queries>
+__global__ __launch_bounds__(256, (Queries ? 2 : 4)) void kv_append_kernel(AppendParams p) {
     constexpr int kRow = W / 16;  // threads a row
     const int tid = threadIdx.x, D = (int)p.c.dim;
-    if (blockIdx.x >= p.kv_groups) {
-        const int64_t row = (int64_t)(blockIdx.x - p.kv_groups) * 4 + (tid >> 6);
-        const int64_t b = row / p.tokens, t = row - b * p.tokens;
-        if (b >= p.batch) return;
-        const int64_t n = p.counts ? p.counts[b] : p.tokens, pos = (int64_t)p.lengths[b] + t;
-        const bool live = t < n && pos >= 0 && pos < p.table_width * p.c.page;
-        const T* q = static_cast<const T*>(p.q) + b * p.q_stride[0] + t * p.q_stride[1];
-        T* out = static_cast<T*>(p.q_out) + row * p.q_heads * D;
-        constexpr int kLanes = 64 / kRow * kRow;  // lanes at work: whole rows
-        const int lane = tid & 63;
-        if (lane >= kLanes) return;
-        const Pieces at = pieces_of(p, lane % kRow, true);
-        float c[8], s[8];
-        if (live && at.turn >= 0) {
-            __builtin_memcpy(c, p.cos + pos * (p.rot / 2) + at.turn, sizeof c);
-            __builtin_memcpy(s, p.sin + pos * (p.rot / 2) + at.turn, sizeof s);
-        }
-        constexpr int kHeads = 64 / kRow;
-        for (int h0 = lane / kRow; h0 < p.q_heads; h0 += 4 * kHeads) {
-            float x[4][2][8];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int h = h0 + u * kHeads;
-                const T* src = q + h * p.q_stride[2];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[u][0][i] = x[u][1][i] = 0.f;
-                if (live && h < p.q_heads) {
-                    if (at.a < D) load8(src + at.a, x[u][0]);
-                    if (at.b < D) load8(src + at.b, x[u][1]);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int h = h0 + u * kHeads;
-                if (h >= p.q_heads) break;
-                if (live && at.turn >= 0) turn_pieces(c, s, p.interleaved, x[u][0], x[u][1]);
-                T y[2][8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    y[0][i] = (T)x[u][0][i];
-                    y[1][i] = (T)x[u][1][i];
-                }
-                if (at.a < D) __builtin_memcpy(out + (int64_t)h * D + at.a, y[0], sizeof y[0]);
-                if (at.b < D) __builtin_memcpy(out + (int64_t)h * D + at.b, y[1], sizeof y[1]);
-            }
-        }
+    if (Queries && blockIdx.x >= p.kv_groups) {
+        rotate_token<T, W>(p, (int64_t)(blockIdx.x - p.kv_groups) * 4 + (tid >> 6));
         return;
     }
     Block k;
@@ -448,23 +457,42 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p) {
     if (tid == 0) *k.scale = scale;
 }
 
-template <typename T>
-int append_launch(AppendParams& p, bool queries, hipStream_t st) {
-    const bool pieces = p.c.dim % 8 == 0 && p.rot % 16 == 0;
-    const int64_t rows = queries ? p.batch * p.tokens : 0, grid = p.kv_groups + (pieces ? (rows + 3) / 4 : rows);
-    if (grid > kMaxGrid) return set_error(TT_UNSUPPORTED, "tt_kv_append: %lld workgroups", (long long)grid);
-    const uint32_t g = (uint32_t)grid;
-    if (!pieces)
-        kv_append_any_kernel<T><<<g, 256, 0, st>>>(p);
-    else if (p.width == 64)
-        kv_append_kernel<T, 64><<<g, 256, 0, st>>>(p);
-    else if (p.width == 128)
-        kv_append_kernel<T, 128><<<g, 256, 0, st>>>(p);
-    else if (p.width == 192)
-        kv_append_kernel<T, 192><<<g, 256, 0, st>>>(p);
-    else
-        kv_append_kernel<T, 256><<<g, 256, 0, st>>>(p);
+// A few workgroups are one launch. Many are two, so that neither kind holds the
+// other's registers: four prompts of 4096 tokens took 108 us as one launch and
+// 93 as two, one token of eight sequences 4.9 us as one.
+constexpr int64_t kOneLaunch = 2048;
+
+template <typename T, int W>
+int append_width(const AppendParams& p, int64_t rows, hipStream_t st) {
+    const int64_t groups = (rows + 3) / 4;
+    if (p.kv_groups + groups <= kOneLaunch) {
+        kv_append_kernel<T, W, true><<<(uint32_t)(p.kv_groups + groups), 256, 0, st>>>(p);
+    } else {
+        kv_append_kernel<T, W, false><<<(uint32_t)p.kv_groups, 256, 0, st>>>(p);
+        if (groups) rotate_queries_kernel<T, W><<<(uint32_t)groups, 256, 0, st>>>(p);
+    }
     return check_launch("tt_kv_append");
+}
+
+template <typename T>
+int append_launch(const AppendParams& p, bool queries, hipStream_t st) {
+    const int64_t rows = queries ? p.batch * p.tokens : 0;
+    if (p.kv_groups + rows > kMaxGrid)
+        return set_error(TT_UNSUPPORTED, "tt_kv_append: %lld workgroups", (long long)(p.kv_groups + rows));
+    if (p.c.dim % 8 != 0 || p.rot % 16 != 0) {
+        kv_append_any_kernel<T><<<(uint32_t)(p.kv_groups + rows), 256, 0, st>>>(p);
+        return check_launch("tt_kv_append");
+    }
+    switch (p.width) {
+        case 64:
+            return append_width<T, 64>(p, rows, st);
+        case 128:
+            return append_width<T, 128>(p, rows, st);
+        case 192:
+            return append_width<T, 192>(p, rows, st);
+        default:
+            return append_width<T, 256>(p, rows, st);
+    }
 }
 
 }  // namespace
