@@ -15,8 +15,9 @@ def q4_weights(codes: torch.Tensor, scales: torch.Tensor, k: int, group: int, ze
     """(n, k) float64 weights: scale * (code - zero)."""
     n = codes.shape[0]
     w = torch.empty((n, k), dtype=torch.float64)
+    wide = codes.to(torch.int64)
     for j in range(k):
-        c = codes[:, j // 2].to(torch.int64)
+        c = wide[:, j // 2]
         c = c // 16 if j % 2 else c % 16
         z = 8.0 if zeros is None else zeros[:, j // group].double()
         w[:, j] = scales[:, j // group].double() * (c.double() - z)

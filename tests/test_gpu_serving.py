@@ -46,7 +46,7 @@ def _q4(n, k, group, dtype, zeros, seed):
 def _check_q4(x, codes, scales, z, k, group, y):
     w = ref.q4_weights(codes, scales, k, group, z)
     want = x.double() @ w.t()
-    ones = ref.q4_weights(codes, scales, k, group, z).abs()
+    ones = w.abs()
     s = scales.double()[:, torch.arange(k) // group]
     size = x.double().abs() @ (ones + 24.0 * s.abs()).t()
     tol = U[y.dtype] * want.abs() + 2.0 ** -24 * (16 + math.sqrt(k)) * size
@@ -77,6 +77,13 @@ def _check_q4(x, codes, scales, z, k, group, y):
         (130, 72, 512, 512),
         (1, 520, 4224, 128),
         (4, 24, 8192, 64),
+        # many rows on both sides
+        (17, 8200, 130, 128),
+        (32, 8320, 1024, 128),
+        (33, 8193, 1290, 256),
+        (64, 8448, 900, 128),
+        (100, 8209, 640, 128),
+        (20, 8288, 250, 32),
     ],
 )
 def test_q4_matmul(hip, m, n, k, group, zeros, dtype):

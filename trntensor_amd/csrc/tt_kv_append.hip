@@ -182,6 +182,29 @@ __device__ __forceinline__ void load8(const T* src, float* x) {
     for (int i = 0; i < 8; ++i) x[i] = to_f32(v[i]);
 }
 
+// Eight elements as they lie in memory.
+template <typename T>
+struct Eight {
+    u32x4 raw[sizeof(T) / 2];
+
+    __device__ __forceinline__ Eight() {}
+    __device__ __forceinline__ explicit Eight(const float* v) {
+        T t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = (T)v[i];
+        __builtin_memcpy(raw, t, sizeof raw);
+    }
+    __device__ __forceinline__ void load(const T* src) { __builtin_memcpy(raw, src, sizeof raw); }
+    __device__ __forceinline__ void store(T* dst) const { __builtin_memcpy(dst, raw, sizeof raw); }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(raw[i / 4][i % 4]);
+        if constexpr (sizeof(T) == 2) {
+            const uint16_t h = (uint16_t)(raw[0][i / 2] >> 16 * (i & 1));
+            return to_f32(__builtin_bit_cast(T, h));
+        }
+    }
+};
+
 // The two pieces of eight elements that one thread takes of a row: for the
 // rotated part a piece and the one it is paired with (the same distance into
 // the other half, or its neighbour), after that neighbours.
@@ -250,30 +273,28 @@ __device__ __forceinline__ void rotate_token(const AppendParams& p, int64_t row)
         __builtin_memcpy(s, p.sin + pos * (p.rot / 2) + at.turn, sizeof s);
     }
     constexpr int kHeads = 64 / kRow;
-    for (int h0 = lane / kRow; h0 < p.q_heads; h0 += 4 * kHeads) {
-        T x[4][2][8];
+    constexpr int kDeep = 2;  // heads of a lane in flight: more take more registers (four: 97 us for 95)
+    for (int h0 = lane / kRow; h0 < p.q_heads; h0 += kDeep * kHeads) {
+        Eight<T> x[kDeep][2];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < kDeep; ++u) {
             const int h = h0 + u * kHeads;
             const T* src = q + h * p.q_stride[2];
             if (live && h < p.q_heads) {
-                if (at.a < D) __builtin_memcpy(x[u][0], src + at.a, sizeof x[u][0]);
-                if (at.b < D) __builtin_memcpy(x[u][1], src + at.b, sizeof x[u][1]);
+                if (at.a < D) x[u][0].load(src + at.a);
+                if (at.b < D) x[u][1].load(src + at.b);
             }
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < kDeep; ++u) {
             const int h = h0 + u * kHeads;
             if (h >= p.q_heads) break;
             float v[2][8];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i / 8][i % 8] = live ? to_f32(x[u][i / 8][i % 8]) : 0.f;
+            for (int i = 0; i < 16; ++i) v[i / 8][i % 8] = live ? x[u][i / 8].get(i % 8) : 0.f;
             if (live && at.turn >= 0) turn_pieces(c, s, p.interleaved, v[0], v[1]);
-            T y[2][8];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) y[i / 8][i % 8] = (T)v[i / 8][i % 8];
-            if (at.a < D) __builtin_memcpy(out + (int64_t)h * D + at.a, y[0], sizeof y[0]);
-            if (at.b < D) __builtin_memcpy(out + (int64_t)h * D + at.b, y[1], sizeof y[1]);
+            if (at.a < D) Eight<T>(v[0]).store(out + (int64_t)h * D + at.a);
+            if (at.b < D) Eight<T>(v[1]).store(out + (int64_t)h * D + at.b);
         }
     }
 }
@@ -459,7 +480,7 @@ __global__ __launch_bounds__(256, (Queries ? 2 : 4)) void kv_append_kernel(Appen
 
 // A few workgroups are one launch. Many are two, so that neither kind holds the
 // other's registers: four prompts of 4096 tokens took 108 us as one launch and
-// 93 as two, one token of eight sequences 4.9 us as one.
+// 95 as two, one token of eight sequences 4.9 us as one.
 constexpr int64_t kOneLaunch = 2048;
 
 template <typename T, int W>

@@ -124,20 +124,6 @@ __device__ __forceinline__ f32x4 mma_f16(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Maximum and sum over the four lanes that share a query column (l, l ^ 16, l ^ 32, l ^ 48).
-__device__ __forceinline__ float column_max(float x) {
-    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float column_sum(float x) {
-    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 // One wavefront's running state for MT blocks of 16 query rows. With lane l,
 // column c = l % 16 is a query row and g = l / 16 a group of four lanes' rows:
 //   scores  s[mt][t][r]  key 16 g + 4 t + r of the tile, query row c
@@ -509,12 +495,12 @@ __device__ __forceinline__ void walk(const AttnParams& p, Wave<T, W, MT>& w, con
         f32x4 s[MT][4];
         tile_scores<T, W, MT>(w, x, s);
         const Scales now = sc;
-        if (i + step < last) {
-            r = rn;
-            const bool ok = settle_runs(p, r, next, sp.held);
-            sc = load_scales(p, r, kh, ok);
-            x.load_k(k_run(p, r, next, kh, W));
-        }
+        // (After the last tile it is loaded again: with the same loads in flight
+        // on every path, the wait for the values need not be one for the keys.)
+        r = rn;
+        const bool ok = settle_runs(p, r, next, sp.held);
+        sc = load_scales(p, r, kh, ok);
+        x.load_k(k_run(p, r, next, kh, W));
         rn = ra;
         __builtin_amdgcn_sched_barrier(0);  // in flight while the tile is folded
         const bool full = sure.sees(p, tile) && __all(now.ok);
@@ -942,10 +928,10 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 ? 2 : 1)) void kv_attention_many_
         for (int n = 0; n < tiles; ++n) {
             const bool more = n + 1 < tiles;
             const int next = tile_of(n + 1);
-            const bool fits = more && settle_runs(p, r, next, all.held);
+            const bool fits = settle_runs(p, r, next, all.held);
             const Runs after = r;
             r = find_runs(p, table, tile_of(n + 2));
-            if (more) load(after, next, fits);
+            load(after, next, fits);
             __builtin_amdgcn_sched_barrier(0);  // in flight while this tile is worked on
             scores(lds[n & 1]);
             const bool full = sure.sees(p, tile) && __all(now.ok);

@@ -322,10 +322,10 @@ __global__ __launch_bounds__(256) void q4_pack_kernel(int N, int K, int chunks, 
     for (int s = 0; s < 4; ++s) {
         const int at = chunk * 64 + s * 16 + (lane >> 4) * 4;
         uint32_t x = 0;
-        if (n < N) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (at + j < bytes) x |= (uint32_t)codes[n * pitch + at + j] << 8 * j;
+        if (n < N && at + 4 <= bytes) {
+            __builtin_memcpy(&x, codes + n * pitch + at, 4);
+        } else if (n < N) {
+            for (int j = 0; at + j < bytes; ++j) x |= (uint32_t)codes[n * pitch + at + j] << 8 * j;
         }
         uint32_t even = x & 0x0f0f0f0fu, odd = x >> 4 & 0x0f0f0f0fu;
         even = (even | even >> 4) & 0x00ff00ffu;

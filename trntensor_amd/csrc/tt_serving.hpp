@@ -58,6 +58,21 @@ __device__ __forceinline__ void split8(const float* x, u32x4* out) {
     }
 }
 
+// Maximum and sum over the four lanes that share a column of an MFMA's result
+// (l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float column_max(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float column_sum(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
 // Codes of one cache row: dim rounded up to a multiple of 64.
 inline int64_t kv_width(int64_t dim) { return (dim + 63) / 64 * 64; }
 
