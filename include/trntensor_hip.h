@@ -286,12 +286,8 @@ int tt_q4_pack(int64_t N, int64_t K, const void* codes, int64_t pitch, void* pac
 typedef struct {
     int64_t dtype, scale_dtype, M, N, K, group, ldx, ldy;
     const void *x, *codes, *scales, *zeros;
-    void *y, *workspace;
-    int64_t workspace_bytes;
+    void *y;
 } tt_q4_args;
-
-/* Device bytes of workspace that tt_q4_matmul needs (may be 0). */
-size_t tt_q4_matmul_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
 
 int tt_q4_matmul(const tt_q4_args* args, void* stream);
 

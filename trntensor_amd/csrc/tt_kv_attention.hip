@@ -745,8 +745,24 @@ __device__ __forceinline__ void join_row(const float* first, const float* rest, 
                                          int l_at, int dim, T* out) {
     const int lane = threadIdx.x & 63;
     auto slot = [&](int i) { return i ? rest + i * stride : first; };
-    float m = -INFINITY;
-    for (int i = lane; i < parts; i += 64) m = fmaxf(m, slot(i)[m_at]);
+    constexpr int kDeep = 8;
+    float x[kDeep][W / 64];
+    auto load = [&](int i) {
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u) {
+            const float* s = slot(i + u < parts ? i + u : parts - 1) + row * W + lane;
+#pragma unroll
+            for (int d = 0; d < W / 64; ++d) x[u][d] = s[d * 64];
+        }
+    };
+    // The first elements, maxima and weights are asked for together: which
+    // memory they come from is a longer way than what is done with them.
+    load(0);
+    const float* own = slot(lane < parts ? lane : parts - 1);
+    float m = own[m_at];
+    const float m_own = m, l_own = own[l_at];
+    __builtin_amdgcn_sched_barrier(0);
+    for (int i = lane + 64; i < parts; i += 64) m = fmaxf(m, slot(i)[m_at]);
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
     const float shift = m == -INFINITY ? 0.f : m;
     float sum = 0.f, o[W / 64] = {};
@@ -755,23 +771,16 @@ __device__ __forceinline__ void join_row(const float* first, const float* rest, 
         float f = 0.f;
         if (i0 + lane < parts) {
             const float* s = slot(i0 + lane);
-            const float l = s[l_at];
+            const float l = i0 ? s[l_at] : l_own;
             if (l != -1.f) {
-                f = exp2f(s[m_at] - shift);
+                f = exp2f((i0 ? s[m_at] : m_own) - shift);
                 sum += l * f;
                 some = true;
             }
         }
         const int n = parts - i0 < 64 ? parts - i0 : 64;
-        constexpr int kDeep = 8;
         for (int i = 0; i < n; i += kDeep) {
-            float x[kDeep][W / 64];
-#pragma unroll
-            for (int u = 0; u < kDeep; ++u) {
-                const float* s = slot(i0 + (i + u < n ? i + u : n - 1)) + row * W + lane;
-#pragma unroll
-                for (int d = 0; d < W / 64; ++d) x[u][d] = s[d * 64];
-            }
+            if (i0 + i > 0) load(i0 + i);
 #pragma unroll
             for (int u = 0; u < kDeep; ++u) {
                 if (i + u >= n) break;

@@ -81,25 +81,27 @@ struct Four {
     }
 };
 
-// One stage of a wavefront's operands: U chunks of 128 columns of 16 R weight
+constexpr int kWaves = 8;  // wavefronts a workgroup
+
+// One stage of a wavefront's operands: a chunk of 128 columns of 16 R weight
 // rows and 16 MT activation rows; GPC scales a chunk and row.
-template <typename T, int SW, int U, int R, int MT, int GPC>
+template <typename T, int SW, int R, int MT, int GPC>
 struct Stage {
-    u32x4 codes[U][R];
-    Four<SW> scales[U][R][GPC], zeros[U][R][GPC];
-    T x[U][MT][4][8];
+    u32x4 codes[R];
+    Four<SW> scales[R][GPC], zeros[R][GPC];
+    T x[MT][4][8];
 };
 
-// R blocks of 16 weight rows and MT of 16 activation rows a wavefront; the KW
+// R blocks of 16 weight rows and MT of 16 activation rows a wavefront; the
 // wavefronts of a workgroup take contiguous shares of the columns, which are
 // summed at the end in their order. GPC: the pieces of a chunk of 128 columns
 // that are scaled one by one, 1 for groups of at least a chunk, else 4.
-template <typename T, int SW, int U, int R, int MT, int GPC, int KW>
-__global__ __launch_bounds__(64 * KW, KW / 4 < 2 ? 2 : KW / 4) void q4_matmul_kernel(Q4Params p) {
+template <typename T, int SW, int R, int MT, int GPC>
+__global__ __launch_bounds__(64 * kWaves, 2) void q4_matmul_kernel(Q4Params p) {
     typedef typename Act<T>::half H;
     constexpr int NP = Act<T>::parts;
     constexpr int kSteps = 4 / GPC;  // MFMA steps of 32 columns a piece
-    __shared__ float so[KW][MT * 16][R * 16 + 4];
+    __shared__ float so[kWaves][MT * 16][R * 16 + 4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
     const int row_blocks = (p.N + 16 * R - 1) / (16 * R);
     const int m_blocks = (p.M + 16 * MT - 1) / (16 * MT);
@@ -115,7 +117,7 @@ __global__ __launch_bounds__(64 * KW, KW / 4 < 2 ? 2 : KW / 4) void q4_matmul_ke
         mb = (blockIdx.x - whole) / tail;
     }
     const int n0 = rb * 16 * R, m0 = mb * 16 * MT;
-    const int per = (p.chunks + KW - 1) / KW;
+    const int per = (p.chunks + kWaves - 1) / kWaves;
     const int first = wave * per, last = first + per < p.chunks ? first + per : p.chunks;
 
     // Rows past the end repeat the last ones: what they give is not stored.
@@ -154,36 +156,32 @@ __global__ __launch_bounds__(64 * KW, KW / 4 < 2 ? 2 : KW / 4) void q4_matmul_ke
         __builtin_memcpy(f.raw, static_cast<const uint8_t*>(base) + ((int64_t)group * scale_pitch + n) * SW, sizeof f.raw);
         return f;
     };
-    typedef Stage<T, SW, U, R, MT, GPC> St;
-    auto load = [&](St& st, int chunk) {
+    typedef Stage<T, SW, R, MT, GPC> St;
+    auto load = [&](St& st, int k) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int k = chunk + u < last ? chunk + u : last - 1;
+        for (int r = 0; r < R; ++r) st.codes[r] = *reinterpret_cast<const u32x4*>(code_row[r] + (int64_t)k * 1024);
+        const bool edge = ragged && k == p.chunks - 1;
 #pragma unroll
-            for (int r = 0; r < R; ++r) st.codes[u][r] = *reinterpret_cast<const u32x4*>(code_row[r] + (int64_t)k * 1024);
-            const bool edge = ragged && k == p.chunks - 1;
+        for (int mt = 0; mt < MT; ++mt) {
+            if (edge) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                if (edge) {
+                for (int s = 0; s < 4; ++s)
+                    __builtin_memcpy(st.x[mt][s], __builtin_assume_aligned(&filled[mt * 16 + c][s * 32 + g * 8], 16),
+                                     sizeof st.x[mt][s]);
+            } else {
+                const T* src = x_row[mt] + k * 128;
 #pragma unroll
-                    for (int s = 0; s < 4; ++s)
-                        __builtin_memcpy(st.x[u][mt][s], __builtin_assume_aligned(&filled[mt * 16 + c][s * 32 + g * 8], 16),
-                                         sizeof st.x[u][mt][s]);
-                } else {
-                    const T* src = x_row[mt] + k * 128;
-#pragma unroll
-                    for (int s = 0; s < 4; ++s) __builtin_memcpy(st.x[u][mt][s], src + s * 32, sizeof st.x[u][mt][s]);
-                }
+                for (int s = 0; s < 4; ++s) __builtin_memcpy(st.x[mt][s], src + s * 32, sizeof st.x[mt][s]);
             }
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int q = 0; q < GPC; ++q) {
-                    const int group = GPC > 1 ? (k * GPC + q) >> p.group_shift : k / p.chunks_per_group;
-                    st.scales[u][r][q] = load_four(p.scales, group, r);
-                    if (p.zeros) st.zeros[u][r][q] = load_four(p.zeros, group, r);
-                }
         }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int q = 0; q < GPC; ++q) {
+                const int group = GPC > 1 ? (k * GPC + q) >> p.group_shift : k / p.chunks_per_group;
+                st.scales[r][q] = load_four(p.scales, group, r);
+                if (p.zeros) st.zeros[r][q] = load_four(p.zeros, group, r);
+            }
     };
     f32x4 out[R][MT];
 #pragma unroll
@@ -192,62 +190,58 @@ __global__ __launch_bounds__(64 * KW, KW / 4 < 2 ? 2 : KW / 4) void q4_matmul_ke
         for (int mt = 0; mt < MT; ++mt) out[r][mt] = f32x4{0, 0, 0, 0};
     const uint32_t ones = one_pair(H());
     const u32x4 one = {ones, ones, ones, ones};
-    auto fold = [&](const St& st, int chunk) {
+    auto fold = [&](const St& st) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (chunk + u >= last) break;
+        for (int q = 0; q < GPC; ++q) {
+            f32x4 sum[R][MT], total[MT];
 #pragma unroll
-            for (int q = 0; q < GPC; ++q) {
-                f32x4 sum[R][MT], total[MT];
+            for (int mt = 0; mt < MT; ++mt) {
+                total[mt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int r = 0; r < R; ++r) sum[r][mt] = f32x4{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int e = 0; e < kSteps; ++e) {
+                const int s = q * kSteps + e;
+                u32x4 b[MT][NP];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
-                    total[mt] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int r = 0; r < R; ++r) sum[r][mt] = f32x4{0, 0, 0, 0};
-                }
-#pragma unroll
-                for (int e = 0; e < kSteps; ++e) {
-                    const int s = q * kSteps + e;
-                    u32x4 b[MT][NP];
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        if constexpr (NP == 1) {
-                            b[mt][0] = __builtin_bit_cast(u32x4, st.x[u][mt][s]);
-                        } else {
-                            split8<NP>(st.x[u][mt][s], b[mt]);
-                        }
-#pragma unroll
-                        for (int i = 0; i < NP; ++i) total[mt] = q4_mma(one, b[mt][i], total[mt], H());
+                    if constexpr (NP == 1) {
+                        b[mt][0] = __builtin_bit_cast(u32x4, st.x[mt][s]);
+                    } else {
+                        split8<NP>(st.x[mt][s], b[mt]);
                     }
 #pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        const u32x4 a = widen_codes(st.codes[u][r][s], H());
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                            for (int i = 0; i < NP; ++i) sum[r][mt] = q4_mma(a, b[mt][i], sum[r][mt], H());
-                    }
+                    for (int i = 0; i < NP; ++i) total[mt] = q4_mma(one, b[mt][i], total[mt], H());
                 }
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    const f32x4 scale = st.scales[u][r][q].get(bf16) * 16.f;
-                    f32x4 off = {1.5f, 1.5f, 1.5f, 1.5f};
-                    if (p.zeros) off = st.zeros[u][r][q].get(bf16) * 0.0625f + 1.f;
+                    const u32x4 a = widen_codes(st.codes[r][s], H());
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) out[r][mt] += scale * (sum[r][mt] - off * total[mt]);
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < NP; ++i) sum[r][mt] = q4_mma(a, b[mt][i], sum[r][mt], H());
                 }
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const f32x4 scale = st.scales[r][q].get(bf16) * 16.f;
+                f32x4 off = {1.5f, 1.5f, 1.5f, 1.5f};
+                if (p.zeros) off = st.zeros[r][q].get(bf16) * 0.0625f + 1.f;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) out[r][mt] += scale * (sum[r][mt] - off * total[mt]);
             }
         }
     };
     if (first < last) {
         St a, b;
         load(a, first);
-        for (int k = first; k < last; k += 2 * U) {
-            if (k + U < last) load(b, k + U);
-            fold(a, k);
-            if (k + U >= last) break;
-            if (k + 2 * U < last) load(a, k + 2 * U);
-            fold(b, k + U);
+        for (int k = first; k < last; k += 2) {
+            if (k + 1 < last) load(b, k + 1);
+            fold(a);
+            if (k + 1 >= last) break;
+            if (k + 2 < last) load(a, k + 2);
+            fold(b);
         }
     }
 #pragma unroll
@@ -255,12 +249,12 @@ __global__ __launch_bounds__(64 * KW, KW / 4 < 2 ? 2 : KW / 4) void q4_matmul_ke
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) *reinterpret_cast<f32x4*>(&so[wave][mt * 16 + c][r * 16 + g * 4]) = out[r][mt];
     __syncthreads();
-    for (int i = threadIdx.x; i < MT * 16 * R * 4; i += 64 * KW) {
+    for (int i = threadIdx.x; i < MT * 16 * R * 4; i += 64 * kWaves) {
         const int m = i / (R * 4), n = i % (R * 4) * 4;
         if (m0 + m >= p.M || n0 + n >= p.N) continue;
         f32x4 v = *reinterpret_cast<const f32x4*>(&so[0][m][n]);
 #pragma unroll
-        for (int w = 1; w < KW; ++w) v += *reinterpret_cast<const f32x4*>(&so[w][m][n]);
+        for (int w = 1; w < kWaves; ++w) v += *reinterpret_cast<const f32x4*>(&so[w][m][n]);
         T* y = static_cast<T*>(p.y) + (int64_t)(m0 + m) * p.ldy + n0 + n;
         if (n0 + n + 4 <= p.N) {
             T t[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
@@ -271,11 +265,11 @@ __global__ __launch_bounds__(64 * KW, KW / 4 < 2 ? 2 : KW / 4) void q4_matmul_ke
     }
 }
 
-template <typename T, int SW, int U, int R, int MT, int GPC, int KW>
+template <typename T, int SW, int R, int MT, int GPC>
 int q4_run(const Q4Params& p, hipStream_t st) {
     const int64_t grid = (int64_t)((p.N + 16 * R - 1) / (16 * R)) * ((p.M + 16 * MT - 1) / (16 * MT));
     if (grid > kMaxGrid / 4) return set_error(TT_UNSUPPORTED, "tt_q4_matmul: %lld workgroups", (long long)grid);
-    q4_matmul_kernel<T, SW, U, R, MT, GPC, KW><<<(uint32_t)grid, 64 * KW, 0, st>>>(p);
+    q4_matmul_kernel<T, SW, R, MT, GPC><<<(uint32_t)grid, 64 * kWaves, 0, st>>>(p);
     return check_launch("tt_q4_matmul");
 }
 
@@ -291,12 +285,12 @@ int q4_shape(const Q4Params& p, hipStream_t st) {
     constexpr bool kWide = sizeof(T) == 4;  // three parts an activation: no room for two blocks of rows
     const int tiles = (p.N + 15) / 16;
     if (p.M <= 16 || kWide) {
-        if (tiles <= 512) return q4_run<T, SW, 1, 1, 1, GPC, 8>(p, st);
-        return q4_run<T, SW, 1, 2, 1, GPC, 8>(p, st);
+        if (tiles <= 512) return q4_run<T, SW, 1, 1, GPC>(p, st);
+        return q4_run<T, SW, 2, 1, GPC>(p, st);
     }
     if constexpr (!kWide) {
-        if (tiles <= 256) return q4_run<T, SW, 1, 1, 2, GPC, 8>(p, st);
-        return q4_run<T, SW, 1, GPC == 1 ? 4 : 2, 2, GPC, 8>(p, st);
+        if (tiles <= 256) return q4_run<T, SW, 1, 2, GPC>(p, st);
+        return q4_run<T, SW, GPC == 1 ? 4 : 2, 2, GPC>(p, st);
     }
     return TT_OK;
 }
@@ -362,11 +356,6 @@ extern "C" int tt_q4_pack(int64_t N, int64_t K, const void* codes, int64_t pitch
     q4_pack_kernel<<<(uint32_t)blocks, 256, 0, static_cast<hipStream_t>(stream)>>>(
         (int)N, (int)K, (int)((K + 127) / 128), static_cast<const uint8_t*>(codes), pitch, static_cast<u32x4*>(packed), count);
     return check_launch("tt_q4_pack");
-}
-
-extern "C" size_t tt_q4_matmul_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
-    (void)dtype, (void)M, (void)N, (void)K;
-    return 0;
 }
 
 extern "C" int tt_q4_matmul(const tt_q4_args* a, void* stream) {

@@ -52,7 +52,6 @@ SIGNATURES = {
     # The serving operators' argument structs travel as packed bytes.
     "tt_q4_packed_bytes": (_sz, [_i64, _i64]),
     "tt_q4_pack": (_int, [_i64, _i64, _vp, _i64, _vp, _vp]),
-    "tt_q4_matmul_workspace_bytes": (_sz, [_int, _i64, _i64, _i64]),
     "tt_q4_matmul": (_int, [ctypes.c_char_p, _vp]),
     "tt_kv_append": (_int, [ctypes.c_char_p, _vp]),
     "tt_kv_attention_workspace_bytes": (_sz, [ctypes.c_char_p]),

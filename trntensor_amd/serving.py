@@ -34,7 +34,7 @@ _CODES = {torch.float32: _lib.TT_F32, torch.bfloat16: _lib.TT_BF16, torch.float1
 FP8 = torch.float8_e4m3fn
 
 # The argument structs of include/trntensor_hip.h, eight bytes a field.
-_Q4_ARGS = struct.Struct("=15q")
+_Q4_ARGS = struct.Struct("=13q")
 _CACHE = struct.Struct("=8q")
 _APPEND_ARGS = struct.Struct("=26q")
 _ATTENTION_ARGS = struct.Struct("=11qd5q")
@@ -132,7 +132,8 @@ def q4_matmul(x: torch.Tensor, w: Q4Matrix) -> torch.Tensor:
     Codes are widened in registers on their way into the matrix units, so the
     weights cross memory at half a byte each; products are summed in 32 bits
     and the result is rounded once to x's dtype. Rows of x need a unit stride
-    and one row pitch, else they are copied.
+    and one row pitch, else they are copied. A row of x that holds an infinity
+    gives infinities or NaN, one that holds NaN gives NaN.
     """
     if w._host is not None and dispatch._use_hip() and isinstance(x, torch.Tensor):
         y = w._host.run(x)
@@ -155,12 +156,9 @@ def q4_matmul(x: torch.Tensor, w: Q4Matrix) -> torch.Tensor:
         x2 = x2.contiguous()
     y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=w.device)
     zeros = w.zeros
-    need = _lib.load().tt_q4_matmul_workspace_bytes(code, m, n, k)
-    ws = torch.empty(need, dtype=torch.uint8, device=w.device) if need else None
     _launch("tt_q4_matmul", w.device, _Q4_ARGS.pack(
         code, w._code, m, n, k, w.group_size, max(x2.stride(0), k), n, x2.data_ptr(), w.packed.data_ptr(),
-        w.scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(), y.data_ptr(),
-        0 if ws is None else ws.data_ptr(), need))
+        w.scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(), y.data_ptr()))
     return y if home == w.device else y.to(home)
 
 
@@ -174,7 +172,7 @@ class KVCache:
     ``k`` is (pages, heads, page_size, width) and ``v`` (pages, heads, width,
     page_size), both ``torch.float8_e4m3fn`` with width = head_dim rounded up
     to a multiple of 64 (keys' codes past head_dim are zeros); ``k_scale`` and
-    ``v_scale`` are float32 (pages, heads). page_size is a multiple of 16,
+    ``v_scale`` are float32 (pages, heads), 2^-64 to 2^120. page_size is a multiple of 16,
     head_dim at most 256. The constructor takes tensors a program holds;
     :meth:`empty` makes a cache. Which pages are whose is the program's
     business: calls take a page table.
@@ -205,8 +203,9 @@ class KVCache:
             if not t.is_contiguous() or t.data_ptr() % 16:
                 raise ValueError(f"{name} must be contiguous and 16-byte aligned")
         for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            if not (torch.frexp(t)[0] == 0.5).all():
-                raise ValueError(f"{name} must be positive powers of two")
+            mantissa, exponent = torch.frexp(t)
+            if not ((mantissa == 0.5) & (exponent > -64) & (exponent <= 121)).all():
+                raise ValueError(f"{name} must be powers of two from 2^-64 to 2^120, those that kv_append takes")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.head_dim, self.page_size, self.num_pages, self.num_heads = int(head_dim), page, pages, heads
         self.device = k.device
@@ -373,7 +372,8 @@ def kv_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, leng
 
     Returns q's shape and dtype; queries that see nothing (empty sequences,
     rows past their count) give zeros. No masked slot has any influence,
-    whatever its page holds.
+    whatever its page holds. Weighted sums are held in 32 bits before they are
+    divided: values of 2^100 and more may overflow them.
     """
     if cache._host is not None and dispatch._use_hip():
         out = cache._host.attention(q, page_table, lengths, counts, cache._scale if scale is None else scale,
