@@ -380,6 +380,50 @@ def test_kv_attention(hip, heads, share, dim, page, tokens, lengths, counts, win
     _attention_case(heads, share, dim, page, tokens, lengths, counts, window, sinks, dtype)
 
 
+@pytest.mark.parametrize(
+    "dtype,heads,share,dim,page,tokens,lengths,counts,window,sinks",
+    [
+        # every block of rows that is taken, whole and with its keys split
+        (torch.bfloat16, 8, 4, 128, 64, 1024, [3000, 2500], None, None, 0),
+        (torch.float16, 8, 4, 96, 32, 1024, [3000, 1100], [1024, 700], None, 0),
+        (torch.bfloat16, 2, 4, 128, 64, 512, [32768], None, None, 0),
+        (torch.float16, 2, 4, 64, 64, 512, [20000], None, None, 0),
+        (torch.bfloat16, 8, 4, 64, 16, 128, [1000] * 8, None, None, 0),
+        (torch.bfloat16, 1, 4, 128, 64, 200, [5000, 0], None, None, 0),
+        (torch.float32, 8, 4, 128, 16, 256, [1500, 900], None, None, 0),
+        (torch.float32, 2, 2, 256, 32, 300, [5000], None, None, 0),
+        (torch.bfloat16, 4, 3, 200, 32, 400, [4000, 100, 0], [400, 30, 0], None, 0),
+        (torch.bfloat16, 8, 4, 128, 64, 1024, [3000, 2500], None, 700, 5),
+        (torch.float16, 8, 4, 128, 64, 600, [600, 2001], None, 100, 130),
+    ],
+)
+def test_kv_attention_many_rows(hip, dtype, heads, share, dim, page, tokens, lengths, counts, window, sinks):
+    """Some tokens of calls too large to check whole; the others are finite."""
+    batch, width, g = len(lengths), -(-max(lengths) // page), torch.Generator().manual_seed(17)
+    dev, want = _cache(batch * width, heads, page, dim, 16)
+    table = torch.randperm(batch * width, generator=g).to(torch.int32).reshape(batch, width)
+    for b, n in enumerate(lengths):
+        for block in range(width):
+            live = min(max(n - block * page, 0), page)
+            dev.k.view(torch.uint8)[int(table[b, block]), :, live:] = 0x7F
+            dev.v.view(torch.uint8)[int(table[b, block]), :, :, live:] = 0xFF
+    q = torch.randn((batch, tokens, heads * share, dim), generator=g).to(dtype)
+    n = None if counts is None else _i32(counts)
+    got = tt.kv_attention(q.cuda(), dev, table.cuda(), _i32(lengths).cuda(), counts=None if n is None else n.cuda(),
+                          window=window, sinks=sinks).cpu()
+    assert got.isfinite().all()
+    for b, held in enumerate(lengths):
+        live = tokens if counts is None else counts[b]
+        picked = {0, 1, 15, 16, 63, 64, live // 2, live - 1, *torch.randint(0, tokens, (6,), generator=g).tolist()}
+        for t in sorted(x for x in picked if 0 <= x < tokens):
+            if t >= live or held - live + t < 0:
+                assert (got[b, t] == 0).all()
+                continue
+            # A token sees what a single query behind its position sees.
+            _check_attention(got[b : b + 1, t : t + 1], q[b : b + 1, t : t + 1], want, table[b : b + 1],
+                             _i32([held - live + t + 1]), None, 1 / math.sqrt(dim), window, sinks)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("scale", [0.0, 2.0, -0.5])
 def test_kv_attention_scale(hip, scale, dtype):

@@ -1048,6 +1048,37 @@ __global__ __launch_bounds__(256) void kv_attention_many_join_kernel(AttnParams 
                    out_row<T>(p, b, kh, row0 + r));
 }
 
+// Workgroups of many rows: blocks of 16 rows a wavefront, wavefronts, and the
+// us that a tile takes with one workgroup on a compute unit and, where two fit,
+// with two (bfloat16, head size 128). Eight wavefronts of two blocks widen a
+// tile for the most rows (2048 tokens on 8192: 268 us, of one block 340, four
+// of one 396); smaller blocks waste less where rows are few or the causal edge
+// is steep (128 tokens on 1024: 27, 22, 20; 2048 on 2048: 80, 64, 76).
+struct Shape {
+    int mt, waves;
+    double alone, both;
+};
+constexpr Shape kShapes[] = {{1, 4, 1.27, 1.85}, {1, 8, 1.47, 1.47}, {2, 8, 2.15, 2.15}};
+
+// What a call is expected to take (us), its keys cut into g ranges. Joining
+// them is a second launch that reads what the first one wrote: 5 us, 0.36 a MB
+// and 0.45 a thousand rows. It pays where blocks leave compute units idle (one
+// block a head, 8192 keys: 278 us whole, 34 in 32 ranges), not where keys are
+// few for their rows (eight times 128 tokens on 1024: 32 us whole, 56 halved).
+double many_cost(const tt_kv_attention_args* a, const Shape& s, int64_t W, int64_t tiles, int64_t blocks, int64_t g,
+                 int64_t slots) {
+    const double width = (W + 64) / 192.0, kind = a->dtype == TT_F32 ? 1.6 : a->dtype == TT_F16 ? 1.3 : 1.0;
+    const double per = (double)((tiles + g - 1) / g), cap = (double)a->table_width * a->cache.page;
+    // Of a prompt's own keys its rows see half.
+    const double seen = a->window > 0 || cap <= 0 ? 1 : 1 - 0.5 * (a->tokens < cap ? a->tokens : cap) / cap;
+    const int64_t n = blocks * g, rounds = (n + slots - 1) / slots;
+    const double start = 2;  // tiles' worth, of every workgroup
+    const double longest = (per + start) * s.alone, all = (per * seen + start) * rounds * (n <= 256 ? s.alone : s.both);
+    const double rows = 16.0 * s.mt * s.waves * blocks;
+    const double join = g > 1 ? 5 + 0.36e-6 * rows * g * (W + 2) * 4 + 0.45e-3 * rows : 0;
+    return (longest > all ? longest : all) * width * kind + join;
+}
+
 // How a call is cut, from what the host knows of it.
 struct Cut {
     bool few, direct;
@@ -1070,23 +1101,44 @@ Cut cut_of(const tt_kv_attention_args* a) {
     if (c.few) {
         c.mt = 1;
         c.row_blocks = 1;
-        c.direct = tiles <= 16;
-        c.groups = 512;
+        // A workgroup a pair needs no second launch to join (about 5 us), but
+        // lets its longest pair decide. us direct / shared, one token of 8 heads
+        // of 128: 8 pairs of 1024 keys 10.8 / 14.4, of 2048 15.4 / 14.1; 64 pairs
+        // of 2048 17.6 / 18.6, of 4096 30.2 / 24.6; 256 pairs of 4096 43.7 / 52.8
+        // (of 1 to 4096 33.6 / 36.0), 512 of 4096 100.7 / 106.3 (57.2 / 61.9);
+        // past what is resident at once, 1024 pairs of 4096 241 / 198, but 2048
+        // of 1500 134 / 170. The table's width is all the host knows of the
+        // lengths: beyond 64 tiles one long sequence among short ones would
+        // hold up its few workgroups.
+        const int most = pairs < 64 ? 16 : pairs < 256 || pairs > 512 ? 32 : 64;
+        c.direct = tiles <= most;
+        c.groups = 512;  // two a compute unit; 256 and 1024 were 8% slower at some length each, level at others
         c.grid = c.direct ? pairs : c.groups;
         c.slots = c.direct ? 0 : 2 * c.groups;
         c.slot_floats = 16 * (W + 2);
     } else {
-        const bool wide = W > 128;
-        c.mt = rows > 128 && !wide && a->dtype != TT_F32 ? 2 : 1;
-        c.waves = rows <= 64 || (wide && a->dtype == TT_F32) ? 4 : 8;
-        const int64_t block = 16 * c.mt * c.waves;
-        c.row_blocks = (int)((rows + block - 1) / block);
-        const int64_t blocks = pairs * c.row_blocks, want = c.waves == 4 ? 512 : 256;
-        int64_t g = blocks >= want ? 1 : (want + blocks - 1) / blocks;
-        if (g > tiles / 4) g = tiles / 4 > 0 ? tiles / 4 : 1;
-        c.groups = (int)g;
-        c.grid = blocks * g;
-        c.slots = g > 1 ? blocks * g : 0;
+        c.mt = c.waves = 0;
+        double best = 0;
+        for (const Shape& s : kShapes) {
+            if ((s.mt == 2 && (W > 128 || a->dtype == TT_F32)) || (s.waves == 8 && W > 128 && a->dtype == TT_F32)) continue;
+            const int64_t block = 16 * s.mt * s.waves, blocks = pairs * ((rows + block - 1) / block);
+            if (c.waves && rows <= block / 2) continue;
+            const int64_t slots = s.waves == 4 && W <= 128 ? 512 : 256, fit = slots / blocks;
+            for (int64_t g = 1;; g = 2 * g < fit ? 2 * g : fit) {
+                const double cost = many_cost(a, s, W, tiles, blocks, g, slots);
+                if (!c.waves || cost < best) {
+                    best = cost;
+                    c.mt = s.mt;
+                    c.waves = s.waves;
+                    c.groups = (int)g;
+                    c.row_blocks = (int)(blocks / pairs);
+                }
+                if (g >= fit || 2 * g > tiles) break;
+            }
+        }
+        const int64_t block = 16 * c.mt * c.waves, blocks = pairs * c.row_blocks;
+        c.grid = blocks * c.groups;
+        c.slots = c.groups > 1 ? blocks * c.groups : 0;
         c.slot_floats = block * (W + 2);
     }
     return c;
