@@ -23,7 +23,8 @@ struct Q4Params {
     void* y;
     int M, N, K, groups, chunks;  // chunks of 128 columns
     int group_shift, chunks_per_group;  // groups below 128 columns: log2(group / 32); else chunks a group
-    int scale_bf16;                     // 16-bit scales: bfloat16, not float16
+    uint32_t zero_mask;                 // all ones where there are zero points, else 0 (and `zeros` is `scales`)
+    uint32_t scale_bf16;                // 16-bit scales: all ones for bfloat16, 0 for float16
 };
 
 __device__ __forceinline__ f32x4 q4_mma(u32x4 a, u32x4 b, f32x4 c, __bf16) {
@@ -69,27 +70,34 @@ __device__ __forceinline__ uint32_t one_pair(_Float16) { return 0x3c003c00u; }
 // Scales or zero points of four neighbouring rows, as stored (SW bytes each).
 template <int SW>
 struct Four {
-    uint32_t raw[SW];
-    __device__ __forceinline__ f32x4 get(bool bf16) const {
+    uint32_t raw __attribute__((ext_vector_type(SW)));
+    // 16-bit ones are bfloat16 where the bits of `bf16` are set, else float16
+    // (not a condition: the compiler would gather all conversions under one
+    // branch, and the floats with them).
+    __device__ __forceinline__ f32x4 get(uint32_t bf16) const {
         if constexpr (SW == 4)
             return f32x4{__uint_as_float(raw[0]), __uint_as_float(raw[1]), __uint_as_float(raw[2]), __uint_as_float(raw[3])};
-        if (bf16)
-            return f32x4{__uint_as_float(raw[0] << 16), __uint_as_float(raw[0] & 0xffff0000u), __uint_as_float(raw[1] << 16),
-                         __uint_as_float(raw[1] & 0xffff0000u)};
-        const f16x2 a = __builtin_bit_cast(f16x2, raw[0]), b = __builtin_bit_cast(f16x2, raw[1]);
-        return f32x4{(float)a[0], (float)a[1], (float)b[0], (float)b[1]};
+        f32x4 v;
+        if constexpr (SW == 2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t pair = raw[i / 2];
+                const float half = (float)__builtin_bit_cast(f16x2, pair)[i & 1];
+                v[i] = __uint_as_float((__float_as_uint(bf16_of(pair, i & 1)) & bf16) | (__float_as_uint(half) & ~bf16));
+            }
+        }
+        return v;
     }
 };
 
 constexpr int kWaves = 8;  // wavefronts a workgroup
 
-// One stage of a wavefront's operands: a chunk of 128 columns of 16 R weight
-// rows and 16 MT activation rows; GPC scales a chunk and row.
-template <typename T, int SW, int R, int MT, int GPC>
-struct Stage {
+// What a wavefront holds of a chunk of 128 columns of its 16 R weight rows: codes
+// and, for GPC pieces of the chunk, scales and zero points (or scales again).
+template <int SW, int R, int GPC>
+struct Chunk {
     u32x4 codes[R];
     Four<SW> scales[R][GPC], zeros[R][GPC];
-    T x[MT][4][8];
 };
 
 // R blocks of 16 weight rows and MT of 16 activation rows a wavefront; the
@@ -102,19 +110,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void q4_matmul_kernel(Q4Params p) {
     constexpr int NP = Act<T>::parts;
     constexpr int kSteps = 4 / GPC;  // MFMA steps of 32 columns a piece
     __shared__ float so[kWaves][MT * 16][R * 16 + 4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int row_blocks = (p.N + 16 * R - 1) / (16 * R);
     const int m_blocks = (p.M + 16 * MT - 1) / (16 * MT);
     // Workgroup i runs on XCD i % 8: the blocks of activation rows that read
     // the same weights follow each other on one XCD, and share its L2.
     int rb, mb;
-    const int tail = row_blocks % kNumXcd, whole = (row_blocks - tail) * m_blocks;
-    if ((int)blockIdx.x < whole) {
+    const int tail = row_blocks % kNumXcd, even = (row_blocks - tail) * m_blocks;
+    if ((int)blockIdx.x < even) {
         rb = blockIdx.x / (kNumXcd * m_blocks) * kNumXcd + blockIdx.x % kNumXcd;
         mb = blockIdx.x / kNumXcd % m_blocks;
     } else {
-        rb = row_blocks - tail + (blockIdx.x - whole) % tail;
-        mb = (blockIdx.x - whole) / tail;
+        rb = row_blocks - tail + (blockIdx.x - even) % tail;
+        mb = (blockIdx.x - even) / tail;
     }
     const int n0 = rb * 16 * R, m0 = mb * 16 * MT;
     const int per = (p.chunks + kWaves - 1) / kWaves;
@@ -126,7 +134,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void q4_matmul_kernel(Q4Params p) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int t = rb * R + r;
-        code_row[r] = p.codes + (int64_t)(t < tiles ? t : tiles - 1) * p.chunks * 1024 + lane * 16;
+        code_row[r] = p.codes + (int64_t)(t < tiles ? t : tiles - 1) * p.chunks * 1024;
     }
     const T* x_row[MT];
 #pragma unroll
@@ -136,52 +144,49 @@ __global__ __launch_bounds__(64 * kWaves, 2) void q4_matmul_kernel(Q4Params p) {
     }
     // A last chunk that the columns do not fill, with zeros behind them.
     __shared__ __attribute__((aligned(16))) T filled[MT * 16][128 + 16 / sizeof(T)];
-    const bool ragged = last == p.chunks && p.K % 128 != 0 && first < last;
-    if (ragged) {
-        const int k0 = (p.chunks - 1) * 128;
-        for (int i = lane; i < MT * 16 * 128; i += 64) {
-            const int m = m0 + i / 128, k = k0 + i % 128;
-            filled[i / 128][i % 128] = k < p.K ? static_cast<const T*>(p.x)[(int64_t)(m < p.M ? m : p.M - 1) * p.ldx + k] : (T)0.f;
+    const bool uneven = p.K % 128 != 0, ragged = uneven && last == p.chunks && first < last;
+    const int whole = ragged ? last - 1 : last;
+    if (uneven) {
+        constexpr int kEach = MT * 16 * 128 / (64 * kWaves);
+        const int k = (p.chunks - 1) * 128 + threadIdx.x % 128;
+        T v[kEach];
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+            const int m = m0 + u * (64 * kWaves / 128) + threadIdx.x / 128;
+            v[u] = static_cast<const T*>(p.x)[(int64_t)(m < p.M ? m : p.M - 1) * p.ldx + (k < p.K ? k : p.K - 1)];
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int u = 0; u < kEach; ++u)
+            filled[u * (64 * kWaves / 128) + threadIdx.x / 128][threadIdx.x % 128] = k < p.K ? v[u] : (T)0.f;
     }
-    const bool bf16 = p.scale_bf16;
+    const uint32_t bf16 = p.scale_bf16, eight = __float_as_uint(8.f);
     const int scale_pitch = (p.N + 15) / 16 * 16;
     auto load_four = [&](const void* base, int group, int r) {
         Four<SW> f;
         group = group < p.groups ? group : p.groups - 1;
-        const int n = n0 + r * 16 < scale_pitch ? n0 + r * 16 + g * 4 : 0;
-        __builtin_memcpy(f.raw, static_cast<const uint8_t*>(base) + ((int64_t)group * scale_pitch + n) * SW, sizeof f.raw);
+        const int n = n0 + r * 16 < scale_pitch ? n0 + r * 16 : 0;
+        f.raw = *reinterpret_cast<const decltype(f.raw)*>(static_cast<const uint8_t*>(base) +
+                                                          ((int64_t)group * scale_pitch + n) * SW + (uint32_t)(g * 4 * SW));
         return f;
     };
-    typedef Stage<T, SW, R, MT, GPC> St;
-    auto load = [&](St& st, int k) {
+    auto load = [&](Chunk<SW, R, GPC>& w, int k) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int r = 0; r < R; ++r) st.codes[r] = *reinterpret_cast<const u32x4*>(code_row[r] + (int64_t)k * 1024);
-        const bool edge = ragged && k == p.chunks - 1;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            if (edge) {
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-                    __builtin_memcpy(st.x[mt][s], __builtin_assume_aligned(&filled[mt * 16 + c][s * 32 + g * 8], 16),
-                                     sizeof st.x[mt][s]);
-            } else {
-                const T* src = x_row[mt] + k * 128;
-#pragma unroll
-                for (int s = 0; s < 4; ++s) __builtin_memcpy(st.x[mt][s], src + s * 32, sizeof st.x[mt][s]);
-            }
-        }
+        for (int r = 0; r < R; ++r) w.codes[r] = *reinterpret_cast<const u32x4*>(code_row[r] + (int64_t)k * 1024 + (uint32_t)(lane * 16));
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int q = 0; q < GPC; ++q) {
                 const int group = GPC > 1 ? (k * GPC + q) >> p.group_shift : k / p.chunks_per_group;
-                st.scales[r][q] = load_four(p.scales, group, r);
-                if (p.zeros) st.zeros[r][q] = load_four(p.zeros, group, r);
+                w.scales[r][q] = load_four(p.scales, group, r);
+                w.zeros[r][q] = load_four(p.zeros, group, r);
             }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    T x[MT][4][8];
+    auto load_x = [&](int s, int k) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) __builtin_memcpy(x[mt][s], x_row[mt] + k * 128 + s * 32, sizeof x[mt][s]);
     };
     f32x4 out[R][MT];
 #pragma unroll
@@ -190,7 +195,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void q4_matmul_kernel(Q4Params p) {
         for (int mt = 0; mt < MT; ++mt) out[r][mt] = f32x4{0, 0, 0, 0};
     const uint32_t ones = one_pair(H());
     const u32x4 one = {ones, ones, ones, ones};
-    auto fold = [&](const St& st) {
+    // Folds a chunk; the activations of chunk `next` take the place of each step's.
+    auto fold = [&](const Chunk<SW, R, GPC>& w, int next, auto reload) {
 #pragma unroll
         for (int q = 0; q < GPC; ++q) {
             f32x4 sum[R][MT], total[MT];
@@ -207,42 +213,76 @@ __global__ __launch_bounds__(64 * kWaves, 2) void q4_matmul_kernel(Q4Params p) {
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     if constexpr (NP == 1) {
-                        b[mt][0] = __builtin_bit_cast(u32x4, st.x[mt][s]);
+                        b[mt][0] = __builtin_bit_cast(u32x4, x[mt][s]);
                     } else {
-                        split8<NP>(st.x[mt][s], b[mt]);
+                        split8<NP>(x[mt][s], b[mt]);
                     }
 #pragma unroll
                     for (int i = 0; i < NP; ++i) total[mt] = q4_mma(one, b[mt][i], total[mt], H());
                 }
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    const u32x4 a = widen_codes(st.codes[r][s], H());
+                    const u32x4 a = widen_codes(w.codes[r][s], H());
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                         for (int i = 0; i < NP; ++i) sum[r][mt] = q4_mma(a, b[mt][i], sum[r][mt], H());
                 }
+                if constexpr (reload.value) load_x(s, next);
             }
+            __builtin_amdgcn_sched_barrier(0);  // scales become floats here, not earlier
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const f32x4 scale = st.scales[r][q].get(bf16) * 16.f;
-                f32x4 off = {1.5f, 1.5f, 1.5f, 1.5f};
-                if (p.zeros) off = st.zeros[r][q].get(bf16) * 0.0625f + 1.f;
+                const f32x4 scale = w.scales[r][q].get(bf16) * 16.f;
+                f32x4 off = w.zeros[r][q].get(bf16);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    off[i] = __builtin_fmaf(__uint_as_float((__float_as_uint(off[i]) & p.zero_mask) | (eight & ~p.zero_mask)),
+                                            0.0625f, 1.f);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) out[r][mt] += scale * (sum[r][mt] - off * total[mt]);
             }
         }
     };
-    if (first < last) {
-        St a, b;
-        load(a, first);
-        for (int k = first; k < last; k += 2) {
-            if (k + 1 < last) load(b, k + 1);
-            fold(a);
-            if (k + 1 >= last) break;
-            if (k + 2 < last) load(a, k + 2);
-            fold(b);
+    // A chunk is folded with the next one in flight, loaded into the other of a
+    // and b; the last is in a, so that an odd number of steps begins with b. No
+    // load hangs on a condition of its own: a wait for one chunk would become one
+    // for all. (Loading the last chunk twice instead costs a wait at the end.)
+    Chunk<SW, R, GPC> a, b;
+    const int final = whole - 1;
+    if (first <= final) {
+        int second = (final - first) & 1;
+        asm volatile("" : "+s"(second));
+        if (second)
+            load(b, first);
+        else
+            load(a, first);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) load_x(s, first);
+        for (int k = first; k < final;) {
+            if (!second) {
+                load(b, ++k);
+                fold(a, k, std::true_type());
+            }
+            second = 0;
+            asm volatile("" : "+s"(second));
+            load(a, ++k);
+            fold(b, k, std::true_type());
         }
+    }
+    if (uneven) __syncthreads();
+    // The last whole chunk, and then the one that the columns do not fill.
+    for (int left = (first < whole) + ragged; left > 0; --left) {
+        if (ragged && left == 1) {
+            load(a, p.chunks - 1);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+                    __builtin_memcpy(x[mt][s], __builtin_assume_aligned(&filled[mt * 16 + c][s * 32 + g * 8], 16),
+                                     sizeof x[mt][s]);
+        }
+        fold(a, 0, std::false_type());
     }
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -275,24 +315,37 @@ int q4_run(const Q4Params& p, hipStream_t st) {
 
 template <typename T, int SW, int GPC>
 int q4_shape(const Q4Params& p, hipStream_t st) {
-    // R weight tiles a wavefront read the same activations: fewer of their bytes
-    // a byte of codes, but fewer wavefronts. us for R = 1 / 2 / 4 (bfloat16,
-    // groups of 128): one row, 4096 x 4096 4.9 / 6.6 / 9.8, 8192 x 4096 7.4 /
-    // 8.5 / 11.2, 16384 x 8192 20.4 / 18.1 / 20.1; 16 rows, 16384 x 8192 36.9 /
-    // 24.5 / 22.7; 32 rows, 4096 x 4096 11.2 / 12.5 / 15.9, 16384 x 8192 69.9 /
-    // 41.9 / 31.2. Four or sixteen wavefronts a workgroup, or two chunks a
-    // stage, were slower at all of these or level.
-    constexpr bool kWide = sizeof(T) == 4;  // three parts an activation: no room for two blocks of rows
-    const int tiles = (p.N + 15) / 16;
-    if (p.M <= 16 || kWide) {
-        if (tiles <= 512) return q4_run<T, SW, 1, 1, GPC>(p, st);
+    // R weight tiles a wavefront share its activations: less of them to read and
+    // to split, but fewer workgroups. `work` counts those of R = 1, of which two
+    // fit a compute unit, and one of the others. us for R = 1 / 2 / 4:
+    //   bfloat16, groups of 128        work 256          512              1024
+    //     1 row     (K 4096, 4096, 8192)  5.2 / 6.5 / 9.8   7.4 / 8.1 / 10.8   20.3 / 16.9 / 20.4
+    //     16 rows                         7.0 / 7.8 / 10.8  11.2 / 9.2 / 11.4  35.8 / 22.6 / 21.4
+    //     32 rows                         10.4 / 11.2 / 13.9  18.0 / 12.4 / 14.8  63.1 / 37.6 / 27.0
+    //   float16, groups of 64
+    //     1 row                           7.9 / 12.4        11.9 / 13.4        35.0 / 40.4
+    //     16 rows                         9.1 / 12.9        15.0 / 13.6        47.5 / 41.5 (1792: 42.1 / 47.4)
+    //     32 rows                         12.0 / 16.1       21.9 / 17.0        78.1 / 52.6
+    //   float32 (three parts an activation: no room for two blocks of rows), groups of 32
+    //     1 row                           9.9 / 13.2        18.5 / 15.9        59.2 / 48.1
+    // Four or sixteen wavefronts a workgroup were slower or level.
+    const int64_t tiles = (p.N + 15) / 16;
+    if constexpr (sizeof(T) == 4) {
+        if (tiles * ((p.M + 15) / 16) <= 256) return q4_run<T, SW, 1, 1, GPC>(p, st);
         return q4_run<T, SW, 2, 1, GPC>(p, st);
+    } else if constexpr (GPC > 1) {
+        if (p.M <= 16) return q4_run<T, SW, 1, 1, GPC>(p, st);
+        if (tiles * ((p.M + 31) / 32) <= 256) return q4_run<T, SW, 1, 2, GPC>(p, st);
+        return q4_run<T, SW, 2, 2, GPC>(p, st);
+    } else if (p.M <= 16) {
+        const int wide = (tiles > 256) + (tiles > 512) - (p.M <= 4);
+        if (wide <= 0) return q4_run<T, SW, 1, 1, GPC>(p, st);
+        return wide == 1 ? q4_run<T, SW, 2, 1, GPC>(p, st) : q4_run<T, SW, 4, 1, GPC>(p, st);
+    } else {
+        const int64_t work = tiles * ((p.M + 31) / 32);
+        if (work <= 256) return q4_run<T, SW, 1, 2, GPC>(p, st);
+        return work <= 512 ? q4_run<T, SW, 2, 2, GPC>(p, st) : q4_run<T, SW, 4, 2, GPC>(p, st);
     }
-    if constexpr (!kWide) {
-        if (tiles <= 256) return q4_run<T, SW, 1, 2, GPC>(p, st);
-        return q4_run<T, SW, GPC == 1 ? 4 : 2, 2, GPC>(p, st);
-    }
-    return TT_OK;
 }
 
 template <typename T>
@@ -379,7 +432,8 @@ extern "C" int tt_q4_matmul(const tt_q4_args* a, void* stream) {
     p.ldy = a->ldy;
     p.x = a->x;
     p.scales = a->scales;
-    p.zeros = a->zeros;
+    p.zeros = a->zeros ? a->zeros : a->scales;
+    p.zero_mask = a->zeros ? ~0u : 0u;
     p.codes = static_cast<const uint8_t*>(a->codes);
     p.y = a->y;
     p.M = (int)a->M;
@@ -390,7 +444,7 @@ extern "C" int tt_q4_matmul(const tt_q4_args* a, void* stream) {
     p.chunks = (int)((a->K + 127) / 128);
     p.chunks_per_group = group >= 128 ? (int)(group / 128) : 1;
     p.group_shift = group == 64 ? 1 : 0;
-    p.scale_bf16 = a->scale_dtype == TT_BF16;
+    p.scale_bf16 = a->scale_dtype == TT_BF16 ? ~0u : 0u;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (a->dtype == TT_F32) return q4_typed<float>(a->scale_dtype, p, group < 128, st);
     if (a->dtype == TT_BF16) return q4_typed<__bf16>(a->scale_dtype, p, group < 128, st);
