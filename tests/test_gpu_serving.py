@@ -84,6 +84,11 @@ def _check_q4(x, codes, scales, z, k, group, y):
         (64, 8448, 900, 128),
         (100, 8209, 640, 128),
         (20, 8288, 250, 32),
+        (2, 8300, 300, 128),
+        (9, 8250, 300, 128),
+        (12, 5000, 390, 128),
+        (20, 4200, 270, 128),
+        (40, 2200, 200, 64),
     ],
 )
 def test_q4_matmul(hip, m, n, k, group, zeros, dtype):
@@ -99,6 +104,16 @@ def test_q4_matmul_scales_of_another_dtype(hip, dtype, scale_dtype):
     codes, scales, z = _q4(50, 256, 64, scale_dtype, True, 4)
     x = torch.randn((3, 256), generator=torch.Generator().manual_seed(5)).to(dtype)
     _check_q4(x, codes, scales, z, 256, 64, tt.q4_matmul(x.cuda(), tt.Q4Matrix(codes.cuda(), scales.cuda(), 256, 64, zeros=z.cuda())))
+
+
+@pytest.mark.parametrize("dtype,scale_dtype", [(torch.bfloat16, torch.float32), (torch.float16, torch.float32),
+                                               (torch.float32, torch.bfloat16), (torch.bfloat16, torch.float16)])
+@pytest.mark.parametrize("m,n,k,group", [(9, 8250, 300, 128), (20, 4200, 270, 128), (20, 8288, 250, 32), (40, 2200, 200, 64)])
+def test_q4_matmul_many_rows_and_scales_of_another_dtype(hip, m, n, k, group, dtype, scale_dtype):
+    codes, scales, z = _q4(n, k, group, scale_dtype, True, m + n)
+    x = torch.randn((m, k), generator=torch.Generator().manual_seed(9)).to(dtype)
+    w = tt.Q4Matrix(codes.cuda(), scales.cuda(), k, group, zeros=z.cuda())
+    _check_q4(x, codes, scales, z, k, group, tt.q4_matmul(x.cuda(), w))
 
 
 def test_q4_matmul_every_code_and_column(hip):

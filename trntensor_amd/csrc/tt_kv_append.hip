@@ -252,6 +252,9 @@ __device__ __forceinline__ void turn_pieces(const float* c, const float* s, bool
 //            run, whose codes lie together in the cache
 //   queries  a wavefront takes a token; a lane's elements are in the same
 //            place of every head, so that it reads its angles once
+// Four prompts of 4096 tokens (8 heads of 128, 32 query heads, 377 MB) take 95
+// us, 4.0 TB/s where a large copy has 5.2; one token of eight sequences 5 us, a
+// launch and the waits for length, page, scale and values one after the other.
 // Head sizes are multiples of 8 here and rotated parts of 16.
 template <typename T, int W>
 __device__ __forceinline__ void rotate_token(const AppendParams& p, int64_t row) {

@@ -32,7 +32,9 @@ struct AttnParams {
 
 constexpr int kTile = 64;     // keys a wavefront takes at a time
 constexpr int kMinTiles = 4;  // fewest tiles worth a workgroup: one per wavefront
-constexpr int kPairCost = 4;  // what starting and joining a pair costs, in tiles
+// What starting and joining a pair costs, in tiles. 1 to 8 are level within 5%
+// at five lengths and batches; 16 takes 90 us for 80 (48 sequences of 4096).
+constexpr int kPairCost = 4;
 
 // A value that all lanes of a wavefront share, for scalar registers.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -84,6 +86,7 @@ __device__ __forceinline__ Span span_of(const AttnParams& p, int b, int row0, in
 // are exact in either 16-bit type. float32 splits into three bfloat16 parts
 // (24 bits); float16 queries are taken as they are, and their probabilities as
 // two bfloat16 parts (16 bits), since scaled values may pass float16's range.
+// bfloat16 ones are rounded to the 8 bits that their result is held in.
 template <typename T>
 struct Parts {
     static constexpr int q = 1, p = 1;
@@ -662,7 +665,12 @@ __device__ __forceinline__ int64_t share_of(const AttnParams& p, int64_t total) 
 // take every fourth tile of the same keys. The key tiles of all (sequence,
 // head) pairs form one list, in which each pair also takes the room of what
 // starting it costs; the workgroups share it evenly whatever the sequences'
-// lengths, and a pair cut by a workgroup's end leaves partial results.
+// lengths, and a pair cut by a workgroup's end leaves partial results. Or, for
+// short tables, each takes a pair whole (cut_of). Bound by the codes' bytes: two
+// sequences of 131071 tokens (8 heads of 128, 534 MB) take 106 us, 5.0 TB/s where
+// a large copy has 5.2; 48 of 1 to 4096, a workgroup a pair, 50 us, 4.0 TB/s, the
+// longest pairs being left at the end; one of 200 tokens 7 us, the launch and a
+// chain of waits (length, page, keys, values).
 // Wavefronts a SIMD is to hold: two where the state of one fits half its registers.
 template <typename T, int W, int MT>
 constexpr int kWavesPerSimd = Parts<T>::q * MT * W > 256 || W > 128 ? 1 : 2;
@@ -740,12 +748,12 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<T, W, 1>)) void kv_attention_fe
 // One query row of `parts` partial results by one wavefront: slot 0 is `first`
 // and slot i > 0 `rest` + i * stride; a slot holds its rows' sums of W elements,
 // and the row's maximum and weight at m_at and l_at (weight -1: no key seen).
-template <typename T, int W>
+// kDeep slots are in flight.
+template <typename T, int W, int kDeep>
 __device__ __forceinline__ void join_row(const float* first, const float* rest, int64_t stride, int parts, int row, int m_at,
                                          int l_at, int dim, T* out) {
     const int lane = threadIdx.x & 63;
     auto slot = [&](int i) { return i ? rest + i * stride : first; };
-    constexpr int kDeep = 8;
     float x[kDeep][W / 64];
     auto load = [&](int i) {
 #pragma unroll
@@ -757,10 +765,10 @@ __device__ __forceinline__ void join_row(const float* first, const float* rest, 
     };
     // The first elements, maxima and weights are asked for together: which
     // memory they come from is a longer way than what is done with them.
-    load(0);
     const float* own = slot(lane < parts ? lane : parts - 1);
     float m = own[m_at];
     const float m_own = m, l_own = own[l_at];
+    load(0);
     __builtin_amdgcn_sched_barrier(0);
     for (int i = lane + 64; i < parts; i += 64) m = fmaxf(m, slot(i)[m_at]);
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
@@ -797,7 +805,8 @@ __device__ __forceinline__ void join_row(const float* first, const float* rest, 
         if (d * 64 + lane < dim) out[d * 64 + lane] = (T)(some ? o[d] / sum : 0.f);
 }
 
-// Joins the partial results of the pairs that were cut: one wavefront a query row.
+// Joins the partial results of the pairs that were cut: one wavefront a query
+// row. 4 to 5 us: a launch, and two waits on memory (lengths, partial results).
 template <typename T, int W>
 __global__ __launch_bounds__(256) void kv_attention_few_join_kernel(AttnParams p) {
     constexpr int64_t kSlot = 16 * (W + 2);
@@ -811,7 +820,7 @@ __global__ __launch_bounds__(256) void kv_attention_few_join_kernel(AttnParams p
     if (g0 == g1) return;
     const float* base = p.part + g0 * 2 * kSlot;
     for (int row = uniform((int)threadIdx.x >> 6); row < sp.live; row += 4)
-        join_row<T, W>(base + kSlot, base, 2 * kSlot, (int)(g1 - g0 + 1), row, 16 * W + row, 16 * W + 16 + row, p.dim,
+        join_row<T, W, 32>(base + kSlot, base, 2 * kSlot, (int)(g1 - g0 + 1), row, 16 * W + row, 16 * W + 16 + row, p.dim,
                        out_row<T>(p, b, kh, row));
 }
 
@@ -819,7 +828,11 @@ __global__ __launch_bounds__(256) void kv_attention_few_join_kernel(AttnParams p
 // them walk the same keys, whose codes the workgroup widens once and puts into
 // LDS as the operands of the products, tile by tile in two buffers: what widens
 // a tile, loads it and reads it is shared by 16 MT NW rows. With `groups` > 1
-// the keys of a row block are cut into that many ranges, joined afterwards.
+// the keys of a row block are cut into that many ranges, joined afterwards. 2048
+// tokens on 8192 (32 heads of 128, 240 GFLOP): 268 us, 0.90 PFLOP/s of the 1.22
+// that a large product reaches. Bound by issue: a tile's exponentials, widening
+// and addresses take the vector units about as long as its products take the
+// matrix units, and with two wavefronts a SIMD the two overlap in part only.
 template <typename T, int W, int MT, int NW>
 __global__ __launch_bounds__(64 * NW, (NW == 8 ? 2 : 1)) void kv_attention_many_kernel(AttnParams p) {
     typedef Wave<T, W, MT> WV;
@@ -1044,7 +1057,7 @@ __global__ __launch_bounds__(256) void kv_attention_many_join_kernel(AttnParams 
     if (per >= all.tiles) return;
     constexpr int64_t kSlot = kRows * (W + 2);
     const float* base = p.part + (((int64_t)b * p.row_blocks + rb) * p.heads + kh) * p.groups * kSlot;
-    join_row<T, W>(base, base, kSlot, (all.tiles + per - 1) / per, r, kRows * W + r, kRows * W + kRows + r, p.dim,
+    join_row<T, W, 8>(base, base, kSlot, (all.tiles + per - 1) / per, r, kRows * W + r, kRows * W + kRows + r, p.dim,
                    out_row<T>(p, b, kh, row0 + r));
 }
 
