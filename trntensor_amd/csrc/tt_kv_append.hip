@@ -56,23 +56,25 @@ struct Block {
     float* scale;
 };
 
+// (Extents and lengths fit 32 bits: a 64-bit division is a hundred instructions.)
 template <typename T>
-__device__ __forceinline__ bool find_block(const AppendParams& p, int64_t w, Block& k) {
-    const int64_t H = p.c.heads, P = p.c.page;
+__device__ __forceinline__ bool find_block(const AppendParams& p, uint32_t w, Block& k) {
+    const uint32_t H = (uint32_t)p.c.heads, P = (uint32_t)p.c.page, blocks = (uint32_t)p.blocks;
     k.is_v = w & 1;
     w >>= 1;
-    const int64_t h = w % H, j = w / H % p.blocks, b = w / H / p.blocks;
+    const uint32_t pair = w / H, h = w - pair * H, b = pair / blocks, j = pair - b * blocks;
     const int64_t len = p.lengths[b];
     int64_t n = p.counts ? p.counts[b] : p.tokens;
     n = n > p.tokens ? p.tokens : n;
     if (len < 0) return false;
     const int64_t end = len + n < p.table_width * P ? len + n : p.table_width * P;
-    k.first = (len / P + j) * P;
+    const int64_t block = (uint32_t)len / P + j;
+    k.first = block * P;
     k.lo = (int)((len > k.first ? len : k.first) - k.first);
     const int64_t hi = (end < k.first + P ? end : k.first + P) - k.first;
     if (k.lo >= hi) return false;
     k.hi = (int)hi;
-    const int64_t page = p.table[b * p.table_stride + k.first / P];
+    const int64_t page = p.table[b * p.table_stride + block];
     if (page < 0 || page >= p.c.pages) return false;
     const int64_t* stride = k.is_v ? p.v_stride : p.k_stride;
     k.x = static_cast<const T*>(k.is_v ? p.v : p.k) + b * stride[0] + h * stride[2] + (k.first - len) * stride[1];
@@ -260,7 +262,8 @@ template <typename T, int W>
 __device__ __forceinline__ void rotate_token(const AppendParams& p, int64_t row) {
     constexpr int kRow = W / 16;  // lanes a head
     const int tid = threadIdx.x, D = (int)p.c.dim;
-    const int64_t b = row / p.tokens, t = row - b * p.tokens;
+    const uint32_t tokens = (uint32_t)p.tokens;
+    const int64_t b = (uint32_t)row / tokens, t = (uint32_t)row - (uint32_t)b * tokens;
     if (b >= p.batch) return;
     const int64_t n = p.counts ? p.counts[b] : p.tokens, pos = (int64_t)p.lengths[b] + t;
     const bool live = t < n && pos >= 0 && pos < p.table_width * p.c.page;
@@ -392,53 +395,47 @@ __global__ __launch_bounds__(256, (Queries ? 2 : 4)) void kv_append_kernel(Appen
     }
     // values
     const int run0 = k.lo / 16, runs = (k.hi + 15) / 16 - run0, P = (int)p.c.page;
-    auto load = [&](int unit, float* v) {
-        const int t = (run0 + unit / (W / 2)) * 16, d = unit % (W / 2) * 2;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = 0.f;
-        if (d >= D) return;
-        const T* src = x + t * k.row_stride + d;
+    struct Run {
         T two[16][2];
-        if (t >= k.lo && t + 16 <= k.hi) {
+    };
+    // Two elements of a run's 16 tokens, zeros in other slots.
+    auto load = [&](int unit, Run& v) {
+        const int t = (run0 + unit / (W / 2)) * 16, d = unit % (W / 2) * 2;
+        const T* src = x + t * k.row_stride + d;
+        if (d < D && t >= k.lo && t + 16 <= k.hi) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) __builtin_memcpy(two[i], src + i * k.row_stride, sizeof two[i]);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                v[i] = to_f32(two[i][0]);
-                v[16 + i] = to_f32(two[i][1]);
-            }
+            for (int i = 0; i < 16; ++i) __builtin_memcpy(v.two[i], src + i * k.row_stride, sizeof v.two[i]);
             return;
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (t + i >= k.lo && t + i < k.hi) {
-                __builtin_memcpy(two[i], src + i * k.row_stride, sizeof two[i]);
-                v[i] = to_f32(two[i][0]);
-                v[16 + i] = to_f32(two[i][1]);
-            }
+        for (int i = 0; i < 16; ++i) {
+            v.two[i][0] = v.two[i][1] = (T)0.f;
+            if (d < D && t + i >= k.lo && t + i < k.hi) __builtin_memcpy(v.two[i], src + i * k.row_stride, sizeof v.two[i]);
+        }
+    };
+    auto each = [&](const Run& v, auto take, uint32_t& most) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) take(most, to_f32(v.two[i / 2][i & 1]));
     };
     const int units = runs * (W / 2);
-    float held[32];
+    Run held;
     if (tid < units) {
         load(tid, held);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) take_max(top, held[i]);
+        each(held, take_max, top);
     }
     for (int u = tid + 256; u < units; u += 256) {
-        float v[32];
+        Run v;
         load(u, v);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) take_max(top, v[i]);
+        each(v, take_max, top);
     }
     top = top_of_all(top);
     const bool wild = top >= kNotFinite;
     if (wild) {
         uint32_t finite = 0;
         for (int u = tid; u < units; u += 256) {
-            float v[32];
+            Run v;
             load(u, v);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) take_finite_max(finite, v[i]);
+            each(v, take_finite_max, finite);
         }
         top = top_of_all(finite);
     }
@@ -452,7 +449,12 @@ __global__ __launch_bounds__(256, (Queries ? 2 : 4)) void kv_append_kernel(Appen
             u32x4* dst = reinterpret_cast<u32x4*>(k.codes + (int64_t)(d + e) * P + t);
             u32x4 c;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] = codes_of(held + e * 16 + i * 4, inv, wild);
+            for (int i = 0; i < 4; ++i) {
+                float v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = to_f32(held.two[4 * i + j][e]);
+                c[i] = codes_of(v, inv, wild);
+            }
             if (t < k.lo || t + 16 > k.hi) {
                 // a run that holds other tokens: earlier ones, or slots not yet taken
                 const u32x4 was = *dst;
