@@ -447,6 +447,41 @@ def test_kv_attention_scale(hip, scale, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens", [1, 20])
+def test_kv_attention_every_code(hip, tokens, dtype):
+    """Sequence c holds code c: as the only value seen it comes back as it is
+    (every code times a power of two is exact in each type here); as a key
+    beside a zero key it weighs as its value says."""
+    codes = torch.arange(256, dtype=torch.uint8)
+    table, lengths = torch.arange(256, dtype=torch.int32)[:, None].cuda(), _i32([tokens] * 256).cuda()
+    value = codes.view(F8).double()
+    finite = value.isfinite()
+    cache = tt.KVCache.empty(256, 1, 64, page_size=32)
+    cache.v.view(torch.uint8)[:, 0, :, :] = codes.cuda()[:, None, None]
+    cache.v_scale.fill_(2.0 ** -3)
+    q = torch.zeros((256, tokens, 1, 64), dtype=dtype)
+    got = tt.kv_attention(q.cuda(), cache, table, lengths).cpu().double()
+    tol = (U[dtype] + 2.0 ** -24 * 32 + (2.0 ** -8 if tokens > 1 and dtype == torch.bfloat16 else 2.0 ** -15 if tokens > 1 else 0))
+    want = (value / 8)[:, None, None, None].expand(got.shape)
+    if tokens == 1:
+        assert torch.equal(got[finite], want[finite])
+    assert ((got - want)[finite].abs() <= tol * want[finite].abs()).all()
+    assert got[~finite].isnan().all() and not got[finite].isnan().any()
+
+    cache.k.view(torch.uint8)[:, 0, tokens - 1, 5] = codes.cuda()
+    cache.k_scale.fill_(2.0 ** -5)
+    cache.v.view(torch.uint8).zero_()
+    cache.v.view(torch.uint8)[:, 0, :, tokens - 1] = 0x38  # 1.0
+    cache.v_scale.fill_(1.0)
+    q[..., 5] = 1
+    got = tt.kv_attention(q.cuda(), cache, table, lengths, scale=0.5).cpu().double()[finite][:, -1, 0]
+    e = torch.exp(value[finite] / 64)
+    want = (e / (e + tokens - 1))[:, None].expand(got.shape)
+    tol = U[dtype] + (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -15) + 2 * 2.0 ** -24 * 24 * 7 + 2.0 ** -24 * 24
+    assert ((got - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_kv_attention_long(hip, dtype):
     """A long sequence beside short ones, for which the work is split and joined."""
     _attention_case(1, 2, 64, 64, 1, [9000, 3, 0, 4097], None, None, 0, dtype)
@@ -574,6 +609,43 @@ def test_a_step_in_a_graph(hip):
         got = out.clone()
         want = _step(x * (1 + i), w_in, w_out, cache, *rest)  # the same slots: written alike
         assert torch.equal(got, want), i
+
+
+def test_calls_without_the_host_path(hip):
+    """What the compiled host path launches is what Python launches."""
+    g = torch.Generator().manual_seed(31)
+    codes, scales, z = _q4(6 * 64, 256, 64, torch.bfloat16, True, 32)
+    w = tt.Q4Matrix(codes.cuda(), scales.cuda(), 256, 64, zeros=z.cuda())
+    angles = torch.rand((128, 32), generator=g)
+    cos, sin = torch.cos(angles).cuda(), torch.sin(angles).cuda()
+    x = torch.randn((3, 40, 256), generator=g).to(torch.bfloat16).cuda()
+    table = torch.arange(6, dtype=torch.int32).view(3, 2).cuda()
+    held, counts = _i32([0, 30, 64]).cuda(), _i32([40, 0, 13]).cuda()
+    found = []
+    for direct in (True, False):
+        cache = tt.KVCache.empty(6, 2, 64, 64)
+        assert w._host is not None and cache._host is not None
+        host = w._host
+        if not direct:
+            w._host = cache._host = None
+        q, k, v = tt.q4_matmul(x, w).view(3, 40, 6, 64).split([2, 2, 2], dim=2)
+        q = tt.kv_append(cache, k, v, table, held, counts=counts, q=q, cos=cos, sin=sin, interleaved=True)
+        o = tt.kv_attention(q, cache, table, held + counts, counts=counts, window=50, sinks=2)
+        found.append([q, o, cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale])
+        w._host = host
+    for a, b in zip(*found):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("bad", [0.0, -1.0, 3.0, 2.0 ** -65, 2.0 ** 121, float("inf"), float("nan")])
+def test_a_cache_takes_powers_of_two_in_range(hip, bad):
+    c = tt.KVCache.empty(2, 1, 64, 16)
+    for ok in (2.0 ** -64, 2.0 ** 120):
+        tt.KVCache(c.k, c.v, torch.full_like(c.k_scale, ok), torch.full_like(c.v_scale, ok), 64)
+    scale = c.v_scale.clone()
+    scale[1, 0] = bad
+    with pytest.raises(ValueError, match="powers of two"):
+        tt.KVCache(c.k, c.v, c.k_scale, scale, 64)
 
 
 def test_results_repeat_bit_for_bit(hip):
