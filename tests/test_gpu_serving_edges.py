@@ -1,0 +1,69 @@
+"""Serving operators on the GPU where their precision and their ranges end,
+against their definitions in float64 (oracle/serving.py). Every tolerance is
+derived at its test, before its first run; u is the unit roundoff of a result's
+dtype (2^-24, 2^-9, 2^-12 for float32, bfloat16, float16).
+"""
+
+import math
+
+import pytest
+import torch
+
+import trntensor_amd as tt
+from oracle import serving as ref
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -9, torch.float16: 2.0 ** -12}
+DTYPES = list(U)
+F8 = torch.float8_e4m3fn
+
+
+def _i32(values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+def _cache(pages, heads, page, dim, seed):
+    """A cache of random codes and scales on the device, and the same as float64 values for the oracle."""
+    g = torch.Generator().manual_seed(seed)
+    w = -(-dim // 64) * 64
+    k, v = ((torch.randn(s, generator=g) * 90).clamp(-448, 448).to(F8)
+            for s in ((pages, heads, page, w), (pages, heads, w, page)))
+    k.view(torch.uint8)[..., dim:] = 0
+    ks, vs = (torch.exp2(torch.randint(-9, -5, (pages, heads), generator=g).float()) for _ in range(2))
+    return (tt.KVCache(k.cuda(), v.cuda(), ks.cuda(), vs.cuda(), head_dim=dim),
+            {"k": k.double(), "v": v.double(), "k_scale": ks.double(), "v_scale": vs.double()})
+
+
+@pytest.mark.parametrize("tokens", [1, 18])
+@pytest.mark.parametrize("low", [-64, -60, -8, 100])
+def test_kv_attention_float32_weights_do_not_depend_on_value_scales(hip, low, tokens):
+    """Two keys of nearly equal weight, in pages whose value scales lie far
+    apart: the values of one page outweigh the other's, so that the result is a
+    weight times that page's value.
+
+    Tolerance: scores are at most 2^-4, so their errors are below 2^-24 of the
+    result. Each of two exponentials errs by a unit in the last place (2^-23)
+    and moves the result p by p (1 - p) <= 1/4 of it; their sum, its reciprocal,
+    the product and the result round by 2^-24 each, the split into parts by
+    2^-24, the product's sums by 2^-24: below 2^-21 of the value in all.
+    """
+    batch, heads, share, dim, page = 16, 4, 4 if tokens == 1 else 1, 64, 16
+    dev, want = _cache(2 * batch, heads, page, dim, 1)
+    # Token 0 in one page, the last in the other: a window of one and one sink.
+    value = torch.tensor(1.0)
+    dev.v.copy_(value.to(F8).expand(dev.v.shape))
+    want["v"].fill_(1.0)
+    scales = torch.exp2(torch.tensor([0.0, low])).repeat(batch)[:, None].expand(2 * batch, heads)
+    dev.v_scale.copy_(scales)
+    want["v_scale"].copy_(scales)
+    table = torch.arange(2 * batch, dtype=torch.int32).reshape(batch, 2)
+    table[1::2] = table[1::2].flip(1)
+    held = 17
+    q = torch.randn((batch, 1, heads * share, dim), generator=torch.Generator().manual_seed(2)) * 2.0 ** -6
+    # More rows than one tile's: the last token's, behind rows that are before the sequence's start.
+    rows = q.expand(batch, tokens, heads * share, dim).contiguous()
+    got = tt.kv_attention(rows.cuda(), dev, table.cuda(), _i32([held] * batch).cuda(), window=1, sinks=1)[:, -1:]
+    out, spread = ref.attention(q, want, table, [held] * batch, None, dim ** -0.5, 1, 1)
+    err = (got.cpu().double() - out).abs() / spread[..., 1:2]
+    assert err.max() <= 2.0 ** -21, f"2^{math.log2(err.max()):.1f} of the values"

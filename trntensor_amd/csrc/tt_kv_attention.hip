@@ -252,14 +252,15 @@ __device__ __forceinline__ const uint8_t* v_run(const AttnParams& p, const Runs&
 
 // The scales of the run whose keys' scores a lane holds, as loaded: what is
 // made of them is made where they are used, not where that would be a wait for
-// them. A value's scale is 2^v_exp(): probabilities are formed times it, as
-// exp2 of one sum, and sums of probabilities are taken with 2^-v_exp().
+// them. A value's scale is a power of two, 2^v_exp(): probabilities enter the
+// second product times it, and their sums are taken with 2^-v_exp().
 struct Scales {
     float k, v;
     bool ok;
 
     __device__ __forceinline__ float key() const { return ok ? k : 0.f; }
     __device__ __forceinline__ float v_exp() const { return ok ? (float)((int)(__float_as_uint(v) >> 23 & 255) - 127) : 0.f; }
+    __device__ __forceinline__ float value() const { return ok ? __uint_as_float(__float_as_uint(v) & 0x7f800000u) : 1.f; }
     // 2^-v_exp() as two bfloat16 values; the low one is that of a float in its upper half.
     __device__ __forceinline__ uint32_t v_inv() const {
         const uint32_t inv = (ok ? 254 - (__float_as_uint(v) >> 23 & 255) : 127u) << 7;
@@ -417,7 +418,11 @@ __device__ __forceinline__ void tile_weights(const AttnParams& p, Wave<T, W, MT>
     const float c = fmaxf(sc.key() * p.scale, 1e-30f);
     const uint32_t inv = sc.v_inv();
     const u32x4 one = {inv, inv, inv, inv};
-    const float v_exp = sc.v_exp();
+    // A value's scale enters as a term of the exponent, which then has up to 7
+    // bits fewer behind the point (2^-18 of a weight at a scale of 2^-64), below
+    // what the parts of 16-bit types keep; float32 weights are multiplied by it.
+    constexpr bool kApart = sizeof(T) == 4;
+    const float v_exp = kApart ? 0.f : sc.v_exp(), v_scale = kApart ? sc.value() : 1.f;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         float top = s[mt][0][0];
@@ -442,12 +447,16 @@ __device__ __forceinline__ void tile_weights(const AttnParams& p, Wave<T, W, MT>
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][2 * h + i / 4][i & 3], c, shift));
-            u32x4 parts[WV::PP];
-            split8<WV::PP>(e, parts);
             if constexpr (!SumOnMfma) {
                 const float sum = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-                w.l[mt][0] += sum * __uint_as_float(inv << 16);
+                w.l[mt][0] += kApart ? sum : sum * __uint_as_float(inv << 16);
             }
+            if constexpr (kApart) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] *= v_scale;
+            }
+            u32x4 parts[WV::PP];
+            split8<WV::PP>(e, parts);
 #pragma unroll
             for (int n = 0; n < WV::PP; ++n) {
                 prob[mt][n][h] = parts[n];
