@@ -1,7 +1,7 @@
 """Serving operators on the GPU where their precision and their ranges end,
 against their definitions in float64 (oracle/serving.py). Every tolerance is
 derived at its test, before its first run; u is the unit roundoff of a result's
-dtype (2^-24, 2^-9, 2^-12 for float32, bfloat16, float16).
+dtype (2^-24, 2^-8, 2^-11 for float32, bfloat16, float16).
 """
 
 import math
@@ -14,7 +14,7 @@ from oracle import serving as ref
 
 pytestmark = pytest.mark.gpu
 
-U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -9, torch.float16: 2.0 ** -12}
+U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 DTYPES = list(U)
 F8 = torch.float8_e4m3fn
 
@@ -67,3 +67,37 @@ def test_kv_attention_float32_weights_do_not_depend_on_value_scales(hip, low, to
     out, spread = ref.attention(q, want, table, [held] * batch, None, dim ** -0.5, 1, 1)
     err = (got.cpu().double() - out).abs() / spread[..., 1:2]
     assert err.max() <= 2.0 ** -21, f"2^{math.log2(err.max()):.1f} of the values"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,held", [(1, 5), (1, 40), (3, 200), (40, 200), (1, 3000)])
+def test_kv_attention_sums_the_weights_that_it_applies(hip, tokens, held, dtype):
+    """Values that lie close together far from zero: rounding a weight may move
+    a result by its share of the values' distance from the result, not of the
+    values, because the weights' sum is that of the rounded ones.
+
+    Tolerance: the result's rounding, u |o|; the weights' (2^-8 in bfloat16,
+    2^-16 in two parts), times sum p |v - o|; an error ds of the scores, 2 ds
+    max |v - o| with ds = 2^-24 (16 + sqrt D) sum |q k| scale; and for sums in
+    32 bits over L keys, and the exponentials, 2^-24 (16 + sqrt L) max |v|.
+    """
+    batch, heads, share, dim, page = 6, 2, 4, 64, 16
+    width = -(-held // page)
+    dev, want = _cache(batch * width, heads, page, dim, 3)
+    v = (1.0 + 0.125 * torch.randint(0, 2, dev.v.shape, generator=torch.Generator().manual_seed(4))).to(F8)
+    dev.v.copy_(v.cuda())
+    dev.v_scale.fill_(1.0)
+    want["v"], want["v_scale"] = v.double(), torch.ones_like(want["v_scale"])
+    table = torch.arange(batch * width, dtype=torch.int32).reshape(batch, width).flip(1).contiguous()
+    q = torch.randn((batch, tokens, heads * share, dim), generator=torch.Generator().manual_seed(5)).to(dtype)
+    lengths = [held] * batch
+    got = tt.kv_attention(q.cuda(), dev, table.cuda(), _i32(lengths).cuda()).cpu().double()
+    out, spread = ref.attention(q, want, table, lengths, None, dim ** -0.5, None, 0)
+    # sum p |v - o| is at most twice p (1 - p) times the values' step, p being the larger ones' weight.
+    p = (out - 1.0) / 0.125
+    apart = 0.25 * p * (1 - p)
+    ds = 2.0 ** -24 * (16 + math.sqrt(dim)) * spread[..., 0:1]
+    tol = (U[dtype] * out.abs() + (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -16) * apart + 2 * ds * 0.125
+           + 2.0 ** -24 * (16 + math.sqrt(held)) * 1.125)
+    err = (got - out).abs()
+    assert (err <= tol).all(), f"{(err / tol).max():.3g} times the tolerance, {(err > tol).sum()} of {err.numel()}"

@@ -409,8 +409,11 @@ __device__ __forceinline__ void mask_scores(const AttnParams& p, Wave<T, W, MT>&
 }
 
 // The weights of one tile's keys, of products s (-inf where masked), as the
-// operands of the second product, and their sum and maximum in the running state.
-template <typename T, int W, int MT, bool SumOnMfma>
+// operands of the second product, and their sum and maximum in the running
+// state. What is summed are the weights as that product takes them: rounding
+// then moves a result in proportion to how far values lie from it, not to
+// their size.
+template <typename T, int W, int MT>
 __device__ __forceinline__ void tile_weights(const AttnParams& p, Wave<T, W, MT>& w, const Scales& sc, f32x4 (&s)[MT][4],
                                              u32x4 (&prob)[MT][Wave<T, W, MT>::PP][2]) {
     typedef Wave<T, W, MT> WV;
@@ -447,10 +450,6 @@ __device__ __forceinline__ void tile_weights(const AttnParams& p, Wave<T, W, MT>
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][2 * h + i / 4][i & 3], c, shift));
-            if constexpr (!SumOnMfma) {
-                const float sum = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-                w.l[mt][0] += kApart ? sum : sum * __uint_as_float(inv << 16);
-            }
             if constexpr (kApart) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) e[i] *= v_scale;
@@ -460,7 +459,7 @@ __device__ __forceinline__ void tile_weights(const AttnParams& p, Wave<T, W, MT>
 #pragma unroll
             for (int n = 0; n < WV::PP; ++n) {
                 prob[mt][n][h] = parts[n];
-                if constexpr (SumOnMfma) w.l[mt] = mma_bf16(one, parts[n], w.l[mt]);
+                w.l[mt] = mma_bf16(one, parts[n], w.l[mt]);
             }
         }
     }
@@ -539,7 +538,7 @@ __device__ __forceinline__ void walk(const AttnParams& p, Wave<T, W, MT>& w, con
             }
         }
         u32x4 prob[MT][WV::PP][2];
-        tile_weights<T, W, MT, false>(p, w, now, s, prob);
+        tile_weights<T, W, MT>(p, w, now, s, prob);
 #pragma unroll
         for (int d = 0; d < W / 16; ++d)
 #pragma unroll
@@ -591,7 +590,7 @@ __device__ __forceinline__ void join_waves(const AttnParams& p, Wave<T, W, 1>& w
     __shared__ float so[4][16][68];
     const int tid = fresh_lane(threadIdx.x), dim = fresh(p.dim);
     const int lane = tid & 63, wave = uniform(tid >> 6), c = lane & 15, g = lane >> 4;
-    const float l = column_sum(w.l[0][0]);
+    const float l = w.l[0][0];
     const bool any = column_sum(w.any[0] ? 1.f : 0.f) > 0.f;
     if (g == 0) {
         sm[wave][c] = w.m[0];
@@ -974,7 +973,7 @@ __global__ __launch_bounds__(64 * NW, (NW == 8 ? 2 : 1)) void kv_attention_many_
                 mask_scores<T, W, MT>(p, w, now.ok, s, tile, mask);
             }
             u32x4 prob[MT][WV::PP][2];
-            tile_weights<T, W, MT, true>(p, w, now, s, prob);
+            tile_weights<T, W, MT>(p, w, now, s, prob);
             if (!full && nan_values[n % 3]) {
                 // Values staged without their NaN, which not every row
                 // sees: it is given to those that do.
