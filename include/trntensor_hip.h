@@ -259,7 +259,10 @@ int tt_strided_contract(int dtype, int n_out, const int64_t* out_shape,
  * Their arguments travel in structs whose fields are all 8 bytes wide, in the
  * order given. Element strides count elements, pitches count bytes. dtype is
  * TT_F32, TT_BF16 or TT_F16; sums, softmax statistics and rotations are held
- * in 32 bits and rounded once at the store.
+ * in 32 bits, results rounded once at the store. What is rounded before that:
+ * tt_kv_attention's weights, to 8 bits (TT_BF16), 16 (TT_F16) or 24 (TT_F32),
+ * as their sum and their product with the values take them; tt_q4_matmul sums
+ * x (1 + code / 16) and takes the offset off, which costs about 2 of 24 bits.
  * --------------------------------------------------------------------- */
 
 /*

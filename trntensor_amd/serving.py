@@ -17,7 +17,10 @@ All three run on torch's current stream and never wait for the device: how
 many tokens each sequence holds, and in which pages, is read there. They have
 no backward pass, and refuse tensors that ask for one. Activations are
 float32, bfloat16 or float16; sums, softmax statistics and rotations are held
-in 32 bits and rounded once. Operands on the host are staged to the weights'
+in 32 bits, and results rounded once to the activations' dtype. Two steps
+before that round too: attention's weights enter the product with the values
+in 8 bits for bfloat16, 16 for float16 and 24 for float32, and 4-bit products
+keep about 22 of the 24 bits. Operands on the host are staged to the weights'
 or cache's device, and the result goes back to the first one's.
 """
 
@@ -131,9 +134,13 @@ def q4_matmul(x: torch.Tensor, w: Q4Matrix) -> torch.Tensor:
 
     Codes are widened in registers on their way into the matrix units, so the
     weights cross memory at half a byte each; products are summed in 32 bits
-    and the result is rounded once to x's dtype. Rows of x need a unit stride
-    and one row pitch, else they are copied. A row of x that holds an infinity
-    gives infinities or NaN, one that holds NaN gives NaN.
+    and the result is rounded once to x's dtype. Summed are x times 1 + code /
+    16, and the share of the offset is taken off, which costs about two of the
+    24 bits: codes that equal their zero point give 2^-22 of sum |x| s 16, not
+    always 0. Rows of x need a unit stride and one row pitch, else they are
+    copied. A row of x that holds an infinity gives infinities or NaN, one that
+    holds NaN gives NaN; sums of x beyond float32's range overflow however small
+    the scales, and so do scales of 2^124 and more.
     """
     if w._host is not None and dispatch._use_hip() and isinstance(x, torch.Tensor):
         y = w._host.run(x)
@@ -372,8 +379,11 @@ def kv_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, leng
 
     Returns q's shape and dtype; queries that see nothing (empty sequences,
     rows past their count) give zeros. No masked slot has any influence,
-    whatever its page holds. Weighted sums are held in 32 bits before they are
-    divided: values of 2^100 and more may overflow them.
+    whatever its page holds. The products of a query and a key's codes, and
+    weighted sums before they are divided, are held in 32 bits: queries of 2^110
+    and values of 2^100 and more may overflow them. bfloat16 calls round the
+    weights to 8 bits before they are summed and applied (float16 16, float32
+    24): a result errs by up to 2^-8 of its values' distance from it.
     """
     if cache._host is not None and dispatch._use_hip():
         out = cache._host.attention(q, page_table, lengths, counts, cache._scale if scale is None else scale,
