@@ -1106,7 +1106,7 @@ double many_cost(const tt_kv_attention_args* a, const Shape& s, int64_t W, int64
 struct Cut {
     bool few, direct;
     int mt, waves, row_blocks, groups;
-    int64_t grid, slots, slot_floats;
+    int64_t grid, join, slots, slot_floats;  // workgroups, and those that join partial results
 };
 
 Cut cut_of(const tt_kv_attention_args* a) {
@@ -1137,6 +1137,7 @@ Cut cut_of(const tt_kv_attention_args* a) {
         c.direct = tiles <= most;
         c.groups = 512;  // two a compute unit; 256 and 1024 were 8% slower at some length each, level at others
         c.grid = c.direct ? pairs : c.groups;
+        c.join = c.direct ? 0 : pairs;
         c.slots = c.direct ? 0 : 2 * c.groups;
         c.slot_floats = 16 * (W + 2);
     } else {
@@ -1161,6 +1162,7 @@ Cut cut_of(const tt_kv_attention_args* a) {
         }
         const int64_t block = 16 * c.mt * c.waves, blocks = pairs * c.row_blocks;
         c.grid = blocks * c.groups;
+        c.join = blocks * 4 * c.mt * c.waves;
         c.slots = c.groups > 1 ? blocks * c.groups : 0;
         c.slot_floats = block * (W + 2);
     }
@@ -1170,10 +1172,7 @@ Cut cut_of(const tt_kv_attention_args* a) {
 template <typename T, int W, int MT, int NW>
 int attn_many(const AttnParams& p, const Cut& c, hipStream_t st) {
     kv_attention_many_kernel<T, W, MT, NW><<<(uint32_t)c.grid, 64 * NW, 0, st>>>(p);
-    if (c.groups > 1) {
-        const uint32_t join = (uint32_t)((int64_t)p.batch * p.heads * p.row_blocks * 4 * MT * NW);
-        kv_attention_many_join_kernel<T, W, 16 * MT * NW><<<join, 256, 0, st>>>(p);
-    }
+    if (c.groups > 1) kv_attention_many_join_kernel<T, W, 16 * MT * NW><<<(uint32_t)c.join, 256, 0, st>>>(p);
     return check_launch("tt_kv_attention");
 }
 
@@ -1181,7 +1180,7 @@ template <typename T, int W>
 int attn_launch(const AttnParams& p, const Cut& c, hipStream_t st) {
     if (c.few) {
         kv_attention_few_kernel<T, W><<<(uint32_t)c.grid, 256, 0, st>>>(p);
-        if (!c.direct) kv_attention_few_join_kernel<T, W><<<(uint32_t)(p.batch * p.heads), 256, 0, st>>>(p);
+        if (c.join) kv_attention_few_join_kernel<T, W><<<(uint32_t)c.join, 256, 0, st>>>(p);
         return check_launch("tt_kv_attention");
     }
     if (c.waves == 4) return attn_many<T, W, 1, 4>(p, c, st);
@@ -1240,9 +1239,8 @@ extern "C" int tt_kv_attention(const tt_kv_attention_args* a, void* stream) {
     if (int rc = check_attention(a)) return rc;
     if (a->batch == 0 || a->tokens == 0) return TT_OK;
     const Cut c = cut_of(a);
-    const int64_t join = a->batch * a->cache.heads * c.row_blocks * 4 * c.mt * c.waves;
-    if (c.grid > kMaxGrid || join > kMaxGrid)
-        return set_error(TT_UNSUPPORTED, "tt_kv_attention: %lld workgroups", (long long)c.grid);
+    if (c.grid > kMaxGrid || c.join > kMaxGrid)
+        return set_error(TT_UNSUPPORTED, "tt_kv_attention: %lld workgroups", (long long)(c.grid > c.join ? c.grid : c.join));
     const int64_t need = c.slots * c.slot_floats * 4;
     if (need > 0 && (!a->workspace || a->workspace_bytes < need || (uintptr_t)a->workspace % 16))
         return set_error(TT_INVALID, "tt_kv_attention: workspace of %lld bytes, need %lld", (long long)a->workspace_bytes,
