@@ -101,3 +101,16 @@ def test_kv_attention_sums_the_weights_that_it_applies(hip, tokens, held, dtype)
            + 2.0 ** -24 * (16 + math.sqrt(held)) * 1.125)
     err = (got - out).abs()
     assert (err <= tol).all(), f"{(err / tol).max():.3g} times the tolerance, {(err > tol).sum()} of {err.numel()}"
+
+
+def test_kv_attention_of_more_row_blocks_than_a_join_would_take(hip):
+    """A million sequences of more than 16 query rows: one launch, whose
+    workgroups need no others to join what they find."""
+    batch, tokens, dim, page = 1_100_000, 17, 16, 32
+    dev, _ = _cache(5, 1, page, dim, 6)
+    table = _i32([[3], [0], [4], [1], [2]]).repeat(batch // 5, 1)
+    q = torch.randn((5, tokens, 1, dim), generator=torch.Generator().manual_seed(7)).to(torch.bfloat16).cuda()
+    lengths = _i32([17, 32, 20, 0, 25])
+    want = tt.kv_attention(q, dev, table[:5].cuda(), lengths.cuda())
+    got = tt.kv_attention(q.repeat(batch // 5, 1, 1, 1), dev, table.cuda(), lengths.repeat(batch // 5).cuda())
+    assert torch.equal(got.view(batch // 5, 5, tokens, 1, dim), want.expand(batch // 5, -1, -1, -1, -1))

@@ -32,3 +32,10 @@ def test_attention_refuses_more_pairs_than_one_launch_has_workgroups(lib, width)
     head is one (short tables) or is joined by one (long tables)."""
     assert _attention(lib, batch=1 << 23, width=width) == _lib.TT_UNSUPPORTED
     assert lib.tt_last_error() == b"tt_kv_attention: 16777216 workgroups"
+
+
+def test_attention_refuses_row_blocks_that_no_launch_holds(lib):
+    """Workgroups of eight wavefronts count twice: 2^23 - 1 of them."""
+    kw = dict(batch=1 << 20, cache=dict(heads=1), q_heads=1, width=1)
+    assert _attention(lib, tokens=10 * 256, **kw) == _lib.TT_UNSUPPORTED
+    assert lib.tt_last_error().startswith(b"tt_kv_attention: ")

@@ -1162,7 +1162,7 @@ Cut cut_of(const tt_kv_attention_args* a) {
         }
         const int64_t block = 16 * c.mt * c.waves, blocks = pairs * c.row_blocks;
         c.grid = blocks * c.groups;
-        c.join = blocks * 4 * c.mt * c.waves;
+        c.join = c.groups > 1 ? blocks * 4 * c.mt * c.waves : 0;
         c.slots = c.groups > 1 ? blocks * c.groups : 0;
         c.slot_floats = block * (W + 2);
     }
@@ -1172,7 +1172,7 @@ Cut cut_of(const tt_kv_attention_args* a) {
 template <typename T, int W, int MT, int NW>
 int attn_many(const AttnParams& p, const Cut& c, hipStream_t st) {
     kv_attention_many_kernel<T, W, MT, NW><<<(uint32_t)c.grid, 64 * NW, 0, st>>>(p);
-    if (c.groups > 1) kv_attention_many_join_kernel<T, W, 16 * MT * NW><<<(uint32_t)c.join, 256, 0, st>>>(p);
+    if (c.join) kv_attention_many_join_kernel<T, W, 16 * MT * NW><<<(uint32_t)c.join, 256, 0, st>>>(p);
     return check_launch("tt_kv_attention");
 }
 
@@ -1239,7 +1239,8 @@ extern "C" int tt_kv_attention(const tt_kv_attention_args* a, void* stream) {
     if (int rc = check_attention(a)) return rc;
     if (a->batch == 0 || a->tokens == 0) return TT_OK;
     const Cut c = cut_of(a);
-    if (c.grid > kMaxGrid || c.join > kMaxGrid)
+    const int64_t most = c.waves > 4 ? kMaxGrid / 2 : kMaxGrid;  // of eight wavefronts: half as many
+    if (c.grid > most || c.join > kMaxGrid)
         return set_error(TT_UNSUPPORTED, "tt_kv_attention: %lld workgroups", (long long)(c.grid > c.join ? c.grid : c.join));
     const int64_t need = c.slots * c.slot_floats * 4;
     if (need > 0 && (!a->workspace || a->workspace_bytes < need || (uintptr_t)a->workspace % 16))
