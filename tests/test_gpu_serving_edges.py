@@ -114,3 +114,17 @@ def test_kv_attention_of_more_row_blocks_than_a_join_would_take(hip):
     want = tt.kv_attention(q, dev, table[:5].cuda(), lengths.cuda())
     got = tt.kv_attention(q.repeat(batch // 5, 1, 1, 1), dev, table.cuda(), lengths.repeat(batch // 5).cuda())
     assert torch.equal(got.view(batch // 5, 5, tokens, 1, dim), want.expand(batch // 5, -1, -1, -1, -1))
+
+
+def test_kv_append_of_more_query_rows_than_a_launch_has_workgroups(hip):
+    """2^24 rows of queries, four a workgroup; most lie past the table's end and give zeros."""
+    tokens, dim, page = 1 << 23, 16, 65536
+    dev = tt.KVCache.empty(2, 1, dim, page)
+    angle = torch.rand((page, dim // 2), generator=torch.Generator().manual_seed(8)).cuda()
+    row = torch.randn((2, 1, 1, dim), generator=torch.Generator().manual_seed(9)).to(torch.bfloat16).cuda()
+    args = (_i32([[0], [1]]).cuda(), _i32([page - 70, page - 20]).cuda())
+    kw = dict(cos=angle.cos(), sin=angle.sin())
+    want = tt.kv_append(dev, *(row.expand(2, 100, 1, dim),) * 2, *args, q=row.expand(2, 100, 1, dim), **kw)
+    got = tt.kv_append(dev, *(row.expand(2, tokens, 1, dim),) * 2, *args, q=row.expand(2, tokens, 1, dim), **kw)
+    assert want[0, :70].ne(0).any() and not want[0, 70:].any() and not want[1, 20:].any()
+    assert torch.equal(got[:, :100], want) and not got[:, 100:].any()

@@ -503,9 +503,11 @@ int append_width(const AppendParams& p, int64_t rows, hipStream_t st) {
 template <typename T>
 int append_launch(const AppendParams& p, bool queries, hipStream_t st) {
     const int64_t rows = queries ? p.batch * p.tokens : 0;
-    if (p.kv_groups + rows > kMaxGrid)
-        return set_error(TT_UNSUPPORTED, "tt_kv_append: %lld workgroups", (long long)(p.kv_groups + rows));
-    if (p.c.dim % 8 != 0 || p.rot % 16 != 0) {
+    const bool any = p.c.dim % 8 != 0 || p.rot % 16 != 0;
+    // (kv_groups is within a launch's limit; four rows of queries are a workgroup, those of a launch of their own.)
+    const int64_t grid = any ? p.kv_groups + rows : (rows + 3) / 4;
+    if (grid > kMaxGrid) return set_error(TT_UNSUPPORTED, "tt_kv_append: %lld workgroups", (long long)grid);
+    if (any) {
         kv_append_any_kernel<T><<<(uint32_t)(p.kv_groups + rows), 256, 0, st>>>(p);
         return check_launch("tt_kv_append");
     }
