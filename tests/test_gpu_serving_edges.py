@@ -8,6 +8,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import trntensor_amd as tt
 from oracle import serving as ref
@@ -128,3 +129,19 @@ def test_kv_append_of_more_query_rows_than_a_launch_has_workgroups(hip):
     got = tt.kv_append(dev, *(row.expand(2, tokens, 1, dim),) * 2, *args, q=row.expand(2, tokens, 1, dim), **kw)
     assert want[0, :70].ne(0).any() and not want[0, 70:].any() and not want[1, 20:].any()
     assert torch.equal(got[:, :100], want) and not got[:, 100:].any()
+
+
+@pytest.mark.parametrize("name", ["x", "attention q", "k", "v", "q"])
+def test_calls_on_the_device_refuse_tangents(hip, name):
+    """The compiled path of ordinary calls does not lose them either."""
+    table, held = _i32([[0, 1], [2, 3]]).cuda(), _i32([3, 0]).cuda()
+    dev, _ = _cache(4, 2, 16, 64, 10)
+    kw = {n: torch.zeros((2, 1, 2, 64), device="cuda") for n in ("k", "v", "q", "attention q", "x")}
+    w = tt.Q4Matrix(torch.zeros((8, 32), dtype=torch.uint8), torch.ones((8, 1)), 64, 64)
+    cos = torch.zeros((32, 32), device="cuda")
+    with forward_ad.dual_level():
+        kw[name] = forward_ad.make_dual(kw[name], torch.ones_like(kw[name]))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            tt.kv_append(dev, kw["k"], kw["v"], table, held, q=kw["q"], cos=cos, sin=cos)
+            tt.kv_attention(kw["attention q"], dev, table, held)
+            tt.q4_matmul(kw["x"], w)

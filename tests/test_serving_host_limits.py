@@ -5,7 +5,9 @@ import struct
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
+import trntensor_amd as tt
 from trntensor_amd.hip import _lib
 
 
@@ -39,3 +41,49 @@ def test_attention_refuses_row_blocks_that_no_launch_holds(lib):
     kw = dict(batch=1 << 20, cache=dict(heads=1), q_heads=1, width=1)
     assert _attention(lib, tokens=10 * 256, **kw) == _lib.TT_UNSUPPORTED
     assert lib.tt_last_error().startswith(b"tt_kv_attention: ")
+
+
+class _Cache:
+    """What the checks before a launch read of a cache."""
+
+    head_dim, num_heads, page_size = 64, 2, 16
+    device = torch.device("cpu")
+    _host = None
+
+
+class _Weights:
+    shape = (8, 64)
+    device = torch.device("cpu")
+    _host = None
+
+
+def _append(mark, name):
+    x, cos = torch.zeros((2, 3, 2, 64)), torch.zeros((64, 32))
+    kw = dict(k=x, v=x, q=x, cos=cos, sin=cos)
+    kw[name] = mark(kw[name])
+    table, held = torch.zeros((2, 4), dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    return tt.kv_append(_Cache(), kw.pop("k"), kw.pop("v"), table, held, **kw)
+
+
+def _attend(mark, name):
+    q = mark(torch.zeros((2, 3, 2, 64)))
+    return tt.kv_attention(q, _Cache(), torch.zeros((2, 4), dtype=torch.int32), torch.zeros(2, dtype=torch.int32))
+
+
+def _multiply(mark, name):
+    return tt.q4_matmul(mark(torch.zeros((3, 64))), _Weights())
+
+
+def _dual(t):
+    return forward_ad.make_dual(t, torch.ones_like(t))
+
+
+ROWS = [(_multiply, "x"), (_attend, "q"), (_append, "k"), (_append, "v"), (_append, "q")]
+
+
+@pytest.mark.parametrize("context", [torch.enable_grad, torch.no_grad])
+@pytest.mark.parametrize("call,name", ROWS)
+def test_calls_refuse_tangents(call, name, context):
+    """A dual tensor does not require grad, and no_grad leaves forward mode on."""
+    with forward_ad.dual_level(), context(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        call(_dual, name)

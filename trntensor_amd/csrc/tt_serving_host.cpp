@@ -12,6 +12,7 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
+#include <torch/csrc/autograd/forward_grad.h>
 
 #include <cstring>
 #include <string>
@@ -72,7 +73,12 @@ int64_t code_of(at::ScalarType t) {
 struct Place {
     c10::DeviceIndex device;
 
-    bool here() const { return c10::hip::current_device() == device; }
+    // Within forward mode (which no_grad leaves on) operands may have tangents: Python looks for them.
+    bool here() const {
+        const bool forward =
+            c10::AutogradState::get_tls_state().get_fw_grad_mode() && torch::autograd::ForwardADLevel::try_get_by_idx(0);
+        return !forward && c10::hip::current_device() == device;
+    }
     bool holds(const Tensor& t) const { return t.is_cuda() && t.device().index() == device && !wants_grad(t); }
     static bool wants_grad(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
     Tensor empty(c10::IntArrayRef sizes, at::ScalarType t) const {

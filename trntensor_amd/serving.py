@@ -30,6 +30,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from .hip import _fastpath, _lib, dispatch, engine
 
@@ -52,10 +53,13 @@ def _check_dtype(what: str, t: torch.Tensor) -> int:
 
 
 def _check_grad(what: str, *tensors) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or detach its operands")
+    for t in tensors:
+        if t is None:
+            continue
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or detach its operands")
+        if torch._C._is_fwd_grad_enabled() and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative: take its operands' primals")
 
 
 def _launch(name: str, device: torch.device, *args) -> None:
