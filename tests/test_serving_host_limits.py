@@ -87,3 +87,11 @@ def test_calls_refuse_tangents(call, name, context):
     """A dual tensor does not require grad, and no_grad leaves forward mode on."""
     with forward_ad.dual_level(), context(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
         call(_dual, name)
+
+
+@pytest.mark.parametrize("name", ["cos", "sin"])
+def test_append_refuses_derivatives_of_angles(name):
+    with pytest.raises(RuntimeError, match="no backward"):
+        _append(lambda t: t.clone().requires_grad_(), name)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        _append(_dual, name)

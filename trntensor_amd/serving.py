@@ -334,7 +334,7 @@ def kv_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table: torc
     if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
         raise RuntimeError("k, v and q must share one dtype")
     v = _rows(cache, v, "v", batch, tokens, cache.num_heads)
-    _check_grad("kv_append", k, v, q)
+    _check_grad("kv_append", k, v, q, cos, sin)
     dispatch.require_hip()
     table, lengths, counts = _schedule(cache, batch, page_table, lengths, counts)
     rot = 0
