@@ -145,3 +145,18 @@ def test_calls_on_the_device_refuse_tangents(hip, name):
             tt.kv_append(dev, kw["k"], kw["v"], table, held, q=kw["q"], cos=cos, sin=cos)
             tt.kv_attention(kw["attention q"], dev, table, held)
             tt.q4_matmul(kw["x"], w)
+
+
+def test_weights_and_caches_that_ask_for_a_gradient(hip):
+    """Refused while gradients are on; taken as numbers under no_grad."""
+    codes = torch.randint(0, 256, (8, 32), generator=torch.Generator().manual_seed(11), dtype=torch.uint8)
+    scales, x = torch.ones((8, 1)), torch.ones((1, 64)).cuda()
+    want = tt.q4_matmul(x, tt.Q4Matrix(codes, scales, 64, 64))
+    with torch.no_grad():
+        assert torch.equal(tt.q4_matmul(x, tt.Q4Matrix(codes, scales.clone().requires_grad_(), 64, 64)), want)
+    c = tt.KVCache.empty(2, 1, 64, 16)
+    ask = c.v_scale.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="KVCache has no backward"):
+        tt.KVCache(c.k, c.v, c.k_scale, ask, 64)
+    with torch.no_grad():
+        tt.KVCache(c.k, c.v, c.k_scale, ask, 64)

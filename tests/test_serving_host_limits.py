@@ -95,3 +95,16 @@ def test_append_refuses_derivatives_of_angles(name):
         _append(lambda t: t.clone().requires_grad_(), name)
     with forward_ad.dual_level(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
         _append(_dual, name)
+
+
+@pytest.mark.parametrize("name", ["scales", "zeros"])
+def test_weights_refuse_scales_that_ask_for_a_derivative(name):
+    """The copies that are laid out would not be theirs any more."""
+    kw = dict(scales=torch.ones((8, 1)), zeros=torch.ones((8, 1)))
+    codes, plain = torch.zeros((8, 32), dtype=torch.uint8), kw[name]
+    kw[name] = plain.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no backward"):
+        tt.Q4Matrix(codes, kw["scales"], 64, 64, zeros=kw["zeros"])
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        kw[name] = _dual(plain)
+        tt.Q4Matrix(codes, kw["scales"], 64, 64, zeros=kw["zeros"])

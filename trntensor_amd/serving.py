@@ -89,7 +89,8 @@ class Q4Matrix:
 
     The weights are laid out once, here, in copies on ``codes``' device (the
     current GPU if that is the host): codes in the tiles that the matrix units
-    take, scales with the output features contiguous.
+    take, scales with the output features contiguous. Scales and zero points
+    that ask for a gradient are refused.
     """
 
     __slots__ = ("packed", "scales", "zeros", "shape", "group_size", "device", "_code", "_host")
@@ -108,6 +109,7 @@ class Q4Matrix:
         for name, t in (("scales", scales), ("zeros", zeros)):
             if t is not None and (tuple(t.shape) != (n, groups) or t.dtype != scales.dtype):
                 raise ValueError(f"{name} must be {scales.dtype} ({n}, {groups}); got {t.dtype} {tuple(t.shape)}")
+        _check_grad("Q4Matrix", scales, zeros)
         dispatch.require_hip()
         device = codes.device if codes.device.type == "cuda" else dispatch._device()
         codes = codes.to(device).contiguous()
@@ -213,6 +215,7 @@ class KVCache:
                 raise RuntimeError(f"a cache's tensors are on one HIP device; {name} is on {t.device}")
             if not t.is_contiguous() or t.data_ptr() % 16:
                 raise ValueError(f"{name} must be contiguous and 16-byte aligned")
+        _check_grad("KVCache", k, v, k_scale, v_scale)
         for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
             mantissa, exponent = torch.frexp(t)
             if not ((mantissa == 0.5) & (exponent > -64) & (exponent <= 121)).all():
