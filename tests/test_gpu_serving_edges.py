@@ -160,3 +160,18 @@ def test_weights_and_caches_that_ask_for_a_gradient(hip):
         tt.KVCache(c.k, c.v, c.k_scale, ask, 64)
     with torch.no_grad():
         tt.KVCache(c.k, c.v, c.k_scale, ask, 64)
+
+
+@pytest.mark.parametrize("k", [1, 7, 127, 129, 1001])
+def test_laid_out_codes_past_the_columns_are_zeros(hip, k):
+    """An odd number of columns leaves half a byte, which may hold anything."""
+    n = 35
+    codes = torch.randint(0, 256, (n, (k + 1) // 2), generator=torch.Generator().manual_seed(k), dtype=torch.uint8)
+    cleared = codes.clone()
+    codes[:, -1] |= 0xF0
+    cleared[:, -1] &= 0x0F
+    scales = torch.ones((n, -(-k // 32)))
+    a, b = (tt.Q4Matrix(c, scales, k, 32) for c in (codes, cleared))
+    assert torch.equal(a.packed, b.packed)
+    x = torch.randn((3, k), generator=torch.Generator().manual_seed(1)).cuda()
+    assert torch.equal(tt.q4_matmul(x, a), tt.q4_matmul(x, b))

@@ -379,6 +379,9 @@ __global__ __launch_bounds__(256) void q4_pack_kernel(int N, int K, int chunks, 
         } else if (n < N) {
             for (int j = 0; at + j < bytes; ++j) x |= (uint32_t)codes[n * pitch + at + j] << 8 * j;
         }
+        // An odd K leaves half a byte, whatever it holds.
+        const int half = bytes - 1 - at;
+        if ((K & 1) && half >= 0 && half < 4) x &= ~(0xf0u << 8 * half);
         uint32_t even = x & 0x0f0f0f0fu, odd = x >> 4 & 0x0f0f0f0fu;
         even = (even | even >> 4) & 0x00ff00ffu;
         odd = (odd | odd >> 4) & 0x00ff00ffu;
