@@ -175,3 +175,39 @@ def test_laid_out_codes_past_the_columns_are_zeros(hip, k):
     assert torch.equal(a.packed, b.packed)
     x = torch.randn((3, k), generator=torch.Generator().manual_seed(1)).cuda()
     assert torch.equal(tt.q4_matmul(x, a), tt.q4_matmul(x, b))
+
+
+def test_weights_and_caches_keep_their_attributes(hip):
+    """Calls go by the memory found at construction: what would change it and be ignored is refused."""
+    c = tt.KVCache.empty(2, 1, 64, 16)
+    w = tt.Q4Matrix(torch.zeros((8, 32), dtype=torch.uint8), torch.ones((8, 1)), 64, 64)
+    for thing in (c, w):
+        for name in [n for n in type(thing).__slots__ if not n.startswith("_")]:
+            with pytest.raises(AttributeError, match=f"{name} is fixed"):
+                setattr(thing, name, getattr(thing, name))
+    c.k.view(torch.uint8).fill_(1)  # what they hold may change
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+@pytest.mark.parametrize("name", ["k", "v", "k_scale", "v_scale", "packed", "scales", "zeros"])
+def test_calls_refuse_tensors_that_were_given_other_memory(hip, name, compiled):
+    c = tt.KVCache.empty(2, 1, 64, 16)
+    ones = torch.ones((8, 1))
+    w = tt.Q4Matrix(torch.zeros((8, 32), dtype=torch.uint8), ones, 64, 64, zeros=ones)
+    if not compiled:
+        c._host = w._host = None
+    x, table, held = torch.zeros((1, 1, 1, 64)).cuda(), _i32([[0, 1]]).cuda(), _i32([3]).cuda()
+    calls = [lambda: tt.kv_append(c, x, x, table, held), lambda: tt.kv_attention(x, c, table, held)]
+    if not hasattr(c, name):
+        calls = [lambda: tt.q4_matmul(x, w)]
+    for call in calls:
+        call()
+    t = getattr(c if hasattr(c, name) else w, name)
+    was = t.data
+    t.data = t.data.clone()
+    for call in calls:
+        with pytest.raises(RuntimeError, match="other memory"):
+            call()
+    t.data = was
+    for call in calls:
+        call()

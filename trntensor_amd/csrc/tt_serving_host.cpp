@@ -107,7 +107,7 @@ class Q4Host {
         const int64_t nd = x.dim();
         tt_q4_args a = args_;
         a.dtype = code_of(x.scalar_type());
-        if (nd < 1 || a.dtype < 0 || !at_.holds(x) || !at_.here() || x.size(nd - 1) != a.K) return py::none();
+        if (nd < 1 || a.dtype < 0 || !unmoved() || !at_.holds(x) || !at_.here() || x.size(nd - 1) != a.K) return py::none();
         if (nd == 2 && x.stride(1) == 1 && x.stride(0) >= a.K) {
             a.M = x.size(0);
             a.ldx = x.stride(0);
@@ -127,6 +127,12 @@ class Q4Host {
     }
 
    private:
+    // The tensors are where they were: else Python reports it.
+    bool unmoved() const {
+        return packed_.data_ptr() == args_.codes && scales_.data_ptr() == args_.scales &&
+               (!zeros_ || zeros_->data_ptr() == args_.zeros);
+    }
+
     Library lib_;
     Tensor packed_, scales_;
     OptTensor zeros_;
@@ -156,7 +162,7 @@ class CacheHost {
         tt_kv_append_args a;
         std::memset(&a, 0, sizeof a);
         a.dtype = code_of(k.scalar_type());
-        if (a.dtype < 0 || k.dim() != 4 || !at_.here()) return declined;
+        if (a.dtype < 0 || k.dim() != 4 || !unmoved() || !at_.here()) return declined;
         a.batch = k.size(0);
         a.tokens = k.size(1);
         if (a.batch < 1 || a.tokens < 1 || !rows(k, a.batch, a.tokens, cache_.heads) || !rows(v, a.batch, a.tokens, cache_.heads) ||
@@ -200,7 +206,7 @@ class CacheHost {
         tt_kv_attention_args a;
         std::memset(&a, 0, sizeof a);
         a.dtype = code_of(q.scalar_type());
-        if (a.dtype < 0 || q.dim() != 4 || !at_.here() || window < 0 || sinks < 0) return py::none();
+        if (a.dtype < 0 || q.dim() != 4 || !unmoved() || !at_.here() || window < 0 || sinks < 0) return py::none();
         a.batch = q.size(0);
         a.tokens = q.size(1);
         a.q_heads = q.size(2);
@@ -231,6 +237,10 @@ class CacheHost {
     }
 
    private:
+    bool unmoved() const {
+        return keep_[0].data_ptr() == cache_.k && keep_[1].data_ptr() == cache_.v && keep_[2].data_ptr() == cache_.k_scale &&
+               keep_[3].data_ptr() == cache_.v_scale;
+    }
     bool rows(const Tensor& t, int64_t batch, int64_t tokens, int64_t heads) const {
         return t.dim() == 4 && t.size(0) == batch && t.size(1) == tokens && t.size(2) == heads && t.size(3) == cache_.dim &&
                (t.stride(3) == 1 || cache_.dim == 1) && at_.holds(t);

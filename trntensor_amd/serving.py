@@ -74,10 +74,26 @@ def _launch(name: str, device: torch.device, *args) -> None:
         _lib.check(st, name)
 
 
+class _Fixed:
+    """Attributes are set once: calls go by the memory and sizes found at construction."""
+
+    __slots__ = ()
+
+    def __setattr__(self, name, value):
+        if not name.startswith("_") and hasattr(self, name):
+            raise AttributeError(f"{type(self).__name__}.{name} is fixed at construction: make another {type(self).__name__}")
+        object.__setattr__(self, name, value)
+
+    def _check_memory(self):
+        """Tensors given other memory since (``t.data = ...``, a resized storage) are not what calls would work on."""
+        if self._memory != tuple(0 if t is None else t.data_ptr() for t in self._tensors()):
+            raise RuntimeError(f"the tensors of a {type(self).__name__} were given other memory: make another one of them")
+
+
 # ---------------------------------------------------------------------------
 # 4-bit weights
 # ---------------------------------------------------------------------------
-class Q4Matrix:
+class Q4Matrix(_Fixed):
     """A weight matrix (out_features, in_features) held in 4 bits:
     ``W[n, k] = scales[n, k // group_size] * (code[n, k] - zeros[n, k // group_size])``.
 
@@ -93,7 +109,7 @@ class Q4Matrix:
     that ask for a gradient are refused.
     """
 
-    __slots__ = ("packed", "scales", "zeros", "shape", "group_size", "device", "_code", "_host")
+    __slots__ = ("packed", "scales", "zeros", "shape", "group_size", "device", "_code", "_host", "_memory")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, in_features: int, group_size: int,
                  zeros: torch.Tensor | None = None):
@@ -120,9 +136,13 @@ class Q4Matrix:
         self.shape = (n, k)
         self.group_size = int(group_size)
         self.device = device
+        self._memory = tuple(0 if t is None else t.data_ptr() for t in self._tensors())
         host = _fastpath.module()
         self._host = None if host is None else host.Q4Host(_fastpath.serving_entries(), self.packed, self.scales, self.zeros,
                                                            n, k, self.group_size, self._code)
+
+    def _tensors(self):
+        return self.packed, self.scales, self.zeros
 
     @staticmethod
     def _by_group(t: torch.Tensor) -> torch.Tensor:
@@ -169,6 +189,7 @@ def q4_matmul(x: torch.Tensor, w: Q4Matrix) -> torch.Tensor:
         x2 = x2.contiguous()
     y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=w.device)
     zeros = w.zeros
+    w._check_memory()
     _launch("tt_q4_matmul", w.device, _Q4_ARGS.pack(
         code, w._code, m, n, k, w.group_size, max(x2.stride(0), k), n, x2.data_ptr(), w.packed.data_ptr(),
         w.scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(), y.data_ptr()))
@@ -178,7 +199,7 @@ def q4_matmul(x: torch.Tensor, w: Q4Matrix) -> torch.Tensor:
 # ---------------------------------------------------------------------------
 # the paged cache
 # ---------------------------------------------------------------------------
-class KVCache:
+class KVCache(_Fixed):
     """Pages of keys and values in 8-bit floats (e4m3), with one power-of-two
     scale for each page and head: a value is its code times its page's scale.
 
@@ -187,12 +208,13 @@ class KVCache:
     to a multiple of 64 (keys' codes past head_dim are zeros); ``k_scale`` and
     ``v_scale`` are float32 (pages, heads), 2^-64 to 2^120. page_size is a multiple of 16,
     head_dim at most 256. The constructor takes tensors a program holds;
-    :meth:`empty` makes a cache. Which pages are whose is the program's
-    business: calls take a page table.
+    :meth:`empty` makes a cache. Its attributes are fixed, what the tensors
+    hold is not. Which pages are whose is the program's business: calls take a
+    page table.
     """
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "head_dim", "page_size", "num_pages", "num_heads", "device", "_packed",
-                 "_scale", "_host")
+                 "_scale", "_host", "_memory")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, head_dim: int):
         if k.dim() != 4:
@@ -224,11 +246,14 @@ class KVCache:
         self.head_dim, self.page_size, self.num_pages, self.num_heads = int(head_dim), page, pages, heads
         self.device = k.device
         self._scale = 1.0 / math.sqrt(self.head_dim)
-        self._packed = _CACHE.pack(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, heads, page,
-                                   self.head_dim)
+        self._memory = tuple(t.data_ptr() for t in self._tensors())
+        self._packed = _CACHE.pack(*self._memory, pages, heads, page, self.head_dim)
         host = _fastpath.module()
         self._host = None if host is None else host.CacheHost(_fastpath.serving_entries(), k, v, k_scale, v_scale,
                                                               self.head_dim)
+
+    def _tensors(self):
+        return self.k, self.v, self.k_scale, self.v_scale
 
     @classmethod
     def empty(cls, num_pages: int, num_heads: int, head_dim: int, page_size: int = 64,
@@ -363,6 +388,7 @@ def kv_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table: torc
         out = torch.empty((batch, tokens, heads, cache.head_dim), dtype=q.dtype, device=cache.device)
     sk, sv, sq = k.stride(), v.stride(), k.stride() if q is None else q.stride()
     if batch and tokens:
+        cache._check_memory()
         _launch("tt_kv_append", cache.device, _APPEND_ARGS.pack(
             code, batch, tokens, heads, rot, bool(interleaved), table.shape[1], table.stride(0), sk[0], sk[1], sk[2],
             sv[0], sv[1], sv[2], sq[0], sq[1], sq[2], k.data_ptr(), v.data_ptr(), q.data_ptr() if heads else 0,
@@ -414,6 +440,7 @@ def kv_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, leng
     table, lengths, counts = _schedule(cache, batch, page_table, lengths, counts)
     out = torch.empty((batch, tokens, heads, dim), dtype=q.dtype, device=cache.device)
     if batch and tokens:
+        cache._check_memory()
         sq = q.stride()
         head = (code, batch, tokens, heads, window or 0, sinks, table.shape[1], table.stride(0), sq[0], sq[1], sq[2],
                 cache._scale if scale is None else float(scale), q.data_ptr(), out.data_ptr(), table.data_ptr(),
