@@ -347,7 +347,7 @@ int tt_kv_append(const tt_kv_append_args* args, void* stream);
  * j <= position and, where window > 0, j > position - window or j < sinks.
  * q is [batch][tokens][q_heads][dim] with strides, out the same, contiguous;
  * q_heads is a multiple of the cache's heads and query head h reads cache head
- * h / (q_heads / heads). Queries that see nothing, and rows past counts[b],
+ * h / (q_heads / heads). scale is finite (below 1e38). Queries that see nothing, and rows past counts[b],
  * give zeros. What masked slots of a page hold has no influence, NaN included.
  */
 typedef struct {

@@ -211,3 +211,10 @@ def test_calls_refuse_tensors_that_were_given_other_memory(hip, name, compiled):
     t.data = was
     for call in calls:
         call()
+
+
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf])
+def test_kv_attention_refuses_a_scale_that_is_no_number(hip, scale):
+    dev, _ = _cache(2, 1, 16, 64, 12)
+    with pytest.raises(ValueError, match="scale"):
+        tt.kv_attention(torch.ones((1, 1, 1, 64)).cuda(), dev, _i32([[0, 1]]).cuda(), _i32([20]).cuda(), scale=scale)

@@ -108,3 +108,9 @@ def test_weights_refuse_scales_that_ask_for_a_derivative(name):
     with forward_ad.dual_level(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
         kw[name] = _dual(plain)
         tt.Q4Matrix(codes, kw["scales"], 64, 64, zeros=kw["zeros"])
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e39])
+def test_attention_refuses_a_scale_that_is_no_number(lib, scale):
+    assert _attention(lib, scale=scale) == _lib.TT_INVALID
+    assert lib.tt_last_error().startswith(b"tt_kv_attention: scale")

@@ -4,6 +4,7 @@
 //
 // in one pass over the keys with the running maximum and sum of a softmax;
 // neither scores nor widened keys and values ever leave registers.
+#include <cmath>
 #include <type_traits>
 
 #include "tt_serving.hpp"
@@ -1211,6 +1212,7 @@ int check_attention(const tt_kv_attention_args* a) {
     if (int rc = check_cache("tt_kv_attention", a->cache)) return rc;
     if (a->batch < 0 || a->tokens < 0 || a->table_width < 0 || a->window < 0 || a->sinks < 0)
         return set_error(TT_INVALID, "tt_kv_attention: negative extent");
+    if (!(std::fabs(a->scale) < 1e38)) return set_error(TT_INVALID, "tt_kv_attention: scale %g", a->scale);
     if (a->q_heads < 1 || a->q_heads % a->cache.heads)
         return set_error(TT_INVALID, "tt_kv_attention: %lld query heads on %lld cache heads", (long long)a->q_heads,
                          (long long)a->cache.heads);

@@ -408,7 +408,7 @@ def kv_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, leng
     first ``counts[b]`` rows of q (all, without counts) are its last tokens.
     The token at position p sees every token up to p or, with ``window``, the
     last ``window`` of those and the first ``sinks`` of the sequence.
-    ``scale`` multiplies the products (1 / sqrt(head_dim) by default).
+    ``scale`` multiplies the products (1 / sqrt(head_dim) by default; finite).
 
     Returns q's shape and dtype; queries that see nothing (empty sequences,
     rows past their count) give zeros. No masked slot has any influence,
