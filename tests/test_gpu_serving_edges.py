@@ -12,28 +12,13 @@ from torch.autograd import forward_ad
 
 import trntensor_amd as tt
 from oracle import serving as ref
+from tests import test_gpu_serving as base
+from tests.test_gpu_serving import F8, _cache, _i32
 
 pytestmark = pytest.mark.gpu
 
 U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 DTYPES = list(U)
-F8 = torch.float8_e4m3fn
-
-
-def _i32(values):
-    return torch.tensor(values, dtype=torch.int32)
-
-
-def _cache(pages, heads, page, dim, seed):
-    """A cache of random codes and scales on the device, and the same as float64 values for the oracle."""
-    g = torch.Generator().manual_seed(seed)
-    w = -(-dim // 64) * 64
-    k, v = ((torch.randn(s, generator=g) * 90).clamp(-448, 448).to(F8)
-            for s in ((pages, heads, page, w), (pages, heads, w, page)))
-    k.view(torch.uint8)[..., dim:] = 0
-    ks, vs = (torch.exp2(torch.randint(-9, -5, (pages, heads), generator=g).float()) for _ in range(2))
-    return (tt.KVCache(k.cuda(), v.cuda(), ks.cuda(), vs.cuda(), head_dim=dim),
-            {"k": k.double(), "v": v.double(), "k_scale": ks.double(), "v_scale": vs.double()})
 
 
 @pytest.mark.parametrize("tokens", [1, 18])
@@ -68,6 +53,29 @@ def test_kv_attention_float32_weights_do_not_depend_on_value_scales(hip, low, to
     out, spread = ref.attention(q, want, table, [held] * batch, None, dim ** -0.5, 1, 1)
     err = (got.cpu().double() - out).abs() / spread[..., 1:2]
     assert err.max() <= 2.0 ** -21, f"2^{math.log2(err.max()):.1f} of the values"
+
+
+@pytest.mark.parametrize("heads,share,dim,page,tokens,lengths", [(2, 4, 128, 64, 1, [5, 40, 64, 130]), (1, 3, 64, 16, 5, [70, 5]),
+                                                                 (2, 1, 192, 32, 40, [90, 300]), (1, 2, 256, 16, 1, [1500])])
+def test_kv_attention_float32_keeps_its_bits(hip, heads, share, dim, page, tokens, lengths):
+    """Queries and weights enter the matrix units as three parts, 24 bits together.
+
+    Tolerance: u |o|; 2^-22 sum p |v| for the exponentials (a unit in the last
+    place), the split and its products; 2 ds max |v| with ds = 2^-24 (16 +
+    sqrt D) sum |q k| scale, small here since the queries are; and 2^-24 (16 +
+    sqrt L) max |v| for the sums over L keys. Two parts would err by 2^-16 p |v|.
+    """
+    batch, width = len(lengths), -(-max(lengths) // page)
+    dev, want = _cache(batch * width, heads, page, dim, 18)
+    table = torch.arange(batch * width, dtype=torch.int32).reshape(batch, width).flip(1).contiguous()
+    q = 0.05 * torch.randn((batch, tokens, heads * share, dim), generator=torch.Generator().manual_seed(19))
+    got = tt.kv_attention(q.cuda(), dev, table.cuda(), _i32(lengths).cuda()).cpu().double()
+    out, spread = ref.attention(q, want, table, lengths, None, dim ** -0.5, None, 0)
+    ds = 2.0 ** -24 * (16 + math.sqrt(dim)) * spread[..., 0:1]
+    tol = (2.0 ** -24 * out.abs() + 2.0 ** -22 * spread[..., 2:3]
+           + (2 * ds + 2.0 ** -24 * (16 + math.sqrt(max(lengths)))) * spread[..., 1:2])
+    err = (got - out).abs()
+    assert (err <= tol).all(), f"{(err / tol.clamp(min=1e-300)).max():.3g} times the tolerance"
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -218,3 +226,143 @@ def test_kv_attention_refuses_a_scale_that_is_no_number(hip, scale):
     dev, _ = _cache(2, 1, 16, 64, 12)
     with pytest.raises(ValueError, match="scale"):
         tt.kv_attention(torch.ones((1, 1, 1, 64)).cuda(), dev, _i32([[0, 1]]).cuda(), _i32([20]).cuda(), scale=scale)
+
+
+# ---------------------------------------------------------------------------
+# sizes and cuts of calls that each take a kernel or a path of their own
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(
+    "heads,share,dim,rot,page,tokens,lengths,counts,interleaved",
+    [
+        # rows of 192 codes, which a wavefront's lanes do not divide evenly
+        (2, 2, 192, 192, 64, 70, [0, 60], [70, 33], False),
+        (1, 9, 160, 64, 32, 40, [5, 31], None, True),
+        (2, 1, 136, 128, 16, 33, [0, 15, 16], None, False),
+        (1, 16, 192, 96, 16, 1, [0, 17, 31], [1, 0, 1], True),
+        (2, 3, 136, 136, 48, 50, [3, 47], None, False),
+        (1, 2, 130, 130, 32, 9, [30], None, True),
+        (3, 1, 176, 16, 128, 300, [100], None, False),
+    ],
+)
+def test_kv_append_of_heads_between_128_and_192(hip, heads, share, dim, rot, page, tokens, lengths, counts, interleaved, dtype):
+    base.test_kv_append(hip, heads, share, dim, rot, page, tokens, lengths, counts, interleaved, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(
+    "heads,share,dim,page,tokens,lengths,counts,window,sinks",
+    [
+        (2, 4, 136, 64, 1, [0, 1, 63, 64, 65, 200], None, None, 0),
+        (1, 2, 160, 16, 3, [3, 64, 130], [3, 0, 2], None, 0),
+        (1, 5, 192, 32, 1, [600], None, 50, 70),
+        (2, 2, 192, 64, 30, [70, 200, 0], [30, 9, 0], None, 0),
+        (1, 3, 136, 48, 70, [150], None, 33, 7),
+        (1, 1, 160, 128, 130, [140, 300], None, None, 0),
+    ],
+)
+def test_kv_attention_of_heads_between_128_and_192(hip, heads, share, dim, page, tokens, lengths, counts, window, sinks, dtype):
+    base._attention_case(heads, share, dim, page, tokens, lengths, counts, window, sinks, dtype)
+
+
+@pytest.mark.parametrize("dtype,tokens", [(torch.bfloat16, 500), (torch.float16, 260), (torch.float32, 130)])
+def test_kv_attention_of_many_rows_and_heads_between_128_and_192(hip, dtype, tokens):
+    for dim in (136, 192):
+        base.test_kv_attention_many_rows(hip, dtype, 2, 3, dim, 32, tokens, [2500, 700], [tokens, 20], None, 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(
+    "heads,share,dim,page,tokens,lengths,counts,window,sinks",
+    [
+        # pairs of sequence and head cut anywhere, over several heads and sequences
+        (3, 2, 128, 64, 1, [5000, 3, 0, 2049], None, None, 0),
+        (8, 2, 192, 32, 1, [3000, 1100], None, None, 0),
+        (2, 4, 256, 16, 3, [2000, 0, 1500], [3, 1, 2], None, 0),
+        (5, 1, 80, 16, 1, [1, 1300, 1, 1200], None, None, 0),
+        # queries before their sequence's start, and rows past their counts
+        (2, 3, 64, 64, 5, [4000, 3, 2100], [5, 5, 0], None, 0),
+        # windows of more tiles than a workgroup takes, and sinks before them
+        (2, 2, 96, 64, 2, [6000, 4000, 9], None, 2000, 70),
+        (4, 1, 128, 128, 1, [9000, 1500], None, 1100, 1),
+        # more sequences than a wavefront looks at together, most of them short or empty
+        (1, 2, 64, 16, 1, [2100, *[n % 5 * 7 for n in range(75)], 700, 0, 1900], None, None, 0),
+    ],
+)
+def test_kv_attention_of_long_tables(hip, heads, share, dim, page, tokens, lengths, counts, window, sinks, dtype):
+    base._attention_case(heads, share, dim, page, tokens, lengths, counts, window, sinks, dtype)
+
+
+def _wide(dtype, heads, share, dim, page, tokens, lengths, width, missing=(), counts=None, seed=51):
+    """Attention through a table of `width` entries, -1 past each sequence's end and at `missing` (sequence, entry)."""
+    dev, want = _cache(sum(-(-n // page) for n in lengths) + 1, heads, page, dim, seed)
+    table = torch.full((len(lengths), width), -1, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(lengths):
+        used = -(-n // page)
+        table[b, :used] = torch.arange(at, at + used, dtype=torch.int32).flip(0)
+        at += used
+    for b, entry in missing:
+        table[b, entry] = -1
+    q = torch.randn((len(lengths), tokens, heads * share, dim), generator=torch.Generator().manual_seed(seed + 1)).to(dtype)
+    n = None if counts is None else _i32(counts)
+    got = tt.kv_attention(q.cuda(), dev, table.cuda(), _i32(lengths).cuda(), counts=None if n is None else n.cuda())
+    base._check_attention(got, q, want, table, lengths, n, 1 / math.sqrt(dim), None, 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens", [1, 20, 70, 300])
+def test_kv_attention_through_tables_wider_than_the_sequences(hip, tokens, dtype):
+    """How a call is cut follows from the table's width, what is there from the lengths."""
+    for lengths in ([300], [70, 0, 310]):
+        _wide(dtype, 1, 2, 64, 16, tokens, lengths, 2000)
+    _wide(dtype, 2, 1, 128, 64, tokens, [330, 90], 700, counts=[tokens, 1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens", [1, 3, 40])
+def test_kv_attention_of_long_sequences_that_miss_pages(hip, tokens, dtype):
+    _wide(dtype, 2, 2, 64, 16, tokens, [3000, 1500], 400, missing=[(0, e) for e in (*range(40, 60), 0, 100, 187)]
+          + [(1, e) for e in range(5, 90)])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k,group", [(300, 700, 520, 128), (513, 200, 390, 64), (257, 330, 640, 32), (400, 130, 1000, 256)])
+def test_q4_matmul_of_hundreds_of_rows(hip, m, n, k, group, dtype):
+    base.test_q4_matmul(hip, m, n, k, group, True, dtype)
+
+
+# ---------------------------------------------------------------------------
+# values at the ends of their types
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_kv_attention_of_infinite_queries(hip, tokens, dtype, value):
+    """A score is then infinite or NaN, and the formula gives NaN: for that
+    query head alone."""
+    dev, _ = _cache(4, 2, 64, 64, 13)
+    table, held = _i32([[2, 0, 3, 1]]).cuda(), _i32([250]).cuda()
+    q = torch.randn((1, tokens, 6, 64), generator=torch.Generator().manual_seed(14)).to(dtype)
+    clean = tt.kv_attention(q.cuda(), dev, table, held)
+    q[0, tokens // 2, 4, 17] = value
+    got = tt.kv_attention(q.cuda(), dev, table, held)
+    bad = torch.zeros(got.shape[:3], dtype=torch.bool, device="cuda")
+    bad[0, tokens // 2, 4] = True
+    assert got[bad].isnan().all() and torch.equal(got[~bad], clean[~bad])
+
+
+def test_float16_operands_below_the_normal_range(hip):
+    """Subnormal activations and queries count as what they are."""
+    g = torch.Generator().manual_seed(15)
+    codes, scales, z = base._q4(70, 256, 64, torch.float32, True, 16)
+    x = (torch.randint(-900, 900, (20, 256), generator=g).double() * 2.0 ** -24).to(torch.float16)
+    assert x.abs().max() < 2.0 ** -14
+    w = tt.Q4Matrix(codes, scales * 2.0 ** 14, 256, 64, zeros=z)
+    base._check_q4(x, codes, scales * 2.0 ** 14, z, 256, 64, tt.q4_matmul(x.cuda(), w))
+    for tokens in (1, 40):
+        dev, want = _cache(4, 1, 64, 64, 17)
+        q = (torch.randint(-900, 900, (1, tokens, 2, 64), generator=g).double() * 2.0 ** -24).to(torch.float16)
+        table = _i32([[2, 0, 3, 1]])
+        got = tt.kv_attention(q.cuda(), dev, table.cuda(), _i32([250]).cuda(), scale=2.0 ** 12)
+        base._check_attention(got, q, want, table, [250], None, 2.0 ** 12, None, 0)
