@@ -3,7 +3,8 @@
 //   o_r = sum_j softmax_j(scale * q_r . k_j) v_j over the keys j that row r sees
 //
 // in one pass over the keys with the running maximum and sum of a softmax;
-// neither scores nor widened keys and values ever leave registers.
+// scores never leave registers, and widened keys and values only, where many
+// query rows share them, for LDS.
 #include <cmath>
 #include <type_traits>
 
@@ -672,6 +673,10 @@ __device__ __forceinline__ int64_t share_of(const AttnParams& p, int64_t total) 
     return per < kMinTiles + kPairCost ? kMinTiles + kPairCost : per;
 }
 
+// Wavefronts a SIMD is to hold: two where the state of one fits half its registers.
+template <typename T, int W, int MT>
+constexpr int kWavesPerSimd = Parts<T>::q * MT * W > 256 || W > 128 ? 1 : 2;
+
 // Few query rows (at most 16 a cache head): the four wavefronts of a workgroup
 // take every fourth tile of the same keys. The key tiles of all (sequence,
 // head) pairs form one list, in which each pair also takes the room of what
@@ -680,12 +685,10 @@ __device__ __forceinline__ int64_t share_of(const AttnParams& p, int64_t total) 
 // short tables, each takes a pair whole (cut_of). Bound by the codes' bytes: two
 // sequences of 131071 tokens (8 heads of 128, 534 MB) take 106 us, 5.0 TB/s where
 // a large copy has 5.2; 48 of 1 to 4096, a workgroup a pair, 50 us, 4.0 TB/s, the
-// longest pairs being left at the end; one of 200 tokens 7 us, the launch and a
-// chain of waits (length, page, keys, values).
-// Wavefronts a SIMD is to hold: two where the state of one fits half its registers.
-template <typename T, int W, int MT>
-constexpr int kWavesPerSimd = Parts<T>::q * MT * W > 256 || W > 128 ? 1 : 2;
-
+// longest pairs being left at the end (all of 4096: 5.2 TB/s at head size 256);
+// one of 200 tokens 7 us, the launch and a chain of waits (length, page, keys,
+// values). 256 pairs of 18 tiles (windows) leave one wavefront a SIMD, which
+// waits on memory 57% of its time.
 template <typename T, int W>
 __global__ __launch_bounds__(256, (kWavesPerSimd<T, W, 1>)) void kv_attention_few_kernel(AttnParams p) {
     const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -817,7 +820,8 @@ __device__ __forceinline__ void join_row(const float* first, const float* rest, 
 }
 
 // Joins the partial results of the pairs that were cut: one wavefront a query
-// row. 4 to 5 us: a launch, and two waits on memory (lengths, partial results).
+// row. A launch and two waits on memory (lengths, partial results): 5 us where
+// nothing is cut, 8 for 32 partial results of each of 16 pairs.
 template <typename T, int W>
 __global__ __launch_bounds__(256) void kv_attention_few_join_kernel(AttnParams p) {
     constexpr int64_t kSlot = 16 * (W + 2);
@@ -841,9 +845,12 @@ __global__ __launch_bounds__(256) void kv_attention_few_join_kernel(AttnParams p
 // a tile, loads it and reads it is shared by 16 MT NW rows. With `groups` > 1
 // the keys of a row block are cut into that many ranges, joined afterwards. 2048
 // tokens on 8192 (32 heads of 128, 240 GFLOP): 268 us, 0.90 PFLOP/s of the 1.22
-// that a large product reaches. Bound by issue: a tile's exponentials, widening
-// and addresses take the vector units about as long as its products take the
-// matrix units, and with two wavefronts a SIMD the two overlap in part only.
+// that a large product reaches. Bound by issue: the products take the matrix
+// units 44% of a wavefront's time, exponentials, widening and addresses the
+// vector units 41%, and with two wavefronts a SIMD the two overlap in part only.
+// float16 takes 354 us and float32 571, head sizes of 64, 192 and 256 193, 417
+// and 500 (bfloat16): rows of more than 128 codes and float32 have no room for
+// two blocks of rows a wavefront.
 template <typename T, int W, int MT, int NW>
 __global__ __launch_bounds__(64 * NW, (NW == 8 ? 2 : 1)) void kv_attention_many_kernel(AttnParams p) {
     typedef Wave<T, W, MT> WV;
@@ -1089,6 +1096,13 @@ constexpr Shape kShapes[] = {{1, 4, 1.27, 1.85}, {1, 8, 1.47, 1.47}, {2, 8, 2.15
 // and 0.45 a thousand rows. It pays where blocks leave compute units idle (one
 // block a head, 8192 keys: 278 us whole, 34 in 32 ranges), not where keys are
 // few for their rows (eight times 128 tokens on 1024: 32 us whole, 56 halved).
+// `width` and `kind` say what 2048 tokens on 8192 take at head sizes 64 to 256
+// within 10% for bfloat16 (256: 14%) and 16% for float16, against the same shape
+// at 128 in bfloat16; float32 of more than 128 codes a row, which has one shape,
+// takes a third longer. Keys
+// are those that the table covers: sequences that are shorter have ranges of
+// few tiles (512 tokens on 512 through a table of 4096 keys or more 33 us, of
+// 512 17; 128 on 1024 29 for 19).
 double many_cost(const tt_kv_attention_args* a, const Shape& s, int64_t W, int64_t tiles, int64_t blocks, int64_t g,
                  int64_t slots) {
     const double width = (W + 64) / 192.0, kind = a->dtype == TT_F32 ? 1.6 : a->dtype == TT_F16 ? 1.3 : 1.0;
@@ -1133,7 +1147,9 @@ Cut cut_of(const tt_kv_attention_args* a) {
         // past what is resident at once, 1024 pairs of 4096 241 / 198, but 2048
         // of 1500 134 / 170. The table's width is all the host knows of the
         // lengths: beyond 64 tiles one long sequence among short ones would
-        // hold up its few workgroups.
+        // hold up its few workgroups. (That bound is this worry's; what was
+        // measured does not cross there.) Short sequences in a table past the
+        // bound pay for the join: 200 keys 12 us, in a table of 1024 keys 7.
         const int most = pairs < 64 ? 16 : pairs < 256 || pairs > 512 ? 32 : 64;
         c.direct = tiles <= most;
         c.groups = 512;  // two a compute unit; 256 and 1024 were 8% slower at some length each, level at others

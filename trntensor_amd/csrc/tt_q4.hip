@@ -104,11 +104,17 @@ struct Chunk {
 // wavefronts of a workgroup take contiguous shares of the columns, which are
 // summed at the end in their order: a row's codes are read once, as 1 KiB a
 // load, by as many wavefronts as there are CUs to hold them. A few rows are
-// bound by the codes' bytes (1 row on 4096 x 14336: 12.3 us, 2.5 TB/s; on
-// 4096 x 4096, 4.6 us, by the launch and three waits on memory one after the
-// other), more by the activations, which every workgroup reads from L2 (32 rows
-// on 16384 x 8192: 27 us, 134 MB of them beside 73 MB of weights). GPC: the pieces of a chunk of 128 columns
-// that are scaled one by one, 1 for groups of at least a chunk, else 4.
+// bound by the codes' bytes (1 row on 16384 x 8192: 16.9 us where they take 14;
+// on 4096 x 4096, 4.6 us, by the launch and three waits on memory one after the
+// other; between them by whole rounds of workgroups on the CUs: 12288, 14336 and
+// 16384 x 4096 take 12.1, 12.4 and 12.8 us), more by the vector units: 32 rows on 16384 x 8192 take 27 us, in which
+// a wavefront issues 506 vector instructions a chunk (codes widened, scales and
+// zero points made floats of either type and applied) beside 40 products. They
+// keep a SIMD's vector unit busy 56% of the time, the matrix unit 18%; the 212 MB
+// that leave L2 are 8 TB/s. Groups of 32 and 64 scale four pieces a chunk (57
+// us), and every 32 rows widen all codes again: 2048 rows on 4096 x 4096 take 206
+// us, 0.33 PFLOP/s (groups of 64: 475 us). GPC: the pieces of a chunk of 128
+// columns that are scaled one by one, 1 for groups of at least a chunk, else 4.
 template <typename T, int SW, int R, int MT, int GPC>
 __global__ __launch_bounds__(64 * kWaves, 2) void q4_matmul_kernel(Q4Params p) {
     typedef typename Act<T>::half H;
@@ -327,10 +333,11 @@ int q4_shape(const Q4Params& p, hipStream_t st) {
     //     1 row     (K 4096, 4096, 8192)  5.2 / 6.5 / 9.8   7.4 / 8.1 / 10.8   20.3 / 16.9 / 20.4
     //     16 rows                         7.0 / 7.8 / 10.8  11.2 / 9.2 / 11.4  35.8 / 22.6 / 21.4
     //     32 rows                         10.4 / 11.2 / 13.9  18.0 / 12.4 / 14.8  63.1 / 37.6 / 27.0
-    //   float16, groups of 64
-    //     1 row                           7.9 / 12.4        11.9 / 13.4        35.0 / 40.4
-    //     16 rows                         9.1 / 12.9        15.0 / 13.6        47.5 / 41.5 (1792: 42.1 / 47.4)
-    //     32 rows                         12.0 / 16.1       21.9 / 17.0        78.1 / 52.6
+    //   16-bit, groups of 64 and 32, zero points                                       1792 (K 4096)
+    //     1 row                           8.8 / 13.8        13.2 / 14.8        40.0 / 43.1        36.3 / 49.0
+    //     16 rows                         9.3 / 14.3        15.4 / 15.0        49.5 / 44.4        43.4 / 51.4
+    //     32 rows                         12.7 / 17.1       23.2 / 17.8        82.2 / 56.9        76.8 / 64.1
+    //     (up to 16 rows stay at R = 1: 2 gains 10% at 1024 and loses 18% at 1792, which no bound on work tells apart)
     //   float32 (three parts an activation: no room for two blocks of rows), groups of 32
     //     1 row                           9.9 / 13.2        18.5 / 15.9        59.2 / 48.1
     // Four or sixteen wavefronts a workgroup were slower or level.
