@@ -108,9 +108,9 @@ struct Chunk {
 // on 4096 x 4096, 4.6 us, by the launch and three waits on memory one after the
 // other; between them by whole rounds of workgroups on the CUs: 12288, 14336 and
 // 16384 x 4096 take 12.1, 12.4 and 12.8 us), more by the vector units: 32 rows on 16384 x 8192 take 27 us, in which
-// a wavefront issues 506 vector instructions a chunk (codes widened, scales and
+// a wavefront issues 448 vector instructions a chunk (codes widened, scales and
 // zero points made floats of either type and applied) beside 40 products. They
-// keep a SIMD's vector unit busy 56% of the time, the matrix unit 18%; the 212 MB
+// issue 56% of a SIMD's time, and keep the matrix unit busy 18%; the 212 MB
 // that leave L2 are 8 TB/s. Groups of 32 and 64 scale four pieces a chunk (57
 // us), and every 32 rows widen all codes again: 2048 rows on 4096 x 4096 take 206
 // us, 0.33 PFLOP/s (groups of 64: 475 us). GPC: the pieces of a chunk of 128
