@@ -275,7 +275,8 @@ def _exact_wide(codes: torch.Tensor, scales: torch.Tensor, rows: int) -> torch.T
 
 
 def _exact_rows8(y: torch.Tensor) -> dict:
-    """Codes' values and scales of 64-bit rows: steps of 2^(e-3) from e = -6 up, ties to even."""
+    """64-bit rows over their blocks' scales, and the scales. What codes stand
+    for is given unrounded, as every other output here."""
     codes, scales = torch.empty_like(y), []
     for j in range(0, y.shape[1], 128):
         part = y[:, j: j + 128]
@@ -283,8 +284,6 @@ def _exact_rows8(y: torch.Tensor) -> dict:
         e = torch.ceil(torch.log2(top / 448.0)).clamp(min=-127.0)
         e = torch.where(top > 448.0 * torch.exp2(e), e + 1.0, e)
         e = torch.where((e > -127.0) & (top <= 448.0 * torch.exp2(e - 1.0)), e - 1.0, e)
-        part = part / torch.exp2(e)[:, None]
-        step = torch.exp2((torch.frexp(part)[1] - 1).clamp(min=-6).double() - 3.0)
-        codes[:, j: j + 128] = torch.round(part / step) * step
+        codes[:, j: j + 128] = part / torch.exp2(e)[:, None]
         scales.append(torch.exp2(e))
     return {"codes": codes, "scales": torch.stack(scales, dim=1)}
