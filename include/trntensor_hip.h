@@ -41,7 +41,7 @@
 extern "C" {
 #endif
 
-#define TT_ABI_VERSION 5
+#define TT_ABI_VERSION 6
 #define TT_MAX_DIMS 8
 
 enum { TT_OK = 0, TT_INVALID = 1, TT_UNSUPPORTED = 2, TT_HIP_ERROR = 3 };
@@ -366,6 +366,95 @@ typedef struct {
 size_t tt_kv_attention_workspace_bytes(const tt_kv_attention_args* args);
 
 int tt_kv_attention(const tt_kv_attention_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The 8-bit chain: activations and weights in 8-bit floats (OCP e4m3, no
+ * infinities) with a scale for each block of 128.
+ *
+ * Rows of `dim` elements in 8 bits are two arrays, contiguous in their rows:
+ * codes [rows][dim rounded up to a multiple of 128], zeros past dim, and
+ * scales [rows][S], a byte e + 127 for the power of two 2^e (e8m0) of each
+ * block of 128, S being the number of blocks rounded up to a multiple of 4 and
+ * the bytes past the blocks zeros. A value is its code times its block's
+ * scale. codes are 16-byte aligned, scales 4-byte.
+ *
+ * Where they are written, e is the smallest one, at least -127, that brings
+ * the block's largest finite magnitude to 448 or below; codes are rounded to
+ * nearest even, infinities become NaN and NaN stays NaN.
+ * --------------------------------------------------------------------- */
+
+/* Scale dtype of weights: the bytes above. */
+#define TT_E8M0 6
+
+/* Rows of `dtype`, of unit stride and x_stride elements apart, into 8 bits. */
+typedef struct {
+    int64_t dtype, rows, dim, x_stride;
+    const void *x;
+    void *codes, *scales;
+} tt_fp8_quantize_args;
+
+int tt_fp8_quantize(const tt_fp8_quantize_args* args, void* stream);
+
+/*
+ * h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight, row by row, in 32
+ * bits. residual and weight may be NULL. The result goes, rounded once, to y
+ * (contiguous, dtype) or, in 8 bits, to codes and scales: the other is NULL.
+ * sum (contiguous, dtype; NULL iff residual is) gets h rounded; y follows from
+ * h as it was before. No result overlaps an operand. eps is finite and not
+ * negative.
+ */
+typedef struct {
+    int64_t dtype, weight_dtype, rows, dim, x_stride, residual_stride;
+    double eps;
+    const void *x, *residual, *weight;
+    void *sum, *y, *codes, *scales;
+} tt_rms_norm_args;
+
+int tt_rms_norm(const tt_rms_norm_args* args, void* stream);
+
+/*
+ * Lays out weight codes for the products below. Row n of `codes` starts at n *
+ * pitch bytes. `packed` (16-byte aligned) takes tt_fp8_packed_bytes(N, K)
+ * bytes: tiles of 16 rows and 128 columns, 2048 bytes each, those of the same
+ * rows together; codes past N and K become zeros. Byte 1024 h + 16 l + j of a
+ * tile is row l % 16, column 64 h + 16 (l / 16) + j.
+ */
+size_t tt_fp8_packed_bytes(int64_t N, int64_t K);
+
+int tt_fp8_pack(int64_t N, int64_t K, const void* codes, int64_t pitch, void* packed, void* stream);
+
+/*
+ * y[m][n] = sum_k x[m][k] w[n][k]: rows in 8 bits times weights laid out by
+ * tt_fp8_pack. scale_dtype TT_F32: w_scales is [ceil(N / 128)][ceil(K / 128)]
+ * floats; TT_E8M0: bytes, [ceil(N / 128)][ceil(K / 128) rounded up to a
+ * multiple of 4], 4-byte aligned. Products are summed in 32 bits; y is [M][N]
+ * of dtype, contiguous.
+ */
+typedef struct {
+    int64_t dtype, scale_dtype, M, N, K;
+    const void *x, *x_scales, *w, *w_scales;
+    void *y;
+} tt_fp8_matmul_args;
+
+int tt_fp8_matmul(const tt_fp8_matmul_args* args, void* stream);
+
+/*
+ * a = x gate^T, b = x up^T, h = act(a) b, both weights (N, K) as above. act is
+ * a / (1 + exp(-a)) (activation 0) or 0.5 a (1 + tanh(sqrt(2 / pi) (a +
+ * 0.044715 a^3))) (activation 1). h goes, rounded once, to y ([M][N] of dtype)
+ * or, in 8 bits, to codes and scales (rows of N elements): the other is NULL.
+ * The workspace (4-byte aligned) is needed for codes only, and may be 0 bytes.
+ */
+typedef struct {
+    int64_t dtype, scale_dtype, activation, M, N, K;
+    const void *x, *x_scales, *gate, *gate_scales, *up, *up_scales;
+    void *y, *codes, *scales, *workspace;
+    int64_t workspace_bytes;
+} tt_fp8_gated_args;
+
+size_t tt_fp8_gated_workspace_bytes(const tt_fp8_gated_args* args);
+
+int tt_fp8_gated_matmul(const tt_fp8_gated_args* args, void* stream);
 
 /*
  * Measurement aid with no counterpart in the reference: `workgroups`

@@ -13,6 +13,7 @@ package.
 __version__ = "0.4.0+mi355x"
 
 from .einsum import einsum, multi_einsum
+from .fp8 import Fp8Matrix, Fp8Rows, fp8_gated_matmul, fp8_matmul, fp8_quantize, rms_norm
 from .hip import HAS_HIP, HAS_NKI, get_backend, set_backend
 from .hip.dispatch import from_device, from_xla, to_device, to_xla
 from .plan import (
@@ -49,4 +50,10 @@ __all__ = [
     "KVCache",
     "kv_append",
     "kv_attention",
+    "Fp8Rows",
+    "Fp8Matrix",
+    "rms_norm",
+    "fp8_quantize",
+    "fp8_matmul",
+    "fp8_gated_matmul",
 ]

@@ -26,6 +26,8 @@ LIB = os.path.join(OUT_DIR, "libtrntensor_hip.so")
 SOURCES = [
     "tt_abi.hip",
     "tt_dd.hip",
+    "tt_fp8.hip",
+    "tt_fp8_rows.hip",
     "tt_gemm.hip",
     "tt_gemm16.hip",
     "tt_gemm16_dma.hip",
