@@ -28,6 +28,7 @@ SOURCES = [
     "tt_dd.hip",
     "tt_fp8.hip",
     "tt_fp8_rows.hip",
+    "tt_fp8_tiles.hip",
     "tt_gemm.hip",
     "tt_gemm16.hip",
     "tt_gemm16_dma.hip",

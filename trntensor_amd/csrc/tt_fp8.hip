@@ -8,86 +8,11 @@
 // sum on its way into the accumulators.
 #include <type_traits>
 
-#include "tt_fp8.hpp"
+#include "tt_fp8_block.hpp"
 
 namespace tt {
 
 namespace {
-
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
-struct Fp8Params {
-    const uint8_t *x, *xs;       // rows and their scales
-    const uint8_t *w[2], *ws[2]; // weights (gate and up)
-    void* y;
-    uint8_t *codes, *scales;
-    int M, N, K, blocks, x_scales;  // blocks of 128 columns; scale bytes of a row
-    int activation;
-};
-
-constexpr uint32_t kOne = 127;  // e8m0 of 1.0
-
-// out += scales * A B^T for 16 rows of either and a block of 128 columns, A being
-// weights. The 8-bit matrix instructions take eight products at a time, align
-// them to the largest and drop what lies 2^-13 below its power of two (measured;
-// sums of eights are added in 24 bits). For results of 16 and 8 bits that is
-// nothing: 2^-16 of a sum of 128 terms of normal distribution. Exact ones
-// (float32 results) have the codes widened to bfloat16, whose products the
-// matrix units add in 32 bits at half the rate.
-template <bool EXACT, bool E8>
-struct Block {
-    u32x4 v[2];
-
-    __device__ __forceinline__ void load(const uint8_t* first, const uint8_t* second) {
-        v[0] = *reinterpret_cast<const u32x4*>(first);
-        v[1] = *reinterpret_cast<const u32x4*>(second);
-    }
-    __device__ __forceinline__ i32x8 operand() const {
-        return i32x8{(int)v[0][0], (int)v[0][1], (int)v[0][2], (int)v[0][3], (int)v[1][0], (int)v[1][1], (int)v[1][2], (int)v[1][3]};
-    }
-    // Eight codes as bfloat16.
-    __device__ __forceinline__ bf16x8 wide(int i) const {
-        u32x4 r;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint32_t c = v[i / 2][i % 2 * 2 + j];
-            r[2 * j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, false));
-            r[2 * j + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, true));
-        }
-        return __builtin_bit_cast(bf16x8, r);
-    }
-};
-
-__device__ __forceinline__ float e8m0_value(uint32_t byte) { return byte ? __uint_as_float(byte << 23) : 0x1p-127f; }
-
-// `sa`: the weights' scale, a byte or a float's bits; `sb`: the byte of this lane's row of x.
-template <bool EXACT, bool E8>
-__device__ __forceinline__ void mma_block(const Block<EXACT, E8>& a, const Block<EXACT, E8>& b, f32x4& out, uint32_t sa, uint32_t sb) {
-    if constexpr (EXACT) {
-        f32x4 sum = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.wide(i), b.wide(i), sum, 0, 0, 0);
-        out += (E8 ? e8m0_value(sa) : __uint_as_float(sa)) * e8m0_value(sb) * sum;
-    } else if constexpr (E8) {
-        out = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.operand(), b.operand(), out, 0, 0, 0, (int)sa, 0, (int)sb);
-    } else {
-        const f32x4 zero = {0, 0, 0, 0};
-        out += __uint_as_float(sa) *
-               __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.operand(), b.operand(), zero, 0, 0, 0, kOne, 0, (int)sb);
-    }
-}
-
-// The scale of a block of weights, as mma_block takes it.
-template <bool E8>
-__device__ __forceinline__ uint32_t weight_scale(const Fp8Params& p, int r, int tile, int k) {
-    return E8 ? p.ws[r][(int64_t)(tile / 8) * p.x_scales + k] : reinterpret_cast<const uint32_t*>(p.ws[r])[(int64_t)(tile / 8) * p.blocks + k];
-}
-
-// act(a) b: both activations are a / (1 + exp(-bend)), since (1 + tanh(z)) / 2 is 1 / (1 + exp(-2 z)).
-__device__ __forceinline__ float gate_value(float a, float b, int activation) {
-    const float bend = activation == 0 ? a : 1.5957691216f * (a + 0.044715f * a * a * a);
-    return a / (1.f + expf(-bend)) * b;
-}
 
 constexpr int kWaves = 8;
 
@@ -212,6 +137,10 @@ int check_product(const char* who, int64_t dtype, int64_t scale_dtype, int64_t M
     return TT_OK;
 }
 
+// Whether a call runs on workgroup tiles. (Their offsets within 256 rows are of 32 bits.)
+bool many_rows_of(int64_t M, int64_t K) { return M >= 128 && K <= 1 << 23; }
+bool many_rows(const Fp8Params& p) { return many_rows_of(p.M, p.K); }
+
 Fp8Params params_of(int64_t M, int64_t N, int64_t K, const void* x, const void* xs) {
     Fp8Params p = {};
     p.x = static_cast<const uint8_t*>(x);
@@ -259,11 +188,13 @@ extern "C" int tt_fp8_matmul(const tt_fp8_matmul_args* a, void* stream) {
     p.ws[0] = static_cast<const uint8_t*>(a->w_scales);
     p.y = a->y;
     hipStream_t st = static_cast<hipStream_t>(stream);
+    if (many_rows(p)) return fp8_tiles(a->dtype, a->scale_dtype == TT_E8M0, false, p, st);
     return a->scale_dtype == TT_E8M0 ? fp8_typed<true, false>(a->dtype, p, st) : fp8_typed<false, false>(a->dtype, p, st);
 }
 
 extern "C" size_t tt_fp8_gated_workspace_bytes(const tt_fp8_gated_args* a) {
-    if (!a || !a->codes || a->M < 1 || a->N < 1) return 0;
+    using namespace tt;
+    if (!a || !a->codes || a->M < 1 || a->N < 1 || a->K < 1 || many_rows_of(a->M, a->K)) return 0;
     return (size_t)a->M * (size_t)a->N * 4;
 }
 
@@ -289,8 +220,11 @@ extern "C" int tt_fp8_gated_matmul(const tt_fp8_gated_args* a, void* stream) {
     p.ws[1] = static_cast<const uint8_t*>(a->up_scales);
     p.activation = (int)a->activation;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    p.y = a->codes ? a->workspace : a->y;
     p.codes = static_cast<uint8_t*>(a->codes);
+    p.scales = static_cast<uint8_t*>(a->scales);
+    p.y = a->y;
+    if (many_rows(p)) return fp8_tiles(a->dtype, a->scale_dtype == TT_E8M0, true, p, st);
+    if (a->codes) p.y = a->workspace;
     if (int rc = a->scale_dtype == TT_E8M0 ? fp8_typed<true, true>(a->dtype, p, st) : fp8_typed<false, true>(a->dtype, p, st)) return rc;
     if (!a->codes) return TT_OK;
     const tt_fp8_quantize_args q = {TT_F32, a->M, a->N, a->N, a->workspace, a->codes, a->scales};
