@@ -22,8 +22,9 @@ def exponent(amax: float) -> int:
 def exponents(x: torch.Tensor) -> torch.Tensor:
     """(rows, blocks) exponents of rows x, from their blocks' largest finite magnitudes."""
     x = torch.where(x.isfinite(), x.double().abs(), 0.0)
-    return torch.tensor([[exponent(row[i: i + 128].max().item()) for i in range(0, x.shape[1], 128)] for row in x],
-                        dtype=torch.int64).reshape(x.shape[0], -(-x.shape[1] // 128))
+    top = torch.stack([x[:, i: i + 128].amax(dim=1) for i in range(0, x.shape[1], 128)], dim=1)
+    limits = 448.0 * torch.exp2(torch.arange(-127, 130, dtype=torch.float64))  # exact
+    return torch.searchsorted(limits, top.contiguous()) - 127
 
 
 def quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

@@ -277,6 +277,20 @@ def test_matmul(hip, m, n, k, e8m0, dtype):
     _check_product(x, w, y)
 
 
+# Many rows and columns, for every tile.
+LARGE = [(4000, 4096, 300), (3900, 4100, 129), (2048, 4000, 640), (1000, 4100, 256), (520, 4096, 700), (250, 4080, 1100), (64, 16400, 513),
+         (30, 16384, 300), (16, 20000, 128), (8200, 257, 200)]
+
+
+@pytest.mark.parametrize("e8m0", [True, False])
+@pytest.mark.parametrize("m,n,k", LARGE)
+def test_matmul_many_rows_and_columns(hip, m, n, k, e8m0):
+    rows, x = _rows8(m, k, m + n)
+    mat, w = _weights8(n, k, k, e8m0)
+    for dtype in DTYPES:
+        _check_product(x, w, tt.fp8_matmul(rows, mat, dtype=dtype))
+
+
 @pytest.mark.parametrize("e8m0", [True, False])
 @pytest.mark.parametrize("m", [128, 300])
 def test_matmul_every_code_and_column(hip, m, e8m0):
@@ -375,3 +389,18 @@ def test_gated_matmul(hip, m, n, k, e8m0, activation):
         err = _gated(x, wg, wu, activation, True)[1]
     small = 2.0 ** -25 if dtype == torch.float16 else 0.0
     assert ((plain.cpu().double() - want).abs() <= U[dtype] * want.abs() + (1 + U[dtype]) * err + small).all()
+
+
+@pytest.mark.parametrize("e8m0", [True, False])
+@pytest.mark.parametrize("m,n,k", [(m, n // 2 + 3, k) for m, n, k in LARGE])
+def test_gated_matmul_many_rows_and_columns(hip, m, n, k, e8m0):
+    rows, x = _rows8(m, k, m + n)
+    gate, wg = _weights8(n, k, k, e8m0)
+    up, wu = _weights8(n, k, k + 1, e8m0)
+    want, err = _gated(x, wg, wu, "silu", False)
+    _check_rows8(tt.fp8_gated_matmul(rows, gate, up), want, err)
+    for dtype in (torch.bfloat16, torch.float32):
+        plain = tt.fp8_gated_matmul(tt.Fp8Rows(rows.codes, rows.scales, dtype), gate, up, fp8=False)
+        if dtype == torch.float32:
+            err = _gated(x, wg, wu, "silu", True)[1]
+        assert ((plain.cpu().double() - want).abs() <= U[dtype] * want.abs() + (1 + U[dtype]) * err).all()

@@ -27,6 +27,7 @@ SOURCES = [
     "tt_abi.hip",
     "tt_dd.hip",
     "tt_fp8.hip",
+    "tt_fp8_gated.hip",
     "tt_fp8_rows.hip",
     "tt_fp8_tiles.hip",
     "tt_gemm.hip",

@@ -16,89 +16,159 @@ namespace {
 
 constexpr int kWaves = 8;
 
-// One workgroup of eight wavefronts a tile of 16 weight rows (two tiles where
-// gated) and 16 MT rows of x; the wavefronts share the columns, and their sums
-// are joined in their order.
-template <typename T, bool EXACT, bool E8, int MT, bool GATED>
-__global__ __launch_bounds__(64 * kWaves) void fp8_rows_kernel(Fp8Params p) {
-    constexpr int R = GATED ? 2 : 1;
-    __shared__ float so[kWaves][R][MT * 16][20];
+// A few rows: one workgroup of eight wavefronts R tiles of 16 weight rows (of
+// either matrix where gated) and 16 rows of x. The wavefronts share the columns,
+// four blocks of 128 in flight each, and their sums are joined in their order.
+template <typename T, bool EXACT, bool E8, int R, bool GATED>
+__global__ __launch_bounds__(64 * kWaves, 4) void fp8_rows_kernel(Fp8Params p) {
+    constexpr int G = GATED ? 2 : 1, U = 4;
+    __shared__ float so[kWaves][G * R][16][20];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
-    const int tiles = (p.N + 15) / 16;
-    const int tile = blockIdx.x % tiles, m0 = blockIdx.x / tiles * 16 * MT;
-    const int per = (p.blocks + kWaves - 1) / kWaves;
+    const int tiles = (p.N + 15) / 16, row_blocks = (tiles + R - 1) / R, m_blocks = (p.M + 15) / 16;
+    // Workgroup i runs on XCD i % 8: the blocks of x's rows that read the same
+    // weights follow each other on one XCD, and share its L2.
+    int rb, mb;
+    const int tail = row_blocks % kNumXcd, even = (row_blocks - tail) * m_blocks;
+    if ((int)blockIdx.x < even) {
+        rb = blockIdx.x / (kNumXcd * m_blocks) * kNumXcd + blockIdx.x % kNumXcd;
+        mb = blockIdx.x / kNumXcd % m_blocks;
+    } else {
+        rb = row_blocks - tail + (blockIdx.x - even) % tail;
+        mb = (blockIdx.x - even) / tail;
+    }
+    const int m0 = mb * 16, per = (p.blocks + kWaves - 1) / kWaves;
     const int first = wave * per, last = first + per < p.blocks ? first + per : p.blocks;
-    const uint8_t *x_row[MT], *s_row[MT];
+    // Rows past the end repeat the last one: what they give is not stored.
+    const int row = m0 + c < p.M ? m0 + c : p.M - 1;
+    const uint8_t* x_row = p.x + (int64_t)row * p.blocks * 128 + g * 16;
+    const uint8_t* s_row = p.xs + (int64_t)row * p.x_scales;
+    const uint8_t* w_tile[G * R];
+    int tile[G * R];
+    f32x4 out[G * R];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        // Rows past the end repeat the last one: what they give is not stored.
-        const int m = m0 + mt * 16 + c < p.M ? m0 + mt * 16 + c : p.M - 1;
-        x_row[mt] = p.x + (int64_t)m * p.blocks * 128 + g * 16;
-        s_row[mt] = p.xs + (int64_t)m * p.x_scales;
+    for (int r = 0; r < G * R; ++r) {
+        tile[r] = rb * R + r / G < tiles ? rb * R + r / G : tiles - 1;
+        w_tile[r] = p.w[r % G] + (int64_t)tile[r] * p.blocks * 2048 + lane * 16;
+        out[r] = f32x4{0, 0, 0, 0};
     }
-    f32x4 out[R][MT];
+    // Loads of `many` blocks ahead of their products. (No condition among them:
+    // the compiler would put each load behind it.)
+    auto fold = [&](auto many, int k) __attribute__((always_inline)) {
+        constexpr int V = decltype(many)::value;
+        Block<EXACT, E8> a[V][G * R], b[V];
+        uint32_t sa[V][G * R], sb;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+        for (int u = 0; u < V; ++u) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) out[r][mt] = f32x4{0, 0, 0, 0};
-    for (int k = first; k < last; ++k) {
-        Block<EXACT, E8> b[MT];
-        uint32_t sb[MT];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            b[mt].load(x_row[mt] + (int64_t)k * 128, x_row[mt] + (int64_t)k * 128 + 64);
-            sb[mt] = s_row[mt][k];
+            for (int r = 0; r < G * R; ++r) {
+                const uint8_t* w = w_tile[r] + (int64_t)(k + u) * 2048;
+                a[u][r].load(w, w + 1024);
+                sa[u][r] = weight_scale<E8>(p, r % G, tile[r], k + u);
+            }
+            b[u].load(x_row + (int64_t)(k + u) * 128, x_row + (int64_t)(k + u) * 128 + 64);
         }
+        // Four scales of the row at once, from where it has four.
+        const int from = k < p.x_scales - 4 ? k : p.x_scales - 4;
+        __builtin_memcpy(&sb, s_row + from, 4);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const uint8_t* src = p.w[r] + ((int64_t)tile * p.blocks + k) * 2048 + lane * 16;
-            Block<EXACT, E8> a;
-            a.load(src, src + 1024);
-            const uint32_t sa = weight_scale<E8>(p, r, tile, k);
+        for (int u = 0; u < V; ++u)
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) mma_block(a, b[mt], out[r][mt], sa, sb[mt]);
-        }
+            for (int r = 0; r < G * R; ++r) mma_block(a[u][r], b[u], out[r], sa[u][r], sb >> (k - from + u) * 8 & 255);
+    };
+    int k = first;
+    for (; k + U <= last; k += U) fold(std::integral_constant<int, U>(), k);
+    if (k + 2 <= last) {
+        fold(std::integral_constant<int, 2>(), k);
+        k += 2;
     }
+    if (k < last) fold(std::integral_constant<int, 1>(), k);
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) *reinterpret_cast<f32x4*>(&so[wave][r][mt * 16 + c][g * 4]) = out[r][mt];
+    for (int r = 0; r < G * R; ++r) *reinterpret_cast<f32x4*>(&so[wave][r][c][g * 4]) = out[r];
     __syncthreads();
-    for (int i = threadIdx.x; i < MT * 16 * 4; i += 64 * kWaves) {
-        const int m = i / 4, n = i % 4 * 4;
-        if (m0 + m >= p.M || tile * 16 + n >= p.N) continue;
-        f32x4 v[R];
+    for (int i = threadIdx.x; i < 16 * R * 4; i += 64 * kWaves) {
+        const int m = i / (R * 4), r = i / 4 % R, n = i % 4 * 4;
+        if (m0 + m >= p.M || (rb * R + r) * 16 + n >= p.N) continue;
+        f32x4 v[G];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            v[r] = *reinterpret_cast<const f32x4*>(&so[0][r][m][n]);
+        for (int q = 0; q < G; ++q) {
+            v[q] = *reinterpret_cast<const f32x4*>(&so[0][r * G + q][m][n]);
 #pragma unroll
-            for (int w = 1; w < kWaves; ++w) v[r] += *reinterpret_cast<const f32x4*>(&so[w][r][m][n]);
+            for (int w = 1; w < kWaves; ++w) v[q] += *reinterpret_cast<const f32x4*>(&so[w][r * G + q][m][n]);
         }
         float y[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = GATED ? gate_value(v[0][j], v[R - 1][j], p.activation) : v[0][j];
-        store_row(static_cast<T*>(p.y) + (int64_t)(m0 + m) * p.N, tile * 16 + n, p.N, y);
+        for (int j = 0; j < 4; ++j) y[j] = GATED ? gate_value(v[0][j], v[G - 1][j], p.activation) : v[0][j];
+        store_row(static_cast<T*>(p.y) + (int64_t)(m0 + m) * p.N, (rb * R + r) * 16 + n, p.N, y);
     }
 }
 
-template <typename T, bool EXACT, bool E8, bool GATED>
-int fp8_rows(const Fp8Params& p, hipStream_t st) {
-    const int64_t tiles = (p.N + 15) / 16;
-    const int mt = p.M <= 16 ? 1 : 2;
-    const int64_t grid = tiles * ((p.M + 16 * mt - 1) / (16 * mt));
+template <bool EXACT, bool E8, int R, bool GATED>
+int rows_run(int kind, const Fp8Params& p, hipStream_t st) {
+    const int64_t grid = ((int64_t)(p.N + 15) / 16 + R - 1) / R * ((p.M + 15) / 16);
     if (grid > kMaxGrid / 2) return set_error(TT_UNSUPPORTED, "8-bit products: %lld workgroups", (long long)grid);
-    if (mt == 1)
-        fp8_rows_kernel<T, EXACT, E8, 1, GATED><<<(uint32_t)grid, 64 * kWaves, 0, st>>>(p);
-    else
-        fp8_rows_kernel<T, EXACT, E8, 2, GATED><<<(uint32_t)grid, 64 * kWaves, 0, st>>>(p);
+    if (kind != kHalf)
+        fp8_rows_kernel<float, EXACT, E8, R, GATED><<<(uint32_t)grid, 64 * kWaves, 0, st>>>(p);
+    else if constexpr (!EXACT) {
+        if (p.bf16)
+            fp8_rows_kernel<__bf16, EXACT, E8, R, GATED><<<(uint32_t)grid, 64 * kWaves, 0, st>>>(p);
+        else
+            fp8_rows_kernel<_Float16, EXACT, E8, R, GATED><<<(uint32_t)grid, 64 * kWaves, 0, st>>>(p);
+    }
     return check_launch("8-bit products");
 }
 
-template <bool E8, bool GATED>
-int fp8_typed(int64_t dtype, const Fp8Params& p, hipStream_t st) {
-    if (GATED && p.codes) return fp8_rows<float, false, E8, GATED>(p, st);
-    if (dtype == TT_F32) return fp8_rows<float, true, E8, GATED>(p, st);
-    return dtype == TT_BF16 ? fp8_rows<__bf16, false, E8, GATED>(p, st) : fp8_rows<_Float16, false, E8, GATED>(p, st);
+// Two weight tiles a workgroup from 512 workgroups on: 32 / 64 rows on 4096 x 4096
+// take 6.5 / 9.1 us with two, 7.8 / 12.7 with one, 9.0 / 9.1 with four; 1 and 16
+// rows (256 workgroups) 5.3 / 6.5 with two, 5.0 / 5.8 with one. Two blocks of x's
+// rows a workgroup were slower for each (64 rows: 9.2 for 9.1 us, 128: 14.3 for 15.0).
+bool two_tiles(const Fp8Params& p) { return (int64_t)((p.N + 15) / 16) * ((p.M + 15) / 16) >= 512 && p.M > 16; }
+
+template <bool EXACT, bool E8, bool GATED>
+int rows_shape(int kind, const Fp8Params& p, hipStream_t st) {
+    if constexpr (!GATED)
+        if (two_tiles(p)) return rows_run<EXACT, E8, 2, GATED>(kind, p, st);
+    return rows_run<EXACT, E8, 1, GATED>(kind, p, st);
+}
+
+template <bool GATED>
+int rows(int kind, bool e8, const Fp8Params& p, hipStream_t st) {
+    if (kind == kExact) return e8 ? rows_shape<true, true, GATED>(kind, p, st) : rows_shape<true, false, GATED>(kind, p, st);
+    return e8 ? rows_shape<false, true, GATED>(kind, p, st) : rows_shape<false, false, GATED>(kind, p, st);
+}
+
+// About how many us the workgroups above take: what they read at 17 TB/s (16 to
+// 64 rows on 4096 x 4096, 60 on 1523 x 7009: 15 to 20).
+double rows_cost(const Fp8Params& p, bool gated) {
+    const int r = gated || two_tiles(p) ? 2 : 1;
+    const double groups = (double)((p.N + 15) / 16) * (gated ? 2 : 1) / r * ((p.M + 15) / 16);
+    return groups * p.blocks * (r * 2048 + (p.M < 16 ? p.M : 16) * 128) / 17e6;
+}
+
+// Offsets within a tile's rows are of 32 bits.
+bool tiles_can(const Fp8Params& p) { return p.K <= 1 << 23; }
+
+constexpr double kLaunch = 3.0;  // us of another launch
+
+// How a gated call into 8 bits goes: on tiles that write codes, or as 32-bit
+// products (on other tiles, or on few rows' workgroups) that a second launch rounds.
+struct GatedPlan {
+    bool tiles, fused;
+    int which;
+};
+
+GatedPlan gated_plan(const Fp8Params& p, int kind) {
+    GatedPlan plan = {false, false, 0};
+    if (!tiles_can(p)) return plan;
+    int which = 0;
+    double best = rows_cost(p, true);
+    const double cost = fp8_gated_tiles_cost(p, kind == kCodes ? kRaw : kind, &which);
+    if (cost < best) plan = {true, false, which}, best = cost;
+    if (kind == kCodes) {
+        const double fused = fp8_gated_tiles_cost(p, kCodes, &which) - kLaunch;
+        if (fused < best) plan = {true, true, which};
+    }
+    return plan;
 }
 
 // One thread 16 bytes of a tile.
@@ -136,10 +206,6 @@ int check_product(const char* who, int64_t dtype, int64_t scale_dtype, int64_t M
     if (M > int64_t(1) << 30) return set_error(TT_UNSUPPORTED, "%s: extents beyond 2^30", who);
     return TT_OK;
 }
-
-// Whether a call runs on workgroup tiles. (Their offsets within 256 rows are of 32 bits.)
-bool many_rows_of(int64_t M, int64_t K) { return M >= 128 && K <= 1 << 23; }
-bool many_rows(const Fp8Params& p) { return many_rows_of(p.M, p.K); }
 
 Fp8Params params_of(int64_t M, int64_t N, int64_t K, const void* x, const void* xs) {
     Fp8Params p = {};
@@ -187,15 +253,18 @@ extern "C" int tt_fp8_matmul(const tt_fp8_matmul_args* a, void* stream) {
     p.w[0] = static_cast<const uint8_t*>(a->w);
     p.ws[0] = static_cast<const uint8_t*>(a->w_scales);
     p.y = a->y;
+    p.bf16 = a->dtype == TT_BF16;
+    const bool exact = a->dtype == TT_F32, e8 = a->scale_dtype == TT_E8M0;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (many_rows(p)) return fp8_tiles(a->dtype, a->scale_dtype == TT_E8M0, false, p, st);
-    return a->scale_dtype == TT_E8M0 ? fp8_typed<true, false>(a->dtype, p, st) : fp8_typed<false, false>(a->dtype, p, st);
+    int which = 0;
+    if (tiles_can(p) && fp8_tiles_cost(p, exact, &which) < rows_cost(p, false)) return fp8_tiles(exact, e8, which, p, st);
+    return rows<false>(exact ? kExact : kHalf, e8, p, st);
 }
 
 extern "C" size_t tt_fp8_gated_workspace_bytes(const tt_fp8_gated_args* a) {
     using namespace tt;
-    if (!a || !a->codes || a->M < 1 || a->N < 1 || a->K < 1 || many_rows_of(a->M, a->K)) return 0;
-    return (size_t)a->M * (size_t)a->N * 4;
+    if (!a || !a->codes || a->M < 1 || a->N < 1 || a->K < 1 || a->M > 1 << 30 || a->N > 1 << 30 || a->K > 1 << 30) return 0;
+    return gated_plan(params_of(a->M, a->N, a->K, nullptr, nullptr), kCodes).fused ? 0 : (size_t)a->M * (size_t)a->N * 4;
 }
 
 extern "C" int tt_fp8_gated_matmul(const tt_fp8_gated_args* a, void* stream) {
@@ -219,13 +288,17 @@ extern "C" int tt_fp8_gated_matmul(const tt_fp8_gated_args* a, void* stream) {
     p.w[1] = static_cast<const uint8_t*>(a->up);
     p.ws[1] = static_cast<const uint8_t*>(a->up_scales);
     p.activation = (int)a->activation;
-    hipStream_t st = static_cast<hipStream_t>(stream);
     p.codes = static_cast<uint8_t*>(a->codes);
     p.scales = static_cast<uint8_t*>(a->scales);
-    p.y = a->y;
-    if (many_rows(p)) return fp8_tiles(a->dtype, a->scale_dtype == TT_E8M0, true, p, st);
-    if (a->codes) p.y = a->workspace;
-    if (int rc = a->scale_dtype == TT_E8M0 ? fp8_typed<true, true>(a->dtype, p, st) : fp8_typed<false, true>(a->dtype, p, st)) return rc;
+    p.bf16 = a->dtype == TT_BF16;
+    const bool e8 = a->scale_dtype == TT_E8M0;
+    const int kind = a->codes ? kCodes : a->dtype == TT_F32 ? kExact : kHalf;
+    const GatedPlan plan = gated_plan(p, kind);
+    p.y = a->codes ? a->workspace : a->y;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (plan.fused) return fp8_gated_tiles(kCodes, e8, plan.which, p, st);
+    const int first = a->codes ? kRaw : kind;
+    if (int rc = plan.tiles ? fp8_gated_tiles(first, e8, plan.which, p, st) : rows<true>(first, e8, p, st)) return rc;
     if (!a->codes) return TT_OK;
     const tt_fp8_quantize_args q = {TT_F32, a->M, a->N, a->N, a->workspace, a->codes, a->scales};
     return tt_fp8_quantize(&q, stream);

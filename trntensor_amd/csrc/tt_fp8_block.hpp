@@ -15,6 +15,7 @@ struct Fp8Params {
     uint8_t *codes, *scales;
     int M, N, K, blocks, x_scales;  // blocks of 128 columns; scale bytes of a row
     int activation;
+    int bf16;  // 16-bit results are bfloat16
 };
 
 constexpr uint32_t kOne = 127;  // e8m0 of 1.0
@@ -52,6 +53,13 @@ struct Block {
 
 __device__ __forceinline__ float e8m0_value(uint32_t byte) { return byte ? __uint_as_float(byte << 23) : 0x1p-127f; }
 
+// The sum of a block of 128 columns with the scales of x's rows alone.
+template <bool EXACT, bool E8>
+__device__ __forceinline__ f32x4 block_sum(const Block<EXACT, E8>& a, const Block<EXACT, E8>& b, uint32_t sb) {
+    const f32x4 zero = {0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.operand(), b.operand(), zero, 0, 0, 0, kOne, 0, (int)sb);
+}
+
 // `sa`: the weights' scale, a byte or a float's bits; `sb`: the byte of this lane's row of x.
 template <bool EXACT, bool E8>
 __device__ __forceinline__ void mma_block(const Block<EXACT, E8>& a, const Block<EXACT, E8>& b, f32x4& out, uint32_t sa, uint32_t sb) {
@@ -63,16 +71,18 @@ __device__ __forceinline__ void mma_block(const Block<EXACT, E8>& a, const Block
     } else if constexpr (E8) {
         out = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.operand(), b.operand(), out, 0, 0, 0, (int)sa, 0, (int)sb);
     } else {
-        const f32x4 zero = {0, 0, 0, 0};
-        out += __uint_as_float(sa) *
-               __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.operand(), b.operand(), zero, 0, 0, 0, kOne, 0, (int)sb);
+        out += __uint_as_float(sa) * block_sum(a, b, sb);
     }
 }
 
-// The scale of a block of weights, as mma_block takes it.
+// The scale of a block of weights, as mma_block takes it: a scalar load, so
+// that no wait for it is one for the vector loads on their way.
 template <bool E8>
 __device__ __forceinline__ uint32_t weight_scale(const Fp8Params& p, int r, int tile, int k) {
-    return E8 ? p.ws[r][(int64_t)(tile / 8) * p.x_scales + k] : reinterpret_cast<const uint32_t*>(p.ws[r])[(int64_t)(tile / 8) * p.blocks + k];
+    typedef const __attribute__((address_space(4))) uint32_t constant_word;
+    const int64_t at = E8 ? (int64_t)(tile / 8) * (p.x_scales / 4) + k / 4 : (int64_t)(tile / 8) * p.blocks + k;
+    const uint32_t word = ((constant_word*)(uintptr_t)p.ws[r])[at];
+    return E8 ? word >> (k & 3) * 8 & 255 : word;
 }
 
 // act(a) b: both activations are a / (1 + exp(-bend)), since (1 + tanh(z)) / 2 is 1 / (1 + exp(-2 z)).
@@ -81,7 +91,14 @@ __device__ __forceinline__ float gate_value(float a, float b, int activation) {
     return a / (1.f + expf(-bend)) * b;
 }
 
-// Many rows: tt_fp8_tiles.hip. dtype is the result's, or -1 for rows in 8 bits.
-int fp8_tiles(int64_t dtype, bool e8, bool gated, const Fp8Params& p, hipStream_t st);
+// What a call's products are summed by and written as.
+enum { kHalf, kExact, kRaw, kCodes };
+
+// Workgroup tiles (tt_fp8_tiles.hip, tt_fp8_gated.hip): about how many us a call
+// takes on the tile that is best for it, and that tile; the call on it.
+double fp8_tiles_cost(const Fp8Params& p, bool exact, int* which);
+int fp8_tiles(bool exact, bool e8, int which, const Fp8Params& p, hipStream_t st);
+double fp8_gated_tiles_cost(const Fp8Params& p, int kind, int* which);
+int fp8_gated_tiles(int kind, bool e8, int which, const Fp8Params& p, hipStream_t st);
 
 }  // namespace tt

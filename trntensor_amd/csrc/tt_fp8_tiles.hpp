@@ -1,0 +1,431 @@
+// Products of many rows in 8 bits with 8-bit weights, and the gated block on
+// two of them (tt_fp8_tiles.hip, tt_fp8_gated.hip): workgroup tiles whose operands are copied global -> LDS by
+// direct loads.
+//
+// A workgroup has WM x WN wavefronts of MB x NB blocks of 16 x 16. A stage is one
+// block of 128 columns: rows of x as eight 16-byte pieces, piece p of row r at
+// position p ^ (r / 2 % 8) so that 16 lanes' reads cover 256 bytes, and weight
+// tiles as they are packed. NS stages are held; a step multiplies one of them:
+//   the rows' blocks one at a time, the next one being read from LDS meanwhile;
+//   before the last one, all reads of the stage are done and the next stage has
+//   arrived: one barrier, behind which this stage's slot is filled again (NS
+//   steps ahead) and the next stage's weights and first rows are read while the
+//   last block is multiplied.
+// The rows' scales come along with each stage, those of the four blocks that its
+// own belongs to, 4 bytes a row. Stages that fill none are a loop of their own:
+// a branch among the products lets the compiler gather them behind it, and all
+// operands in registers before it.
+#pragma once
+
+#include <type_traits>
+
+#include "tt_fp8_block.hpp"
+
+namespace tt {
+
+namespace {
+
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+    return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+
+// Values that all lanes share, for scalar registers.
+__device__ __forceinline__ unsigned uniform(unsigned x) { return (unsigned)__builtin_amdgcn_readfirstlane((int)x); }
+__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
+    const uint64_t v = (uint64_t)(uintptr_t)p;
+    return (const uint8_t*)(uintptr_t)((uint64_t)uniform((unsigned)v) | (uint64_t)uniform((unsigned)(v >> 32)) << 32);
+}
+
+// Direct loads, 16 and 4 bytes a lane, to LDS address `to` (uniform) + 16 or 4 *
+// lane, from base (uniform) + offset, for all lanes (`on` ~0) or none (0). They are assembly so
+// that the compiler does not take them for writes that every LDS read has to wait
+// for; the kernel's own waits and barriers order them, and loads of no lane count
+// in those waits as any other. Nothing else here uses M0, and all lanes are on.
+__device__ __forceinline__ void copy16(unsigned to, const uint8_t* base, uint32_t offset, unsigned on) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
+                 :
+                 : "s"(uniform(to)), "v"(offset), "s"(uniform(base)), "s"(uniform(on))
+                 : "memory", "m0");
+}
+__device__ __forceinline__ void copy4(unsigned to, const uint8_t* base, uint32_t offset, unsigned on) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b64 exec, -1"
+                 :
+                 : "s"(uniform(to)), "v"(offset), "s"(uniform(base)), "s"(uniform(on))
+                 : "memory", "m0");
+}
+
+// s_waitcnt immediates: vmcnt in bits 3:0 and 15:14, expcnt 6:4 (7: no wait), lgkmcnt 11:8.
+constexpr int wait_vm(int n) { return (n & 15) | (n >> 4) << 14 | 0xf70; }
+constexpr int kWaitLds = ~0xf00;  // and lgkmcnt(0)
+
+// What the result is written as.
+struct Half {};    // bfloat16 or float16, as the call says
+struct Single {};  // float32, of exact sums
+struct Raw {};     // float32, of the 8-bit matrix instructions' sums
+struct Codes {};   // rows in 8 bits
+
+template <typename T, bool E8, bool GATED, int WM, int WN, int MB, int NB, int NS>
+__global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p, int tiles_m, int tiles_n) {
+    constexpr bool CODES = std::is_same<T, Codes>::value, EXACT = std::is_same<T, Single>::value;
+    constexpr int NW = WM * WN, BM = WM * MB * 16;
+    constexpr int NT = WN * NB;                          // weight tiles of 16 rows a stage
+    constexpr int BN = GATED ? NT * 8 : NT * 16;         // columns of the result
+    constexpr int XB = BM * 128, WB = NT * 2048, STAGE = XB + WB;  // bytes
+    constexpr int XI = XB / 1024 / NW, WI = WB / 1024 / NW;  // direct loads a wavefront a stage
+    constexpr int SI = (BM + 63) / 64;                   // wavefronts that load the rows' scales
+    constexpr int SB = SI * 256;                         // bytes of a four of them
+    constexpr int FOURS = 4;                             // of them held
+    constexpr int GM = GATED ? 2 : 1;                    // weight matrices
+    constexpr int WS = E8 ? FOURS : 16;                  // scales held of each: fours of bytes, or floats, of 64 tiles
+    constexpr int PER = XI + WI + 1;                     // direct loads a wavefront a stage
+    constexpr bool TWICE = NS >= 4;                      // registers hold the operands of two stages
+    constexpr int AHEAD = NS == 2 ? 1 : 0;               // stages that lines are asked of L2 before their direct loads
+    static_assert(XI * 1024 * NW == XB && WI * 1024 * NW == WB && NW >= SI + GM && MB % 2 == 0 && NB % 2 == 0, "tile");
+    // The stages held belong to at most FOURS fours.
+    static_assert(NS >= 2 && NS <= 9 && (NS - 1) * PER < 64, "stages");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * STAGE + FOURS * SB + GM * WS * 256 + (AHEAD ? NW * 256 : 0)];
+    const unsigned lds0 = lds_address(lds), ldss = lds0 + NS * STAGE, ldsw = ldss + FOURS * SB;
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+    const int wm = wave / WN, wn = wave % WN;
+
+    // Each XCD walks a contiguous range of tiles, four tiles of rows at a time.
+    const int total = tiles_m * tiles_n;
+    const int id = (int)xcd_remap(blockIdx.x, total);
+    constexpr int kGroup = 4;
+    const int grp = id / (kGroup * tiles_n), rest = id - grp * kGroup * tiles_n;
+    const int high = tiles_m - grp * kGroup < kGroup ? tiles_m - grp * kGroup : kGroup;
+    const int m0 = (grp * kGroup + rest % high) * BM, n0 = rest / high * BN;
+
+    // What this lane's direct loads read: rows past the end repeat the last one,
+    // weight tiles past the end the last one, and what they give is not stored.
+    const int64_t pitch = (int64_t)p.blocks * 128;
+    const uint8_t* x_base = p.x + m0 * pitch;
+    uint32_t x_off[XI];
+#pragma unroll
+    for (int i = 0; i < XI; ++i) {
+        const int r = (wave * XI + i) * 8 + (lane >> 3);
+        const int row = m0 + r < p.M ? r : p.M - 1 - m0;
+        x_off[i] = (uint32_t)(row * pitch) + (((lane & 7) ^ (r >> 1 & 7)) * 16);
+    }
+    const int last_tile = (p.N + 15) / 16 - 1;
+    const uint8_t* w_base[WI];
+#pragma unroll
+    for (int i = 0; i < WI; ++i) {
+        const int at = (wave * WI + i) / 2, j = at % NB;
+        int t = GATED ? n0 / 16 + at / NB * (NB / 2) + j % (NB / 2) : n0 / 16 + at;
+        t = t < last_tile ? t : last_tile;
+        w_base[i] = uniform(p.w[GATED ? j / (NB / 2) : 0] + (int64_t)t * p.blocks * 2048 + (wave * WI + i) % 2 * 1024);
+    }
+    const uint32_t w_off = lane * 16;
+    // The first wavefronts load the rows' scales, a row a lane; the others those
+    // of the weights, a tile a lane (as often as there are more lanes).
+    const bool of_rows = wave < SI;
+    const int matrix = (wave - SI) & (GM - 1);
+    uint32_t s_off;
+    const uint8_t* s_base;
+    if (of_rows) {
+        const int r = wave * 64 + lane;
+        s_base = p.xs + (int64_t)m0 * p.x_scales;
+        s_off = (uint32_t)((m0 + r < p.M ? r : p.M - 1 - m0) * (int64_t)p.x_scales);
+    } else {
+        const int pitch_ws = E8 ? p.x_scales : p.blocks * 4, t0 = n0 / 16, t = t0 + lane % (NT / GM);
+        s_base = p.ws[matrix] + (int64_t)(t0 / 8) * pitch_ws;
+        s_off = (uint32_t)(((t < last_tile ? t : last_tile) / 8 - t0 / 8) * pitch_ws);
+    }
+    const unsigned s_to = of_rows ? ldss + wave * 256 : ldsw + matrix * WS * 256;
+
+    // Direct loads [from, to) of a stage, whose place in LDS is `slot`; of no lane past the last stage.
+    auto fill = [&](int stage, int slot, int from, int to) __attribute__((always_inline)) {
+        const unsigned on = stage < p.blocks ? ~0u : 0u;
+#pragma unroll
+        for (int i = from; i < to; ++i) {
+            if (i < XI)
+                copy16(lds0 + slot + (wave * XI + i) * 1024, x_base + (int64_t)stage * 128, x_off[i], on);
+            else if (i < XI + WI)
+                copy16(lds0 + slot + XB + (wave * WI + i - XI) * 1024, w_base[i - XI] + (int64_t)stage * 2048, w_off, on);
+            else
+                copy4(s_to + (of_rows ? (stage >> 2) % FOURS * SB : (E8 ? stage >> 2 : stage) % WS * 256),
+                      s_base + (of_rows || E8 ? stage >> 2 : stage) * 4, s_off, on);
+        }
+    };
+
+    // Two stages in LDS leave a direct load one step to arrive in, which is less
+    // than a line takes that is not in L2: each line is asked for two steps earlier
+    // by one of the workgroups that share it (four of the same weights, eight or
+    // more of the same rows, on one XCD), as one word of it to a place nobody reads.
+    // A wavefront whose turn it is not asks for one line that it has.
+    const uint8_t* line = nullptr;
+    int line_step = 0;
+    if constexpr (AHEAD > 0) {
+        constexpr int XL = BM / 64, WL = NT / 4;  // wavefronts that have all lines
+        static_assert(XL + WL <= NW, "a line a lane");
+        line = x_base;
+        if (wave < XL) {
+            const int r = wave * 64 + lane;
+            if (rest / high % XL == wave) {
+                line += (m0 + r < p.M ? r : p.M - 1 - m0) * pitch;
+                line_step = 128;
+            }
+        } else if (wave < XL + WL && rest % high % WL == wave - XL) {
+            const int at = (wave - XL) * 4 + lane / 16, j = at % NB;
+            int t = GATED ? n0 / 16 + at / NB * (NB / 2) + j % (NB / 2) : n0 / 16 + at;
+            t = t < last_tile ? t : last_tile;
+            line = p.w[GATED ? j / (NB / 2) : 0] + (int64_t)t * p.blocks * 2048 + lane % 16 * 128;
+            line_step = 2048;
+        }
+    }
+    auto ask = [&](int stage) __attribute__((always_inline)) {
+        const int s = stage < p.blocks ? stage : p.blocks - 1;
+        const uint8_t* from = line + (int64_t)s * line_step;
+        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off"
+                     :
+                     : "s"(uniform(ldsw + GM * WS * 256 + wave * 256)), "v"(from)
+                     : "memory", "m0");
+    };
+
+    // Where this lane reads its operands of 16 rows or 16 weight rows.
+    const int sw = c >> 1 & 7;
+    const uint8_t* xr0 = lds + (wm * MB * 16 + c) * 128 + (g ^ sw) * 16;
+    const uint8_t* xr1 = lds + (wm * MB * 16 + c) * 128 + ((g + 4) ^ sw) * 16;
+    const uint8_t* wr = lds + XB + wn * NB * 2048 + lane * 16;
+    const uint8_t* sr = lds + NS * STAGE + (wm * MB * 16 + c) * 4;
+    const uint8_t* wsr = lds + NS * STAGE + FOURS * SB + wn * (NB / GM) * 4;  // the wavefront's weights lie in one block of 128
+
+    f32x4 acc[NB][MB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int m = 0; m < MB; ++m) acc[n][m] = f32x4{0, 0, 0, 0};
+    const int nk = p.blocks;
+    // With float scales a product waits for its predecessor's multiplication, which runs beside it.
+    constexpr bool FLOATS = !E8 && !EXACT;
+    typedef Block<EXACT, E8> B;
+    f32x4 sum;
+    auto scaled = [&](int n, int m, const uint32_t (&ws)[GM]) __attribute__((always_inline)) {
+        acc[n][m] += __uint_as_float(ws[GATED ? n / (NB / 2) : 0]) * sum;
+    };
+    auto product = [&](int n, int m, const B& w, const B& x, const uint32_t (&ws)[GM], uint32_t sb) __attribute__((always_inline)) {
+        if constexpr (FLOATS) {
+            const f32x4 next = block_sum(w, x, sb);
+            __builtin_amdgcn_sched_barrier(0);
+            if (n > 0) scaled(n - 1, m, ws);
+            if (n == 0 && m > 0) scaled(NB - 1, m - 1, ws);
+            __builtin_amdgcn_sched_barrier(0);
+            sum = next;
+        } else {
+            mma_block(w, x, acc[n][m], ws[GATED ? n / (NB / 2) : 0], sb);
+        }
+    };
+    auto read_x = [&](B& x, uint32_t& xs, int slot, int m, int stage) __attribute__((always_inline)) {
+        x.load(xr0 + slot + m * 2048, xr1 + slot + m * 2048);
+        xs = *reinterpret_cast<const uint32_t*>(sr + (stage >> 2) % FOURS * SB + m * 64);
+    };
+    auto read_w = [&](B& w, int slot, int n) __attribute__((always_inline)) {
+        w.load(wr + slot + n * 2048, wr + slot + n * 2048 + 1024);
+    };
+    auto read_ws = [&](uint32_t (&ws)[GM], int stage) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < GM; ++i) ws[i] = *reinterpret_cast<const uint32_t*>(wsr + (i * WS + (E8 ? stage >> 2 : stage) % WS) * 256);
+    };
+    auto take_ws = [&](uint32_t (&ws)[GM], int stage) __attribute__((always_inline)) {
+        if constexpr (E8)
+#pragma unroll
+            for (int i = 0; i < GM; ++i) ws[i] = ws[i] >> (stage & 3) * 8 & 255;
+    };
+    int slot = 0, last = (NS - 1) * STAGE;
+    if constexpr (!TWICE) {
+        constexpr int XR = MB % 4 == 0 ? 4 : 2, LEAD = XR / 2;  // blocks of rows in registers, and read ahead
+        // Products that a stage's direct loads are spread over, some of them behind
+        // the barrier and the rest in the next step.
+        constexpr int SPREAD = MB * NB * 7 / 16, LATE = PER * (LEAD * NB < SPREAD ? LEAD * NB : SPREAD) / SPREAD;
+        B w[NB], x[XR];
+        uint32_t xs[XR], ws[GM], next_ws[GM];
+        auto step = [&](int stage) __attribute__((always_inline)) {
+            const int next = slot == (NS - 1) * STAGE ? 0 : slot + STAGE;
+#pragma unroll
+            for (int m = 0; m < MB; ++m) {
+                if (m == MB - LEAD) {
+                    // The next stage was filled before NS - 2 others.
+                    __builtin_amdgcn_s_waitcnt(wait_vm((NS - 2) * PER + (AHEAD > 0)) & kWaitLds);
+                    asm volatile("s_barrier" ::: "memory");
+                }
+                const uint32_t sb = xs[m % XR] >> (stage & 3) * 8 & 255;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    product(n, m, w[n], x[m % XR], ws, sb);
+                    __builtin_amdgcn_sched_barrier(0);
+                    // Past the last stage these read what the slot holds, for nothing.
+                    if (n == 0) {
+                        if (m < MB - LEAD)
+                            read_x(x[(m + LEAD) % XR], xs[(m + LEAD) % XR], slot, m + LEAD, stage);
+                        else
+                            read_x(x[(m + LEAD) % XR], xs[(m + LEAD) % XR], next, m + LEAD - MB, stage + 1);
+                    }
+                    if (m == MB - 1) read_w(w[n], next, n);
+                    if (m == MB - 1 && n == 0) read_ws(next_ws, stage + 1);
+                    const int at = ((m - (MB - LEAD) + MB) % MB) * NB + n;  // products since the barrier
+                    const bool before = m < MB - LEAD;
+                    if (at < SPREAD) fill(stage + NS - before, before ? last : slot, PER * at / SPREAD, PER * (at + 1) / SPREAD);
+                    if constexpr (AHEAD > 0)
+                        if (at == SPREAD - 1) ask(stage + NS - before + AHEAD);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if constexpr (FLOATS) scaled(NB - 1, MB - 1, ws);
+#pragma unroll
+            for (int i = 0; i < GM; ++i) ws[i] = next_ws[i];
+            take_ws(ws, stage + 1);
+            last = slot;
+            slot = next;
+        };
+#pragma unroll
+        for (int s = 0; s < NS; ++s) fill(s, s * STAGE, 0, s < NS - 1 ? PER : LATE);
+        __builtin_amdgcn_s_waitcnt(wait_vm((NS - 2) * PER + LATE));
+        asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+        for (int n = 0; n < NB; ++n) read_w(w[n], 0, n);
+        read_ws(ws, 0);
+        take_ws(ws, 0);
+#pragma unroll
+        for (int m = 0; m < LEAD; ++m) read_x(x[m], xs[m], 0, m, 0);
+        for (int stage = 0; stage < nk; ++stage) step(stage);
+    } else {
+        B w[2][NB], x[2][MB];
+        uint32_t xs[2][MB], ws[2][GM];
+        auto step = [&](auto parity, int stage) __attribute__((always_inline)) {
+            constexpr int P = decltype(parity)::value;
+            const int next = slot == (NS - 1) * STAGE ? 0 : slot + STAGE;
+            take_ws(ws[P], stage);
+#pragma unroll
+            for (int m = 0; m < MB; ++m) {
+                const uint32_t sb = xs[P][m] >> (stage & 3) * 8 & 255;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    product(n, m, w[P][n], x[P][m], ws[P], sb);
+                    __builtin_amdgcn_sched_barrier(0);
+                    // The next stage's operands (past the last stage, what the slot holds).
+                    const int at = m * NB + n;
+                    if (at == 0) read_ws(ws[P ^ 1], stage + 1);
+                    if (at < NB) read_w(w[P ^ 1][at], next, at);
+                    if (at >= MB * NB - MB) read_x(x[P ^ 1][at - (MB * NB - MB)], xs[P ^ 1][at - (MB * NB - MB)], next, at - (MB * NB - MB), stage + 1);
+                    fill(stage + NS - 1, last, PER * at / (MB * NB), PER * (at + 1) / (MB * NB));
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if constexpr (FLOATS) scaled(NB - 1, MB - 1, ws[P]);
+            // The stage after the next was filled before NS - 3 others.
+            __builtin_amdgcn_s_waitcnt(wait_vm((NS - 3) * PER));
+            asm volatile("s_barrier" ::: "memory");
+            last = slot;
+            slot = next;
+        };
+#pragma unroll
+        for (int s = 0; s < NS - 1; ++s) fill(s, s * STAGE, 0, PER);
+        __builtin_amdgcn_s_waitcnt(wait_vm((NS - 3) * PER));
+        asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+        for (int n = 0; n < NB; ++n) read_w(w[0][n], 0, n);
+        read_ws(ws[0], 0);
+#pragma unroll
+        for (int m = 0; m < MB; ++m) read_x(x[0][m], xs[0][m], 0, m, 0);
+        int stage = 0;
+        for (; stage + 1 < nk; stage += 2) {
+            step(std::integral_constant<int, 0>(), stage);
+            step(std::integral_constant<int, 1>(), stage + 1);
+        }
+        if (stage < nk) step(std::integral_constant<int, 0>(), stage);
+    }
+    __builtin_amdgcn_s_waitcnt(wait_vm(0));
+
+    if constexpr (!CODES) {
+        constexpr int N = GATED ? NB / 2 : NB;  // column blocks of the result a wavefront
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+            const int row = m0 + (wm * MB + m) * 16 + c;
+            if (row >= p.M) continue;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = GATED ? gate_value(acc[n][m][i], acc[n + NB - N][m][i], p.activation) : acc[n][m][i];
+                const int64_t at = (int64_t)row * p.N;
+                const int col = n0 + (wn * N + n) * 16 + g * 4;
+                if constexpr (!std::is_same<T, Half>::value)
+                    store_row(static_cast<float*>(p.y) + at, col, p.N, v);
+                else if (p.bf16)
+                    store_row(static_cast<__bf16*>(p.y) + at, col, p.N, v);
+                else
+                    store_row(static_cast<_Float16*>(p.y) + at, col, p.N, v);
+            }
+        }
+    } else {
+        // Rows in 8 bits: the tile has all of a block's 128 columns.
+        constexpr int N = NB / 2;
+        static_assert(!CODES || (GATED && BN == 128), "a block of 128 a tile");
+        float* top = reinterpret_cast<float*>(lds);                // [WN][BM]
+        uint8_t* out = lds + WN * BM * 4;                          // [BM][144]
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+            float amax = 0.f;
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float v = gate_value(acc[n][m][i], acc[n + N][m][i], p.activation);
+                    if (n0 + (wn * N + n) * 16 + g * 4 + i >= p.N) v = 0.f;
+                    acc[n][m][i] = v;
+                    amax = fmaxf(amax, finite_magnitude(v));
+                }
+            amax = column_max(amax);
+            if (g == 0) top[wn * BM + (wm * MB + m) * 16 + c] = amax;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+            const int r = (wm * MB + m) * 16 + c;
+            float amax = top[r];
+#pragma unroll
+            for (int i = 1; i < WN; ++i) amax = fmaxf(amax, top[i * BM + r]);
+            const uint32_t byte = fp8_scale_byte(amax);
+            const float inv = fp8_scale_inverse(byte);
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const f32x4 v = acc[n][m] * inv;
+                *reinterpret_cast<uint32_t*>(out + r * 144 + (wn * N + n) * 16 + g * 4) = fp8_high(v[2], v[3], fp8_low(v[0], v[1]));
+            }
+            const int64_t blocks = fp8_blocks(p.N), per_row = fp8_scales(p.N);
+            if (wn == 0 && m0 + r < p.M) {
+                uint8_t* to = p.scales + (m0 + r) * per_row + n0 / 128;
+                if (g == 0) to[0] = (uint8_t)byte;
+                if (g > 0 && n0 + 128 >= p.N && n0 / 128 + g < per_row) to[g] = 0;  // past the blocks
+            }
+            if (m == MB - 1) {
+                __syncthreads();
+                for (int i = threadIdx.x; i < BM * 8; i += 64 * NW)
+                    if (m0 + i / 8 < p.M)
+                        *reinterpret_cast<u32x4*>(p.codes + ((m0 + i / 8) * blocks * 128 + n0 + i % 8 * 16)) =
+                            *reinterpret_cast<const u32x4*>(out + i / 8 * 144 + i % 8 * 16);
+            }
+        }
+    }
+}
+
+template <typename T, bool E8, bool GATED, int WM, int WN, int MB, int NB, int NS>
+int tiles_run(const Fp8Params& p, hipStream_t st) {
+    constexpr int BM = WM * MB * 16, BN = WN * NB * (GATED ? 8 : 16);
+    const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
+    if (tm * tn > kMaxGrid / 2) return set_error(TT_UNSUPPORTED, "8-bit products: %lld tiles", (long long)(tm * tn));
+    fp8_tiles_kernel<T, E8, GATED, WM, WN, MB, NB, NS><<<(uint32_t)(tm * tn), 64 * WM * WN, 0, st>>>(p, (int)tm, (int)tn);
+    return check_launch("8-bit products");
+}
+
+// Steps of 256 workgroups that tiles of bm x bn take, times what a step takes.
+inline double tiles_cost(const Fp8Params& p, int bm, int bn, double step) {
+    const int64_t tiles = (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn);
+    return (double)((tiles + 255) / 256) * step;
+}
+
+}  // namespace
+}  // namespace tt
