@@ -34,6 +34,8 @@ def no_gpu(monkeypatch):
 class _Matrix:
     """What the checks before a launch read of weights."""
 
+    _host = None
+
     def __init__(self, n=64, k=256, scale_dtype=torch.float32):
         self.shape, self.scale_dtype, self.device = (n, k), scale_dtype, torch.device("cpu")
 

@@ -32,9 +32,14 @@ struct Library {
     decltype(&tt_kv_attention) kv_attention;
     decltype(&tt_last_error) last_error;
     decltype(&tt_status_string) status_string;
+    decltype(&tt_fp8_quantize) fp8_quantize;
+    decltype(&tt_rms_norm) rms_norm;
+    decltype(&tt_fp8_matmul) fp8_matmul;
+    decltype(&tt_fp8_gated_workspace_bytes) gated_bytes;
+    decltype(&tt_fp8_gated_matmul) gated_matmul;
 
     explicit Library(const std::vector<int64_t>& a) {
-        TORCH_CHECK(a.size() == 6, "Library: six entry points expected");
+        TORCH_CHECK(a.size() == 11, "Library: eleven entry points expected");
         for (int64_t p : a) TORCH_CHECK(p != 0, "Library: null entry point");
         q4_matmul = reinterpret_cast<decltype(q4_matmul)>(a[0]);
         kv_append = reinterpret_cast<decltype(kv_append)>(a[1]);
@@ -42,6 +47,11 @@ struct Library {
         kv_attention = reinterpret_cast<decltype(kv_attention)>(a[3]);
         last_error = reinterpret_cast<decltype(last_error)>(a[4]);
         status_string = reinterpret_cast<decltype(status_string)>(a[5]);
+        fp8_quantize = reinterpret_cast<decltype(fp8_quantize)>(a[6]);
+        rms_norm = reinterpret_cast<decltype(rms_norm)>(a[7]);
+        fp8_matmul = reinterpret_cast<decltype(fp8_matmul)>(a[8]);
+        gated_bytes = reinterpret_cast<decltype(gated_bytes)>(a[9]);
+        gated_matmul = reinterpret_cast<decltype(gated_matmul)>(a[10]);
     }
 
     void check(int rc, const char* what) const {
@@ -265,6 +275,175 @@ class CacheHost {
     tt_kv_cache cache_;
 };
 
+// Codes and scales of rows in 8 bits, as the kernels lay them out.
+struct Rows8 {
+    Tensor codes, scales;
+
+    Rows8(const Place& at, int64_t rows, int64_t dim) {
+        const int64_t blocks = (dim + 127) / 128;
+        codes = at.empty({rows, blocks * 128}, at::kByte);
+        scales = at.empty({rows, (blocks + 3) / 4 * 4}, at::kByte);
+    }
+};
+
+// Rows of `dim` elements of unit stride, `stride` elements apart; false where they are not.
+bool rows_of(const Tensor& x, int64_t& rows, int64_t& dim, int64_t& stride) {
+    const int64_t nd = x.dim();
+    if (nd < 1 || x.size(nd - 1) < 1) return false;
+    dim = x.size(nd - 1);
+    if (nd == 2 && x.stride(1) == 1) {
+        rows = x.size(0);
+        stride = x.stride(0);
+        return true;
+    }
+    rows = x.numel() / dim;
+    stride = dim;
+    return x.is_contiguous();
+}
+
+// Norms and quantization.
+class RowsHost {
+   public:
+    explicit RowsHost(const std::vector<int64_t>& entries) : lib_(entries) {}
+
+    // (codes, scales), or None
+    py::object quantize(const Tensor& x) const {
+        tt_fp8_quantize_args a;
+        a.dtype = code_of(x.scalar_type());
+        const Place at{x.device().index()};
+        if (a.dtype < 0 || !at.holds(x) || !at.here() || !rows_of(x, a.rows, a.dim, a.x_stride)) return py::none();
+        const Rows8 out(at, a.rows, a.dim);
+        a.x = x.data_ptr();
+        a.codes = out.codes.data_ptr();
+        a.scales = out.scales.data_ptr();
+        lib_.check(lib_.fp8_quantize(&a, at.stream()), "tt_fp8_quantize");
+        return py::make_tuple(out.codes, out.scales);
+    }
+
+    // (norm or codes, scales or None, sum or None), or None
+    py::object norm(const Tensor& x, const OptTensor& weight, const OptTensor& residual, double eps, bool fp8) const {
+        tt_rms_norm_args a;
+        std::memset(&a, 0, sizeof a);
+        a.dtype = code_of(x.scalar_type());
+        const Place at{x.device().index()};
+        if (a.dtype < 0 || !at.holds(x) || !at.here() || !rows_of(x, a.rows, a.dim, a.x_stride) || !(eps >= 0.0) || eps >= 1e38)
+            return py::none();
+        if (weight) {
+            a.weight_dtype = code_of(weight->scalar_type());
+            if (a.weight_dtype < 0 || weight->dim() != 1 || weight->size(0) != a.dim || !weight->is_contiguous() || !at.holds(*weight))
+                return py::none();
+            a.weight = weight->data_ptr();
+        }
+        Tensor sum;
+        if (residual) {
+            int64_t rows, dim;
+            if (residual->sizes() != x.sizes() || residual->scalar_type() != x.scalar_type() || !at.holds(*residual) ||
+                !rows_of(*residual, rows, dim, a.residual_stride))
+                return py::none();
+            sum = at.empty(x.sizes(), x.scalar_type());
+            a.residual = residual->data_ptr();
+            a.sum = sum.data_ptr();
+        }
+        a.eps = eps;
+        a.x = x.data_ptr();
+        Tensor first, second;
+        if (fp8) {
+            const Rows8 out(at, a.rows, a.dim);
+            first = out.codes;
+            second = out.scales;
+            a.codes = first.data_ptr();
+            a.scales = second.data_ptr();
+        } else {
+            first = at.empty(x.sizes(), x.scalar_type());
+            a.y = first.data_ptr();
+        }
+        lib_.check(lib_.rms_norm(&a, at.stream()), "tt_rms_norm");
+        return py::make_tuple(first, fp8 ? py::cast(second) : py::none(), residual ? py::cast(sum) : py::none());
+    }
+
+   private:
+    Library lib_;
+};
+
+// 8-bit weights. Rows come as their two arrays, whose shapes Fp8Rows vouches for.
+class Fp8Host {
+   public:
+    Fp8Host(const std::vector<int64_t>& entries, const Tensor& packed, const Tensor& scales, int64_t n, int64_t k, bool e8m0)
+        : lib_(entries), packed_(packed), scales_(scales), at_{packed.device().index()}, n_(n), k_(k), code_(e8m0 ? TT_E8M0 : TT_F32) {}
+
+    py::object run(const Tensor& codes, const Tensor& scales, const std::vector<int64_t>& shape, at::ScalarType dtype) const {
+        tt_fp8_matmul_args a;
+        a.dtype = code_of(dtype);
+        if (a.dtype < 0 || !at_.here() || !takes(codes, shape)) return py::none();
+        a.scale_dtype = code_;
+        a.M = codes.size(0);
+        a.N = n_;
+        a.K = k_;
+        a.x = codes.data_ptr();
+        a.x_scales = scales.data_ptr();
+        a.w = packed_.data_ptr();
+        a.w_scales = scales_.data_ptr();
+        const Tensor y = at_.empty(result(shape), dtype);
+        a.y = y.data_ptr();
+        lib_.check(lib_.fp8_matmul(&a, at_.stream()), "tt_fp8_matmul");
+        return py::cast(y);
+    }
+
+    // (result or codes, scales or None), or None; this matrix is the gate's.
+    py::object gated(const Fp8Host& up, const Tensor& codes, const Tensor& scales, const std::vector<int64_t>& shape,
+                     at::ScalarType dtype, int64_t activation, bool fp8) const {
+        tt_fp8_gated_args a;
+        std::memset(&a, 0, sizeof a);
+        a.dtype = code_of(dtype);
+        if (a.dtype < 0 || !at_.here() || !takes(codes, shape) || up.n_ != n_ || up.k_ != k_ || up.code_ != code_ ||
+            up.at_.device != at_.device)
+            return py::none();
+        a.scale_dtype = code_;
+        a.activation = activation;
+        a.M = codes.size(0);
+        a.N = n_;
+        a.K = k_;
+        a.x = codes.data_ptr();
+        a.x_scales = scales.data_ptr();
+        a.gate = packed_.data_ptr();
+        a.gate_scales = scales_.data_ptr();
+        a.up = up.packed_.data_ptr();
+        a.up_scales = up.scales_.data_ptr();
+        Tensor first, second, room;
+        if (fp8) {
+            const Rows8 out(at_, a.M, n_);
+            first = out.codes;
+            second = out.scales;
+            a.codes = first.data_ptr();
+            a.scales = second.data_ptr();
+            a.workspace_bytes = static_cast<int64_t>(lib_.gated_bytes(&a));
+            if (a.workspace_bytes) {
+                room = at_.empty({a.workspace_bytes}, at::kByte);
+                a.workspace = room.data_ptr();
+            }
+        } else {
+            first = at_.empty(result(shape), dtype);
+            a.y = first.data_ptr();
+        }
+        lib_.check(lib_.gated_matmul(&a, at_.stream()), "tt_fp8_gated_matmul");
+        return py::make_tuple(first, fp8 ? py::cast(second) : py::none());
+    }
+
+   private:
+    bool takes(const Tensor& codes, const std::vector<int64_t>& shape) const {
+        return codes.is_cuda() && codes.device().index() == at_.device && !shape.empty() && shape.back() == k_ && n_ > 0;
+    }
+    std::vector<int64_t> result(std::vector<int64_t> shape) const {
+        shape.back() = n_;
+        return shape;
+    }
+
+    Library lib_;
+    Tensor packed_, scales_;
+    Place at_;
+    int64_t n_, k_, code_;
+};
+
 }  // namespace
 
 void bind_serving(py::module_& m) {
@@ -276,4 +455,12 @@ void bind_serving(py::module_& m) {
         .def(py::init<const std::vector<int64_t>&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t>())
         .def("append", &CacheHost::append)
         .def("attention", &CacheHost::attention);
+    py::class_<RowsHost>(m, "RowsHost")
+        .def(py::init<const std::vector<int64_t>&>())
+        .def("quantize", &RowsHost::quantize)
+        .def("norm", &RowsHost::norm);
+    py::class_<Fp8Host>(m, "Fp8Host")
+        .def(py::init<const std::vector<int64_t>&, const Tensor&, const Tensor&, int64_t, int64_t, bool>())
+        .def("run", &Fp8Host::run)
+        .def("gated", &Fp8Host::gated);
 }

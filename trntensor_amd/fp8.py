@@ -26,7 +26,7 @@ import struct
 import torch
 
 from . import serving
-from .hip import _lib, dispatch
+from .hip import _fastpath, _lib, dispatch
 from .serving import FP8, _check_dtype, _check_grad, _CODES, _Fixed
 
 E8M0 = torch.float8_e8m0fnu
@@ -64,6 +64,15 @@ def _rows(t: torch.Tensor, device: torch.device) -> torch.Tensor:
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
+def _shaped(t: torch.Tensor, lead, last: int) -> torch.Tensor:
+    """Two-dimensional rows, of which `last` elements count, in their own shape."""
+    if t.shape[1] != last:
+        t = t[:, :last]
+    if len(lead) == 1:
+        return t
+    return t.unflatten(0, lead) if lead else t[0]
+
+
 class Fp8Rows(_Fixed):
     """Activations (..., features) in 8-bit floats, with one power of two for
     each row and block of 128 features: a value is its code times its scale.
@@ -95,7 +104,12 @@ class Fp8Rows(_Fixed):
         self._scales[:, : want[-1]] = scales.to(device).view(torch.uint8).reshape(-1, want[-1])
 
     def _set(self, shape, dtype, codes, scales):
-        self.shape, self.dtype, self.device, self._codes, self._scales = torch.Size(shape), dtype, codes.device, codes, scales
+        put = object.__setattr__
+        put(self, "shape", shape)
+        put(self, "dtype", dtype)
+        put(self, "device", codes.device)
+        put(self, "_codes", codes)
+        put(self, "_scales", scales)
 
     @classmethod
     def _of(cls, shape, dtype, codes, scales) -> "Fp8Rows":
@@ -106,13 +120,12 @@ class Fp8Rows(_Fixed):
     @property
     def codes(self) -> torch.Tensor:
         """float8_e4m3fn (..., features); rows start every multiple of 128 codes."""
-        return self._codes.view(FP8)[:, : self.shape[-1]].unflatten(0, self.shape[:-1] or (1,)).view(self.shape)
+        return _shaped(self._codes.view(FP8), self.shape[:-1], self.shape[-1])
 
     @property
     def scales(self) -> torch.Tensor:
         """float8_e8m0fnu (..., ceil(features / 128)); rows start every multiple of 4 scales."""
-        shape = (*self.shape[:-1], _blocks(self.shape[-1]))
-        return self._scales.view(E8M0)[:, : shape[-1]].unflatten(0, shape[:-1] or (1,)).view(shape)
+        return _shaped(self._scales.view(E8M0), self.shape[:-1], _blocks(self.shape[-1]))
 
     def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         """The rows' values, in ``dtype`` (the rows' one if None)."""
@@ -143,7 +156,7 @@ class Fp8Matrix(_Fixed):
     take. Operands that ask for a gradient are refused.
     """
 
-    __slots__ = ("shape", "device", "scale_dtype", "_packed", "_scales")
+    __slots__ = ("shape", "device", "scale_dtype", "_packed", "_scales", "_host")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dtype != FP8 or codes.dim() != 2 or codes.shape[1] < 1:
@@ -167,6 +180,9 @@ class Fp8Matrix(_Fixed):
         self.shape = (n, k)
         self.device = device
         self.scale_dtype = scales.dtype
+        host = _fastpath.module()
+        self._host = None if host is None else host.Fp8Host(_fastpath.serving_entries(), self._packed, self._scales, n, k,
+                                                            scales.dtype == E8M0)
 
     @classmethod
     def quantize(cls, weights: torch.Tensor) -> "Fp8Matrix":
@@ -207,6 +223,11 @@ def fp8_quantize(x: torch.Tensor) -> Fp8Rows:
     even. Infinities become NaN (the format has none), and NaN stays NaN. Rows
     need a unit stride and one row pitch, else they are copied.
     """
+    host = _fastpath.rows_host()
+    if host is not None and dispatch._use_hip() and isinstance(x, torch.Tensor):
+        out = host.quantize(x)
+        if out is not None:
+            return Fp8Rows._of(x.shape, x.dtype, *out)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"x must be (..., features); got {tuple(x.shape)}")
     code = _check_dtype("x", x)
@@ -232,6 +253,12 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
     rounding. Squares are summed in 32 bits: magnitudes of 2^63 and more overflow
     them. Rows need a unit stride and one row pitch, else they are copied.
     """
+    host = _fastpath.rows_host()
+    if host is not None and dispatch._use_hip() and isinstance(x, torch.Tensor):
+        out = host.norm(x, weight, residual, eps, fp8)
+        if out is not None:
+            y = Fp8Rows._of(x.shape, x.dtype, out[0], out[1]) if fp8 else out[0]
+            return y if residual is None else (y, out[2])
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"x must be (..., features); got {tuple(x.shape)}")
     dim = x.shape[-1]
@@ -302,6 +329,10 @@ def fp8_matmul(x: Fp8Rows | torch.Tensor, w: Fp8Matrix, *, dtype: torch.dtype | 
     of each block of 128 before its weights' scale multiplies it. NaN in a row
     gives NaN in the row's result.
     """
+    if w._host is not None and isinstance(x, Fp8Rows) and dispatch._use_hip():
+        y = w._host.run(x._codes, x._scales, x.shape, x.dtype if dtype is None else dtype)
+        if y is not None:
+            return y
     home = None if isinstance(x, Fp8Rows) else x.device
     x = _operand("fp8_matmul", x, w)
     code = _CODES.get(x.dtype if dtype is None else dtype)
@@ -334,12 +365,16 @@ def fp8_gated_matmul(x: Fp8Rows | torch.Tensor, gate: Fp8Matrix, up: Fp8Matrix, 
     kind = _ACTIVATIONS.get(activation)
     if kind is None:
         raise ValueError(f"activation must be one of {tuple(_ACTIVATIONS)}; got {activation!r}")
+    if gate._host is not None and up._host is not None and isinstance(x, Fp8Rows) and dispatch._use_hip():
+        out = gate._host.gated(up._host, x._codes, x._scales, x.shape, x.dtype, kind, fp8)
+        if out is not None:
+            return Fp8Rows._of(torch.Size((*x.shape[:-1], gate.shape[0])), x.dtype, *out) if fp8 else out[0]
     home = None if isinstance(x, Fp8Rows) else x.device
     x = _operand("fp8_gated_matmul", x, gate)
     dispatch.require_hip()
     n, k = gate.shape
     device = gate.device
-    shape = (*x.shape[:-1], n)
+    shape = torch.Size((*x.shape[:-1], n))
     y = codes = scales = None
     if fp8:
         codes, scales = _room(shape, device)

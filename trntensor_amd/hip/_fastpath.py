@@ -22,6 +22,7 @@ PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
 
 _module = None
 _table = None
+_rows = None
 _error: str | None = None
 _tried = False
 
@@ -46,7 +47,7 @@ def module():
         spec = importlib.util.spec_from_file_location("tt_fastpath", PATH)
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
-        for name in ("LaunchTable", "Q4Host", "CacheHost"):
+        for name in ("LaunchTable", "Q4Host", "CacheHost", "RowsHost", "Fp8Host"):
             getattr(mod, name)
         _module = mod
     except (ImportError, OSError, AttributeError) as exc:
@@ -67,10 +68,22 @@ def table(max_entries: int):
 
 
 def serving_entries() -> list[int]:
-    """The library's entry points that Q4Host and CacheHost call, by address."""
+    """The library's entry points that the serving operators' host path calls, by address."""
     lib = _lib.load()
     return [_addr(fn) for fn in (lib.tt_q4_matmul, lib.tt_kv_append, lib.tt_kv_attention_workspace_bytes,
-                                 lib.tt_kv_attention, lib.tt_last_error, lib.tt_status_string)]
+                                 lib.tt_kv_attention, lib.tt_last_error, lib.tt_status_string, lib.tt_fp8_quantize,
+                                 lib.tt_rms_norm, lib.tt_fp8_matmul, lib.tt_fp8_gated_workspace_bytes,
+                                 lib.tt_fp8_gated_matmul)]
+
+
+def rows_host():
+    """The process's RowsHost (created on first use), or None with the reason in error()."""
+    global _rows
+    if _rows is None:
+        mod = module()
+        if mod is not None:
+            _rows = mod.RowsHost(serving_entries())
+    return _rows
 
 
 def error() -> str | None:
