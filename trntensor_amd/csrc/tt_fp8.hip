@@ -296,6 +296,8 @@ extern "C" int tt_fp8_gated_matmul(const tt_fp8_gated_args* a, void* stream) {
     const GatedPlan plan = gated_plan(p, kind);
     p.y = a->codes ? a->workspace : a->y;
     hipStream_t st = static_cast<hipStream_t>(stream);
+    if (a->codes && !plan.fused && fp8_quantize_grid(a->M, a->N) > kMaxGrid)
+        return set_error(TT_UNSUPPORTED, "%s: %lld rows of %lld", who, (long long)a->M, (long long)a->N);
     if (plan.fused) return fp8_gated_tiles(kCodes, e8, plan.which, p, st);
     const int first = a->codes ? kRaw : kind;
     if (int rc = plan.tiles ? fp8_gated_tiles(first, e8, plan.which, p, st) : rows<true>(first, e8, p, st)) return rc;

@@ -7,6 +7,8 @@
 // matrix instructions take both as they are.
 #pragma once
 
+#include <type_traits>
+
 #include "tt_serving.hpp"
 
 namespace tt {
@@ -14,6 +16,17 @@ namespace tt {
 inline __host__ __device__ int64_t fp8_blocks(int64_t dim) { return (dim + 127) / 128; }
 inline __host__ __device__ int64_t fp8_width(int64_t dim) { return fp8_blocks(dim) * 128; }
 inline __host__ __device__ int64_t fp8_scales(int64_t dim) { return (fp8_blocks(dim) + 3) / 4 * 4; }
+
+// Lanes that a row takes in tt_fp8_quantize, eight elements each (or 256 a piece of
+// 2048 elements), and its workgroups of 256.
+inline int fp8_quantize_lanes(int64_t dim) {
+    const int64_t blocks = fp8_blocks(dim);
+    return blocks <= 1 ? 16 : blocks <= 2 ? 32 : blocks <= 4 ? 64 : blocks <= 8 ? 128 : 256;
+}
+inline int64_t fp8_quantize_grid(int64_t rows, int64_t dim) {
+    const int each = 256 / fp8_quantize_lanes(dim);
+    return each > 1 ? (rows + each - 1) / each : rows * ((dim + 2047) / 2048);
+}
 
 // The e8m0 byte of a block whose largest finite magnitude is amax: the
 // smallest e >= -127 with amax <= 448 * 2^e. 448 is 1.75 * 2^8, so that e is
@@ -53,8 +66,9 @@ __device__ __forceinline__ uint32_t fp8_high(float a, float b, uint32_t old) {
 }
 
 // Eight values of a row, from column `col` on (a multiple of 8), as codes and,
-// from the first of the 16 lanes that hold a block, its scale. All lanes of a
-// block call it, values past dim are zeros; `blocks` is fp8_blocks(dim).
+// from the first of the 16 lanes that hold a block, its scale (and zeros past the
+// last one). All lanes of a block call it, values past dim are zeros; `blocks` is
+// fp8_blocks(dim).
 __device__ __forceinline__ void fp8_store8(const float (&v)[8], int64_t col, int64_t blocks, uint8_t* codes, uint8_t* scales) {
     float amax = finite_magnitude(v[0]);
 #pragma unroll
@@ -68,22 +82,47 @@ __device__ __forceinline__ void fp8_store8(const float (&v)[8], int64_t col, int
             w[i] = fp8_high(v[4 * i + 2] * inv, v[4 * i + 3] * inv, fp8_low(v[4 * i] * inv, v[4 * i + 1] * inv));
         *reinterpret_cast<u32x2*>(codes + col) = w;
     }
-    if ((threadIdx.x & 15) == 0 && col < (blocks + 3) / 4 * 4 * 128) scales[col / 128] = (uint8_t)byte;
-}
-
-// N elements from p + col on as floats, zeros from `dim` on.
-template <int N, typename T>
-__device__ __forceinline__ void load_row(const T* p, int64_t col, int64_t dim, float (&v)[N]) {
-    if (col + N <= dim) {
-        T t[N];
-        __builtin_memcpy(t, p + col, sizeof t);
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = to_f32(t[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = col + i < dim ? to_f32(p[col + i]) : 0.f;
+    if ((threadIdx.x & 15) == 0 && col < blocks * 128) {
+        scales[col / 128] = (uint8_t)byte;
+        if (col / 128 == blocks - 1)
+            for (int64_t past = blocks; past < (blocks + 3) / 4 * 4; ++past) scales[past] = 0;
     }
 }
+
+// Eight elements of a row from column `col` on, zeros from `dim` on, as loaded:
+// what is made of them is made where they are used, so that several loads are on
+// their way at once.
+template <typename T>
+struct Eight {
+    u32x4 raw[sizeof(T) / 2];
+
+    __device__ __forceinline__ void load(const T* p, int col, int dim) {
+        if (col + 8 <= dim) {
+            __builtin_memcpy(raw, p + col, sizeof raw);
+            return;
+        }
+        typedef typename std::conditional<sizeof(T) == 2, uint16_t, uint32_t>::type U;
+        const U* u = reinterpret_cast<const U*>(p);
+        uint32_t t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = u[col + i < dim ? col + i : dim - 1];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (col + i >= dim) t[i] = 0;
+        if constexpr (sizeof(T) == 2) {
+            raw[0] = u32x4{t[0] | t[1] << 16, t[2] | t[3] << 16, t[4] | t[5] << 16, t[6] | t[7] << 16};
+        } else {
+            raw[0] = u32x4{t[0], t[1], t[2], t[3]};
+            raw[1] = u32x4{t[4], t[5], t[6], t[7]};
+        }
+    }
+    // Element i; 16-bit ones are bfloat16 if `bf16`, else float16.
+    __device__ __forceinline__ float get(int i, bool bf16 = std::is_same<T, __bf16>::value) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(raw[i / 4][i % 4]);
+        const uint32_t pair = raw[0][i / 2];
+        return bf16 ? bf16_of(pair, i % 2) : (float)__builtin_bit_cast(f16x2, pair)[i % 2];
+    }
+};
 
 template <int N, typename T>
 __device__ __forceinline__ void store_row(T* p, int64_t col, int64_t dim, const float (&v)[N]) {
