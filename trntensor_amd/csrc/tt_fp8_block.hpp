@@ -85,10 +85,17 @@ __device__ __forceinline__ uint32_t weight_scale(const Fp8Params& p, int r, int 
     return E8 ? word >> (k & 3) * 8 & 255 : word;
 }
 
-// act(a) b: both activations are a / (1 + exp(-bend)), since (1 + tanh(z)) / 2 is 1 / (1 + exp(-2 z)).
+// act(a) b: both activations are a / (1 + exp(-bend)), since (1 + tanh(z)) / 2 is 1 /
+// (1 + exp(-2 z)). The hardware's exponential (of base 2) and reciprocal err by a
+// unit each, which costs nothing next to the products' sums; with a full division
+// and exponential a tile of 256 x 128 values took 14 us for @ beside its products.
+template <int ACTIVATION>
+__device__ __forceinline__ float gate_value(float a, float b) {
+    const float bend = ACTIVATION == 0 ? a : 1.5957691216f * (a + 0.044715f * a * a * a);
+    return a * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504089f * bend)) * b;
+}
 __device__ __forceinline__ float gate_value(float a, float b, int activation) {
-    const float bend = activation == 0 ? a : 1.5957691216f * (a + 0.044715f * a * a * a);
-    return a / (1.f + expf(-bend)) * b;
+    return activation == 0 ? gate_value<0>(a, b) : gate_value<1>(a, b);
 }
 
 // What a call's products are summed by and written as.

@@ -339,24 +339,40 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
     __builtin_amdgcn_s_waitcnt(wait_vm(0));
 
     if constexpr (!CODES) {
+        // Through LDS, so that what is stored together is rows' whole lines: stored from
+        // the accumulators, 32 bytes of a row each, a tile of 256 x 256 took 6 us for @.
         constexpr int N = GATED ? NB / 2 : NB;  // column blocks of the result a wavefront
+        typedef typename std::conditional<std::is_same<T, Half>::value, uint16_t, uint32_t>::type E;
+        constexpr int PITCH = BN * sizeof(E) + 16, PIECES = BN * sizeof(E) / 16, EACH = 16 / sizeof(E);
+        static_assert(BM * PITCH <= (int)sizeof lds, "the result fits in LDS");
+        __syncthreads();
 #pragma unroll
-        for (int m = 0; m < MB; ++m) {
-            const int row = m0 + (wm * MB + m) * 16 + c;
-            if (row >= p.M) continue;
+        for (int m = 0; m < MB; ++m)
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                float v[4];
+                E e[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = GATED ? gate_value(acc[n][m][i], acc[n + NB - N][m][i], p.activation) : acc[n][m][i];
-                const int64_t at = (int64_t)row * p.N;
-                const int col = n0 + (wn * N + n) * 16 + g * 4;
-                if constexpr (!std::is_same<T, Half>::value)
-                    store_row(static_cast<float*>(p.y) + at, col, p.N, v);
-                else if (p.bf16)
-                    store_row(static_cast<__bf16*>(p.y) + at, col, p.N, v);
-                else
-                    store_row(static_cast<_Float16*>(p.y) + at, col, p.N, v);
+                for (int i = 0; i < 4; ++i) {
+                    const float v = GATED ? gate_value(acc[n][m][i], acc[n + NB - N][m][i], p.activation) : acc[n][m][i];
+                    if constexpr (sizeof(E) == 4)
+                        e[i] = __float_as_uint(v);
+                    else
+                        e[i] = p.bf16 ? __builtin_bit_cast(uint16_t, (__bf16)v) : __builtin_bit_cast(uint16_t, (_Float16)v);
+                }
+                __builtin_memcpy(__builtin_assume_aligned(lds + ((wm * MB + m) * 16 + c) * PITCH + ((wn * N + n) * 16 + g * 4) * sizeof(E), 8), e, sizeof e);
+            }
+        __syncthreads();
+        for (int i = threadIdx.x; i < BM * PIECES; i += 64 * NW) {
+            const int row = m0 + i / PIECES, col = n0 + i % PIECES * EACH;
+            if (row >= p.M || col >= p.N) continue;
+            const E* from = reinterpret_cast<const E*>(lds + i / PIECES * PITCH) + i % PIECES * EACH;
+            E* to = static_cast<E*>(p.y) + (int64_t)row * p.N + col;
+            if (col + EACH <= p.N) {
+                E e[EACH];
+                __builtin_memcpy(e, __builtin_assume_aligned(from, 16), sizeof e);
+                __builtin_memcpy(to, e, sizeof e);
+            } else {
+                for (int j = 0; j < p.N - col; ++j) to[j] = from[j];
             }
         }
     } else {
@@ -366,18 +382,45 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
         float* top = reinterpret_cast<float*>(lds);                // [WN][BM]
         uint8_t* out = lds + WN * BM * 4;                          // [BM][144]
         __syncthreads();
+        auto values = [&](auto activation) __attribute__((always_inline)) {
+#pragma unroll
+            for (int m = 0; m < MB; ++m)
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        acc[n][m][i] = gate_value<decltype(activation)::value>(acc[n][m][i], acc[n + N][m][i]);
+        };
+        if (p.activation == 0)
+            values(std::integral_constant<int, 0>());
+        else
+            values(std::integral_constant<int, 1>());
+        if (n0 + 128 > p.N) {
+#pragma unroll
+            for (int m = 0; m < MB; ++m)
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (n0 + (wn * N + n) * 16 + g * 4 + i >= p.N) acc[n][m][i] = 0.f;
+        }
 #pragma unroll
         for (int m = 0; m < MB; ++m) {
-            float amax = 0.f;
+            float amax = 0.f;  // NaN has no part in it
 #pragma unroll
             for (int n = 0; n < N; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float v = gate_value(acc[n][m][i], acc[n + N][m][i], p.activation);
-                    if (n0 + (wn * N + n) * 16 + g * 4 + i >= p.N) v = 0.f;
-                    acc[n][m][i] = v;
-                    amax = fmaxf(amax, finite_magnitude(v));
-                }
+                for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(acc[n][m][i]));
+            if (__any(amax == INFINITY)) {  // infinities become NaN
+                amax = 0.f;
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (fabsf(acc[n][m][i]) == INFINITY) acc[n][m][i] = NAN;
+                        amax = fmaxf(amax, fabsf(acc[n][m][i]));
+                    }
+            }
             amax = column_max(amax);
             if (g == 0) top[wn * BM + (wm * MB + m) * 16 + c] = amax;
         }
@@ -392,8 +435,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
             const float inv = fp8_scale_inverse(byte);
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                const f32x4 v = acc[n][m] * inv;
-                *reinterpret_cast<uint32_t*>(out + r * 144 + (wn * N + n) * 16 + g * 4) = fp8_high(v[2], v[3], fp8_low(v[0], v[1]));
+                const f32x4 v = acc[n][m] * inv;  // 448 at most
+                const uint32_t low = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+                *reinterpret_cast<uint32_t*>(out + r * 144 + (wn * N + n) * 16 + g * 4) =
+                    (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], (int)low, true);
             }
             const int64_t blocks = fp8_blocks(p.N), per_row = fp8_scales(p.N);
             if (wn == 0 && m0 + r < p.M) {
