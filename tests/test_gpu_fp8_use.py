@@ -1,0 +1,263 @@
+"""The 8-bit chain as a program uses it: the operators one after the other, on
+streams of their own, in captured graphs that share weights, from several
+threads, and through the C interface between guard bytes.
+
+Tolerances of the chain, fixed before its first run: each product takes operands
+that are off by half a step of 8 bits (2^-4 of each value, 2^-10 of a block's scale
+for the smallest) against the chain in 64 bits that rounds at the same places;
+what differs there is which of two neighbouring codes a value next to their middle
+gets. An operator's own result differs from the 64-bit one by at most 2^-13 of a
+row's norm, so that at most about 2^-13 / 2^-4 = 2^-9 of the values change their
+code, by 2^-3 each: 2^-4.5 2^-3 < 2^-7 of the norm an operator, 2^-5 for three of
+them in a row with the final rounding.
+"""
+
+import ctypes
+import struct
+import threading
+
+import pytest
+import torch
+
+import trntensor_amd as tt
+from oracle import fp8 as ref
+from trntensor_amd.hip import _fastpath, _lib
+
+pytestmark = pytest.mark.gpu
+
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def _randn(shape, seed, dtype=torch.float32, size=1.0):
+    return (size * torch.randn(shape, generator=torch.Generator().manual_seed(seed))).to(dtype)
+
+
+def _matrix(n, k, seed, e8m0=True):
+    mat = tt.Fp8Matrix.quantize(_randn((n, k), seed, size=k ** -0.5).cuda())
+    if e8m0:
+        return mat
+    codes = (100.0 * _randn((n, k), seed)).clamp(-448.0, 448.0).to(E4M3)
+    scales = 0.01 * k ** -0.5 * (0.5 + torch.rand((-(-n // 128), -(-k // 128)), generator=torch.Generator().manual_seed(seed)))
+    return tt.Fp8Matrix(codes.cuda(), scales.cuda())
+
+
+def _feed_forward(x, y, w, layer):
+    """A pre-norm feed-forward block with the residual stream."""
+    h, x = tt.rms_norm(y, w, residual=x, fp8=True)
+    h = tt.fp8_gated_matmul(h, layer["gate"], layer["up"])
+    return tt.fp8_matmul(h, layer["down"]), x
+
+
+def _layer(hidden, mlp, seed):
+    return {"gate": _matrix(mlp, hidden, seed), "up": _matrix(mlp, hidden, seed + 1), "down": _matrix(hidden, mlp, seed + 2)}
+
+
+def _values(mat):
+    """The weights that a matrix stands for, through its products with the unit vectors."""
+    return tt.fp8_matmul(torch.eye(mat.shape[1]).cuda(), mat).t().cpu().double()
+
+
+@pytest.mark.parametrize("rows,hidden,mlp", [(1, 256, 640), (5, 192, 320), (70, 384, 1000), (300, 512, 768)])
+def test_chain_against_64_bits(hip, rows, hidden, mlp):
+    layer = _layer(hidden, mlp, 1)
+    x, y, w = _randn((rows, hidden), 4, torch.bfloat16), _randn((rows, hidden), 5, torch.bfloat16), 1 + 0.1 * _randn((hidden,), 6)
+    out, stream = _feed_forward(x.cuda(), y.cuda(), w.cuda(), layer)
+
+    def rounded(v):
+        codes, e = ref.quantize(v)
+        return codes * ref.spread(torch.exp2(e.double()), v.shape[1])
+
+    h, total = ref.rms_norm(y, w, x, 1e-6)
+    h = rounded(h)
+    h = rounded(ref.act(h @ _values(layer["gate"]).t(), "silu") * (h @ _values(layer["up"]).t()))
+    want = h @ _values(layer["down"]).t()
+    assert ((stream.cpu().double() - total).abs() <= 2.0 ** -8 * 1.01 * total.abs()).all()
+    assert (out.cpu().double() - want).norm() <= 2.0 ** -5 * want.norm()
+
+
+@pytest.mark.parametrize("fast", [True, False])
+def test_calls_give_the_same_with_and_without_the_host_path(hip, monkeypatch, fast):
+    if not fast:
+        monkeypatch.setattr(_fastpath, "rows_host", lambda: None)
+        monkeypatch.setattr(_fastpath, "module", lambda: None)
+    layer, floats = _layer(320, 500, 10), _matrix(77, 320, 13, e8m0=False)
+    for lead in ((), (3,), (2, 4), (0,), (2, 0, 3)):
+        x, y = (_randn((*lead, 320), s, torch.float16).cuda() for s in (14, 15))
+        w = _randn((320,), 16, torch.float32).cuda()
+        rows, total = tt.rms_norm(y, w, residual=x, fp8=True)
+        plain, total2 = tt.rms_norm(y, w, residual=x)
+        assert torch.equal(total, total2) and plain.shape == x.shape and rows.shape == x.shape
+        again = tt.fp8_quantize(y)
+        assert again.codes.shape == (*lead, 320) and again.scales.shape == (*lead, 3)
+        h = tt.fp8_gated_matmul(rows, layer["gate"], layer["up"], activation="gelu_tanh")
+        assert h.shape == (*lead, 500) and h.dtype == torch.float16
+        assert tt.fp8_gated_matmul(rows, layer["gate"], layer["up"], fp8=False).shape == (*lead, 500)
+        for z in (tt.fp8_matmul(h, layer["down"]), tt.fp8_matmul(rows, layer["up"], dtype=torch.float32)):
+            assert z.shape[:-1] == torch.Size(lead)
+        got = (rows._codes, rows._scales, total, plain, again._codes, h._codes, h._scales, tt.fp8_matmul(rows, floats))
+        expected = _EXPECTED.setdefault(lead, got)
+        for a, b in zip(got, expected):
+            assert torch.equal(a, b)
+
+
+_EXPECTED = {}
+
+
+def test_results_repeat_bit_for_bit_and_do_not_depend_on_earlier_calls(hip):
+    layer = _layer(1024, 1500, 20)
+    for rows in (1, 20, 100, 600):
+        x, y, w = _randn((rows, 1024), 21, torch.bfloat16).cuda(), _randn((rows, 1024), 22, torch.bfloat16).cuda(), torch.ones(1024).cuda()
+        first = _feed_forward(x, y, w, layer)
+        for _ in range(3):
+            _feed_forward(y, x, 2 * w, layer)
+            again = _feed_forward(x, y, w, layer)
+            assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+def test_streams_that_share_weights(hip):
+    """Calls on four streams at once, with no wait between them."""
+    layer = _layer(512, 900, 30)
+    inputs = [(_randn((m, 512), 31 + m, torch.bfloat16).cuda(), _randn((m, 512), 32 + m, torch.bfloat16).cuda()) for m in (1, 17, 130, 400)]
+    w = torch.ones(512).cuda()
+    want = [_feed_forward(x, y, w, layer) for x, y in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in inputs]
+    for _ in range(5):
+        got = []
+        for s, (x, y) in zip(streams, inputs):
+            with torch.cuda.stream(s):
+                got.append(_feed_forward(x, y, w, layer))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_two_graphs_that_share_weights(hip):
+    """Each captured with its own buffers, replayed in turn with eager calls between, and checked each time."""
+    layer = _layer(384, 700, 40)
+    w = torch.ones(384).cuda()
+    buffers, graphs, outs = [], [], []
+    for m in (2, 150):
+        x, y = torch.zeros((m, 384), dtype=torch.bfloat16, device="cuda"), torch.zeros((m, 384), dtype=torch.bfloat16, device="cuda")
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _feed_forward(x, y, w, layer)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(_feed_forward(x, y, w, layer))
+        buffers.append((x, y))
+        graphs.append(graph)
+    for step in range(4):
+        for i in (step % 2, 1 - step % 2):
+            x, y = buffers[i]
+            x.copy_(_randn(x.shape, 41 + step, torch.bfloat16))
+            y.copy_(_randn(x.shape, 51 + step, torch.bfloat16))
+            graphs[i].replay()
+            want = _feed_forward(x, y, w, layer)
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i][0], want[0]) and torch.equal(outs[i][1], want[1])
+
+
+def test_threads_that_share_weights(hip):
+    layer = _layer(256, 400, 60)
+    w = torch.ones(256).cuda()
+    inputs = [(_randn((m, 256), 61 + m, torch.bfloat16).cuda(), _randn((m, 256), 62 + m, torch.bfloat16).cuda()) for m in (1, 33, 257)]
+    want = [_feed_forward(x, y, w, layer) for x, y in inputs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = _feed_forward(*inputs[i], w, layer)
+                torch.cuda.current_stream().synchronize()
+                if not (torch.equal(got[0], want[i][0]) and torch.equal(got[1], want[i][1])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(inputs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_operands_are_not_written(hip):
+    layer = _layer(300, 420, 70)
+    for m in (3, 260):
+        x, y = _randn((m, 300), 71, torch.float16).cuda(), _randn((m, 300), 72, torch.float16).cuda()
+        rows = tt.fp8_quantize(x)
+        before = [t.clone() for t in (x, y, rows._codes, rows._scales, layer["gate"]._packed, layer["gate"]._scales)]
+        tt.rms_norm(x, residual=y, fp8=True)
+        tt.fp8_gated_matmul(rows, layer["gate"], layer["up"])
+        tt.fp8_matmul(rows, layer["gate"])
+        for a, b in zip(before, (x, y, rows._codes, rows._scales, layer["gate"]._packed, layer["gate"]._scales)):
+            assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------
+# the C interface: nothing outside a result is written
+# ---------------------------------------------------------------------------
+class _Guarded:
+    """`size` bytes on the device with 4 KiB of 0xA5 on either side."""
+
+    def __init__(self, size):
+        self.all = torch.full((size + 8192,), 0xA5, dtype=torch.uint8, device="cuda")
+        self.size = size
+
+    @property
+    def ptr(self):
+        return self.all.data_ptr() + 4096
+
+    def check(self):
+        assert (self.all[:4096] == 0xA5).all() and (self.all[4096 + self.size:] == 0xA5).all()
+        return self.all[4096: 4096 + self.size]
+
+
+def _call(name, fmt, *fields):
+    lib = _lib.load()
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    status = getattr(lib, name)(struct.pack(fmt, *fields), stream)
+    assert status == 0, lib.tt_last_error()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (3, 130, 257), (17, 200, 128), (100, 257, 300), (300, 129, 700), (513, 1030, 200), (4100, 4110, 129)])
+@pytest.mark.parametrize("e8m0", [True, False])
+def test_c_calls_stay_in_their_results(hip, m, n, k, e8m0):
+    gate, up = _matrix(n, k, 80, e8m0), _matrix(n, k, 81, e8m0)
+    x = _randn((m, k), 82, torch.bfloat16).cuda()
+    width, per_row = -(-k // 128) * 128, -(-(-(-k // 128)) // 4) * 4
+    codes, scales = _Guarded(m * width), _Guarded(m * per_row)
+    _call("tt_fp8_quantize", "=7q", _lib.TT_BF16, m, k, k, x.data_ptr(), codes.ptr, scales.ptr)
+    rows = tt.fp8_quantize(x)
+    assert torch.equal(codes.check().view(m, width), rows._codes) and torch.equal(scales.check().view(m, per_row), rows._scales)
+    total, codes2, scales2 = _Guarded(m * k * 2), _Guarded(m * width), _Guarded(m * per_row)
+    _call("tt_rms_norm", "=6qd7q", _lib.TT_BF16, 0, m, k, k, k, 1e-6, x.data_ptr(), x.data_ptr(), 0, total.ptr, 0, codes2.ptr, scales2.ptr)
+    normed, h = tt.rms_norm(x, residual=x, fp8=True)
+    assert torch.equal(codes2.check().view(m, width), normed._codes) and torch.equal(scales2.check().view(m, per_row), normed._scales)
+    assert torch.equal(total.check().view(torch.bfloat16).view(m, k), h)
+    plain = _Guarded(m * k * 2)
+    _call("tt_rms_norm", "=6qd7q", _lib.TT_BF16, 0, m, k, k, 0, 1e-6, x.data_ptr(), 0, 0, 0, plain.ptr, 0, 0)
+    assert torch.equal(plain.check().view(torch.bfloat16).view(m, k), tt.rms_norm(x))
+    kind = _lib.TT_E8M0 if e8m0 else _lib.TT_F32
+    for dtype, code in ((torch.bfloat16, _lib.TT_BF16), (torch.float16, _lib.TT_F16), (torch.float32, _lib.TT_F32)):
+        y = _Guarded(m * n * dtype.itemsize)
+        _call("tt_fp8_matmul", "=10q", code, kind, m, n, k, rows._codes.data_ptr(), rows._scales.data_ptr(), gate._packed.data_ptr(),
+              gate._scales.data_ptr(), y.ptr)
+        assert torch.equal(y.check().view(dtype).view(m, n), tt.fp8_matmul(rows, gate, dtype=dtype))
+        y = _Guarded(m * n * dtype.itemsize)
+        head = (code, kind, 0, m, n, k, rows._codes.data_ptr(), rows._scales.data_ptr(), gate._packed.data_ptr(), gate._scales.data_ptr(),
+                up._packed.data_ptr(), up._scales.data_ptr())
+        _call("tt_fp8_gated_matmul", "=17q", *head, y.ptr, 0, 0, 0, 0)
+        want = tt.fp8_gated_matmul(tt.Fp8Rows(rows.codes, rows.scales, dtype), gate, up, fp8=False)
+        assert torch.equal(y.check().view(dtype).view(m, n), want)
+    width, per_row = -(-n // 128) * 128, -(-(-(-n // 128)) // 4) * 4
+    codes, scales = _Guarded(m * width), _Guarded(m * per_row)
+    query = struct.pack("=17q", *head, 0, codes.ptr, scales.ptr, 0, 0)
+    room = _Guarded(_lib.load().tt_fp8_gated_workspace_bytes(query))
+    _call("tt_fp8_gated_matmul", "=17q", *head, 0, codes.ptr, scales.ptr, room.ptr, room.size)
+    room.check()
+    want = tt.fp8_gated_matmul(rows, gate, up)
+    assert torch.equal(codes.check().view(m, width), want._codes) and torch.equal(scales.check().view(m, per_row), want._scales)
