@@ -1,11 +1,12 @@
-"""A small decoder with 4-bit weights and a paged 8-bit cache, answering several
-prompts at once: one ragged pass over the prompts, then one token of every
+"""A small decoder with 4-bit or 8-bit weights and a paged 8-bit cache, answering
+several prompts at once: one ragged pass over the prompts, then one token of every
 sequence at a time, the step captured in a HIP graph.
 
-    python examples/decode.py [--layers 4] [--batch 8] [--prompt 500] [--tokens 64]
+    python examples/decode.py [--layers 4] [--batch 8] [--prompt 500] [--tokens 64] [--fp8]
 
 Weights are random: what it shows is how q4_matmul, kv_append and kv_attention
-run together, and what a step costs.
+run together or, with --fp8, rms_norm, fp8_matmul and fp8_gated_matmul around the
+same cache, and what a step costs.
 """
 
 import argparse
@@ -29,26 +30,41 @@ def random_q4(out_features: int, in_features: int, group: int, g: torch.Generato
     return tt.Q4Matrix(codes.cuda(), scales.to(torch.bfloat16).cuda(), in_features, group)
 
 
+def random_fp8(out_features: int, in_features: int, g: torch.Generator) -> tt.Fp8Matrix:
+    """Random weights that keep their operand's size, in 8 bits."""
+    return tt.Fp8Matrix.quantize(torch.randn((out_features, in_features), generator=g).cuda() / math.sqrt(in_features))
+
+
 class Decoder:
-    """Pre-norm layers of grouped-query attention and a gated MLP."""
+    """Pre-norm layers of grouped-query attention and a gated MLP, with weights in 4 bits or, with fp8, in 8."""
 
     def __init__(self, layers=4, hidden=1024, q_heads=8, kv_heads=2, head_dim=128, mlp=2816, vocab=4096, group=128,
-                 max_tokens=2048, pages=512, page_size=64, seed=0):
+                 max_tokens=2048, pages=512, page_size=64, seed=0, fp8=False):
         g = torch.Generator().manual_seed(seed)
         self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
         self.page_size = page_size
         self.embed = torch.randn((vocab, hidden), generator=g).to(torch.bfloat16).cuda()
         width = (q_heads + 2 * kv_heads) * head_dim
-        self.layers = [{"qkv": random_q4(width, hidden, group, g), "out": random_q4(hidden, q_heads * head_dim, group, g),
-                        "up": random_q4(2 * mlp, hidden, group, g), "down": random_q4(hidden, mlp, group, g),
-                        "cache": tt.KVCache.empty(pages, kv_heads, head_dim, page_size)} for _ in range(layers)]
-        self.head = random_q4(vocab, hidden, group, g)
+        self.fp8 = fp8
+        if fp8:
+            self.layers = [{"qkv": random_fp8(width, hidden, g), "out": random_fp8(hidden, q_heads * head_dim, g),
+                            "gate": random_fp8(mlp, hidden, g), "up": random_fp8(mlp, hidden, g),
+                            "down": random_fp8(hidden, mlp, g),
+                            "cache": tt.KVCache.empty(pages, kv_heads, head_dim, page_size)} for _ in range(layers)]
+            self.head = random_fp8(vocab, hidden, g)
+        else:
+            self.layers = [{"qkv": random_q4(width, hidden, group, g), "out": random_q4(hidden, q_heads * head_dim, group, g),
+                            "up": random_q4(2 * mlp, hidden, group, g), "down": random_q4(hidden, mlp, group, g),
+                            "cache": tt.KVCache.empty(pages, kv_heads, head_dim, page_size)} for _ in range(layers)]
+            self.head = random_q4(vocab, hidden, group, g)
         angles = torch.arange(max_tokens)[:, None] * 10000.0 ** (-torch.arange(0, head_dim, 2) / head_dim)
         self.cos, self.sin = torch.cos(angles).float().cuda(), torch.sin(angles).float().cuda()
 
     def forward(self, tokens, table, held, total, counts=None):
         """Hidden states (batch, T, hidden) of T new tokens of every sequence, of
         which counts count; `held` and `total` are the lengths before and after."""
+        if self.fp8:
+            return self.forward8(tokens, table, held, total, counts)
         B, T = tokens.shape
         HQ, H, D = self.q_heads, self.kv_heads, self.head_dim
         x = self.embed[tokens]
@@ -63,9 +79,28 @@ class Decoder:
             x = x + tt.q4_matmul(F.silu(gate) * up, layer["down"])
         return F.rms_norm(x, norm)
 
+    def forward8(self, tokens, table, held, total, counts=None):
+        """The same with weights in 8 bits: activations are in 8 bits wherever a product
+        reads them, and each norm adds what came before it to the residual stream."""
+        B, T = tokens.shape
+        HQ, H, D = self.q_heads, self.kv_heads, self.head_dim
+        x = self.embed[tokens]
+        h = tt.rms_norm(x, fp8=True)
+        for i, layer in enumerate(self.layers):
+            if i:
+                h, x = tt.rms_norm(y, residual=x, fp8=True)
+            qkv = tt.fp8_matmul(h, layer["qkv"]).view(B, T, HQ + 2 * H, D)
+            q, k, v = qkv.split([HQ, H, H], dim=2)
+            q = tt.kv_append(layer["cache"], k, v, table, held, counts=counts, q=q, cos=self.cos, sin=self.sin)
+            o = tt.kv_attention(q, layer["cache"], table, total, counts=counts)
+            y = tt.fp8_matmul(o.flatten(2), layer["out"])
+            h, x = tt.rms_norm(y, residual=x, fp8=True)
+            y = tt.fp8_matmul(tt.fp8_gated_matmul(h, layer["gate"], layer["up"]), layer["down"])
+        return tt.rms_norm(y, residual=x)[0]
+
     def next_token(self, x):
         """The likeliest next token after hidden states (batch, hidden)."""
-        return tt.q4_matmul(x, self.head).argmax(-1)
+        return (tt.fp8_matmul if self.fp8 else tt.q4_matmul)(x, self.head).argmax(-1)
 
 
 @torch.no_grad()
@@ -116,9 +151,10 @@ def main():
     a = argparse.ArgumentParser()
     for name, value in (("layers", 4), ("batch", 8), ("prompt", 500), ("tokens", 64)):
         a.add_argument(f"--{name}", type=int, default=value)
+    a.add_argument("--fp8", action="store_true", help="8-bit weights and activations")
     a = a.parse_args()
     model = Decoder(layers=a.layers, max_tokens=(a.prompt + a.tokens + 64) // 64 * 64,
-                    pages=a.batch * ((a.prompt + a.tokens) // 64 + 1))
+                    pages=a.batch * ((a.prompt + a.tokens) // 64 + 1), fp8=a.fp8)
     g = torch.Generator().manual_seed(1)
     prompts = [torch.randint(0, 4096, (max(1, a.prompt - 37 * i % a.prompt),), generator=g) for i in range(a.batch)]
     eager, slow = answer(model, prompts, a.tokens, graph=False)
