@@ -114,7 +114,8 @@ def test_product_checks(no_gpu):
 
 
 def test_fixed_attributes():
-    rows = tt.Fp8Rows._of((2, 3), torch.float32, torch.zeros((2, 128), dtype=torch.uint8), torch.zeros((2, 4), dtype=torch.uint8))
+    rows = tt.Fp8Rows._of((2, 3), torch.float32, torch.zeros((2, 128), dtype=torch.uint8).view(E4M3),
+                          torch.zeros((2, 4), dtype=torch.uint8).view(E8M0))
     with pytest.raises(AttributeError, match="fixed"):
         rows.dtype = torch.float16
     with pytest.raises(AttributeError):

@@ -53,11 +53,15 @@ def _values(rows):
     return codes, scales, codes * ref.spread(scales, k)
 
 
+def _bytes(t):
+    return t.view(torch.uint8)
+
+
 def _check_padding(rows):
     """What lies past the features and blocks is zeros: the products read it."""
     k = rows.shape[-1]
-    assert not rows._codes[:, k:].any()
-    assert not rows._scales[:, -(-k // 128):].any()
+    assert not _bytes(rows._codes)[:, k:].any()
+    assert not _bytes(rows._scales)[:, -(-k // 128):].any()
 
 
 def _check_quantized(x, rows):
@@ -135,12 +139,12 @@ def test_quantize_strides_shapes_and_host(hip):
     assert host.device.type == "cuda"
     _check_quantized(wide[:, 0, :192].cpu(), host)
     rows = tt.Fp8Rows(host.codes, host.scales, dtype=torch.float32)
-    assert torch.equal(rows._codes, host._codes) and torch.equal(rows._scales, host._scales) and rows.dtype == torch.float32
+    assert torch.equal(_bytes(rows._codes), _bytes(host._codes)) and torch.equal(_bytes(rows._scales), _bytes(host._scales)) and rows.dtype == torch.float32
     _, _, values = _values(host)
     assert torch.equal(rows.dequantize().cpu().double(), values)
     one = tt.fp8_quantize(wide[0, 0, :130])
     rows = tt.Fp8Rows(one.codes.cpu(), one.scales.cpu())
-    assert rows.shape == (130,) and torch.equal(rows._codes, one._codes) and torch.equal(rows._scales, one._scales)
+    assert rows.shape == (130,) and torch.equal(_bytes(rows._codes), _bytes(one._codes)) and torch.equal(_bytes(rows._scales), _bytes(one._scales))
 
 
 # ---------------------------------------------------------------------------
@@ -334,7 +338,7 @@ def test_matmul_nan_stays_in_its_row(hip, m, e8m0):
     rows, x = _rows8(m, k, 5)
     mat, w = _weights8(n, k, 6, e8m0)
     clean = tt.fp8_matmul(rows, mat)
-    rows._codes[m // 2, 170] = 0x7F
+    _bytes(rows._codes)[m // 2, 170] = 0x7F
     y = tt.fp8_matmul(rows, mat)
     assert y[m // 2].isnan().all()
     keep = torch.arange(m) != m // 2

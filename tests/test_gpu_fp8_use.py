@@ -32,6 +32,10 @@ def _randn(shape, seed, dtype=torch.float32, size=1.0):
     return (size * torch.randn(shape, generator=torch.Generator().manual_seed(seed))).to(dtype)
 
 
+def _bytes(t):
+    return t.view(torch.uint8)
+
+
 def _matrix(n, k, seed, e8m0=True):
     mat = tt.Fp8Matrix.quantize(_randn((n, k), seed, size=k ** -0.5).cuda())
     if e8m0:
@@ -94,7 +98,7 @@ def test_calls_give_the_same_with_and_without_the_host_path(hip, monkeypatch, fa
         assert tt.fp8_gated_matmul(rows, layer["gate"], layer["up"], fp8=False).shape == (*lead, 500)
         for z in (tt.fp8_matmul(h, layer["down"]), tt.fp8_matmul(rows, layer["up"], dtype=torch.float32)):
             assert z.shape[:-1] == torch.Size(lead)
-        got = (rows._codes, rows._scales, total, plain, again._codes, h._codes, h._scales, tt.fp8_matmul(rows, floats))
+        got = (_bytes(rows._codes), _bytes(rows._scales), total, plain, _bytes(again._codes), _bytes(h._codes), _bytes(h._scales), tt.fp8_matmul(rows, floats))
         expected = _EXPECTED.setdefault(lead, got)
         for a, b in zip(got, expected):
             assert torch.equal(a, b)
@@ -189,11 +193,11 @@ def test_operands_are_not_written(hip):
     for m in (3, 260):
         x, y = _randn((m, 300), 71, torch.float16).cuda(), _randn((m, 300), 72, torch.float16).cuda()
         rows = tt.fp8_quantize(x)
-        before = [t.clone() for t in (x, y, rows._codes, rows._scales, layer["gate"]._packed, layer["gate"]._scales)]
+        before = [t.clone() for t in (x, y, _bytes(rows._codes), _bytes(rows._scales), layer["gate"]._packed, layer["gate"]._scales)]
         tt.rms_norm(x, residual=y, fp8=True)
         tt.fp8_gated_matmul(rows, layer["gate"], layer["up"])
         tt.fp8_matmul(rows, layer["gate"])
-        for a, b in zip(before, (x, y, rows._codes, rows._scales, layer["gate"]._packed, layer["gate"]._scales)):
+        for a, b in zip(before, (x, y, _bytes(rows._codes), _bytes(rows._scales), layer["gate"]._packed, layer["gate"]._scales)):
             assert torch.equal(a, b)
 
 
@@ -232,11 +236,11 @@ def test_c_calls_stay_in_their_results(hip, m, n, k, e8m0):
     codes, scales = _Guarded(m * width), _Guarded(m * per_row)
     _call("tt_fp8_quantize", "=7q", _lib.TT_BF16, m, k, k, x.data_ptr(), codes.ptr, scales.ptr)
     rows = tt.fp8_quantize(x)
-    assert torch.equal(codes.check().view(m, width), rows._codes) and torch.equal(scales.check().view(m, per_row), rows._scales)
+    assert torch.equal(codes.check().view(m, width), _bytes(rows._codes)) and torch.equal(scales.check().view(m, per_row), _bytes(rows._scales))
     total, codes2, scales2 = _Guarded(m * k * 2), _Guarded(m * width), _Guarded(m * per_row)
     _call("tt_rms_norm", "=6qd7q", _lib.TT_BF16, 0, m, k, k, k, 1e-6, x.data_ptr(), x.data_ptr(), 0, total.ptr, 0, codes2.ptr, scales2.ptr)
     normed, h = tt.rms_norm(x, residual=x, fp8=True)
-    assert torch.equal(codes2.check().view(m, width), normed._codes) and torch.equal(scales2.check().view(m, per_row), normed._scales)
+    assert torch.equal(codes2.check().view(m, width), _bytes(normed._codes)) and torch.equal(scales2.check().view(m, per_row), _bytes(normed._scales))
     assert torch.equal(total.check().view(torch.bfloat16).view(m, k), h)
     plain = _Guarded(m * k * 2)
     _call("tt_rms_norm", "=6qd7q", _lib.TT_BF16, 0, m, k, k, 0, 1e-6, x.data_ptr(), 0, 0, 0, plain.ptr, 0, 0)
@@ -260,4 +264,4 @@ def test_c_calls_stay_in_their_results(hip, m, n, k, e8m0):
     _call("tt_fp8_gated_matmul", "=17q", *head, 0, codes.ptr, scales.ptr, room.ptr, room.size)
     room.check()
     want = tt.fp8_gated_matmul(rows, gate, up)
-    assert torch.equal(codes.check().view(m, width), want._codes) and torch.equal(scales.check().view(m, per_row), want._scales)
+    assert torch.equal(codes.check().view(m, width), _bytes(want._codes)) and torch.equal(scales.check().view(m, per_row), _bytes(want._scales))

@@ -281,8 +281,8 @@ struct Rows8 {
 
     Rows8(const Place& at, int64_t rows, int64_t dim) {
         const int64_t blocks = (dim + 127) / 128;
-        codes = at.empty({rows, blocks * 128}, at::kByte);
-        scales = at.empty({rows, (blocks + 3) / 4 * 4}, at::kByte);
+        codes = at.empty({rows, blocks * 128}, at::kFloat8_e4m3fn);
+        scales = at.empty({rows, (blocks + 3) / 4 * 4}, at::kFloat8_e8m0fnu);
     }
 };
 

@@ -64,13 +64,13 @@ def _rows(t: torch.Tensor, device: torch.device) -> torch.Tensor:
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _shaped(t: torch.Tensor, lead, last: int) -> torch.Tensor:
+def _shaped(t: torch.Tensor, shape, last: int) -> torch.Tensor:
     """Two-dimensional rows, of which `last` elements count, in their own shape."""
     if t.shape[1] != last:
-        t = t[:, :last]
-    if len(lead) == 1:
+        t = t.narrow(1, 0, last)
+    if len(shape) == 2:
         return t
-    return t.unflatten(0, lead) if lead else t[0]
+    return t.unflatten(0, shape[:-1]) if len(shape) > 2 else t[0]
 
 
 class Fp8Rows(_Fixed):
@@ -100,8 +100,8 @@ class Fp8Rows(_Fixed):
         device = _home("Fp8Rows", codes, scales)
         self._set(codes.shape, dtype, *_room(codes.shape, device, torch.zeros))
         features = codes.shape[-1]
-        self._codes[:, :features] = codes.to(device).view(torch.uint8).reshape(-1, features)
-        self._scales[:, : want[-1]] = scales.to(device).view(torch.uint8).reshape(-1, want[-1])
+        self._codes.view(torch.uint8)[:, :features] = codes.to(device).view(torch.uint8).reshape(-1, features)
+        self._scales.view(torch.uint8)[:, : want[-1]] = scales.to(device).view(torch.uint8).reshape(-1, want[-1])
 
     def _set(self, shape, dtype, codes, scales):
         put = object.__setattr__
@@ -120,12 +120,12 @@ class Fp8Rows(_Fixed):
     @property
     def codes(self) -> torch.Tensor:
         """float8_e4m3fn (..., features); rows start every multiple of 128 codes."""
-        return _shaped(self._codes.view(FP8), self.shape[:-1], self.shape[-1])
+        return _shaped(self._codes, self.shape, self.shape[-1])
 
     @property
     def scales(self) -> torch.Tensor:
         """float8_e8m0fnu (..., ceil(features / 128)); rows start every multiple of 4 scales."""
-        return _shaped(self._scales.view(E8M0), self.shape[:-1], _blocks(self.shape[-1]))
+        return _shaped(self._scales, self.shape, _blocks(self.shape[-1]))
 
     def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         """The rows' values, in ``dtype`` (the rows' one if None)."""
@@ -139,8 +139,8 @@ class Fp8Rows(_Fixed):
 def _room(shape, device: torch.device, make=torch.empty):
     """Codes and scales of rows of this shape as the kernels lay them out."""
     count, blocks = math.prod(shape[:-1]), _blocks(shape[-1])
-    return (make((count, blocks * BLOCK), dtype=torch.uint8, device=device),
-            make((count, -(-blocks // 4) * 4), dtype=torch.uint8, device=device))
+    return (make((count, blocks * BLOCK), dtype=torch.uint8, device=device).view(FP8),
+            make((count, -(-blocks // 4) * 4), dtype=torch.uint8, device=device).view(E8M0))
 
 
 class Fp8Matrix(_Fixed):
