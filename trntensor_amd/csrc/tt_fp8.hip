@@ -148,7 +148,11 @@ double rows_cost(const Fp8Params& p, bool gated) {
 // Offsets within a tile's rows are of 32 bits.
 bool tiles_can(const Fp8Params& p) { return p.K <= 1 << 23; }
 
-constexpr double kLaunch = 3.0;  // us of another launch
+// us that a second launch and the float32 values between the two take: tiles that
+// write codes / a second launch, M x N x K: 4 x 2816 x 1024 8.2 / 11.5, 100 x 2816
+// x 2048 11.0 / 11.6, 500 x 2816 x 2048 15.3 / 18.9, 128 x 12288 x 4096 32.8 / 35.5,
+// but 16 x 12288 x 4096 28.3 / 25.8, 183 x 2176 x 5888 24.3 / 20.8.
+constexpr double kLaunch = 7.0;
 
 // How a gated call into 8 bits goes: on tiles that write codes, or as 32-bit
 // products (on other tiles, or on few rows' workgroups) that a second launch rounds.
@@ -296,12 +300,10 @@ extern "C" int tt_fp8_gated_matmul(const tt_fp8_gated_args* a, void* stream) {
     const GatedPlan plan = gated_plan(p, kind);
     p.y = a->codes ? a->workspace : a->y;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (a->codes && !plan.fused && fp8_quantize_grid(a->M, a->N) > kMaxGrid)
+    if (a->codes && !plan.fused && a->M * ((a->N + 2047) / 2048) > kMaxGrid)
         return set_error(TT_UNSUPPORTED, "%s: %lld rows of %lld", who, (long long)a->M, (long long)a->N);
     if (plan.fused) return fp8_gated_tiles(kCodes, e8, plan.which, p, st);
     const int first = a->codes ? kRaw : kind;
     if (int rc = plan.tiles ? fp8_gated_tiles(first, e8, plan.which, p, st) : rows<true>(first, e8, p, st)) return rc;
-    if (!a->codes) return TT_OK;
-    const tt_fp8_quantize_args q = {TT_F32, a->M, a->N, a->N, a->workspace, a->codes, a->scales};
-    return tt_fp8_quantize(&q, stream);
+    return a->codes ? fp8_gated_round(e8, p, st) : TT_OK;
 }

@@ -54,8 +54,8 @@ __device__ __forceinline__ float max_of_16(float x) {
 }
 
 // A value already divided by its block's scale, for the conversion: finite ones
-// are at most 448, infinities become NaN (the format has none).
-__device__ __forceinline__ float fp8_operand(float x) { return fabsf(x) <= kFp8Max ? x : NAN; }
+// are at most 448 (or round to it), infinities become NaN (the format has none).
+__device__ __forceinline__ float fp8_operand(float x) { return fabsf(x) < INFINITY ? x : NAN; }
 
 // Two floats as codes in the low or the high half of `old`.
 __device__ __forceinline__ uint32_t fp8_low(float a, float b) {
@@ -69,11 +69,9 @@ __device__ __forceinline__ uint32_t fp8_high(float a, float b, uint32_t old) {
 // from the first of the 16 lanes that hold a block, its scale (and zeros past the
 // last one). All lanes of a block call it, values past dim are zeros; `blocks` is
 // fp8_blocks(dim).
-__device__ __forceinline__ void fp8_store8(const float (&v)[8], int64_t col, int64_t blocks, uint8_t* codes, uint8_t* scales) {
-    float amax = finite_magnitude(v[0]);
-#pragma unroll
-    for (int i = 1; i < 8; ++i) amax = fmaxf(amax, finite_magnitude(v[i]));
-    const uint32_t byte = fp8_scale_byte(max_of_16(amax));
+// `amax` is the block's largest magnitude.
+__device__ __forceinline__ void fp8_store8(const float (&v)[8], float amax, int64_t col, int64_t blocks, uint8_t* codes, uint8_t* scales) {
+    const uint32_t byte = fp8_scale_byte(amax);
     const float inv = fp8_scale_inverse(byte);
     if (col < blocks * 128) {
         u32x2 w;
@@ -87,6 +85,13 @@ __device__ __forceinline__ void fp8_store8(const float (&v)[8], int64_t col, int
         if (col / 128 == blocks - 1)
             for (int64_t past = blocks; past < (blocks + 3) / 4 * 4; ++past) scales[past] = 0;
     }
+}
+
+__device__ __forceinline__ void fp8_store8(const float (&v)[8], int64_t col, int64_t blocks, uint8_t* codes, uint8_t* scales) {
+    float amax = finite_magnitude(v[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) amax = fmaxf(amax, finite_magnitude(v[i]));
+    fp8_store8(v, max_of_16(amax), col, blocks, codes, scales);
 }
 
 // Eight elements of a row from column `col` on, zeros from `dim` on, as loaded:

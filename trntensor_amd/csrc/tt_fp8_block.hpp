@@ -51,7 +51,10 @@ struct Block {
     }
 };
 
-__device__ __forceinline__ float e8m0_value(uint32_t byte) { return byte ? __uint_as_float(byte << 23) : 0x1p-127f; }
+// 2^(byte - 127); byte 255 is NaN.
+__device__ __forceinline__ float e8m0_value(uint32_t byte) {
+    return __uint_as_float(byte == 0 ? 0x400000u : byte == 255 ? 0x7fc00000u : byte << 23);
+}
 
 // The sum of a block of 128 columns with the scales of x's rows alone.
 template <bool EXACT, bool E8>
@@ -88,7 +91,8 @@ __device__ __forceinline__ uint32_t weight_scale(const Fp8Params& p, int r, int 
 // act(a) b: both activations are a / (1 + exp(-bend)), since (1 + tanh(z)) / 2 is 1 /
 // (1 + exp(-2 z)). The hardware's exponential (of base 2) and reciprocal err by a
 // unit each, which costs nothing next to the products' sums; with a full division
-// and exponential a tile of 256 x 128 values took 14 us for @ beside its products.
+// and exponential a round of tiles of 256 x 128 values took 14.2 us, with these 10.6
+// (2048 x 16384 from one block of columns, four rounds: 56.6 and 42.6 us).
 template <int ACTIVATION>
 __device__ __forceinline__ float gate_value(float a, float b) {
     const float bend = ACTIVATION == 0 ? a : 1.5957691216f * (a + 0.044715f * a * a * a);
@@ -97,6 +101,61 @@ __device__ __forceinline__ float gate_value(float a, float b) {
 __device__ __forceinline__ float gate_value(float a, float b, int activation) {
     return activation == 0 ? gate_value<0>(a, b) : gate_value<1>(a, b);
 }
+
+// A wavefront's part of a gated block's two products for one row and column, in 32
+// bits: 16 columns of the operands a lane, from lane number `first` of `lanes` on. The
+// sum of a wavefront's parts is in every lane.
+template <bool E8, int UNROLL>
+__device__ __forceinline__ void exact_parts(const Fp8Params& p, int row, int col, int first, int lanes, float (&sum)[2]) {
+    const uint8_t* x = p.x + (int64_t)row * p.blocks * 128;
+    const uint8_t* xs = p.xs + (int64_t)row * p.x_scales;
+    const int64_t tile = (int64_t)(col / 16) * p.blocks * 2048 + col % 16 * 16;
+    sum[0] = sum[1] = 0.f;
+#pragma unroll UNROLL
+    for (int piece = first; piece < p.blocks * 8; piece += lanes) {
+        const int k = piece / 8, q = piece % 8;
+        const u32x4 a = *reinterpret_cast<const u32x4*>(x + (int64_t)k * 128 + q * 16);
+        const float scale = e8m0_value(xs[k]);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const u32x4 b = *reinterpret_cast<const u32x4*>(p.w[w] + tile + (int64_t)k * 2048 + q / 4 * 1024 + q % 4 * 256);
+            const float ws = E8 ? e8m0_value(p.ws[w][(int64_t)(col / 128) * p.x_scales + k])
+                                : reinterpret_cast<const float*>(p.ws[w])[(int64_t)(col / 128) * p.blocks + k];
+            float part = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int ca = (int)a[i], cb = (int)b[i];
+                part = __builtin_fmaf(__builtin_amdgcn_cvt_f32_fp8(ca, 0), __builtin_amdgcn_cvt_f32_fp8(cb, 0), part);
+                part = __builtin_fmaf(__builtin_amdgcn_cvt_f32_fp8(ca, 1), __builtin_amdgcn_cvt_f32_fp8(cb, 1), part);
+                part = __builtin_fmaf(__builtin_amdgcn_cvt_f32_fp8(ca, 2), __builtin_amdgcn_cvt_f32_fp8(cb, 2), part);
+                part = __builtin_fmaf(__builtin_amdgcn_cvt_f32_fp8(ca, 3), __builtin_amdgcn_cvt_f32_fp8(cb, 3), part);
+            }
+            sum[w] += part * (scale * ws);
+        }
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        sum[0] += __shfl_xor(sum[0], off, kWave);
+        sum[1] += __shfl_xor(sum[1], off, kWave);
+    }
+}
+
+// The block's value there as a magnitude; 0 where it is not finite.
+__device__ __forceinline__ float exact_gated(const float (&sum)[2], int activation) {
+    return finite_magnitude(gate_value(sum[0], sum[1], activation));
+}
+
+// Values of the 8-bit matrix instructions are about 2^-16 of a sum off, which decides
+// a block's scale where its largest value is next to 448 times a power of two:
+// where it is within 2^-12 of that (one block in 1500), those of the block's values
+// that come within 2^-11 of the largest are computed again in 32 bits, so that
+// scales are those of 32-bit sums. A workgroup of tiles takes about 2 us longer
+// for it (5 to 6 with a wavefront a value instead of all of them).
+__device__ __forceinline__ bool near_border(float amax) {
+    const int off = (int)(__float_as_uint(amax) & 0x7fffffu) - 0x600000;
+    return off <= 3584 && off >= -3584 && amax >= 0x1p-100f;
+}
+constexpr float kCandidate = 1.f - 0x1p-11f;
 
 // What a call's products are summed by and written as.
 enum { kHalf, kExact, kRaw, kCodes };
@@ -107,5 +166,7 @@ double fp8_tiles_cost(const Fp8Params& p, bool exact, int* which);
 int fp8_tiles(bool exact, bool e8, int which, const Fp8Params& p, hipStream_t st);
 double fp8_gated_tiles_cost(const Fp8Params& p, int kind, int* which);
 int fp8_gated_tiles(int kind, bool e8, int which, const Fp8Params& p, hipStream_t st);
+// What kRaw wrote to y, into codes and scales.
+int fp8_gated_round(bool e8, const Fp8Params& p, hipStream_t st);
 
 }  // namespace tt

@@ -25,10 +25,12 @@ __device__ __forceinline__ float wave_sum32(float v) {
     return v;
 }
 
-// W: float, or __bf16 for weights of either 16-bit type. LANES lanes a row (a wavefront, or the workgroup), eight elements of it a pass.
-// Up to PASSES passes stay in registers: rows are read once, all loads of a row in
-// flight, and 8192 rows of 8192 with the residual stream take 90 us where a
-// copy of as many bytes takes 92. Longer rows (PASSES 0) are read again, from L2.
+// W: float, or __bf16 for weights of either 16-bit type. LANES lanes a row (a
+// wavefront, or the workgroup), eight elements of it a pass. HBM bounds it: up to
+// PASSES passes stay in registers, so that rows are read once, all loads of a row
+// in flight, and 8192 rows of 8192 with the residual stream take 87 us where a copy
+// of as many bytes takes 92. Longer rows (PASSES 0) are read again, from L2. Rows of
+// up to 1024 take a wavefront: 500 of 1007 4.7 us, with a workgroup each 5.4.
 template <typename T, typename W, int LANES, int PASSES>
 __global__ __launch_bounds__(kThreads) void rms_norm_kernel(RowParams p) {
     constexpr int STEP = LANES * 8, HELD = PASSES > 0 ? PASSES : 1;
@@ -50,7 +52,7 @@ __global__ __launch_bounds__(kThreads) void rms_norm_kernel(RowParams p) {
     float v[HELD][8], power = 0.f;
     Eight<W> w[HELD];
     // Of long rows the weights come once the sum is known: their registers would
-    // halve the wavefronts that a CU holds (4096 rows of 16384: 122 us for @).
+    // halve the wavefronts that a CU holds (4096 rows of 16384: 122 us early, 94 so).
     constexpr bool EARLY = PASSES > 0 && PASSES <= 2;
     if constexpr (PASSES > 0) {
         Eight<T> a[PASSES], b[PASSES];
