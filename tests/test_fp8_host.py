@@ -185,6 +185,35 @@ def test_c_refusals(lib):
         assert _gated(lib, ws=0) == _lib.TT_INVALID and _gated(lib, ws_bytes=need - 1) == _lib.TT_INVALID
 
 
+def test_c_refusals_of_calls_beyond_the_grid(lib):
+    """Calls whose extents are allowed one by one, but not together."""
+    big = 1 << 30
+    for dtype in (_lib.TT_F32, _lib.TT_BF16):
+        for kind in (_lib.TT_F32, _lib.TT_E8M0):
+            for k in (128, big):  # on tiles, and where their offsets do not reach
+                assert _product(lib, dtype=dtype, sdtype=kind, M=big, N=big, K=k) == _lib.TT_UNSUPPORTED
+                for out in (dict(y=256, codes=0, scales=0), dict(y=0, codes=256, scales=256, ws_bytes=1 << 62)):
+                    assert _gated(lib, dtype=dtype, sdtype=kind, M=big, N=big, K=k, **out) == _lib.TT_UNSUPPORTED
+    assert _gated(lib, query=True, M=3, N=200, K=(1 << 23) + 1) == 3 * 200 * 4  # no tiles: 32-bit products in between
+    assert _quantize(lib, rows=(1 << 31) - 1, dim=big, stride=big) == _lib.TT_UNSUPPORTED
+
+
+def test_rows_given_other_memory_are_refused(no_gpu):
+    def rows(count=2, codes=256, scales=4):
+        return tt.Fp8Rows._of((2, 256), torch.float32, torch.zeros((count, codes), dtype=torch.uint8).view(E4M3),
+                              torch.zeros((count, scales), dtype=torch.uint8).view(E8M0))
+
+    rows()._check_memory()
+    for bad in (rows(count=1), rows(codes=128), rows(scales=8)):
+        for call in (lambda: tt.fp8_matmul(bad, _Matrix()), lambda: tt.fp8_gated_matmul(bad, _Matrix(), _Matrix())):
+            with pytest.raises(RuntimeError, match="other memory"):
+                call()
+    short = rows()
+    short._codes.untyped_storage().resize_(500)
+    with pytest.raises(RuntimeError, match="other memory"):
+        tt.fp8_matmul(short, _Matrix())
+
+
 def test_c_pack_refusals(lib):
     assert lib.tt_fp8_packed_bytes(17, 129) == 2 * 2 * 2048 and lib.tt_fp8_packed_bytes(0, 5) == 0
     for args in ((-1, 8, 256, 8, 256), (4, 0, 256, 4, 256), (4, 8, 0, 8, 256), (4, 8, 256, 8, 0), (4, 9, 256, 8, 256), (4, 8, 256, 8, 264)):

@@ -265,3 +265,77 @@ def test_c_calls_stay_in_their_results(hip, m, n, k, e8m0):
     room.check()
     want = tt.fp8_gated_matmul(rows, gate, up)
     assert torch.equal(codes.check().view(m, width), _bytes(want._codes)) and torch.equal(scales.check().view(m, per_row), _bytes(want._scales))
+
+
+# ---------------------------------------------------------------------------
+# refusals that the checks of the usual form hand on
+# ---------------------------------------------------------------------------
+def test_refusals(hip):
+    mat, other = _matrix(128, 256, 90), _matrix(128, 300, 91)
+    x, w = torch.ones((4, 256), device="cuda"), torch.ones(256, device="cuda")
+    rows = tt.fp8_quantize(x)
+
+    def asks(t):
+        return t.clone().requires_grad_()
+
+    for call, kind in (
+        (lambda: tt.fp8_quantize(x.double()), NotImplementedError),
+        (lambda: tt.fp8_quantize(x.long()), NotImplementedError),
+        (lambda: tt.fp8_quantize(x[:, :0]), ValueError),
+        (lambda: tt.fp8_quantize(asks(x)), RuntimeError),
+        (lambda: tt.rms_norm(asks(x), w), RuntimeError),
+        (lambda: tt.rms_norm(x, asks(w)), RuntimeError),
+        (lambda: tt.rms_norm(x, w, residual=asks(x)), RuntimeError),
+        (lambda: tt.rms_norm(x, w[:255]), ValueError),
+        (lambda: tt.rms_norm(x, w.double()), NotImplementedError),
+        (lambda: tt.rms_norm(x, w, residual=x[:3]), ValueError),
+        (lambda: tt.rms_norm(x, w, residual=x.half()), ValueError),
+        (lambda: tt.rms_norm(x, w, eps=-1.0), ValueError),
+        (lambda: tt.rms_norm(x, w, eps=float("nan")), ValueError),
+        (lambda: tt.fp8_matmul(rows, other), ValueError),
+        (lambda: tt.fp8_matmul(x, other), ValueError),
+        (lambda: tt.fp8_matmul(asks(x), mat), RuntimeError),
+        (lambda: tt.fp8_matmul(rows, mat, dtype=torch.float64), NotImplementedError),
+        (lambda: tt.fp8_gated_matmul(rows, mat, other), ValueError),
+        (lambda: tt.fp8_gated_matmul(rows, other, other), ValueError),
+        (lambda: tt.fp8_gated_matmul(rows, mat, _matrix(128, 256, 92, e8m0=False)), ValueError),
+        (lambda: tt.fp8_gated_matmul(rows, mat, mat, activation="relu"), ValueError),
+    ):
+        with pytest.raises(kind):
+            call()
+    with torch.no_grad():  # nothing asks here
+        assert torch.equal(tt.rms_norm(asks(x), asks(w)), tt.rms_norm(x, w))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: tt.fp8_quantize(dual), lambda: tt.rms_norm(dual, w), lambda: tt.rms_norm(x, w, residual=dual),
+                     lambda: tt.fp8_matmul(dual, mat), lambda: tt.fp8_gated_matmul(dual, mat, mat)):
+            with pytest.raises(RuntimeError):
+                call()
+
+
+@pytest.mark.parametrize("which", ["codes", "scales"])
+def test_rows_whose_tensors_were_resized_are_refused(hip, which):
+    mat = _matrix(128, 512, 93)
+    for change in (lambda t: t.resize_(16, t.shape[1]), lambda t: t.resize_(4, t.shape[1]), lambda t: t.resize_(t.shape[1], 8),
+                   lambda t: t.untyped_storage().resize_(8), lambda t: t.untyped_storage().resize_(0)):
+        rows = tt.fp8_quantize(torch.ones((8, 512), device="cuda"))
+        tt.fp8_matmul(rows, mat)
+        change(getattr(rows, which))
+        for call in (lambda: tt.fp8_matmul(rows, mat), lambda: tt.fp8_gated_matmul(rows, mat, mat)):
+            with pytest.raises(RuntimeError, match="other memory"):
+                call()
+
+
+def test_rows_of_other_shapes_share_a_layout(hip):
+    """One, two and more dimensions, and widths that need no padding and that do."""
+    for shape in ((512,), (3, 512), (2, 3, 512), (2, 3, 130), (130,), (3, 256), (0, 512), (2, 0, 130)):
+        x = _randn(shape, 94).cuda()
+        rows = tt.fp8_quantize(x)
+        assert rows.codes.shape == shape and rows.scales.shape == (*shape[:-1], -(-shape[-1] // 128))
+        flat = tt.fp8_quantize(x.reshape(-1, shape[-1]))
+        assert torch.equal(_bytes(rows.codes.contiguous()).view(-1), _bytes(flat.codes.contiguous()).view(-1))
+        assert torch.equal(_bytes(rows.scales.contiguous()).view(-1), _bytes(flat.scales.contiguous()).view(-1))
+        mat = _matrix(96, shape[-1], 95)
+        assert torch.equal(tt.fp8_matmul(rows, mat).view(-1, 96), tt.fp8_matmul(flat, mat))
+        again = tt.Fp8Rows(rows.codes, rows.scales, torch.float32)
+        assert torch.equal(again.dequantize(), rows.dequantize())

@@ -365,7 +365,7 @@ class RowsHost {
     Library lib_;
 };
 
-// 8-bit weights. Rows come as their two arrays, whose shapes Fp8Rows vouches for.
+// 8-bit weights. Rows come as their two arrays and the shape they were made in.
 class Fp8Host {
    public:
     Fp8Host(const std::vector<int64_t>& entries, const Tensor& packed, const Tensor& scales, int64_t n, int64_t k, bool e8m0)
@@ -374,7 +374,7 @@ class Fp8Host {
     py::object run(const Tensor& codes, const Tensor& scales, const std::vector<int64_t>& shape, at::ScalarType dtype) const {
         tt_fp8_matmul_args a;
         a.dtype = code_of(dtype);
-        if (a.dtype < 0 || !at_.here() || !takes(codes, shape)) return py::none();
+        if (a.dtype < 0 || !at_.here() || !takes(codes, scales, shape)) return py::none();
         a.scale_dtype = code_;
         a.M = codes.size(0);
         a.N = n_;
@@ -395,7 +395,7 @@ class Fp8Host {
         tt_fp8_gated_args a;
         std::memset(&a, 0, sizeof a);
         a.dtype = code_of(dtype);
-        if (a.dtype < 0 || !at_.here() || !takes(codes, shape) || up.n_ != n_ || up.k_ != k_ || up.code_ != code_ ||
+        if (a.dtype < 0 || !at_.here() || !takes(codes, scales, shape) || up.n_ != n_ || up.k_ != k_ || up.code_ != code_ ||
             up.at_.device != at_.device)
             return py::none();
         a.scale_dtype = code_;
@@ -430,8 +430,17 @@ class Fp8Host {
     }
 
    private:
-    bool takes(const Tensor& codes, const std::vector<int64_t>& shape) const {
-        return codes.is_cuda() && codes.device().index() == at_.device && !shape.empty() && shape.back() == k_ && n_ > 0;
+    // (Users hold both tensors, and may have resized them.)
+    bool takes(const Tensor& codes, const Tensor& scales, const std::vector<int64_t>& shape) const {
+        if (shape.empty() || shape.back() != k_ || n_ < 1) return false;
+        int64_t count = 1;
+        for (size_t i = 0; i + 1 < shape.size(); ++i) count *= shape[i];
+        const int64_t blocks = (k_ + 127) / 128;
+        return whole(codes, count, blocks * 128) && whole(scales, count, (blocks + 3) / 4 * 4);
+    }
+    bool whole(const Tensor& t, int64_t rows, int64_t width) const {
+        return t.is_cuda() && t.device().index() == at_.device && t.dim() == 2 && t.size(0) == rows && t.size(1) == width &&
+               t.is_contiguous() && static_cast<int64_t>(t.storage().nbytes()) >= t.storage_offset() + rows * width;
     }
     std::vector<int64_t> result(std::vector<int64_t> shape) const {
         shape.back() = n_;

@@ -68,9 +68,7 @@ def _shaped(t: torch.Tensor, shape, last: int) -> torch.Tensor:
     """Two-dimensional rows, of which `last` elements count, in their own shape."""
     if t.shape[1] != last:
         t = t.narrow(1, 0, last)
-    if len(shape) == 2:
-        return t
-    return t.unflatten(0, shape[:-1]) if len(shape) > 2 else t[0]
+    return t.unflatten(0, shape[:-1]) if len(shape) > 1 else t[0]
 
 
 class Fp8Rows(_Fixed):
@@ -98,34 +96,45 @@ class Fp8Rows(_Fixed):
         _check_grad("Fp8Rows", codes, scales)
         dispatch.require_hip()
         device = _home("Fp8Rows", codes, scales)
-        self._set(codes.shape, dtype, *_room(codes.shape, device, torch.zeros))
+        self.shape = codes.shape
+        self.dtype = dtype
+        self.device = device
+        self._codes, self._scales = _room(codes.shape, device, torch.zeros)
         features = codes.shape[-1]
         self._codes.view(torch.uint8)[:, :features] = codes.to(device).view(torch.uint8).reshape(-1, features)
         self._scales.view(torch.uint8)[:, : want[-1]] = scales.to(device).view(torch.uint8).reshape(-1, want[-1])
 
-    def _set(self, shape, dtype, codes, scales):
-        put = object.__setattr__
-        put(self, "shape", shape)
-        put(self, "dtype", dtype)
-        put(self, "device", codes.device)
-        put(self, "_codes", codes)
-        put(self, "_scales", scales)
-
-    @classmethod
-    def _of(cls, shape, dtype, codes, scales) -> "Fp8Rows":
-        rows = cls.__new__(cls)
-        rows._set(shape, dtype, codes, scales)
+    @staticmethod
+    def _of(shape, dtype, codes, scales) -> "Fp8Rows":
+        rows = _new(Fp8Rows)
+        _put_shape(rows, shape)
+        _put_dtype(rows, dtype)
+        _put_device(rows, codes.device)
+        _put_codes(rows, codes)
+        _put_scales(rows, scales)
         return rows
+
+    def _check_memory(self):
+        """Tensors that were resized or given other memory since are not what products would read."""
+        count, blocks = math.prod(self.shape[:-1]), _blocks(self.shape[-1])
+        for t, width in ((self._codes, blocks * BLOCK), (self._scales, -(-blocks // 4) * 4)):
+            if (t.device != self.device or tuple(t.shape) != (count, width) or not t.is_contiguous()
+                    or t.untyped_storage().nbytes() < t.storage_offset() + count * width):
+                raise RuntimeError("the tensors of an Fp8Rows were given other memory: make another one of them")
 
     @property
     def codes(self) -> torch.Tensor:
         """float8_e4m3fn (..., features); rows start every multiple of 128 codes."""
-        return _shaped(self._codes, self.shape, self.shape[-1])
+        shape = self.shape
+        n = shape[-1]
+        return self._codes if len(shape) == 2 and n % BLOCK == 0 else _shaped(self._codes, shape, n)
 
     @property
     def scales(self) -> torch.Tensor:
         """float8_e8m0fnu (..., ceil(features / 128)); rows start every multiple of 4 scales."""
-        return _shaped(self._scales, self.shape, _blocks(self.shape[-1]))
+        shape = self.shape
+        n = shape[-1]
+        return self._scales if len(shape) == 2 and n % (4 * BLOCK) == 0 else _shaped(self._scales, shape, _blocks(n))
 
     def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         """The rows' values, in ``dtype`` (the rows' one if None)."""
@@ -134,6 +143,11 @@ class Fp8Rows(_Fixed):
 
     def __repr__(self) -> str:
         return f"Fp8Rows({tuple(self.shape)}, dtype={self.dtype}, device={self.device})"
+
+
+# What sets the attributes of rows that an operator has made (no check in between).
+_new = Fp8Rows.__new__
+_put_shape, _put_dtype, _put_device, _put_codes, _put_scales = (getattr(Fp8Rows, name).__set__ for name in Fp8Rows.__slots__)
 
 
 def _room(shape, device: torch.device, make=torch.empty):
@@ -313,6 +327,7 @@ def _operand(what: str, x, w: Fp8Matrix) -> Fp8Rows:
         raise ValueError(f"x must be (..., {w.shape[1]}); got {tuple(x.shape)}")
     if x.device != w.device:
         raise RuntimeError(f"x is on {x.device}, the weights on {w.device}")
+    x._check_memory()
     return x
 
 
