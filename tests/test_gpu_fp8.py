@@ -408,3 +408,73 @@ def test_gated_matmul_many_rows_and_columns(hip, m, n, k, e8m0):
         if dtype == torch.float32:
             err = _gated(x, wg, wu, "silu", True)[1]
         assert ((plain.cpu().double() - want).abs() <= U[dtype] * want.abs() + (1 + U[dtype]) * err).all()
+
+
+@pytest.mark.parametrize("e8m0", [True, False])
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 128), (40, 1024, 500), (300, 2048, 256), (512, 8192, 128)])
+def test_gated_scales_next_to_a_border(hip, m, n, k, e8m0):
+    """Scales are those of 32-bit sums where the largest value is next to 448 times a
+    power of two. All products are positive, so that a sum errs by its roundings
+    relative to itself: in 32 bits 15 of a lane's 16 terms, two of its scale, and six
+    and seven where lanes and wavefronts are joined, 31 2^-24 with what is of second
+    order. silu passes 1.3 of that on, and the activation adds 8 2^-24: 80 2^-24
+    in all. With float scales the blocks of 128 columns have, for one row each,
+    their largest value 160 2^-24 above or below the border."""
+    band = 80 * 2.0 ** -24
+    blocks, kb = -(-n // 128), -(-k // 128)
+    rand = torch.Generator().manual_seed(m + n)
+
+    def positive(rows, cols):
+        return torch.randn((rows, cols), generator=rand).abs().to(E4M3)
+
+    x, g, u = positive(m, k), positive(n, k), positive(n, k)
+    gs = torch.full((blocks, kb), 4.0 / k)
+    us = 0.5 + torch.rand((blocks, kb), generator=rand)
+    if e8m0:
+        gs, us = torch.full((blocks, kb), 2.0 ** (2 - k.bit_length())), torch.ones((blocks, kb))
+    else:
+        us[:] = us[:, :1]  # one factor for all of a block's columns
+
+    def exact():
+        def product(w, s):
+            return x.double() @ ref.weights(w.double(), s.double()).t()
+
+        a = product(g, gs)
+        return (a / (1.0 + torch.exp(-a)) * product(u, us)).view(m, blocks, 128).amax(dim=2)
+
+    if not e8m0:
+        top = exact()
+        for b in range(blocks):
+            value = top[17 * b % m, b].item()
+            border = 448.0 * 2.0 ** round(math.log2(value / 448.0))
+            us[b] *= border * (1.0 + (2 * band if b % 2 else -2 * band)) / value
+    want = exact()
+    e = torch.ceil(torch.log2(want / 448.0))
+    border = want / (448.0 * 2.0 ** torch.round(torch.log2(want / 448.0))) - 1.0
+    sure = border.abs() > band
+    assert sure.sum() > 0.99 * sure.numel()
+    if not e8m0:
+        assert (sure & (border.abs() < 3 * band)).sum() >= blocks
+        to_w = [tt.Fp8Matrix(w.cuda(), s.cuda()) for w, s in ((g, gs), (u, us))]
+    else:
+        to_w = [tt.Fp8Matrix(w.cuda(), (torch.log2(s) + 127).to(torch.uint8).view(E8M0).cuda()) for w, s in ((g, gs), (u, us))]
+    rows = tt.Fp8Rows(x.cuda(), torch.full((m, kb), 127, dtype=torch.uint8).view(E8M0).cuda())
+    got = tt.fp8_gated_matmul(rows, *to_w)
+    assert torch.equal(got.scales.float().log2().cpu()[sure], e.float()[sure])
+    codes = got.codes.float().view(m, blocks, 128).amax(dim=2)
+    assert (codes >= 224.0).all() and (codes <= 448.0).all()
+
+
+@pytest.mark.parametrize("m", [1, 300])
+def test_scale_of_255_is_nan(hip, m):
+    x, scales = torch.ones((m, 256)).to(E4M3), torch.full((m, 2), 127, dtype=torch.uint8)
+    scales[m // 2, 1] = 255
+    w = tt.Fp8Matrix(torch.ones((256, 256)).to(E4M3).cuda(), torch.ones((2, 2)).cuda())
+    for dtype in DTYPES:
+        y = tt.fp8_matmul(tt.Fp8Rows(x.cuda(), scales.view(E8M0).cuda(), dtype), w).cpu()
+        assert y[m // 2].isnan().all() and (y[torch.arange(m) != m // 2] == 256.0).all()
+    byte = torch.tensor([[127, 255], [127, 127]], dtype=torch.uint8)
+    w = tt.Fp8Matrix(torch.ones((256, 256)).to(E4M3).cuda(), byte.view(E8M0).cuda())
+    for dtype in DTYPES:
+        y = tt.fp8_matmul(torch.ones((m, 256), dtype=dtype).cuda(), w).cpu()
+        assert y[:, :128].isnan().all() and (y[:, 128:] == 256.0).all()
