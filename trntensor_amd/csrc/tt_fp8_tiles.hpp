@@ -79,7 +79,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
     constexpr int WS = E8 ? FOURS : 16;                  // scales held of each: fours of bytes, or floats, of 64 tiles
     constexpr int PER = XI + WI + 1;                     // direct loads a wavefront a stage
     constexpr bool TWICE = NS >= 4;                      // registers hold the operands of two stages
-    constexpr int AHEAD = NS == 2 ? 1 : 0;               // stages that lines are asked of L2 before their direct loads
+    constexpr bool FLOATS = !E8 && !EXACT;
+    constexpr int AHEAD = NS == 2 && !FLOATS ? 1 : 0;    // stages that lines are asked of L2 before their direct loads
     static_assert(XI * 1024 * NW == XB && WI * 1024 * NW == WB && NW >= SI + GM && MB % 2 == 0 && NB % 2 == 0, "tile");
     // The stages held belong to at most FOURS fours.
     static_assert(NS >= 2 && NS <= 9 && (NS - 1) * PER < 64, "stages");
@@ -154,7 +155,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
     // than a line takes that is not in L2: each line is asked for a step earlier
     // by one of the workgroups that share it (four of the same weights, eight or
     // more of the same rows, on one XCD), as one word of it to a place nobody reads.
-    // A wavefront whose turn it is not asks for one line that it has.
+    // A wavefront whose turn it is not asks for one line that it has. 4096 x 8192 x 8192
+    // takes 204 us with it, 217 without; with float scales, whose steps are longer, it
+    // costs what it saves (242 / 239).
     const uint8_t* line = nullptr;
     int line_step = 0;
     if constexpr (AHEAD > 0) {
@@ -198,21 +201,28 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
 #pragma unroll
         for (int m = 0; m < MB; ++m) acc[n][m] = f32x4{0, 0, 0, 0};
     const int nk = p.blocks;
-    // With float scales a product waits for its predecessor's multiplication, which runs beside it.
-    constexpr bool FLOATS = !E8 && !EXACT;
+    // With float scales a block's sum is multiplied when DEPTH products after it are on
+    // their way: two 26.0 us for 1024 x 4096 x 4096, one 27.6, three 26.3; 249 / 256 /
+    // 247 for 2048 x 16384 x 4096 gated, with one sum less to hold than three.
+    constexpr int DEPTH = 2;
     typedef Block<EXACT, E8> B;
-    f32x4 sum;
-    auto scaled = [&](int n, int m, const uint32_t (&ws)[GM]) __attribute__((always_inline)) {
-        acc[n][m] += __uint_as_float(ws[GATED ? n / (NB / 2) : 0]) * sum;
+    f32x4 sum[DEPTH];
+    auto scaled = [&](int at, const uint32_t (&ws)[GM]) __attribute__((always_inline)) {
+        acc[at % NB][at / NB] += __uint_as_float(ws[GATED ? at % NB / (NB / 2) : 0]) * sum[at % DEPTH];
+    };
+    auto last_scaled = [&](const uint32_t (&ws)[GM]) __attribute__((always_inline)) {
+        if constexpr (FLOATS)
+#pragma unroll
+            for (int i = DEPTH; i > 0; --i) scaled(MB * NB - i, ws);
     };
     auto product = [&](int n, int m, const B& w, const B& x, const uint32_t (&ws)[GM], uint32_t sb) __attribute__((always_inline)) {
         if constexpr (FLOATS) {
+            const int at = m * NB + n;
             const f32x4 next = block_sum(w, x, sb);
             __builtin_amdgcn_sched_barrier(0);
-            if (n > 0) scaled(n - 1, m, ws);
-            if (n == 0 && m > 0) scaled(NB - 1, m - 1, ws);
+            if (at >= DEPTH) scaled(at - DEPTH, ws);
             __builtin_amdgcn_sched_barrier(0);
-            sum = next;
+            sum[at % DEPTH] = next;
         } else {
             mma_block(w, x, acc[n][m], ws[GATED ? n / (NB / 2) : 0], sb);
         }
@@ -272,7 +282,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            if constexpr (FLOATS) scaled(NB - 1, MB - 1, ws);
+            last_scaled(ws);
 #pragma unroll
             for (int i = 0; i < GM; ++i) ws[i] = next_ws[i];
             take_ws(ws, stage + 1);
@@ -313,7 +323,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            if constexpr (FLOATS) scaled(NB - 1, MB - 1, ws[P]);
+            last_scaled(ws[P]);
             // The stage after the next was filled before NS - 3 others.
             __builtin_amdgcn_s_waitcnt(wait_vm((NS - 3) * PER));
             asm volatile("s_barrier" ::: "memory");
