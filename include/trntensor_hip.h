@@ -376,7 +376,7 @@ int tt_kv_attention(const tt_kv_attention_args* args, void* stream);
  * scales [rows][S], a byte e + 127 for the power of two 2^e (e8m0) of each
  * block of 128, S being the number of blocks rounded up to a multiple of 4 and
  * the bytes past the blocks zeros. A value is its code times its block's
- * scale. codes are 16-byte aligned, scales 4-byte.
+ * scale (byte 255: NaN). codes are 16-byte aligned, scales 4-byte.
  *
  * Where they are written, e is the smallest one, at least -127, that brings
  * the block's largest finite magnitude to 448 or below; codes are rounded to
@@ -427,8 +427,10 @@ int tt_fp8_pack(int64_t N, int64_t K, const void* codes, int64_t pitch, void* pa
  * y[m][n] = sum_k x[m][k] w[n][k]: rows in 8 bits times weights laid out by
  * tt_fp8_pack. scale_dtype TT_F32: w_scales is [ceil(N / 128)][ceil(K / 128)]
  * floats; TT_E8M0: bytes, [ceil(N / 128)][ceil(K / 128) rounded up to a
- * multiple of 4], 4-byte aligned. Products are summed in 32 bits; y is [M][N]
- * of dtype, contiguous.
+ * multiple of 4], 4-byte aligned. Products are summed in 32 bits where dtype is
+ * TT_F32 (a row's scale times a weight's is then a float32: 2^-126 to 2^127), else
+ * by the 8-bit matrix instructions, eight at a time in 13 bits below the largest.
+ * y is [M][N] of dtype, contiguous.
  */
 typedef struct {
     int64_t dtype, scale_dtype, M, N, K;
@@ -443,7 +445,9 @@ int tt_fp8_matmul(const tt_fp8_matmul_args* args, void* stream);
  * a / (1 + exp(-a)) (activation 0) or 0.5 a (1 + tanh(sqrt(2 / pi) (a +
  * 0.044715 a^3))) (activation 1). h goes, rounded once, to y ([M][N] of dtype)
  * or, in 8 bits, to codes and scales (rows of N elements): the other is NULL.
- * The workspace (4-byte aligned) is needed for codes only, and may be 0 bytes.
+ * Products are summed as above, codes by the 8-bit instructions whatever dtype is;
+ * a block's scale follows 32-bit sums where those leave it open. The workspace
+ * (4-byte aligned) is needed for codes only, and may be 0 bytes: up to 4 M N.
  */
 typedef struct {
     int64_t dtype, scale_dtype, activation, M, N, K;
