@@ -339,3 +339,16 @@ def test_rows_of_other_shapes_share_a_layout(hip):
         assert torch.equal(tt.fp8_matmul(rows, mat).view(-1, 96), tt.fp8_matmul(flat, mat))
         again = tt.Fp8Rows(rows.codes, rows.scales, torch.float32)
         assert torch.equal(again.dequantize(), rows.dequantize())
+
+
+def test_views_that_stand_for_their_negatives(hip):
+    x, w, r = (_randn(s, 96 + i).cuda() for i, s in enumerate(((5, 256), (256,), (5, 256))))
+    nx, nw, nr = (torch._neg_view(-t) for t in (x, w, r))
+    assert torch.equal(nx, x) and nx.is_neg()
+    assert torch.equal(_bytes(tt.fp8_quantize(nx).codes), _bytes(tt.fp8_quantize(x).codes))
+    for got, want in zip(tt.rms_norm(nx, nw, residual=nr), tt.rms_norm(x, w, residual=r)):
+        assert torch.equal(got, want)
+    assert torch.equal(tt.rms_norm(x, nw), tt.rms_norm(x, w)) and torch.equal(tt.rms_norm(x, residual=nr)[0], tt.rms_norm(x, residual=r)[0])
+    mat = _matrix(64, 256, 97)
+    assert torch.equal(tt.fp8_matmul(nx, mat), tt.fp8_matmul(x, mat))
+    assert torch.equal(tt.fp8_matmul(x, tt.Fp8Matrix.quantize(torch._neg_view(-r.cpu()))), tt.fp8_matmul(x, tt.Fp8Matrix.quantize(r)))

@@ -289,7 +289,7 @@ struct Rows8 {
 // Rows of `dim` elements of unit stride, `stride` elements apart; false where they are not.
 bool rows_of(const Tensor& x, int64_t& rows, int64_t& dim, int64_t& stride) {
     const int64_t nd = x.dim();
-    if (nd < 1 || x.size(nd - 1) < 1) return false;
+    if (nd < 1 || x.size(nd - 1) < 1 || x.is_neg()) return false;
     dim = x.size(nd - 1);
     if (nd == 2 && x.stride(1) == 1) {
         rows = x.size(0);
@@ -330,7 +330,8 @@ class RowsHost {
             return py::none();
         if (weight) {
             a.weight_dtype = code_of(weight->scalar_type());
-            if (a.weight_dtype < 0 || weight->dim() != 1 || weight->size(0) != a.dim || !weight->is_contiguous() || !at.holds(*weight))
+            if (a.weight_dtype < 0 || weight->dim() != 1 || weight->size(0) != a.dim || !weight->is_contiguous() || weight->is_neg() ||
+                !at.holds(*weight))
                 return py::none();
             a.weight = weight->data_ptr();
         }

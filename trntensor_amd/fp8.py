@@ -62,8 +62,7 @@ def _home(what: str, *tensors) -> torch.device:
 
 def _rows(t: torch.Tensor, device: torch.device) -> torch.Tensor:
     """`t` as (rows, elements) on the device, its elements of unit stride."""
-    if t.device != device:
-        t = t.to(device)
+    t = t.to(device).resolve_neg()
     t = t if t.dim() == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
@@ -299,7 +298,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
         r2 = _rows(residual, device)
         total = torch.empty(x.shape, dtype=x.dtype, device=device)
     if weight is not None:
-        weight = weight.to(device).contiguous()
+        weight = weight.to(device).resolve_neg().contiguous()
     y = codes = scales = None
     if fp8:
         codes, scales = _room(x.shape, device)
