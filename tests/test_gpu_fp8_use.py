@@ -352,3 +352,77 @@ def test_views_that_stand_for_their_negatives(hip):
     mat = _matrix(64, 256, 97)
     assert torch.equal(tt.fp8_matmul(nx, mat), tt.fp8_matmul(x, mat))
     assert torch.equal(tt.fp8_matmul(x, tt.Fp8Matrix.quantize(torch._neg_view(-r.cpu()))), tt.fp8_matmul(x, tt.Fp8Matrix.quantize(r)))
+
+
+# ---------------------------------------------------------------------------
+# offsets past 32 bits: the last rows give what they give alone
+#
+# Calls of other sizes sum a block's products alike and up to 64 blocks in another
+# order: 64 additions and eight joins of at most 2^-23 of a running sum each, which is
+# 64 blocks' largest at most, 72 64 2^-23 < 10^-3 of it. Two roundings to bfloat16
+# are 2^-8 apart, two codes next to each other 2^-3.
+# ---------------------------------------------------------------------------
+MANY = (1 << 31) // 8192 + 5
+
+
+def _ends(k, seed):
+    """MANY rows of k elements, zeros but for the last seven, and those."""
+    last = _randn((7, k), seed, torch.bfloat16).cuda()
+    x = torch.zeros((MANY, k), dtype=torch.bfloat16, device="cuda")
+    x[-7:] = last
+    return x, last
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_rows_past_32_bits(hip, residual):
+    x, last = _ends(8192, 98)
+    w = _randn((8192,), 99).cuda()
+    if not residual:
+        got, want = tt.fp8_quantize(x), tt.fp8_quantize(last)
+        assert torch.equal(_bytes(got.codes[-7:]), _bytes(want.codes)) and torch.equal(_bytes(got.scales[-7:]), _bytes(want.scales))
+        assert not _bytes(got.codes[:-7]).any() and not _bytes(got.scales[:-7]).any()
+        mat = _matrix(20, 8192, 100)
+        y = tt.fp8_matmul(got, mat)
+        few = tt.fp8_matmul(want, mat).double()
+        assert not y[:-7].any() and ((y[-7:].double() - few).abs() <= 2.0 ** -8 * few.abs() + 1e-3 * few.abs().max()).all()
+    got = tt.rms_norm(x, w, residual=x if residual else None, fp8=True)
+    want = tt.rms_norm(last, w, residual=last if residual else None, fp8=True)
+    if residual:
+        assert torch.equal(got[1][-7:], want[1]) and not got[1][:-7].any()
+        got, want = got[0], want[0]
+    assert torch.equal(_bytes(got.codes[-7:]), _bytes(want.codes)) and torch.equal(_bytes(got.scales[-7:]), _bytes(want.scales))
+
+
+@pytest.mark.parametrize("e8m0", [True, False])
+def test_results_past_32_bits(hip, e8m0):
+    n, k = 8200, 128
+    x, last = _ends(k, 101)
+    gate, up = _matrix(n, k, 102, e8m0), _matrix(n, k, 103, e8m0)
+    rows, few = tt.fp8_quantize(x), tt.fp8_quantize(last)
+    for call in (lambda r: tt.fp8_matmul(r, gate), lambda r: tt.fp8_gated_matmul(r, gate, up, fp8=False)):
+        y, want = call(rows), call(few).double()
+        assert not y[:-7].any() and ((y[-7:].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-3 * want.abs().max()).all()
+        del y
+    got, want = tt.fp8_gated_matmul(rows, gate, up), tt.fp8_gated_matmul(few, gate, up)
+    assert not _bytes(got.codes[:-7]).any()
+    a, b = tt.Fp8Rows(got.codes[-7:], got.scales[-7:]).dequantize().double(), want.dequantize().double()
+    assert ((a - b).abs() <= 2.0 ** -3 * b.abs() + 1e-3 * b.abs().max()).all()
+
+
+@pytest.mark.parametrize("m", [1, 100])
+def test_weights_past_32_bits(hip, m):
+    """Rows of weights that repeat give columns that repeat, in whatever half of the memory they lie."""
+    k = 8192
+    codes = torch.zeros((MANY, k), dtype=torch.uint8, device="cuda")
+    few = (100.0 * _randn((144, k), 104)).clamp(-448.0, 448.0).to(E4M3).cuda()
+    first = (MANY - 144) // 128 * 128
+    codes[first: first + 144] = _bytes(few)
+    scales = torch.full((-(-MANY // 128), k // 128), 0.01, device="cuda")
+    mat, small = tt.Fp8Matrix(codes.view(E4M3), scales), tt.Fp8Matrix(few, scales[:2])
+    del codes
+    x = tt.fp8_quantize(_randn((m, k), 105, torch.bfloat16).cuda())
+    for call in (tt.fp8_matmul, lambda r, w: tt.fp8_gated_matmul(r, w, w, fp8=False)):
+        y, want = call(x, mat), call(x, small).double()
+        part = y[:, first: first + 144].double()
+        assert ((part - want).abs() <= 2.0 ** -8 * want.abs() + 1e-3 * want.abs().max()).all()
+        assert not y[:, :first].any() and not y[:, first + 144:].any()
