@@ -478,3 +478,48 @@ def test_scale_of_255_is_nan(hip, m):
     for dtype in DTYPES:
         y = tt.fp8_matmul(torch.ones((m, 256), dtype=dtype).cuda(), w).cpu()
         assert y[:, :128].isnan().all() and (y[:, 128:] == 256.0).all()
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("m,n,k", [(1, 300, 200), (17, 300, 512), (70, 1030, 256), (300, 2048, 256), (513, 4100, 128)])
+def test_gated_values_that_are_not_finite(hip, m, n, k, activation):
+    """NaN stays in its row; what passes float32's range is NaN in 8 bits and has no part in its block's scale.
+
+    A sum is surely finite where the magnitudes of its blocks' sums add up to less
+    than 2^128, since running sums in any order stay below that, and surely not
+    where itself is beyond it: its last addition, if not one before. Where only
+    running sums or a block's pass it (a multiply-add may hold one that does),
+    either is right."""
+    rows, x = _rows8(m, k, m + n)
+    gate, wg = _weights8(n, k, k, False)
+    g = torch.Generator().manual_seed(n)
+    codes = (100.0 * torch.randn((n, k), generator=g)).clamp(-448.0, 448.0).to(E4M3)
+    scales = 2.0 ** -16 * (0.5 + torch.rand((-(-n // 128), -(-k // 128)), generator=g))
+    scales[1] = 2.0 ** 121  # the second block of columns: values on both sides of the range's end
+    up, wu = tt.Fp8Matrix(codes, scales), ref.weights(codes, scales)[128:256]
+    clean = tt.fp8_gated_matmul(rows, gate, up, activation=activation)
+    got = clean.codes[:, 128:256].float().cpu()
+
+    h, err = _gated(x, wg[128:256], wu * 2.0 ** -100, activation, False)
+    end, off = 2.0 ** 28, _sum_error(x, wu * 2.0 ** -100, False)
+    parts = torch.stack([(x[:, i: i + 128] @ wu[:, i: i + 128].t()).abs() * 2.0 ** -100 for i in range(0, k, 128)])
+    b = (x @ wu.t()).abs() * 2.0 ** -100
+    fine = (parts.sum(dim=0) + off < end) & (h.abs() + err < end)
+    bad = (b - off >= end) | (h.abs() - err >= end)
+    assert not (fine & bad).any() and fine.any() and bad.any() and (fine | bad).float().mean() > 0.5
+    assert got[fine].isfinite().all() and got[bad].isnan().all()
+    low = torch.where(fine, h.abs() - err, torch.zeros_like(h)).amax(dim=1)
+    high = torch.where(fine, h.abs() + err, torch.zeros_like(h)).amax(dim=1)
+    sure = (fine | bad).all(dim=1) & (low > 0)
+    e = torch.ceil(torch.log2(low.clamp(min=1e-300) / 448.0))
+    sure &= e == torch.ceil(torch.log2(high.clamp(min=1e-300) / 448.0))
+    assert torch.equal(clean.scales[:, 1].float().log2().cpu()[sure], (e + 100)[sure].float())
+
+    rest = torch.cat((clean.codes[:, :128], clean.codes[:, 256:]), dim=1).float()
+    assert rest.isfinite().all()
+    row = m // 2
+    _bytes(rows._codes)[row, k // 2] = 0x7F
+    got = tt.fp8_gated_matmul(rows, gate, up, activation=activation)
+    assert got.codes[row].float().isnan().all() and (_bytes(got.scales)[row] == 0).all()
+    keep = torch.arange(m) != row
+    assert torch.equal(_bytes(got.codes)[keep], _bytes(clean.codes)[keep]) and torch.equal(_bytes(got.scales)[keep], _bytes(clean.scales)[keep])
