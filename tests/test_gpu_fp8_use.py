@@ -426,3 +426,40 @@ def test_weights_past_32_bits(hip, m):
         part = y[:, first: first + 144].double()
         assert ((part - want).abs() <= 2.0 ** -8 * want.abs() + 1e-3 * want.abs().max()).all()
         assert not y[:, :first].any() and not y[:, first + 144:].any()
+
+
+@pytest.mark.parametrize("m", [1, 20])
+def test_columns_past_what_tiles_reach(hip, m):
+    """More than 2^23 columns, all but some thousand zeros. A sum errs by 2^-24 for each
+    of 3000 terms of either sign, and what the 8-bit instructions drop of eight products
+    is at most seven times 2^-13 of the largest, 7 2^-13 of all magnitudes; the activation
+    is no steeper than 1.13, and results round by 2^-9."""
+    n, k = 40, (1 << 23) + 200
+    g = torch.Generator().manual_seed(m)
+    where = torch.cat((torch.randint(0, k, (3000,), generator=g).unique(), torch.tensor([k - 1]))).unique()
+    x = torch.zeros((m, k), dtype=torch.bfloat16)
+    x[:, where] = torch.randn((m, len(where)), generator=g).to(torch.bfloat16)
+    rows = tt.fp8_quantize(x.cuda())
+    xv = rows.dequantize(torch.float32)[:, where.cuda()].cpu().double()
+    assert ((xv - x[:, where].double()).abs() <= 2.0 ** -4 * x[:, where].double().abs() + 2.0 ** -10 * 2.0 ** -6).all()
+    mats, values = [], []
+    for seed in (1, 2):
+        codes = torch.zeros((n, k), dtype=torch.uint8, device="cuda")
+        few = (50.0 * torch.randn((n, len(where)), generator=g)).clamp(-448.0, 448.0).to(E4M3)
+        codes[:, where.cuda()] = _bytes(few).cuda()
+        mats.append(tt.Fp8Matrix(codes.view(E4M3), torch.full((1, -(-k // 128)), 2.0 ** -11, device="cuda")))
+        values.append(few.double() * 2.0 ** -11)
+    (gate, up), (wg, wu) = mats, values
+    a, b = xv @ wg.t(), xv @ wu.t()
+    da, db = (7 * 2.0 ** -13 + 3000 * 2.0 ** -24) * (xv.abs() @ wg.abs().t()), (7 * 2.0 ** -13 + 3000 * 2.0 ** -24) * (xv.abs() @ wu.abs().t())
+    assert ((tt.fp8_matmul(rows, gate).cpu().double() - a).abs() <= 2.0 ** -8 * a.abs() + 1.01 * da).all()
+    exact = tt.fp8_matmul(rows, gate, dtype=torch.float32).cpu().double()
+    assert ((exact - a).abs() <= 2.0 ** -23 * a.abs() + 3000 * 2.0 ** -24 * (xv.abs() @ wg.abs().t())).all()
+    h, err = a / (1 + torch.exp(-a)) * b, 1.13 * b.abs() * da + a.abs() * db + 1.13 * da * db
+    assert ((tt.fp8_gated_matmul(rows, gate, up, fp8=False).cpu().double() - h).abs() <= 2.0 ** -8 * h.abs() + 1.01 * err).all()
+    got = tt.fp8_gated_matmul(rows, gate, up)
+    step = 2.0 ** -10 * got.scales.float().cpu().double()
+    assert ((got.dequantize(torch.float32).cpu().double() - h).abs() <= 2.0 ** -4 * h.abs() + 1.07 * err + step).all()
+    norm = tt.rms_norm(x.cuda()).cpu().double()
+    want = x.double() / torch.sqrt((x.double() ** 2).mean(dim=1, keepdim=True) + 1e-6)
+    assert ((norm - want).abs() <= (2.0 ** -8 + 2.0 ** -9) * want.abs()).all()
