@@ -40,17 +40,19 @@ __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
 // lane, from base (uniform) + offset, for all lanes (`on` ~0) or none (0). They are assembly so
 // that the compiler does not take them for writes that every LDS read has to wait
 // for; the kernel's own waits and barriers order them, and loads of no lane count
-// in those waits as any other. Nothing else here uses M0, and all lanes are on.
-__device__ __forceinline__ void copy16(unsigned to, const uint8_t* base, uint32_t offset, unsigned on) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
+// in those waits as any other. Nothing else here uses M0, and all lanes are on. The
+// no-operations keep the five wait states from a vector instruction that writes a
+// scalar register to a load that reads it, and the one from a write of M0.
+__device__ __forceinline__ void copy16(unsigned to, const uint8_t* base, uint32_t offset, uint64_t on) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b64 exec, %3\n\ts_nop 2\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
                  :
-                 : "s"(uniform(to)), "v"(offset), "s"(uniform(base)), "s"(uniform(on))
+                 : "s"(uniform(to)), "v"(offset), "s"(uniform(base)), "s"(on)
                  : "memory", "m0");
 }
-__device__ __forceinline__ void copy4(unsigned to, const uint8_t* base, uint32_t offset, unsigned on) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b64 exec, -1"
+__device__ __forceinline__ void copy4(unsigned to, const uint8_t* base, uint32_t offset, uint64_t on) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b64 exec, %3\n\ts_nop 2\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b64 exec, -1"
                  :
-                 : "s"(uniform(to)), "v"(offset), "s"(uniform(base)), "s"(uniform(on))
+                 : "s"(uniform(to)), "v"(offset), "s"(uniform(base)), "s"(on)
                  : "memory", "m0");
 }
 
@@ -138,7 +140,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
 
     // Direct loads [from, to) of a stage, whose place in LDS is `slot`; of no lane past the last stage.
     auto fill = [&](int stage, int slot, int from, int to) __attribute__((always_inline)) {
-        const unsigned on = stage < p.blocks ? ~0u : 0u;
+        const uint64_t on = stage < p.blocks ? ~0ull : 0ull;
 #pragma unroll
         for (int i = from; i < to; ++i) {
             if (i < XI)
@@ -181,7 +183,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
     auto ask = [&](int stage) __attribute__((always_inline)) {
         const int s = stage < p.blocks ? stage : p.blocks - 1;
         const uint8_t* from = line + (int64_t)s * line_step;
-        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off"
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
                      :
                      : "s"(uniform(ldsw + GM * WS * 256 + wave * 256)), "v"(from)
                      : "memory", "m0");
