@@ -37,12 +37,14 @@ __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
 }
 
 // Direct loads, 16 and 4 bytes a lane, to LDS address `to` (uniform) + 16 or 4 *
-// lane, from base (uniform) + offset, for all lanes (`on` ~0) or none (0). They are assembly so
-// that the compiler does not take them for writes that every LDS read has to wait
-// for; the kernel's own waits and barriers order them, and loads of no lane count
-// in those waits as any other. Nothing else here uses M0, and all lanes are on. The
-// no-operations keep the five wait states from a vector instruction that writes a
-// scalar register to a load that reads it, and the one from a write of M0.
+// lane, from base (uniform) + offset, for all lanes (`on` ~0) or none (0). They are
+// assembly so that the compiler does not take them for writes that every LDS read
+// has to wait for; the kernel's own waits and barriers order them. Loads of no lane
+// count in those waits as any other: in a call of one block of columns all but the
+// first stage's are such, and no other wait than one that leaves as many of them
+// stands between that stage and its use. Nothing else here uses M0, and all lanes
+// are on. The no-operations keep the five wait states from a vector instruction that
+// writes a scalar register to a load that reads it, and the one from a write of M0.
 __device__ __forceinline__ void copy16(unsigned to, const uint8_t* base, uint32_t offset, uint64_t on) {
     asm volatile("s_mov_b32 m0, %0\n\ts_mov_b64 exec, %3\n\ts_nop 2\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
                  :
