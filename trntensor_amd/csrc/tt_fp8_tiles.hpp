@@ -45,16 +45,16 @@ __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
 // stands between that stage and its use. Nothing else here uses M0, and all lanes
 // are on. The no-operations keep the five wait states from a vector instruction that
 // writes a scalar register to a load that reads it, and the one from a write of M0.
-__device__ __forceinline__ void copy16(unsigned to, const uint8_t* base, uint32_t offset, uint64_t on) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b64 exec, %3\n\ts_nop 2\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
+__device__ __forceinline__ void copy16(unsigned to, const uint8_t* base, uint32_t offset, unsigned on) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
                  :
-                 : "s"(uniform(to)), "v"(offset), "s"(uniform(base)), "s"(on)
+                 : "s"(uniform(to)), "v"(offset), "s"(uniform(base)), "s"(uniform(on))
                  : "memory", "m0");
 }
-__device__ __forceinline__ void copy4(unsigned to, const uint8_t* base, uint32_t offset, uint64_t on) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b64 exec, %3\n\ts_nop 2\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b64 exec, -1"
+__device__ __forceinline__ void copy4(unsigned to, const uint8_t* base, uint32_t offset, unsigned on) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\ts_nop 1\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b64 exec, -1"
                  :
-                 : "s"(uniform(to)), "v"(offset), "s"(uniform(base)), "s"(on)
+                 : "s"(uniform(to)), "v"(offset), "s"(uniform(base)), "s"(uniform(on))
                  : "memory", "m0");
 }
 
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
 
     // Direct loads [from, to) of a stage, whose place in LDS is `slot`; of no lane past the last stage.
     auto fill = [&](int stage, int slot, int from, int to) __attribute__((always_inline)) {
-        const uint64_t on = stage < p.blocks ? ~0ull : 0ull;
+        const unsigned on = stage < p.blocks ? ~0u : 0u;
 #pragma unroll
         for (int i = from; i < to; ++i) {
             if (i < XI)
