@@ -29,33 +29,29 @@ __device__ __forceinline__ unsigned lds_address(const void* p) {
     return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 
-// Values that all lanes share, for scalar registers.
-__device__ __forceinline__ unsigned uniform(unsigned x) { return (unsigned)__builtin_amdgcn_readfirstlane((int)x); }
+// Values that all lanes share, for scalar registers, with the five wait states from a
+// vector instruction that writes one to a load that reads it: the compiler does not
+// keep them to loads in assembly.
+__device__ __forceinline__ unsigned uniform(unsigned x) {
+    unsigned r = (unsigned)__builtin_amdgcn_readfirstlane((int)x);
+    asm volatile("s_nop 4" : "+s"(r));
+    return r;
+}
 __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
     const uint64_t v = (uint64_t)(uintptr_t)p;
     return (const uint8_t*)(uintptr_t)((uint64_t)uniform((unsigned)v) | (uint64_t)uniform((unsigned)(v >> 32)) << 32);
 }
 
-// Direct loads, 16 and 4 bytes a lane, to LDS address `to` (uniform) + 16 or 4 *
-// lane, from base (uniform) + offset, for all lanes (`on` ~0) or none (0). They are
-// assembly so that the compiler does not take them for writes that every LDS read
-// has to wait for; the kernel's own waits and barriers order them. Loads of no lane
-// count in those waits as any other: in a call of one block of columns all but the
-// first stage's are such, and no other wait than one that leaves as many of them
-// stands between that stage and its use. Nothing else here uses M0, and all lanes
-// are on. The no-operations keep the five wait states from a vector instruction that
-// writes a scalar register to a load that reads it, and the one from a write of M0.
-__device__ __forceinline__ void copy16(unsigned to, const uint8_t* base, uint32_t offset, unsigned on) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
-                 :
-                 : "s"(uniform(to)), "v"(offset), "s"(uniform(base)), "s"(uniform(on))
-                 : "memory", "m0");
+// Direct loads, 16 and 4 bytes a lane, to LDS address `to` + 16 or 4 * lane, from base
+// + offset; `to` and base are scalars. They are assembly so that the compiler does not
+// take them for writes that every LDS read has to wait for; the kernel's own waits
+// and barriers order them. Nothing else here uses M0, and all lanes are on. The
+// no-operation is the wait state from a write of M0 to its use.
+__device__ __forceinline__ void copy16(unsigned to, const uint8_t* base, uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(offset), "s"(base) : "memory", "m0");
 }
-__device__ __forceinline__ void copy4(unsigned to, const uint8_t* base, uint32_t offset, unsigned on) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\ts_nop 1\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b64 exec, -1"
-                 :
-                 : "s"(uniform(to)), "v"(offset), "s"(uniform(base)), "s"(uniform(on))
-                 : "memory", "m0");
+__device__ __forceinline__ void copy4(unsigned to, const uint8_t* base, uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(to), "v"(offset), "s"(base) : "memory", "m0");
 }
 
 // s_waitcnt immediates: vmcnt in bits 3:0 and 15:14, expcnt 6:4 (7: no wait), lgkmcnt 11:8.
@@ -89,7 +85,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
     // The stages held belong to at most FOURS fours.
     static_assert(NS >= 2 && NS <= 9 && (NS - 1) * PER < 64, "stages");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * STAGE + FOURS * SB + GM * WS * 256 + (AHEAD ? NW * 256 : 0)];
-    const unsigned lds0 = lds_address(lds), ldss = lds0 + NS * STAGE, ldsw = ldss + FOURS * SB;
+    const unsigned lds0 = uniform(lds_address(lds)), ldss = lds0 + NS * STAGE, ldsw = ldss + FOURS * SB;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int wm = wave / WN, wn = wave % WN;
@@ -105,7 +101,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
     // What this lane's direct loads read: rows past the end repeat the last one,
     // weight tiles past the end the last one, and what they give is not stored.
     const int64_t pitch = (int64_t)p.blocks * 128;
-    const uint8_t* x_base = p.x + m0 * pitch;
+    const uint8_t* x_base = uniform(p.x + m0 * pitch);
     uint32_t x_off[XI];
 #pragma unroll
     for (int i = 0; i < XI; ++i) {
@@ -114,15 +110,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
         x_off[i] = (uint32_t)(row * pitch) + (((lane & 7) ^ (r >> 1 & 7)) * 16);
     }
     const int last_tile = (p.N + 15) / 16 - 1;
-    const uint8_t* w_base[WI];
+    // A wavefront's weight tiles are of one matrix, or half of them of either.
+    constexpr int WT = WI / 2, MATS = GATED && WT > NB / 2 ? 2 : 1, WE = WT / MATS;  // tiles, matrices, tiles of each
+    static_assert(WI % 2 == 0 && (!GATED || (MATS == 1 ? NB / 2 % WT == 0 : WT == NB)), "tiles of one matrix");
+    auto weight_tile = [&](int at) __attribute__((always_inline)) {
+        const int t = GATED ? n0 / 16 + at / NB * (NB / 2) + at % NB % (NB / 2) : n0 / 16 + at;
+        return t < last_tile ? t : last_tile;
+    };
+    const uint8_t* w_base[MATS];
+    uint32_t w_off[WT];  // at most 15 tiles on
 #pragma unroll
-    for (int i = 0; i < WI; ++i) {
-        const int at = (wave * WI + i) / 2, j = at % NB;
-        int t = GATED ? n0 / 16 + at / NB * (NB / 2) + j % (NB / 2) : n0 / 16 + at;
-        t = t < last_tile ? t : last_tile;
-        w_base[i] = uniform(p.w[GATED ? j / (NB / 2) : 0] + (int64_t)t * p.blocks * 2048 + (wave * WI + i) % 2 * 1024);
+    for (int i = 0; i < MATS; ++i) {
+        const int at = wave * WT + i * WE, t0 = weight_tile(at);
+        w_base[i] = uniform(p.w[GATED ? at % NB / (NB / 2) : 0] + (int64_t)t0 * p.blocks * 2048);
+#pragma unroll
+        for (int e = 0; e < WE; ++e) w_off[i * WE + e] = (uint32_t)(weight_tile(at + e) - t0) * (uint32_t)p.blocks * 2048 + lane * 16;
     }
-    const uint32_t w_off = lane * 16;
     // The first wavefronts load the rows' scales, a row a lane; the others those
     // of the weights, a tile a lane (as often as there are more lanes).
     const bool of_rows = wave < SI;
@@ -138,20 +141,31 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
         s_base = p.ws[matrix] + (int64_t)(t0 / 8) * pitch_ws;
         s_off = (uint32_t)(((t < last_tile ? t : last_tile) / 8 - t0 / 8) * pitch_ws);
     }
+    s_base = uniform(s_base);
+    // Fours of bytes lie at the multiples of four, floats at four times their stage.
+    const bool fours = of_rows || E8;
+    const uint32_t s_held = fours ? 4 * FOURS - 4 : WS - 1, s_shift = of_rows ? 6 + (SI > 1) + (SI > 2) : fours ? 6 : 8;
+    static_assert(SI == 1 || SI == 2 || SI == 4, "bytes of a four: 256 SI");
     const unsigned s_to = of_rows ? ldss + wave * 256 : ldsw + matrix * WS * 256;
 
-    // Direct loads [from, to) of a stage, whose place in LDS is `slot`; of no lane past the last stage.
+    // Direct loads [from, to) of a stage, whose place in LDS is `slot`. Past the last
+    // stage they are of that once more, for nothing: what stands between two products
+    // counts, and a mask is four scalar instructions a load. With it, a base for each
+    // load and signed and 64-bit arithmetic, 4096 x 8192 x 8192 took 217 us (now 210), with
+    // float scales 231 (224), 1024 x 4096 x 4096 with them 24.7 (22.0), 2048 x 16384 x 4096
+    // gated 222 (215).
+    const unsigned x_to = lds0 + wave * XI * 1024, w_to = lds0 + XB + wave * WI * 1024;
     auto fill = [&](int stage, int slot, int from, int to) __attribute__((always_inline)) {
-        const unsigned on = stage < p.blocks ? ~0u : 0u;
+        const uint32_t at = stage < p.blocks ? stage : p.blocks - 1;
+        const uint8_t* x = x_base + at * 128;
 #pragma unroll
         for (int i = from; i < to; ++i) {
             if (i < XI)
-                copy16(lds0 + slot + (wave * XI + i) * 1024, x_base + (int64_t)stage * 128, x_off[i], on);
+                copy16(x_to + slot + i * 1024, x, x_off[i]);
             else if (i < XI + WI)
-                copy16(lds0 + slot + XB + (wave * WI + i - XI) * 1024, w_base[i - XI] + (int64_t)stage * 2048, w_off, on);
+                copy16(w_to + slot + (i - XI) * 1024, w_base[(i - XI) / 2 / WE] + (at * 2048 + (i - XI) % 2 * 1024), w_off[(i - XI) / 2]);
             else
-                copy4(s_to + (of_rows ? (stage >> 2) % FOURS * SB : (E8 ? stage >> 2 : stage) % WS * 256),
-                      s_base + (of_rows || E8 ? stage >> 2 : stage) * 4, s_off, on);
+                copy4(s_to + ((at & s_held) << s_shift), s_base + (fours ? at & ~3u : at * 4), s_off);
         }
     };
 
@@ -162,33 +176,30 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
     // A wavefront whose turn it is not asks for one line that it has. 4096 x 8192 x 8192
     // takes 204 us with it, 217 without; with float scales, whose steps are longer, it
     // costs what it saves (242 / 239).
-    const uint8_t* line = nullptr;
+    const uint8_t* line = x_base;
+    uint32_t line_off = 0;
     int line_step = 0;
     if constexpr (AHEAD > 0) {
         constexpr int XL = BM / 64, WL = NT / 4;  // wavefronts that have all lines
-        static_assert(XL + WL <= NW, "a line a lane");
-        line = x_base;
+        static_assert(XL + WL <= NW && (!GATED || NB == 4), "a line a lane, of one matrix a wavefront");
         if (wave < XL) {
             const int r = wave * 64 + lane;
             if (rest / high % XL == wave) {
-                line += (m0 + r < p.M ? r : p.M - 1 - m0) * pitch;
+                line_off = (uint32_t)((m0 + r < p.M ? r : p.M - 1 - m0) * pitch);
                 line_step = 128;
             }
         } else if (wave < XL + WL && rest % high % WL == wave - XL) {
-            const int at = (wave - XL) * 4 + lane / 16, j = at % NB;
-            int t = GATED ? n0 / 16 + at / NB * (NB / 2) + j % (NB / 2) : n0 / 16 + at;
-            t = t < last_tile ? t : last_tile;
-            line = p.w[GATED ? j / (NB / 2) : 0] + (int64_t)t * p.blocks * 2048 + lane % 16 * 128;
+            // Four neighbouring tiles, gated ones of the one matrix or of the other.
+            const int q = wave - XL, t0 = n0 / 16 + (GATED ? q / 2 : q) * 4, t = t0 + lane / 16;
+            const int least = t0 < last_tile ? t0 : last_tile;
+            line = uniform(p.w[GATED ? q & 1 : 0] + (int64_t)least * p.blocks * 2048);
+            line_off = (uint32_t)((t < last_tile ? t : last_tile) - least) * (uint32_t)p.blocks * 2048 + lane % 16 * 128;
             line_step = 2048;
         }
     }
     auto ask = [&](int stage) __attribute__((always_inline)) {
         const int s = stage < p.blocks ? stage : p.blocks - 1;
-        const uint8_t* from = line + (int64_t)s * line_step;
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
-                     :
-                     : "s"(uniform(ldsw + GM * WS * 256 + wave * 256)), "v"(from)
-                     : "memory", "m0");
+        copy4(ldsw + GM * WS * 256 + wave * 256, line + (uint32_t)s * (uint32_t)line_step, line_off);
     };
 
     // Where this lane reads its operands of 16 rows or 16 weight rows.
@@ -233,14 +244,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
     };
     auto read_x = [&](B& x, uint32_t& xs, int slot, int m, int stage) __attribute__((always_inline)) {
         x.load(xr0 + slot + m * 2048, xr1 + slot + m * 2048);
-        xs = *reinterpret_cast<const uint32_t*>(sr + (stage >> 2) % FOURS * SB + m * 64);
+        xs = *reinterpret_cast<const uint32_t*>(sr + ((stage >> 2) & (FOURS - 1)) * SB + m * 64);
     };
     auto read_w = [&](B& w, int slot, int n) __attribute__((always_inline)) {
         w.load(wr + slot + n * 2048, wr + slot + n * 2048 + 1024);
     };
     auto read_ws = [&](uint32_t (&ws)[GM], int stage) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < GM; ++i) ws[i] = *reinterpret_cast<const uint32_t*>(wsr + (i * WS + (E8 ? stage >> 2 : stage) % WS) * 256);
+        for (int i = 0; i < GM; ++i) ws[i] = *reinterpret_cast<const uint32_t*>(wsr + (i * WS + ((E8 ? stage >> 2 : stage) & (WS - 1))) * 256);
     };
     auto take_ws = [&](uint32_t (&ws)[GM], int stage) __attribute__((always_inline)) {
         if constexpr (E8)
