@@ -262,8 +262,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
     if constexpr (!TWICE) {
         constexpr int XR = MB % 4 == 0 ? 4 : 2, LEAD = XR / 2;  // blocks of rows in registers, and read ahead
         // Products that a stage's direct loads are spread over, some of them behind
-        // the barrier and the rest in the next step.
-        constexpr int SPREAD = MB * NB * 7 / 16, LATE = PER * (LEAD * NB < SPREAD ? LEAD * NB : SPREAD) / SPREAD;
+        // the barrier and the rest in the next step: half of them 204 us for 4096 x 8192 x
+        // 8192, 7 of 16 210, 9 207, 5 217; with float scales 228, 225, 229 and 225.
+        constexpr int SPREAD = MB * NB * (FLOATS ? 7 : 8) / 16, LATE = PER * (LEAD * NB < SPREAD ? LEAD * NB : SPREAD) / SPREAD;
         B w[NB], x[XR];
         uint32_t xs[XR], ws[GM], next_ws[GM];
         auto step = [&](int stage) __attribute__((always_inline)) {
@@ -293,7 +294,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
                     const bool before = m < MB - LEAD;
                     if (at < SPREAD) fill(stage + NS - before, before ? last : slot, PER * at / SPREAD, PER * (at + 1) / SPREAD);
                     if constexpr (AHEAD > 0)
-                        if (at == SPREAD - 1) ask(stage + NS - before + AHEAD);
+                        if (at == SPREAD) ask(stage + NS - before + AHEAD);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
