@@ -90,7 +90,8 @@ __device__ __forceinline__ uint32_t weight_scale(const Fp8Params& p, int r, int 
 
 // act(a) b: both activations are a / (1 + exp(-bend)), since (1 + tanh(z)) / 2 is 1 /
 // (1 + exp(-2 z)). The hardware's exponential (of base 2) and reciprocal err by a
-// unit each, which costs nothing next to the products' sums; with a full division
+// unit each, which costs nothing next to the products' sums (past a = -87 the
+// exponential is infinite, and what would be below 10^-36 is 0); with a full division
 // and exponential a round of tiles of 256 x 128 values took 14.2 us, with these 10.6
 // (2048 x 16384 from one block of columns, four rounds: 56.6 and 42.6 us).
 template <int ACTIVATION>
