@@ -158,6 +158,14 @@ __device__ __forceinline__ bool near_border(float amax) {
 }
 constexpr float kCandidate = 1.f - 0x1p-11f;
 
+// What a block's scale goes by where its largest value `amax` is near a border and
+// `again` is that of the 32-bit sums: they say on which side of the border it lies,
+// and no more. Where large terms cancel they can be anywhere, but the codes are
+// made of the values that gave amax, which have to stay within the scale.
+__device__ __forceinline__ float decided(float amax, float again) {
+    return fminf(fmaxf(again, amax * kCandidate), amax * (1.f + 0x1p-11f));
+}
+
 // What a call's products are summed by and written as.
 enum { kHalf, kExact, kRaw, kCodes };
 

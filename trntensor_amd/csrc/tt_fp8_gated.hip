@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) void gated_round_kernel(Fp8Params p, int piece
                 if (lane / 16 == l / 16) again = fmaxf(again, h);
             }
         }
-        if (near_border(amax) && left > 0 && again > 0.f) amax = again;
+        if (near_border(amax) && left > 0 && again > 0.f) amax = decided(amax, again);
     }
     fp8_store8(v, amax, col, blocks, p.codes + (int64_t)row * blocks * 128, p.scales + (int64_t)row * ((blocks + 3) / 4 * 4));
 }

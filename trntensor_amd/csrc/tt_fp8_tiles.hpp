@@ -501,7 +501,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(Fp8Params p,
             float amax = top[r];
 #pragma unroll
             for (int i = 1; i < WN; ++i) amax = fmaxf(amax, top[i * BM + r]);
-            if (near_border(amax) && count <= LIST && again[r] > 0.f) amax = again[r];
+            if (near_border(amax) && count <= LIST && again[r] > 0.f) amax = decided(amax, again[r]);
             const uint32_t byte = fp8_scale_byte(amax);
             const float inv = fp8_scale_inverse(byte);
 #pragma unroll
