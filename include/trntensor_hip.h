@@ -400,8 +400,9 @@ int tt_fp8_quantize(const tt_fp8_quantize_args* args, void* stream);
  * bits. residual and weight may be NULL. The result goes, rounded once, to y
  * (contiguous, dtype) or, in 8 bits, to codes and scales: the other is NULL.
  * sum (contiguous, dtype; NULL iff residual is) gets h rounded; y follows from
- * h as it was before. No result overlaps an operand. eps is finite and not
- * negative.
+ * h as it was before. No result overlaps an operand. eps is finite, below 1e38 and not
+ * negative. Magnitudes of h below 2^63 are taken whatever dim is; the squares of
+ * larger ones may overflow, and y is zeros then.
  */
 typedef struct {
     int64_t dtype, weight_dtype, rows, dim, x_stride, residual_stride;

@@ -1,6 +1,8 @@
 // Rows into 8 bits (tt_fp8_quantize), and the root-mean-square norm with the
 // residual stream's addition (tt_rms_norm):
 //   h = x + residual,  y = h / sqrt(mean(h^2) + eps) * weight
+#include <cmath>
+
 #include "tt_fp8.hpp"
 
 namespace tt {
@@ -16,13 +18,26 @@ struct RowParams {
     int64_t x_stride, r_stride, rows;
     int dim, blocks;
     int weight_dtype;
-    float eps;
+    float eps, eps_root;
+    double eps_exact;
 };
 
 __device__ __forceinline__ float wave_sum32(float v) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
     return v;
+}
+
+__device__ __forceinline__ float wave_max32(float v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, kWave));
+    return v;
+}
+
+// 2^-e of a positive float of exponent e (2^127 at most).
+__device__ __forceinline__ float inverse_power(float x) {
+    const uint32_t field = 254u - (__float_as_uint(x) >> 23);
+    return __uint_as_float((field < 254u ? field : 254u) << 23);
 }
 
 // W: float, or __bf16 for weights of either 16-bit type. LANES lanes a row (a
@@ -84,15 +99,57 @@ __global__ __launch_bounds__(kThreads) void rms_norm_kernel(RowParams p) {
             for (int i = 0; i < 8; ++i) power += v[0][i] * v[0][i];
         }
     }
-    power = wave_sum32(power);
-    if constexpr (LANES > kWave) {
-        if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = power;
+    // The wavefronts' sums or maxima of a row, in their order.
+    auto joined = [&](float value, auto join) __attribute__((always_inline)) {
+        if constexpr (LANES == kWave) return value;
+        if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = value;
         __syncthreads();
-        power = 0.f;
+        value = part[0];
 #pragma unroll
-        for (int i = 0; i < kThreads / kWave; ++i) power += part[i];
+        for (int i = 1; i < kThreads / kWave; ++i) value = join(value, part[i]);
+        return value;
+    };
+    auto add = [](float a, float b) __attribute__((always_inline)) { return a + b; };
+    float mean = joined(wave_sum32(power), add) / (float)p.dim + p.eps;
+    // Squares of elements from 2^55 on may pass 2^128 in a row, and below 2^-50 lose bits or
+    // vanish, which counts where eps is as small. Such rows (all lanes have one mean) are summed
+    // again, times a power of two that brings the larger of their top and eps's root to 1.
+    // From 2^63 on they stay as they are: zeros over an infinite mean.
+    float lift = 1.f;
+    if (!(mean >= 0x1p-100f && mean < INFINITY)) {
+        auto each = [&](auto use) __attribute__((always_inline)) {
+            if constexpr (PASSES > 0) {
+#pragma unroll
+                for (int u = 0; u < PASSES; ++u) use(v[u]);
+            } else {
+                for (int col = first; col < p.dim; col += STEP) {
+                    total(col, v[0]);
+                    use(v[0]);
+                }
+            }
+        };
+        float top = 0.f;
+        each([&](const float (&h)[8]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(h[i]));
+        });
+        if constexpr (LANES > kWave) __syncthreads();
+        top = joined(wave_max32(top), [](float a, float b) __attribute__((always_inline)) { return fmaxf(a, b); });
+        const float high = fmaxf(top, p.eps_root);
+        if (high > 0.f && top < 0x1p63f) {
+            lift = inverse_power(high);
+            power = 0.f;
+            each([&](float (&h)[8]) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[i] *= lift, power += h[i] * h[i];
+            });
+            if constexpr (LANES > kWave) __syncthreads();
+            mean = joined(wave_sum32(power), add) / (float)p.dim + (float)(p.eps_exact * lift * lift);
+        } else if (high == 0.f && p.eps_exact > 0.0) {
+            mean = 1.f;  // zeros over an eps that is none in 32 bits
+        }
     }
-    const float scale = 1.f / sqrtf(power / (float)p.dim + p.eps);
+    const float scale = 1.f / sqrtf(mean);
     auto finish = [&](int col, float (&v)[8], const Eight<W>& w) __attribute__((always_inline)) {
         // Past the row's end these stay zeros, whatever the scale.
 #pragma unroll
@@ -117,6 +174,8 @@ __global__ __launch_bounds__(kThreads) void rms_norm_kernel(RowParams p) {
         for (int col = first; col < end; col += STEP) {
             if (p.weight) w[0].load(weight, col, p.dim);
             total(col, v[0]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[0][i] *= lift;
             finish(col, v[0], w[0]);
         }
     }
@@ -202,6 +261,8 @@ extern "C" int tt_rms_norm(const tt_rms_norm_args* a, void* stream) {
     p.rows = a->rows;
     p.weight_dtype = (int)a->weight_dtype;
     p.eps = (float)a->eps;
+    p.eps_root = (float)std::sqrt(a->eps);
+    p.eps_exact = a->eps;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const bool wide = a->weight && a->weight_dtype == TT_F32;
     if (a->dtype == TT_F32) return wide ? rms_norm_run<float, float>(p, st) : rms_norm_run<float, __bf16>(p, st);

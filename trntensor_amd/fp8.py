@@ -270,8 +270,10 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
     ``weight`` (features,) in any of the three (ones if None). Returns the norm
     in x's dtype or, with ``fp8``, as :class:`Fp8Rows`; with a residual, a pair
     of the norm and h in x's dtype. The norm follows from h before that
-    rounding. Squares are summed in 32 bits: magnitudes of 2^63 and more overflow
-    them. Rows need a unit stride and one row pitch, else they are copied.
+    rounding. Squares are summed in 32 bits, those of rows that would overflow or
+    vanish there again with a power of two taken out: any magnitudes below 2^63 are
+    taken, whatever the width. Larger ones may overflow, and the row's norm is zeros
+    then. Rows need a unit stride and one row pitch, else they are copied.
     """
     host = _fastpath.rows_host()
     if host is not None and dispatch._use_hip() and isinstance(x, torch.Tensor):
