@@ -181,23 +181,26 @@ __global__ __launch_bounds__(kThreads) void rms_norm_kernel(RowParams p) {
     }
 }
 
+// Workgroups: four rows each up to 1024 elements, else one.
+int64_t rms_norm_grid(int64_t rows, int64_t dim) { return dim <= 1024 ? (rows + 3) / 4 : rows; }
+
 template <typename T, typename W>
 int rms_norm_run(const RowParams& p, hipStream_t st) {
-    const uint32_t rows = (uint32_t)p.rows, quarter = (uint32_t)((p.rows + 3) / 4);
+    const uint32_t grid = (uint32_t)rms_norm_grid(p.rows, p.dim);
     if (p.dim <= 512)
-        rms_norm_kernel<T, W, 64, 1><<<quarter, kThreads, 0, st>>>(p);
+        rms_norm_kernel<T, W, 64, 1><<<grid, kThreads, 0, st>>>(p);
     else if (p.dim <= 1024)
-        rms_norm_kernel<T, W, 64, 2><<<quarter, kThreads, 0, st>>>(p);
+        rms_norm_kernel<T, W, 64, 2><<<grid, kThreads, 0, st>>>(p);
     else if (p.dim <= 2048)
-        rms_norm_kernel<T, W, 256, 1><<<rows, kThreads, 0, st>>>(p);
+        rms_norm_kernel<T, W, 256, 1><<<grid, kThreads, 0, st>>>(p);
     else if (p.dim <= 4096)
-        rms_norm_kernel<T, W, 256, 2><<<rows, kThreads, 0, st>>>(p);
+        rms_norm_kernel<T, W, 256, 2><<<grid, kThreads, 0, st>>>(p);
     else if (p.dim <= 8192)
-        rms_norm_kernel<T, W, 256, 4><<<rows, kThreads, 0, st>>>(p);
+        rms_norm_kernel<T, W, 256, 4><<<grid, kThreads, 0, st>>>(p);
     else if (p.dim <= 16384)
-        rms_norm_kernel<T, W, 256, 8><<<rows, kThreads, 0, st>>>(p);
+        rms_norm_kernel<T, W, 256, 8><<<grid, kThreads, 0, st>>>(p);
     else
-        rms_norm_kernel<T, W, 256, 0><<<rows, kThreads, 0, st>>>(p);
+        rms_norm_kernel<T, W, 256, 0><<<grid, kThreads, 0, st>>>(p);
     return check_launch("tt_rms_norm");
 }
 
@@ -227,7 +230,7 @@ int check_rows(const char* who, int64_t dtype, int64_t rows, int64_t dim) {
     constexpr int64_t kMost = int64_t(1) << 30;
     if (!serving_dtype(dtype)) return set_error(TT_UNSUPPORTED, "%s: dtype %lld (TT_F32, TT_BF16, TT_F16)", who, (long long)dtype);
     if (rows < 0 || dim < 1) return set_error(TT_INVALID, "%s: %lld rows of %lld", who, (long long)rows, (long long)dim);
-    if (rows > kMaxGrid || dim > kMost) return set_error(TT_UNSUPPORTED, "%s: %lld rows of %lld", who, (long long)rows, (long long)dim);
+    if (rows > kMost << 10 || dim > kMost) return set_error(TT_UNSUPPORTED, "%s: %lld rows of %lld", who, (long long)rows, (long long)dim);
     return TT_OK;
 }
 
@@ -241,6 +244,8 @@ extern "C" int tt_rms_norm(const tt_rms_norm_args* a, void* stream) {
     if (a->weight && !serving_dtype(a->weight_dtype))
         return set_error(TT_UNSUPPORTED, "tt_rms_norm: weight dtype %lld (TT_F32, TT_BF16, TT_F16)", (long long)a->weight_dtype);
     if (!(a->eps >= 0.0) || a->eps > 1e38) return set_error(TT_INVALID, "tt_rms_norm: eps %g", a->eps);
+    if (rms_norm_grid(a->rows, a->dim) > kMaxGrid)
+        return set_error(TT_UNSUPPORTED, "tt_rms_norm: %lld rows of %lld", (long long)a->rows, (long long)a->dim);
     if (a->rows == 0) return TT_OK;
     if (!a->x || !a->residual != !a->sum || !a->codes != !a->scales || !a->y == !a->codes)
         return set_error(TT_INVALID, "tt_rms_norm: NULL pointer, or both of y and codes");
