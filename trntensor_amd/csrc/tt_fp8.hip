@@ -107,9 +107,14 @@ template <bool EXACT, bool E8, int R, bool GATED>
 int rows_run(int kind, const Fp8Params& p, hipStream_t st) {
     const int64_t grid = ((int64_t)(p.N + 15) / 16 + R - 1) / R * ((p.M + 15) / 16);
     if (grid > kMaxGrid / 2) return set_error(TT_UNSUPPORTED, "8-bit products: %lld workgroups", (long long)grid);
-    if (kind != kHalf)
-        fp8_rows_kernel<float, EXACT, E8, R, GATED><<<(uint32_t)grid, 64 * kWaves, 0, st>>>(p);
-    else if constexpr (!EXACT) {
+    // Results in 32 bits are exact sums or, of the gated block, what a second launch rounds.
+    if constexpr (EXACT || GATED) {
+        if (EXACT || kind == kRaw) {
+            fp8_rows_kernel<float, EXACT, E8, R, GATED><<<(uint32_t)grid, 64 * kWaves, 0, st>>>(p);
+            return check_launch("8-bit products");
+        }
+    }
+    if constexpr (!EXACT) {
         if (p.bf16)
             fp8_rows_kernel<__bf16, EXACT, E8, R, GATED><<<(uint32_t)grid, 64 * kWaves, 0, st>>>(p);
         else

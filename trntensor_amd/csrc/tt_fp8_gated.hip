@@ -7,11 +7,12 @@ namespace {
 
 template <typename T, bool E8>
 int tiles_of(int which, const Fp8Params& p, hipStream_t st) {
+    // Raw results of these two would have a block's 128 columns: written as codes at once.
+    if constexpr (!std::is_same<T, Raw>::value) {
+        if (which == 0) return tiles_run<T, E8, true, 2, 4, 8, 4, 2>(p, st);
+        if (which == 1) return tiles_run<T, E8, true, 2, 4, 4, 4, 3>(p, st);
+    }
     switch (which) {
-        case 0:
-            return tiles_run<T, E8, true, 2, 4, 8, 4, 2>(p, st);
-        case 1:
-            return tiles_run<T, E8, true, 2, 4, 4, 4, 3>(p, st);
         case 2:
             return tiles_run<T, E8, true, 2, 2, 4, 4, 4>(p, st);
         case 3:
@@ -100,9 +101,10 @@ double fp8_gated_tiles_cost(const Fp8Params& p, int kind, int* which) {
             if (i == 0 || cost < best) best = cost, *which = i;
         }
     } else {
-        for (int i = 0; i < 5; ++i) {
+        const int first = kind == kRaw ? 2 : 0;
+        for (int i = first; i < 5; ++i) {
             const double cost = tiles_cost(p, shapes[i][0], shapes[i][1], steps[i]);
-            if (i == 0 || cost < best) best = cost, *which = i;
+            if (i == first || cost < best) best = cost, *which = i;
         }
     }
     return best * p.blocks;
