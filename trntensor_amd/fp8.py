@@ -349,8 +349,9 @@ def fp8_matmul(x: Fp8Rows | torch.Tensor, w: Fp8Matrix, *, dtype: torch.dtype | 
     ``x`` is :class:`Fp8Rows`, or a tensor that is quantized first, as by
     :func:`fp8_quantize`. The result is rounded once to ``dtype`` (that of x if
     None); how products are summed follows from that dtype, as at the top of this
-    module: in 32 bits for float32. With float32 scales a block of 128 is summed
-    before its weights' scale multiplies it. A row's scale times a weight's has to
+    module: in 32 bits for float32. With float32 scales a block of 128 is summed,
+    times its row's scale, before its weights' scale multiplies it. Sums that pass
+    float32's range on the way are infinite. A row's scale times a weight's has to
     be a float32 (2^-126 to 2^127) for float32 results. NaN in a row gives NaN in the
     row's result, and so do its block's codes under a scale of NaN (byte 255).
     """
@@ -378,8 +379,8 @@ def fp8_gated_matmul(x: Fp8Rows | torch.Tensor, gate: Fp8Matrix, up: Fp8Matrix, 
 
     ``x`` is as :func:`fp8_matmul` takes it; ``gate`` and ``up`` are weights of
     one shape, with scales of one dtype. ``activation`` is "silu", a / (1 +
-    exp(-a)), or "gelu_tanh", a (1 + tanh(sqrt(2 / pi) (a + 0.044715 a^3))) / 2.
-    The result is rounded once: to 8 bits as :func:`fp8_quantize` does, or without
+    exp(-a)), or "gelu_tanh", a (1 + tanh(sqrt(2 / pi) (a + 0.044715 a^3))) / 2;
+    what is below 10^-36 of it counts as 0. The result is rounded once: to 8 bits as :func:`fp8_quantize` does, or without
     ``fp8`` to x's dtype; sums are as in :func:`fp8_matmul`. A block's scale follows
     sums in 32 bits where the other ones leave it open, within 2^-12 of a power of two's
     border (unless many values share it). Returns
