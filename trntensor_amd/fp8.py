@@ -223,8 +223,8 @@ class Fp8Matrix(_Fixed):
             size = torch.where(part.isfinite(), part.abs(), 0.0).amax(dim=(0, 2))
             fraction, e = torch.frexp(size)
             e = torch.where(size > 0, e - 9 + (fraction > 0.875).int(), -127).clamp(min=-127)
-            # 2^-e from its bits: torch.ldexp takes a power, off by a unit for some exponents on a
-            # GPU, and in the default dtype.
+            # 2^-e from its bits: powers that a GPU computes are a unit off for some exponents
+            # (halfway weights would go to the odd code), and have the default dtype's range.
             inverse = (127 - e).bitwise_left_shift(23).view(torch.float32)
             part = torch.where(part.isfinite(), part * inverse[:, None], math.nan).to(FP8)
             codes[i * BLOCK: i * BLOCK + rows] = part.view(rows, -1)[:, :k]
