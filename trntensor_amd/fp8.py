@@ -378,13 +378,13 @@ def fp8_gated_matmul(x: Fp8Rows | torch.Tensor, gate: Fp8Matrix, up: Fp8Matrix, 
     """``act(x @ gate.T) * (x @ up.T)``, the first half of a gated feed-forward block.
 
     ``x`` is as :func:`fp8_matmul` takes it; ``gate`` and ``up`` are weights of
-    one shape, with scales of one dtype. ``activation`` is "silu", a / (1 +
-    exp(-a)), or "gelu_tanh", a (1 + tanh(sqrt(2 / pi) (a + 0.044715 a^3))) / 2;
-    what is below 10^-36 of it counts as 0. The result is rounded once: to 8 bits as :func:`fp8_quantize` does, or without
-    ``fp8`` to x's dtype; sums are as in :func:`fp8_matmul`. A block's scale follows
+    one shape, with scales of one dtype. ``activation`` is "silu", a / (1 + exp(-a)), or
+    "gelu_tanh", a (1 + tanh(sqrt(2 / pi) (a + 0.044715 a^3))) / 2; what is below 10^-36 of
+    it counts as 0. The result is rounded once: to 8 bits as :func:`fp8_quantize` does, or
+    without ``fp8`` to x's dtype; sums are as in :func:`fp8_matmul`. A block's scale follows
     sums in 32 bits where the other ones leave it open, within 2^-12 of a power of two's
-    border (unless many values share it). Returns
-    :class:`Fp8Rows` or a tensor (..., out_features).
+    border (unless many values share it). Returns :class:`Fp8Rows` or a tensor (...,
+    out_features).
     """
     if gate.shape != up.shape or gate.scale_dtype != up.scale_dtype:
         raise ValueError(f"gate and up must be alike; got {gate} and {up}")
